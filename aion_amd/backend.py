@@ -35,6 +35,13 @@ def quantize_blocks(dtype, values, quant_axis):
     return out
 
 
+def _pair(buffers):
+    """Handles of one or two buffers, 0 for the second of one."""
+    if not 1 <= len(buffers) <= 2:
+        raise AionHipError(hip.INVALID_ARGUMENT, "%d buffers: one of keys, or one of keys and one of values" % len(buffers))
+    return buffers[0].handle, buffers[1].handle if len(buffers) == 2 else 0
+
+
 class DeviceBuffer:
     def __init__(self, backend, handle, nbytes):
         self.backend, self.handle, self.nbytes = backend, handle, nbytes
@@ -422,6 +429,30 @@ class HipBackend:
         """StepSequenceAppend with rows and cache of one element type, F16 or F32 (cpu/exec/sequence_append.zig:12-104)."""
         self._check(self._lib.aionhip_step_sequence_append(self._ctx, dtype, cache.handle, new_kv.handle, end_index.handle, b, s, t_cap,
                                                            row_elems, 1 if rolling else 0))
+
+    def cache_quant_bytes(self, dtype, b, t_cap, h, d):
+        """Bytes of a cache of `t_cap` rows held in 8 (Q8_0) or 4 (Q4_0) bits."""
+        n = int(self._lib.aionhip_cache_quant_bytes(dtype, b, t_cap, h, d))
+        if n == 0:
+            raise AionHipError(hip.INVALID_ARGUMENT, "cache_quant_bytes(dtype=%r, b=%d, t_cap=%d, h=%d, d=%d)" % (dtype, b, t_cap, h, d))
+        return n
+
+    def step_append_quant(self, dtype, caches, rows, write_index, shape, src_dtype=F32, rolling=False):
+        """Rows of keys, or of keys and values (lists of one or two buffers), quantised into their caches; shape = (b, s, t_cap, h, d)."""
+        (kc, vc), (k, v) = _pair(caches), _pair(rows)
+        self._check(self._lib.aionhip_step_append_quant(self._ctx, dtype, kc, k, vc, v, src_dtype, write_index.handle, *shape, 1 if rolling else 0))
+
+    def step_rope_append_quant(self, dtype, q_out, q, k, v, k_cache, v_cache, positions, write_index, b, s, t_cap, h_q, h_kv, d,
+                               base=10000.0, scale_factor=1.0, proportion=1.0, rolling=False):
+        """RoPE1D(q), RoPE1D(k) -> quantised append of k and v, one launch."""
+        self._check(self._lib.aionhip_step_rope_append_quant(
+            self._ctx, dtype, q_out.handle, q.handle, k.handle, v.handle, k_cache.handle, v_cache.handle, positions.handle, write_index.handle,
+            b, s, t_cap, h_q, h_kv, d, base, scale_factor, proportion, 1 if rolling else 0))
+
+    def step_cache_read(self, dtype, outs, caches, first, shape, out_dtype=F32, rolling=False):
+        """Steps first[b] .. +s of one or two quantised caches (lists of buffers) as rows [b, s, h, d]; shape = (b, s, t_cap, h, d)."""
+        (ko, vo), (kc, vc) = _pair(outs), _pair(caches)
+        self._check(self._lib.aionhip_step_cache_read(self._ctx, dtype, out_dtype, ko, kc, vo, vc, first.handle, *shape, 1 if rolling else 0))
 
     def cache_grow(self, dst, src, outer, old_run_bytes, new_run_bytes):
         """dst [outer, new_run_bytes] <- the runs of src [outer, old_run_bytes], zero elsewhere (storage/manager/grow.zig:37-78)."""

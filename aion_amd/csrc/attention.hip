@@ -25,6 +25,8 @@
 // (cpu/kernels/fast_math.zig:79-92, rel. err 4e-5), so results agree to ~1e-4, not bitwise.
 #include "attention_flash.h"
 
+#include "cache_quant.h"
+
 #include <type_traits>
 
 namespace {
@@ -407,7 +409,9 @@ bool dtype_ok(int d) { return d == AIONHIP_F32 || d == AIONHIP_F16 || d == AIONH
 int run_attention(aionhip_ctx *ctx, const aionhip_attention *p, const PreparedAct *prepared) {
     if (!ctx || !p) return AIONHIP_INVALID_ARGUMENT;
     if ((!p->out && !prepared) || !p->q || !p->k || !p->v) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: null operand");
-    if (!dtype_ok(p->q_dtype) || !dtype_ok(p->kv_dtype)) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: q/kv dtype must be f32, f16 or bf16");
+    const bool quant = cq::is_quant(p->kv_dtype);
+    if (!dtype_ok(p->q_dtype) || !(quant || dtype_ok(p->kv_dtype)))
+        return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: q dtype must be f32, f16 or bf16, kv dtype one of these, q8_0 or q4_0");
     if (p->h_kv == 0 || p->h_q == 0 || p->h_q % p->h_kv != 0) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: h_q %zu is not a multiple of h_kv %zu", p->h_q, p->h_kv);
     if (p->d_k == 0 || p->d_v == 0) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: zero head size");
     if (p->batch == 0 || p->l_q == 0) return AIONHIP_OK;
@@ -415,6 +419,9 @@ int run_attention(aionhip_ctx *ctx, const aionhip_attention *p, const PreparedAc
     if (p->batch > lim || p->l_q > lim || p->t_kv > lim || p->h_q > 65535 || p->d_k > 65535 || p->d_v > 65535 ||
         p->batch * p->h_kv > 65535 || p->l_q * (p->h_q / p->h_kv) > lim)
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
+
+    if (quant && prepared) return rows_not_prepared(ctx, "quantized caches");
+    if (quant && p->t_kv) return run_attention_quant(ctx, p);
 
     AttnArgs a{};
     a.q = (const void *)(uintptr_t)p->q;

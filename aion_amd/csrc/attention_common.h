@@ -191,5 +191,7 @@ constexpr int PF_ROWS = 128, PF_TK = 64;
 // whether the prefill kernel takes this call (head size 64, 128 or 256; K/V f16 or bf16; not the hi+lo precise mode)
 bool prefill_takes(const AttnArgs &a, int d);
 int launch_prefill(aionhip_ctx *ctx, AttnArgs &a, int d);
+// the step over q8_0 / q4_0 caches of at least one row (attention_quant.hip)
+int run_attention_quant(aionhip_ctx *ctx, const aionhip_attention *p);
 
 }  // namespace attn

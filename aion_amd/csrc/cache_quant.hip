@@ -1,0 +1,264 @@
+// Writing rows into caches held in 8 or 4 bits and reading them back (the layout: cache_quant.h). One pass over the data each; what a call
+// of a few rows costs is its launch, what one of many rows costs is memory.
+#include "cache_quant.h"
+
+#include <cmath>
+#include <cstring>
+
+namespace {
+using namespace cq;
+
+template <typename T> T *dp(aionhip_handle h) { return reinterpret_cast<T *>((uintptr_t)h); }
+
+// eight values of any alignment their type allows (global memory takes wide accesses at any address)
+__device__ __forceinline__ void load8(const void *src, int dtype, size_t i, float (&x)[8]) {
+    if (dtype == AIONHIP_F32) {
+        __builtin_memcpy(x, (const float *)src + i, 32);
+        return;
+    }
+    unsigned short h[8];
+    __builtin_memcpy(h, (const unsigned short *)src + i, 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(h[j])) : __uint_as_float((unsigned)h[j] << 16);
+}
+
+// the row of a cache that step `t` of a sequence lives in, or -1: outside of a linear cache, or before the first step
+__device__ __forceinline__ long row_of(long t, int t_cap, int rolling) {
+    if (t < 0) return -1;
+    if (rolling) return (long)((unsigned long)t % (unsigned long)t_cap);
+    return t < (long)t_cap ? t : -1;
+}
+
+// four lanes store a block: `at` = its head's row, `col` = the lane's first element
+template <int DT>
+__device__ __forceinline__ void store_block8(unsigned char *codes, __half *scales, size_t unit, long row, int tp, int d, int col, const float (&x)[8]) {
+    unsigned word[2];
+    __half scale;
+    quantize8<DT>(x, word, scale);
+    if (row < 0) return;                                       // (behind the exchange between the lanes)
+    if constexpr (DT == AIONHIP_Q8_0) {
+        unsigned char *o = codes + (unit * tp + (size_t)row) * d + col;
+        *(uint2 *)o = make_uint2(word[0], word[1]);
+    } else {
+        *(unsigned *)(codes + (unit * tp + (size_t)row) * (d / 2) + col / 2) = word[0];
+    }
+    if ((col & 31) == 0) scales[(unit * (d / 32) + col / 32) * tp + (size_t)row] = scale;
+}
+
+struct Pair {
+    unsigned char *codes[2];
+    __half *scales[2];
+    const void *rows[2];
+};
+
+// SequenceAppend with the quantization in it: a thread holds eight elements, four threads a block. Threads run over a head's tokens before the next
+// head's, so that a workgroup's codes are one run.
+template <int DT>
+__global__ __launch_bounds__(256) void append_quant_kernel(Pair p, const int *write_index, int src_dtype, int s_len, int t_cap, int tp, int h, int d, int rolling, size_t total) {
+    const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (gid >= total) return;
+    const int which = blockIdx.y, per = d / 8;
+    const int col = (int)(gid % per) * 8;
+    const size_t rest = gid / per, unit = rest / s_len;                     // unit: sequence and head
+    const int s = (int)(rest % s_len), b = (int)(unit / h), head = (int)(unit % h);
+    const int at = write_index[b];
+    float x[8];
+    load8(p.rows[which], src_dtype, (((size_t)b * s_len + s) * h + head) * d + col, x);
+    store_block8<DT>(p.codes[which], p.scales[which], unit, row_of((long)at + s, t_cap, rolling), tp, d, col, x);
+}
+
+// RoPE1D on q and k, and the append of k and v, for the tokens of one step: a thread holds eight elements of one head of one token. What it rotates
+// with lies half a head away, in another thread, and is read a second time rather than exchanged. The bits of aionhip_step_rope and aionhip_step_append_quant.
+template <int DT>
+__global__ __launch_bounds__(256) void rope_append_quant_kernel(float *q_out, const float *q, const float *k, const float *v, Cache kc, Cache vc, const int *positions,
+                                                                const int *write_index, int s_len, int t_cap, int tp, int h_q, int h_kv, int d, int rope_pairs,
+                                                                const float *freq, int rolling, size_t total) {
+    const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (gid >= total) return;
+    const int per = d / 8, slots = h_q + 2 * h_kv, half = d / 2;
+    const int col = (int)(gid % per) * 8;
+    const int slot = (int)(gid / per % slots);
+    const size_t tok = gid / ((size_t)per * slots);
+    const bool is_q = slot < h_q, is_v = slot >= h_q + h_kv;
+    const int head = is_q ? slot : is_v ? slot - h_q - h_kv : slot - h_q;
+    const size_t row0 = is_q ? (tok * h_q + head) * d : (tok * h_kv + head) * d;
+    const float *src = is_q ? q : is_v ? v : k;
+    const int pos = positions[tok], at = write_index[tok / s_len];
+    float x[8];
+    load8(src, AIONHIP_F32, row0 + col, x);
+    const bool high = col >= half;
+    const int first = high ? col - half : col;                               // of its eight pairs (half a head is a multiple of sixteen)
+    if (!is_v && first < rope_pairs) {
+        float other[8];
+        load8(src, AIONHIP_F32, row0 + (high ? first : col + half), other);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (first + i >= rope_pairs) continue;
+            float sn, cs, yl, yh;
+            sincosf((float)pos * freq[first + i], &sn, &cs);
+            rope_rotate(high ? other[i] : x[i], high ? x[i] : other[i], sn, cs, yl, yh);
+            x[i] = high ? yh : yl;
+        }
+    }
+    if (is_q) {
+        __builtin_memcpy(q_out + row0 + col, x, 32);
+        return;                                                              // (whole blocks: the four lanes of one leave together)
+    }
+    const size_t b = tok / s_len;
+    const long row = row_of((long)at + (long)(tok % s_len), t_cap, rolling);
+    const Cache &c = is_v ? vc : kc;
+    store_block8<DT>(c.codes, c.scales, b * h_kv + head, row, tp, d, col, x);
+}
+
+struct ReadPair {
+    const unsigned char *codes[2];
+    const __half *scales[2];
+    void *out[2];
+};
+
+// Rows first[b] .. first[b] + s_len - 1 as numbers, in the order they leave: a thread has eight elements, a row that the cache does not hold is zeros.
+// The product of a code and a scale is exact in f32 and rounded once.
+template <int DT, int OUT>
+__global__ __launch_bounds__(256) void cache_read_kernel(ReadPair p, const int *first, int s_len, int t_cap, int tp, int h, int d, int rolling, size_t total) {
+    const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (gid >= total) return;
+    const int which = blockIdx.y, per = d / 8;
+    const int col = (int)(gid % per) * 8;
+    const size_t rest = gid / per;
+    const int head = (int)(rest % h);
+    const size_t tok = rest / h, b = tok / s_len;
+    const long row = row_of((long)first[b] + (long)(tok % s_len), t_cap, rolling);
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row >= 0) {
+        const size_t unit = b * h + head;
+        const float scale = __half2float(p.scales[which][(unit * (d / 32) + col / 32) * tp + (size_t)row]);
+        if constexpr (DT == AIONHIP_Q8_0) {
+            const uint2 w = *(const uint2 *)(p.codes[which] + (unit * tp + (size_t)row) * d + col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)((int)((i < 4 ? w.x : w.y) >> (8 * (i & 3)) & 255u) - 128) * scale;
+        } else {
+            const unsigned w = *(const unsigned *)(p.codes[which] + (unit * tp + (size_t)row) * (d / 2) + col / 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (float)((int)(w >> (4 * i) & 15u) - 8) * scale;
+        }
+    }
+    if constexpr (OUT == AIONHIP_F32) {
+        __builtin_memcpy((float *)p.out[which] + gid * 8, x, 32);
+    } else {
+        unsigned short o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (OUT == AIONHIP_F16) o[i] = __half_as_ushort(__float2half_rn(x[i]));
+            else o[i] = __builtin_bit_cast(unsigned short, (__bf16)x[i]);
+        }
+        __builtin_memcpy((unsigned short *)p.out[which] + gid * 8, o, 16);
+    }
+}
+
+int check_shape(aionhip_ctx *ctx, const char *who, int dtype, size_t b, size_t s, size_t t_cap, size_t h, size_t d) {
+    if (!is_quant(dtype)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: caches are q8_0 or q4_0, not dtype %d", who, dtype);
+    if (d % 32 != 0) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: head size %zu is not a multiple of 32", who, d);
+    if (d > MAX_HEAD || h > MAX_HEADS || t_cap > MAX_ROWS || b > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: dimension too large", who);
+    if (s > t_cap) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: %zu tokens exceed the cache capacity %zu", who, s, t_cap);
+    if (b && h && d && t_cap && !aionhip_cache_quant_bytes(dtype, b, t_cap, h, d)) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: size overflow", who);
+    return AIONHIP_OK;
+}
+// workgroups of 256 threads, each with eight of `values` elements
+int grid_of(aionhip_ctx *ctx, const char *who, size_t values, unsigned *grid) {
+    const size_t wgs = (values / 8 + 255) / 256;
+    if (wgs > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
+    *grid = (unsigned)wgs;
+    return AIONHIP_OK;
+}
+int check_cache(aionhip_ctx *ctx, const char *who, aionhip_handle c) {
+    return c & 15 ? set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: a cache begins at a multiple of 16 bytes", who) : AIONHIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t aionhip_cache_quant_bytes(int dtype, size_t b, size_t t_cap, size_t h, size_t d) {
+    if (!is_quant(dtype) || !b || !t_cap || !h || !d || d % 32 != 0 || d > MAX_HEAD || h > MAX_HEADS || t_cap > MAX_ROWS) return 0;
+    const size_t rows = h * padded(t_cap), row = row_bytes(dtype, d) + d / 32 * 2;          // < 2^48 * 2^17
+    if (rows > ((size_t)1 << 46) || b > ((size_t)1 << 62) / (rows * row)) return 0;
+    return b * rows * row;
+}
+
+int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cache, aionhip_handle k, aionhip_handle v_cache, aionhip_handle v, int src_dtype,
+                              aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (!k_cache || !k || !write_index || !v_cache != !v) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: null operand");
+    if (src_dtype != AIONHIP_F32 && src_dtype != AIONHIP_F16 && src_dtype != AIONHIP_BF16)
+        return set_err(ctx, AIONHIP_UNSUPPORTED, "append_quant: rows are f32, f16 or bf16, not dtype %d", src_dtype);
+    if (k_cache == v_cache) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: keys and values in one cache");
+    int rc = check_shape(ctx, "append_quant", dtype, b, s, t_cap, h, d);
+    if (!rc) rc = check_cache(ctx, "append_quant", k_cache | v_cache);
+    if (rc || !b || !s || !h || !d) return rc;
+    const size_t total = b * s * h * d;
+    unsigned grid;
+    if ((rc = grid_of(ctx, "append_quant", total, &grid))) return rc;
+    const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
+    const Pair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k), dp<void>(v)}};
+    ProfScope scope(ctx, "append_quant");
+    launch_k(ctx, dtype == AIONHIP_Q8_0 ? append_quant_kernel<AIONHIP_Q8_0> : append_quant_kernel<AIONHIP_Q4_0>, dim3(grid, v ? 2 : 1), dim3(256), 0, p,
+             dp<const int>(write_index), src_dtype, (int)s, (int)t_cap, (int)padded(t_cap), (int)h, (int)d, rolling ? 1 : 0, total / 8);
+    LAUNCH_CHECK(ctx, "append_quant");
+    return AIONHIP_OK;
+}
+
+int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q_out, aionhip_handle q, aionhip_handle k, aionhip_handle v, aionhip_handle k_cache,
+                                   aionhip_handle v_cache, aionhip_handle positions, aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h_q, size_t h_kv,
+                                   size_t d, float base_frequency, float scale_factor, float rope_proportion, int rolling) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (!q_out || !q || !k || !v || !k_cache || !v_cache || !positions || !write_index) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: null operand");
+    if (!(base_frequency > 0.f) || !(base_frequency < INFINITY) || !(scale_factor > 0.f) || !(scale_factor < INFINITY) || !(rope_proportion >= 0.f && rope_proportion <= 1.f))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: base/scale must be positive and finite, proportion in [0,1]");
+    if (k_cache == v_cache) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: keys and values in one cache");
+    if (q_out == q) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: q is read again while q_out is written");
+    int rc = check_shape(ctx, "rope_append_quant", dtype, b, s, t_cap, h_kv, d);
+    if (!rc) rc = check_cache(ctx, "rope_append_quant", k_cache | v_cache);
+    if (rc || !b || !s || !h_q || !h_kv || !d) return rc;
+    if (h_q > MAX_HEADS) return set_err(ctx, AIONHIP_UNSUPPORTED, "rope_append_quant: dimension too large");
+    const size_t half = d / 2, total = b * s * (h_q + 2 * h_kv) * d;
+    unsigned grid;
+    if ((rc = grid_of(ctx, "rope_append_quant", total, &grid))) return rc;
+    size_t rope_pairs = (size_t)floorf(rope_proportion * (float)half);
+    if (rope_pairs > half) rope_pairs = half;
+    const float freq_step = (float)pow((double)base_frequency, (double)(-2.0f / (float)d));
+    const float *freq = nullptr;
+    if ((rc = rope_table(ctx, (int)rope_pairs, freq_step, scale_factor, &freq))) return rc;
+    ProfScope scope(ctx, "rope_append_quant");
+    launch_k(ctx, dtype == AIONHIP_Q8_0 ? rope_append_quant_kernel<AIONHIP_Q8_0> : rope_append_quant_kernel<AIONHIP_Q4_0>, dim3(grid), dim3(256), 0, dp<float>(q_out),
+             dp<const float>(q), dp<const float>(k), dp<const float>(v), view(k_cache, dtype, b, t_cap, h_kv, d), view(v_cache, dtype, b, t_cap, h_kv, d),
+             dp<const int>(positions), dp<const int>(write_index), (int)s, (int)t_cap, (int)padded(t_cap), (int)h_q, (int)h_kv, (int)d, (int)rope_pairs, freq,
+             rolling ? 1 : 0, total / 8);
+    LAUNCH_CHECK(ctx, "rope_append_quant");
+    return AIONHIP_OK;
+}
+
+int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_handle k_out, aionhip_handle k_cache, aionhip_handle v_out, aionhip_handle v_cache,
+                            aionhip_handle first, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (!k_out || !k_cache || !first || !v_out != !v_cache) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "cache_read: null operand");
+    if (out_dtype != AIONHIP_F32 && out_dtype != AIONHIP_F16 && out_dtype != AIONHIP_BF16)
+        return set_err(ctx, AIONHIP_UNSUPPORTED, "cache_read: rows are f32, f16 or bf16, not dtype %d", out_dtype);
+    int rc = check_shape(ctx, "cache_read", dtype, b, s, t_cap, h, d);
+    if (!rc) rc = check_cache(ctx, "cache_read", k_cache | v_cache);
+    if (rc || !b || !s || !h || !d) return rc;
+    const size_t total = b * s * h * d;
+    unsigned grid;
+    if ((rc = grid_of(ctx, "cache_read", total, &grid))) return rc;
+    const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
+    const ReadPair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k_out), dp<void>(v_out)}};
+    const auto kernel = dtype == AIONHIP_Q8_0 ? (out_dtype == AIONHIP_F32 ? cache_read_kernel<AIONHIP_Q8_0, AIONHIP_F32>
+                                                 : out_dtype == AIONHIP_F16 ? cache_read_kernel<AIONHIP_Q8_0, AIONHIP_F16> : cache_read_kernel<AIONHIP_Q8_0, AIONHIP_BF16>)
+                                              : (out_dtype == AIONHIP_F32 ? cache_read_kernel<AIONHIP_Q4_0, AIONHIP_F32>
+                                                 : out_dtype == AIONHIP_F16 ? cache_read_kernel<AIONHIP_Q4_0, AIONHIP_F16> : cache_read_kernel<AIONHIP_Q4_0, AIONHIP_BF16>);
+    ProfScope scope(ctx, "cache_read");
+    launch_k(ctx, kernel, dim3(grid, v_out ? 2 : 1), dim3(256), 0, p, dp<const int>(first), (int)s, (int)t_cap, (int)padded(t_cap), (int)h, (int)d, rolling ? 1 : 0, total / 8);
+    LAUNCH_CHECK(ctx, "cache_read");
+    return AIONHIP_OK;
+}
+
+}  // extern "C"

@@ -254,7 +254,9 @@ typedef struct aionhip_attention {
     aionhip_handle out, q, k, v, query_positions, kv_lengths;
     size_t batch, l_q, t_kv, h_q, h_kv, d_k, d_v;
     int q_dtype;   /* F32 | F16 | BF16 */
-    int kv_dtype;  /* F32 | F16 | BF16 */
+    int kv_dtype;  /* F32 | F16 | BF16, or Q8_0 | Q4_0: caches as aionhip_cache_quant_bytes describes them (t_kv = their capacity,
+                    * head sizes multiples of 32 up to 1024). Such a step keeps f32 accuracy (about 1e-6), whatever
+                    * aionhip_set_attention_precise says. */
     float scale, attn_logits_soft_cap;
     uint32_t window_left, window_right, window_chunk;
     /* 1: k and v are rolling caches (storage/cache.zig:35-38, 202-207): logical key t lives in row t % T,
@@ -265,8 +267,8 @@ typedef struct aionhip_attention {
 int aionhip_step_attention(aionhip_ctx *ctx, const aionhip_attention *p);
 /* aionhip_step_attention and the matmul of its output rows (w: k = h_q * d_v, C [batch * l_q, n] with row pitch ldc, 0: n) on the exact GEMM, in two
  * launches: the attention kernel writes the rows as the GEMM reads them; p->out is not used. The results are those of the two calls to the bit.
- * AIONHIP_UNSUPPORTED, with nothing launched, where the step would cut its keys into segments (long prompts of few heads, few queries over a long
- * cache) or run on the generic kernel, or the matmul on another one (a few rows, the bf16 modes): issue the two calls. */
+ * AIONHIP_UNSUPPORTED, with nothing launched, where the caches are quantized, where the step would cut its keys into segments (long prompts of few heads, few
+ * queries over a long cache) or run on the generic kernel, or the matmul on another one (a few rows, the bf16 modes): issue the two calls. */
 int aionhip_step_attention_matmul(aionhip_ctx *ctx, const aionhip_attention *p, const aionhip_weight *w, aionhip_handle c, size_t ldc, float alpha,
                                   float beta);
 /* f32 queries over an f16/bf16 cache: off (default) = q rounded to the cache element type, one MFMA
@@ -326,6 +328,28 @@ int aionhip_step_gather_rows(aionhip_ctx *ctx, int table_dtype, aionhip_handle o
 int aionhip_step_append_f16(aionhip_ctx *ctx, aionhip_handle cache, aionhip_handle src_f32, aionhip_handle write_index,
                             size_t b, size_t s, size_t t_cap, size_t row_elems, int rolling);
 int aionhip_step_cast_f32_f16(aionhip_ctx *ctx, aionhip_handle out_f16, aionhip_handle x_f32, size_t n);
+/* Caches held in 8 or 4 bits (dtype AIONHIP_Q8_0 or AIONHIP_Q4_0), for sequences whose keys and values would not fit, or whose reading bounds a decode
+ * step: 34 or 18 bytes to 32 elements instead of 64. aion quantizes weights only; the arithmetic of a block is that of aionhip_quantize_blocks.
+ * A cache for b sequences of up to t_cap rows of h heads of d elements (d a multiple of 32) is ONE buffer of aionhip_cache_quant_bytes bytes (0: arguments out of
+ * range) that begins at a multiple of 16 bytes: codes [B,H,Tp,D * bits / 8] first, Tp = t_cap rounded up to 64, then one f16 scale to every 32 elements,
+ * [B,H,D / 32,Tp]. A code is stored with 128 (q8_0) or 8 (q4_0, the even element in the low half of a byte) added, an element is code * scale. Rows
+ * that were never written may hold anything, as long as no step is told to read them. A linear cache grows by two aionhip_cache_grow calls, one for the codes
+ * (outer b * h, runs of Tp * D * bits / 8 bytes) and one for the scales (outer b * h * d / 32, runs of Tp * 2). */
+size_t aionhip_cache_quant_bytes(int dtype, size_t b, size_t t_cap, size_t h, size_t d);
+/* StepSequenceAppend into such caches, the quantization included: rows k (and v; v_cache and v may both be 0) [B,S,H,D] of src_dtype F32, F16 or BF16 go to
+ * token index write_index[b] .. +S (i32 [B] on device) as aionhip_step_append_f16 places them: rolling = 1 to row t % t_cap; a row outside of a linear cache
+ * is not written. An infinity or a NaN makes its block of 32 read back as NaN. */
+int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cache, aionhip_handle k, aionhip_handle v_cache, aionhip_handle v, int src_dtype,
+                              aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling);
+/* aionhip_step_rope_append over such caches (rolling = 1: rings): RoPE1D on q and k, quantization and append of k and v as one launch, the
+ * bits of aionhip_step_rope followed by aionhip_step_append_quant. q_out is not q. */
+int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q_out, aionhip_handle q, aionhip_handle k, aionhip_handle v, aionhip_handle k_cache,
+                                   aionhip_handle v_cache, aionhip_handle positions, aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h_q, size_t h_kv,
+                                   size_t d, float base_frequency, float scale_factor, float rope_proportion, int rolling);
+/* Rows back out of such caches: out [B,S,H,D] of out_dtype F32, F16 or BF16 = the elements of steps first[b] .. +S (i32 [B] on device), of k_cache and, unless v_out
+ * and v_cache are both 0, of v_cache; rolling = 1: step t is in row t % t_cap. Steps before the first, or past the end of a linear cache, read as zeros. */
+int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_handle k_out, aionhip_handle k_cache, aionhip_handle v_out, aionhip_handle v_cache,
+                            aionhip_handle first, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling);
 /* StepSequenceAppend as the step itself (runtime/executable.zig:193-206, cpu/exec/sequence_append.zig:12-104): cache
  * [B,T,H,D] and new_kv [B,S,H,D] of the same element type `dtype` (AIONHIP_F16 or AIONHIP_F32), end_index i32 [B] on the
  * device; rows go to token index end_index[b] .. +S (rolling = 1: to row t % T). A row that would fall outside a linear
