@@ -14,6 +14,7 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE_KEYS = 32;
+constexpr float REF_NONE = -3.402823466e38f;      // the reference of what holds no key
 
 struct AttnArgs {
     const void *q, *k, *v;

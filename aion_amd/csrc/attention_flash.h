@@ -21,7 +21,6 @@ struct FlashCfg {
     static constexpr int LDS_BYTES = Q_OFF + 16 * Q_ROW;
 };
 constexpr int SPLIT_NW = 8;
-constexpr float REF_NONE = -3.402823466e38f;      // the reference of what holds no key
 constexpr int MEET_PARTS = 32;     // parts that the merging workgroup adds in one tree, with all of their loads in flight
 
 // HILO: q and the probabilities are fed to the MFMAs as a high and a low half-precision part
