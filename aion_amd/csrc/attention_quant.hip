@@ -139,7 +139,43 @@ __device__ __forceinline__ float fma_half(float x, unsigned pair, int k, float y
     const h2 h = __builtin_bit_cast(h2, pair);
     return fmaf(x, (float)(k ? h.y : h.x), y);
 }
+// In the body of a rare condition: or the compiler computes what it changes for every tile and selects, and has both forms in registers
+__device__ __forceinline__ void stay_branch() { asm volatile(""); }
+// A zero that the compiler does not know: fma_half with it stays one instruction (a product alone is a conversion and a multiplication)
+__device__ __forceinline__ float opaque_zero() {
+    float z = 0.f;
+    asm volatile("" : "+v"(z));
+    return z;
+}
 __device__ __forceinline__ unsigned pack_half(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+
+// A query row times a power of two that leaves its largest element in [1, 2): shrink = 2^-e, grow = 2^e, both normal floats. A row that holds no finite maximum stays as it is.
+struct Power2 {
+    float shrink, grow;
+    __device__ __forceinline__ explicit Power2(float amax) {
+        const unsigned e = amax < INFINITY ? min(max(__float_as_uint(amax) >> 23, 2u), 252u) : 127u;
+        shrink = __uint_as_float((254u - e) << 23);
+        grow = __uint_as_float(e << 23);
+    }
+};
+// eight elements of a block times `by` as the sum of two f16 each, in the order of K's codes
+template <int DT>
+__device__ __forceinline__ void split_query(const float (&q)[8], float by, u32x4 (&op)[2]) {
+    float x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = q[element_slot<DT>(j)] * by;
+        y[j] = x[j] - (float)(_Float16)x[j];
+    }
+    op[0] = u32x4{pack2<AIONHIP_F16>(x[0], x[1]), pack2<AIONHIP_F16>(x[2], x[3]), pack2<AIONHIP_F16>(x[4], x[5]), pack2<AIONHIP_F16>(x[6], x[7])};
+    op[1] = u32x4{pack2<AIONHIP_F16>(y[0], y[1]), pack2<AIONHIP_F16>(y[2], y[3]), pack2<AIONHIP_F16>(y[4], y[5]), pack2<AIONHIP_F16>(y[6], y[7])};
+}
+
+// cap * tanh(s * by) * log2(e), as 1 - 2 / (e^2x + 1): off by less than 2^-22 of the cap wherever s lies, without a branch
+__device__ __forceinline__ float capped(float s, float by, float cap) {
+    const float t = __builtin_amdgcn_exp2f(s * by * (2.f * LOG2E));
+    return cap * LOG2E * fmaf(-2.f, __builtin_amdgcn_rcpf(t + 1.f), 1.f);
+}
 
 // N transposing reads (8 rows x 16 bytes within sixteen lanes: lane 2 r + q gives the address of half q of row r, lane i gets byte i of the rows), complete
 // when the statement is. The builtin would wait for every load in flight, whose target LDS may be.
@@ -361,31 +397,25 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         load_k(t);
         load_v(t);
     }
-    amax = groups4_max(amax);
-    const int e_q = amax < INFINITY ? max((int)(__float_as_uint(amax) >> 23), 2) : 127;           // (1 <= the biased exponents of 2^-e and 2^e <= 254)
-    const float shrink_q = __uint_as_float((unsigned)(254 - min(e_q, 253)) << 23), grow_q = __uint_as_float((unsigned)min(e_q, 253) << 23);
-    const float sign = a.scale < 0.f ? -shrink_q : shrink_q;
-    const float row_scale = fabsf(a.scale) * grow_q;
-    const float to_log2 = a.soft_cap > 0.f ? 1.f : row_scale * LOG2E;
+    const Power2 by(groups4_max(amax));
+    const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
+    const float row_scale = fabsf(a.scale) * by.grow;
+    const float to_log2 = a.soft_cap > 0.f ? 1.f : fmaxf(row_scale * LOG2E, 1e-30f);          // (not zero: the score of a key that is not seen is minus infinity)
+    const float zero = opaque_zero();
+    const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
     u32x4 q_op[Cfg::Q_LDS ? 1 : KK][2];
     const unsigned q_addr = (unsigned)(size_t)(lds_void *)lds + lane * 16;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-        float x[8], y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = kk % REP == sub ? qx[kk][element_slot<DT>(j)] * sign : 0.f;
-            y[j] = x[j] - (float)(_Float16)x[j];
-        }
-        const u32x4 high{pack2<AIONHIP_F16>(x[0], x[1]), pack2<AIONHIP_F16>(x[2], x[3]), pack2<AIONHIP_F16>(x[4], x[5]), pack2<AIONHIP_F16>(x[6], x[7])};
-        const u32x4 low{pack2<AIONHIP_F16>(y[0], y[1]), pack2<AIONHIP_F16>(y[2], y[3]), pack2<AIONHIP_F16>(y[4], y[5]), pack2<AIONHIP_F16>(y[6], y[7])};
+        u32x4 op[2];
+        split_query<DT>(qx[kk], kk % REP == sub ? sign : 0.f, op);
         if constexpr (Cfg::Q_LDS) {                                           // (every wavefront has the same rows: each stores its share of the blocks)
             if (kk % NW == wave) {
-                asm volatile("ds_write_b128 %0, %1 offset:%3\n\tds_write_b128 %0, %2 offset:%4" ::"v"(q_addr), "v"(high), "v"(low), "n"(kk * 2048), "n"(kk * 2048 + 1024) : "memory");
+                asm volatile("ds_write_b128 %0, %1 offset:%3\n\tds_write_b128 %0, %2 offset:%4" ::"v"(q_addr), "v"(op[0]), "v"(op[1]), "n"(kk * 2048), "n"(kk * 2048 + 1024) : "memory");
             }
         } else {
-            q_op[kk][0] = high;
-            q_op[kk][1] = low;
+            q_op[kk][0] = op[0];
+            q_op[kk][1] = op[1];
         }
     }
     if constexpr (Cfg::Q_LDS) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (no wait for the loads in flight)
@@ -443,7 +473,7 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = h * 4 + j;
-                    s[key] = fma_half(d[h][j], ksc[st][key >> 3][(key & 7) >> 1], key & 1, st ? s[key] : 0.f);
+                    s[key] = fma_half(d[h][j], ksc[st][key >> 3][(key & 7) >> 1], key & 1, st ? s[key] : zero);
                 }
         }
         if (more) {
@@ -458,8 +488,9 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
             }
         }
         if (a.soft_cap > 0.f) {
+            stay_branch();
 #pragma unroll
-            for (int j = 0; j < KG; ++j) s[j] = a.soft_cap * tanhf(s[j] * row_scale / a.soft_cap) * LOG2E;
+            for (int j = 0; j < KG; ++j) s[j] = capped(s[j], row_scale * inv_cap, a.soft_cap);
         }
         // -- which keys this row sees; whole tiles that every row sees need no mask
         bool whole = row0 + TK <= a.T;
@@ -467,15 +498,18 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
             const int first = row0 < wrap ? base + row0 : base + row0 - a.ring;
             whole = whole && !(row0 < wrap && row0 + TK > wrap) && first >= full_lo && first + TK <= full_hi;
         }
-        unsigned seen = 0xFFFFu;
         if (!whole) {
-            seen = 0u;
+            stay_branch();                                                    // a key that is not seen: no score, and a scale of zero (what is there may be anything)
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
                 const int p = row0 + g * KG + j, key = p < wrap ? base + p : base + p - a.ring;
                 const bool ok = p < a.T && key >= lo && key < hi;
-                seen |= ok ? 1u << j : 0u;
                 s[j] = ok ? s[j] : -INFINITY;
+#pragma unroll
+                for (int st = 0; st < SETS; ++st) {
+                    const unsigned w = vsc[st][j >> 3][(j & 7) >> 1];
+                    vsc[st][j >> 3][(j & 7) >> 1] = ok ? w : w & (j & 1 ? 0xFFFFu : 0xFFFF0000u);
+                }
             }
         }
         float mx = s[0];
@@ -488,22 +522,9 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         float p[16], sum = 0.f;
 #pragma unroll
         for (int j = 0; j < KG; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], to_log2, -ref));
-        if (!whole) {
-#pragma unroll
-            for (int j = 0; j < KG; ++j) p[j] = seen >> j & 1 ? p[j] : 0.f;
-        }
         m_run = m_new;
         // -- the largest P' of the column, and the shift that keeps it in range
-        if (!whole) {                                                         // (the scale of a key that is not seen may be anything)
-#pragma unroll
-            for (int st = 0; st < SETS; ++st)
-#pragma unroll
-                for (int j = 0; j < KG; ++j) {
-                    const unsigned w = vsc[st][j >> 3][(j & 7) >> 1];
-                    vsc[st][j >> 3][(j & 7) >> 1] = seen >> j & 1 ? w : w & (j & 1 ? 0xFFFFu : 0xFFFF0000u);
-                }
-        }
-        auto times_scale = [&](int st, int j) __attribute__((always_inline)) { return fma_half(p[j], vsc[st][j >> 3][(j & 7) >> 1], j & 1, 0.f); };
+        auto times_scale = [&](int st, int j) __attribute__((always_inline)) { return fma_half(p[j], vsc[st][j >> 3][(j & 7) >> 1], j & 1, zero); };
         float pv[Cfg::PV_TWICE ? 1 : SETS][KG], top = 0.f;
 #pragma unroll
         for (int st = 0; st < SETS; ++st)
@@ -767,12 +788,413 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
     return launch_decode<DT, D, 1>(ctx, a);
 }
 
+// --------------------------------------------------------------------------------------------------------------------- many query rows
+// A workgroup has ROWS query rows, 32 to a wavefront (16 at head size 256), and walks its keys a tile at a time. What bounds it is the arithmetic, so the
+// conversions are made once for all of its rows: eight wavefronts turn a tile's codes into operands in LDS while they multiply the tile before it
+// (two stages, one barrier a tile).
+//   K: the codes as f16, exact, [block][lane group][row of a sub-tile] of 16 bytes: an operand is one read, and its scale goes onto the product (a block long).
+//     The query row is the sum of two f16, as in quant_decode_kernel.
+//   V: here the scale can go onto the value, which many rows share: code * scale (19 bits) as the sum of two bf16 (whose exponents hold any of them),
+//     P as well, and of the four products the smallest is left out, 2^-18. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
+// A scale that is not finite would reach rows that do not see its key (0 * NaN): such a value is taken as zero and the rows that do see it get their NaN by hand.
+template <int DT, int D>
+struct PromptCfg {
+    static constexpr int WAVES = 8, TK = D > 128 ? 32 : 64, CT = D > 128 ? 1 : 2, ROWS = WAVES * 16 * CT;
+    static constexpr int RB = DT == AIONHIP_Q8_0 ? D : D / 2;
+    static constexpr int K_BYTES = TK * D * 2, V_BYTES = TK * D * 2, S_BYTES = D / 32 * TK * 2;       // V_BYTES: of either part
+    static constexpr int STAGE = K_BYTES + 2 * V_BYTES + S_BYTES;
+    static constexpr int LDS_BYTES = 2 * STAGE + WAVES * 512 + 64;
+};
+typedef __attribute__((ext_vector_type(2))) int v2i;
+typedef __attribute__((address_space(3))) v2i lds_v2i;
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split sp) {
+    using Cfg = PromptCfg<DT, D>;
+    constexpr int WAVES = Cfg::WAVES, TK = Cfg::TK, CT = Cfg::CT, RB = Cfg::RB, CH = RB / 16, KK = D / 32, MT = D / 16;
+    constexpr int H = TK / 16, KG = TK / 4, STEPS = KG / 8;                  // sub-tiles; keys of a lane; products they make
+    constexpr int K_ALL = TK * RB / 512, KI = (K_ALL + WAVES - 1) / WAVES;   // loads of a tile, 512 bytes each: of K, and of V
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    // longest first: the last rows of all units, then those before them
+    const int units = a.B * a.Hkv, group_tiles = (sp.row_tiles * 16 + Cfg::ROWS - 1) / Cfg::ROWS;
+    const int per_place = units * sp.nseg, place = group_tiles - 1 - (int)(blockIdx.x / per_place), rest = (int)(blockIdx.x % per_place);
+    const int unit = rest / sp.nseg, seg = rest - unit * sp.nseg, b = unit / a.Hkv, hk = unit - b * a.Hkv;
+    const int rows_total = a.L * a.groups, row_first = place * Cfg::ROWS + wave * 16 * CT;
+
+    // ---- query rows (past the last one: that one again)
+    int lo[CT], hi[CT];
+    int uni_lo = INT_MAX, uni_hi = 0, full_lo = 0, full_hi = INT_MAX;        // of the wavefront's rows
+    size_t qbase[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int r = min(row_first + ct * 16 + n, rows_total - 1), li = r / a.groups;
+        qbase[ct] = (((size_t)b * a.L + li) * a.Hq + hk * a.groups + (r - li * a.groups)) * D;
+        visible(a, b, li, lo[ct], hi[ct]);
+        if (hi[ct] <= lo[ct]) lo[ct] = hi[ct] = 0;
+        uni_lo = min(uni_lo, rows16_min_i(hi[ct] > lo[ct] ? lo[ct] : INT_MAX));
+        uni_hi = max(uni_hi, rows16_max_i(hi[ct]));
+        full_lo = max(full_lo, rows16_max_i(lo[ct]));
+        full_hi = min(full_hi, rows16_min_i(hi[ct]));
+    }
+    // ---- the workgroup's keys
+    int *meet_lds = (int *)(lds + 2 * Cfg::STAGE + WAVES * 512);
+    if (threadIdx.x == 0) {
+        meet_lds[0] = INT_MAX;
+        meet_lds[1] = 0;
+        meet_lds[2] = meet_lds[3] = 0;                                       // one more than the last tile with a value whose scale is not finite, by stages
+    }
+    __syncthreads();
+    if (lane == 0) {
+        atomicMin(&meet_lds[0], uni_lo);
+        atomicMax(&meet_lds[1], uni_hi);
+    }
+    __syncthreads();
+    const int wg_lo = __builtin_amdgcn_readfirstlane(meet_lds[0]), wg_hi = __builtin_amdgcn_readfirstlane(meet_lds[1]);
+    const int kv_end = clip_kv_end(a.ring, a.T, a.kv_lengths ? a.kv_lengths[b] : a.T);
+    const int wrap = a.ring ? kv_end % a.ring : INT_MAX, base = a.ring ? kv_end - wrap : 0;      // (rings by their rows: see quant_decode_kernel)
+    int first_tile = 0, count = 0;
+    const int all_tiles = (a.T + TK - 1) / TK;
+    if (wg_hi > wg_lo) {
+        const int p0 = phys_key(a.ring, wg_lo);
+        first_tile = p0 / TK;
+        const long span = (long)(p0 % TK) + (wg_hi - wg_lo);
+        count = (int)min((long)all_tiles, (span + TK - 1) / TK + (a.ring && (long)p0 + (wg_hi - wg_lo) > a.ring ? 1 : 0));
+    }
+    const int per = (count + sp.nseg - 1) / sp.nseg, t0 = seg * per, t_end = min((seg + 1) * per, count);
+    auto row0_of = [&](int i) { const int x = first_tile + i; return (x >= all_tiles ? x - all_tiles : x) * TK; };
+
+    const size_t unit_rows = (size_t)unit * a.Tp;
+    const unsigned char *kc = a.k.codes + unit_rows * RB, *vc = a.v.codes + unit_rows * RB;
+    const __half *ks = a.k.scales + unit_rows * KK, *vs = a.v.scales + unit_rows * KK;
+
+    const float zero = opaque_zero();
+    // ---- a tile on its way: 512 bytes to an instruction, K in order, V as eight keys x 16 bytes to sixteen lanes
+    u32x2 kraw[KI], vraw[KI];
+    u32x4 vscale[KI], kscale{};
+    auto v_octet = [&](int j) { return ((j * WAVES + wave) * 4 + g) / CH; };
+    auto v_chunk = [&](int j) { return ((j * WAVES + wave) * 4 + g) % CH; };
+    auto request = [&](int i) __attribute__((always_inline)) {
+        const int row0 = row0_of(i);
+#pragma unroll
+        for (int j = 0; j < KI; ++j)
+            if (K_ALL % WAVES == 0 || j * WAVES + wave < K_ALL) {
+                kraw[j] = *(const u32x2 *)(kc + (size_t)row0 * RB + (j * WAVES + wave) * 512 + lane * 8);
+                const int key = row0 + v_octet(j) * 8;
+                vraw[j] = *(const u32x2 *)(vc + (size_t)(key + (n >> 1)) * RB + v_chunk(j) * 16 + (n & 1) * 8);
+                vscale[j] = *(const u32x4 *)(vs + (size_t)(DT == AIONHIP_Q8_0 ? v_chunk(j) / 2 : v_chunk(j)) * a.Tp + key);
+            }
+        if (threadIdx.x < KK * TK / 8) kscale = *(const u32x4 *)(ks + (size_t)(threadIdx.x / (TK / 8)) * a.Tp + row0 + (int)(threadIdx.x % (TK / 8)) * 8);
+    };
+    auto convert = [&](int i, int stage) __attribute__((always_inline)) {
+        unsigned char *k_op = lds + stage * Cfg::STAGE, *v_op = k_op + Cfg::K_BYTES, *s_op = v_op + 2 * Cfg::V_BYTES, *swap = lds + 2 * Cfg::STAGE + wave * 512;
+        if (threadIdx.x < KK * TK / 8) *(u32x4 *)(s_op + threadIdx.x * 16) = kscale;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < KI; ++j)
+            if (K_ALL % WAVES == 0 || j * WAVES + wave < K_ALL) {
+                const int off = (j * WAVES + wave) * 512 + lane * 8, key = off / RB, piece = off % RB / 8;
+                const int pos = key % KG / 4 * 16 + key / KG * 4 + key % 4;
+                if constexpr (DT == AIONHIP_Q8_0) {
+                    *(u32x4 *)(k_op + (piece * TK + pos) * 16) = halves_q8(kraw[j].x, kraw[j].y);
+                } else {
+                    *(u32x4 *)(k_op + (piece * 2 * TK + pos) * 16) = halves_q4(kraw[j].x);
+                    *(u32x4 *)(k_op + ((piece * 2 + 1) * TK + pos) * 16) = halves_q4(kraw[j].y);
+                }
+                *(u32x2 *)(swap + lane * 8) = vraw[j];
+                v2i w{};
+#if defined(__HIP_DEVICE_COMPILE__)   // the builtin exists in the device pass only
+                w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(lds_void *)(swap + lane * 8));
+#endif
+                u32x4 sc = vscale[j];
+                bool bad = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bad |= (sc[k] & 0x7C00u) == 0x7C00u || (sc[k] & 0x7C000000u) == 0x7C000000u;
+                if (__any(bad)) {
+                    odd = true;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if ((sc[k] & 0x7C00u) == 0x7C00u) sc[k] &= 0xFFFF0000u;
+                        if ((sc[k] & 0x7C000000u) == 0x7C000000u) sc[k] &= 0xFFFFu;
+                    }
+                }
+                // x: pairs of codes of the keys ka, kb; stored at column `col` of the octet
+                auto store = [&](const u32x4 &x, int col) __attribute__((always_inline)) {
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const unsigned word = x[k >> 1];
+                        const h2 pair = __builtin_bit_cast(h2, word);
+                        const int key = key_slot<DT>(k);
+                        v[key] = fma_half(k & 1 ? (float)pair.y : (float)pair.x, sc[key >> 1], key & 1, zero);
+                    }
+                    u32x4 high, low;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        high[k] = pack2<AIONHIP_BF16>(v[2 * k], v[2 * k + 1]);
+                        low[k] = pack2<AIONHIP_BF16>(v[2 * k] - __uint_as_float(high[k] << 16), v[2 * k + 1] - __uint_as_float(high[k] & 0xFFFF0000u));
+                    }
+                    unsigned char *o = v_op + (v_octet(j) * D + col) * 16;
+                    *(u32x4 *)o = high;
+                    *(u32x4 *)(o + Cfg::V_BYTES) = low;
+                };
+                if constexpr (DT == AIONHIP_Q8_0) {
+                    store(halves_q8((unsigned)w.x, (unsigned)w.y), v_chunk(j) * 16 + n);
+                } else {
+                    const u32x4 x = halves_q4((unsigned)w.x), y = halves_q4((unsigned)w.y);
+                    store(u32x4{x.x, x.z, y.x, y.z}, v_chunk(j) * 32 + n);
+                    store(u32x4{x.y, x.w, y.y, y.w}, v_chunk(j) * 32 + 16 + n);
+                }
+            }
+        if (odd && lane == 0) meet_lds[2 + stage] = i + 1;
+    };
+
+    if (t0 < t_end) request(t0);
+    // ---- Q^T, two parts of eight elements of each block
+    const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
+    u32x4 q_op[CT][KK][2];
+    float row_scale[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        float x[KK][8], amax = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            if (a.q_dtype == AIONHIP_F32) {
+                __builtin_memcpy(x[kk], (const float *)a.q + qbase[ct] + kk * 32 + g * 8, 32);
+            } else {
+                unsigned short y[8];
+                __builtin_memcpy(y, (const unsigned short *)a.q + qbase[ct] + kk * 32 + g * 8, 16);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(y[j])) : bf16_bits_to_f32(y[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[kk][j]));
+        }
+        const Power2 by(groups4_max(amax));
+        row_scale[ct] = fabsf(a.scale) * by.grow;
+        const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) split_query<DT>(x[kk], sign, q_op[ct][kk]);
+    }
+
+    f32x4 acc[CT][MT];
+    float m_ref[CT], l_run[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        m_ref[ct] = REF_NONE;
+        l_run[ct] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[ct][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    if (t0 < t_end) {
+        convert(t0, 0);
+        if (t0 + 1 < t_end) request(t0 + 1);
+    }
+    __syncthreads();
+    for (int i = t0; i < t_end; ++i) {
+        const int stage = (i - t0) & 1, row0 = row0_of(i);
+        if (i + 1 < t_end) {
+            convert(i + 1, stage ^ 1);
+            if (i + 2 < t_end) request(i + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned char *k_op = lds + stage * Cfg::STAGE, *v_op = k_op + Cfg::K_BYTES, *s_op = v_op + 2 * Cfg::V_BYTES;
+        // keys of the tile: `first` the first row's, one after the other but where a ring begins again
+        const int first = row0 < wrap ? base + row0 : base + row0 - a.ring;
+        const bool plain = row0 + TK <= a.T && !(row0 < wrap && row0 + TK > wrap);
+        if (!plain || (first < uni_hi && first + TK > uni_lo)) {
+            float s[CT][KG];
+#pragma unroll
+            for (int o = 0; o < H / 2; ++o)                                   // two sub-tiles: four products (two) on their way
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    u32x4 k8[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) k8[h] = *(const u32x4 *)(k_op + ((kk * 4 + g) * TK + (o * 2 + h) * 16 + n) * 16);
+                    const u32x4 sc = *(const u32x4 *)(s_op + (kk * TK + g * KG + o * 8) * 2);
+                    f32x4 d[CT][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ++ct) d[ct][h] = mfma16<AIONHIP_F16>(k8[h], q_op[ct][kk][0], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ++ct) d[ct][h] = mfma16<AIONHIP_F16>(k8[h], q_op[ct][kk][1], d[ct][h]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) s[ct][o * 8 + j] = fma_half(d[ct][j >> 2][j & 3], sc[j >> 1], j & 1, kk ? s[ct][o * 8 + j] : zero);
+                }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)                                   // (or the products of the second column group would wait, unscaled, behind the first's softmax)
+#pragma unroll
+                for (int j = 0; j < KG; ++j) asm volatile("" : "+v"(s[ct][j]));
+            __builtin_amdgcn_sched_barrier(0);
+            const bool whole = plain && first >= full_lo && first + TK <= full_hi;
+            u32x4 ph[CT][STEPS], pl[CT][STEPS];
+            auto sees = [&](int ct, int p) __attribute__((always_inline)) {
+                const int key = p < wrap ? base + p : base + p - a.ring;
+                return p < a.T && key >= lo[ct] && key < hi[ct];
+            };
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                float to_log2 = fmaxf(row_scale[ct] * LOG2E, 1e-30f);
+                if (a.soft_cap > 0.f) {
+                    stay_branch();
+                    to_log2 = 1.f;
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) s[ct][j] = capped(s[ct][j], row_scale[ct] * inv_cap, a.soft_cap);
+                }
+                if (!whole) {
+                    int p0 = row0 + g * KG;
+                    asm volatile("" : "+v"(p0));                              // (made anew for each column group, not kept)
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) s[ct][j] = sees(ct, p0 + j) ? s[ct][j] : -INFINITY;
+                }
+                float mx = s[ct][0];
+#pragma unroll
+                for (int j = 1; j < KG; ++j) mx = fmaxf(mx, s[ct][j]);
+                mx = groups4_max(mx) * to_log2;
+                // the reference follows the maximum only where that has grown by 2^8: an exponential of up to 2^8 is as exact as one of up to one
+                if (__any(mx > m_ref[ct] + 8.f)) {
+                    stay_branch();
+                    const float m_new = mx > m_ref[ct] + 8.f ? mx : m_ref[ct];
+                    const float alpha = __builtin_amdgcn_exp2f(m_ref[ct] - m_new);
+                    m_ref[ct] = m_new;
+                    l_run[ct] *= alpha;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) acc[ct][mt] *= alpha;
+                }
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < KG; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[ct][j], to_log2, -m_ref[ct]));
+                    s[ct][j] = p;
+                    sum += p;
+                }
+                l_run[ct] += sum;
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = s[ct][step * 8 + 2 * k], y = s[ct][step * 8 + 2 * k + 1];
+                        const unsigned high = pack2<AIONHIP_BF16>(x, y);
+                        ph[ct][step][k] = high;
+                        pl[ct][step][k] = pack2<AIONHIP_BF16>(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xFFFF0000u));
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step) {
+                    const unsigned char *o = v_op + ((g * STEPS + step) * D + mt * 16 + n) * 16;
+                    const u32x4 vh = *(const u32x4 *)o, vl = *(const u32x4 *)(o + Cfg::V_BYTES);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vh, ph[ct][step], acc[ct][mt]);
+                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vh, pl[ct][step], acc[ct][mt]);
+                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vl, ph[ct][step], acc[ct][mt]);
+                    }
+                    if (mt % 2 == 1 && step == STEPS - 1) __builtin_amdgcn_sched_barrier(0);
+                }
+            if (meet_lds[2 + stage] == i + 1) {
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        float gone = 0.f;
+#pragma unroll 1
+                        for (int j = 0; j < KG; ++j) {
+                            const float v = __half2float(vs[(size_t)kk * a.Tp + row0 + g * KG + j]);
+                            if (sees(ct, row0 + g * KG + j) && !(fabsf(v) < INFINITY)) gone = 1.f;
+                        }
+                        if (groups4_max(gone) > 0.f) acc[ct][2 * kk] = acc[ct][2 * kk + 1] = f32x4{NAN, NAN, NAN, NAN};
+                    }
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const float l = groups4_sum(l_run[ct]);
+        const int r = row_first + ct * 16 + n;
+        if (r >= rows_total) continue;
+        float *o;
+        float inv = 1.f;
+        if (sp.nseg == 1) {
+            const int li = r / a.groups;
+            o = a.out + (((size_t)b * a.L + li) * a.Hq + hk * a.groups + (r - li * a.groups)) * D;
+            inv = l != 0.f ? 1.f / l : 0.f;
+        } else {
+            float *part = sp.parts + (((size_t)unit * sp.row_tiles + r / 16) * sp.nseg + seg) * Part<D, 1>::FLOATS;
+            o = part + n * D;
+            if (g == 0) {
+                part[16 * D + 2 * n] = m_ref[ct];
+                part[16 * D + 2 * n + 1] = l;
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const f32x4 x = acc[ct][2 * kk] * inv, y = acc[ct][2 * kk + 1] * inv;
+            f32x4 first4, second4;
+            int at, next;
+            if constexpr (DT == AIONHIP_Q8_0) {
+                first4 = x, second4 = y, at = kk * 32 + g * 4, next = 16;
+            } else {
+                first4 = f32x4{x.x, y.x, x.y, y.y}, second4 = f32x4{x.z, y.z, x.w, y.w}, at = kk * 32 + g * 8, next = 4;
+            }
+            __builtin_memcpy(o + at, &first4, 16);
+            __builtin_memcpy(o + at + next, &second4, 16);
+        }
+    }
+}
+
+template <int DT, int D>
+int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
+    using Cfg = PromptCfg<DT, D>;
+    const int cus = ctx->cu_count > 0 ? ctx->cu_count : 256;
+    const long rows = (long)a.L * a.groups, units = (long)a.B * a.Hkv, wgs = units * ((rows + Cfg::ROWS - 1) / Cfg::ROWS);
+    Split sp{};
+    sp.row_tiles = (int)((rows + 15) / 16);
+    long keys = a.T;
+    if (a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + Cfg::TK);
+    const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
+    sp.nseg = (int)max(1L, min(min((long)cus / wgs, 16L), key_tiles / 4));
+    if (wgs * sp.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
+    if (sp.nseg > 1) {
+        if (const int rc = ensure_scratch2(ctx, (size_t)units * sp.row_tiles * sp.nseg * Part<D, 1>::FLOATS * sizeof(float))) return rc;
+        sp.parts = (float *)ctx->scratch2;
+    }
+    static std::atomic<uint64_t> attr{0};
+    if (const int rc = allow_lds(ctx, attr, (const void *)quant_prompt_kernel<DT, D>, Cfg::LDS_BYTES)) return rc;
+    {
+        ProfScope scope(ctx, "attn_quant_prompt");
+        launch_k(ctx, quant_prompt_kernel<DT, D>, dim3((unsigned)(wgs * sp.nseg)), dim3(Cfg::WAVES * 64), Cfg::LDS_BYTES, a, sp);
+    }
+    if (sp.nseg > 1) {
+        ProfScope scope(ctx, "attn_quant_merge");
+        launch_k(ctx, quant_merge_kernel<D, 1>, dim3((unsigned)(sp.row_tiles * MERGE_SHARES), (unsigned)units), dim3(NW * 64), 0, a, sp);
+    }
+    LAUNCH_CHECK(ctx, "attn_quant_prompt");
+    return AIONHIP_OK;
+}
+
+template <int DT, int D>
+int launch_rows(aionhip_ctx *ctx, const QuantArgs &a) {
+    if ((long)a.L * a.groups > 64) return launch_prompt<DT, D>(ctx, a);
+    return launch_decode_rows<DT, D>(ctx, a);
+}
+
 template <int DT>
 int launch(aionhip_ctx *ctx, const QuantArgs &a) {
     if (a.d_k == a.d_v) {
-        if (a.d_k == 64) return launch_decode_rows<DT, 64>(ctx, a);
-        if (a.d_k == 128) return launch_decode_rows<DT, 128>(ctx, a);
-        if (a.d_k == 256) return launch_decode_rows<DT, 256>(ctx, a);
+        if (a.d_k == 64) return launch_rows<DT, 64>(ctx, a);
+        if (a.d_k == 128) return launch_rows<DT, 128>(ctx, a);
+        if (a.d_k == 256) return launch_rows<DT, 256>(ctx, a);
     }
     return launch_generic<DT>(ctx, a);
 }
