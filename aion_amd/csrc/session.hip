@@ -5,7 +5,7 @@
 // The list is checked as a whole before its first launch (tags, dtypes, shapes), the way the reference validates a program
 // before it executes it (runtime/executable.zig:413-470 validate): a list with a step this device does not run fails with
 // nothing done.
-#include "common.h"
+#include "cache_quant.h"
 
 #include <cmath>
 #include <cstring>
@@ -27,9 +27,11 @@ size_t elems(const aionhip_tensor_ref &t) {
     for (uint32_t d = 0; d < t.rank; ++d) n *= (size_t)t.shape[d];
     return n;
 }
-// bytes of a tensor as aion stores it: 34 / 18 bytes per 32 elements for the block formats (backend/types.zig:41-59)
+bool is_quant_cache(const aionhip_tensor_ref &t) { return (t.flags & AIONHIP_TENSOR_QUANT_CACHE) && t.rank == 4 && cq::is_quant(t.dtype); }
+// bytes of a tensor as aion stores it: 34 / 18 bytes per 32 elements for the block formats (backend/types.zig:41-59), and of a quantized cache
 size_t bytes_of(const aionhip_tensor_ref &t) {
     const size_t n = elems(t);
+    if (is_quant_cache(t)) return aionhip_cache_quant_bytes(t.dtype, t.shape[0], t.shape[1], t.shape[2], t.shape[3]);
     switch (t.dtype) {
     case AIONHIP_F32: case AIONHIP_I32: return n * 4;
     case AIONHIP_F16: case AIONHIP_BF16: return n * 2;
@@ -254,8 +256,11 @@ int aionhip_session::check(size_t i, const aionhip_step &st) {
             return bad("Attention: out is [B, L, Hq, Dv]");
         if (st.in[3].handle && (!is_i32(st.in[3]) || elems(st.in[3]) != q.shape[0] * q.shape[1])) return bad("Attention: query_positions i32 [B, L]");
         if (st.in[4].handle && (!is_i32(st.in[4]) || elems(st.in[4]) != q.shape[0])) return bad("Attention: kv_lengths i32 [B]");
-        for (const aionhip_tensor_ref *t : {&q, &k})
-            if (t->dtype != AIONHIP_F32 && t->dtype != AIONHIP_F16 && t->dtype != AIONHIP_BF16) return unsupported("Attention: f32, f16 or bf16 operands");
+        for (const aionhip_tensor_ref *t : {&q, &k}) {
+            if (t == &k && is_quant_cache(k) && is_quant_cache(v)) continue;
+            if (t->dtype != AIONHIP_F32 && t->dtype != AIONHIP_F16 && t->dtype != AIONHIP_BF16) return unsupported("Attention: f32, f16 or bf16 operands, or quantized caches");
+        }
+        if (is_quant_cache(k) && (k.shape[3] % 32 != 0 || v.shape[3] % 32 != 0)) return bad("Attention: head sizes over quantized caches are multiples of 32");
         if (k.shape[2] == 0 || q.shape[2] % k.shape[2] != 0) return bad("Attention: query heads are a multiple of the kv heads");
         return AIONHIP_OK;
     }
@@ -294,8 +299,13 @@ int aionhip_session::check(size_t i, const aionhip_step &st) {
     case AIONHIP_STEP_SEQUENCE_APPEND: {
         const aionhip_tensor_ref &cache = st.out, &nk = st.in[0], &end = st.in[1];
         if (!cache.handle || !nk.handle || cache.rank != 4 || nk.rank != 4) return bad("SequenceAppend: rank-4 cache and rows");
-        if (cache.dtype != nk.dtype) return bad("SequenceAppend: cache and rows of one type");
-        if (cache.dtype != AIONHIP_F16 && cache.dtype != AIONHIP_F32) return unsupported("SequenceAppend: an f16 or f32 cache");
+        if (is_quant_cache(cache)) {
+            if (nk.dtype != AIONHIP_F32 && nk.dtype != AIONHIP_F16 && nk.dtype != AIONHIP_BF16) return unsupported("SequenceAppend: f32, f16 or bf16 rows into a quantized cache");
+            if (cache.shape[3] % 32 != 0) return bad("SequenceAppend: the head size of a quantized cache is a multiple of 32");
+        } else {
+            if (cache.dtype != nk.dtype) return bad("SequenceAppend: cache and rows of one type");
+            if (cache.dtype != AIONHIP_F16 && cache.dtype != AIONHIP_F32) return unsupported("SequenceAppend: an f16 or f32 cache, or a quantized one");
+        }
         if (cache.shape[0] != nk.shape[0] || cache.shape[2] != nk.shape[2] || cache.shape[3] != nk.shape[3]) return bad("SequenceAppend: rows are [B, S, H, D] of the cache's B, H, D");
         if (!is_i32(end) || elems(end) != cache.shape[0]) return bad("SequenceAppend: end_index i32 [B]");
         return AIONHIP_OK;
@@ -386,8 +396,12 @@ int aionhip_session::run_one(size_t i, const aionhip_step &st) {
     }
     case AIONHIP_STEP_SEQUENCE_APPEND: {
         const aionhip_tensor_ref &cache = st.out, &nk = st.in[0];
-        rc = aionhip_step_sequence_append(ctx, cache.dtype, cache.handle, nk.handle, st.in[1].handle, cache.shape[0], nk.shape[1], cache.shape[1],
-                                          cache.shape[2] * cache.shape[3], (cache.flags & AIONHIP_TENSOR_ROLLING) ? 1 : 0);
+        if (is_quant_cache(cache))
+            rc = aionhip_step_append_quant(ctx, cache.dtype, cache.handle, nk.handle, 0, 0, nk.dtype, st.in[1].handle, cache.shape[0], nk.shape[1], cache.shape[1],
+                                           cache.shape[2], cache.shape[3], (cache.flags & AIONHIP_TENSOR_ROLLING) ? 1 : 0);
+        else
+            rc = aionhip_step_sequence_append(ctx, cache.dtype, cache.handle, nk.handle, st.in[1].handle, cache.shape[0], nk.shape[1], cache.shape[1],
+                                              cache.shape[2] * cache.shape[3], (cache.flags & AIONHIP_TENSOR_ROLLING) ? 1 : 0);
         break;
     }
     case AIONHIP_STEP_CAST:
@@ -560,6 +574,36 @@ size_t aionhip_session::try_fused(const aionhip_step *steps, size_t count, size_
                                                         xq.shape[2], xk.shape[2], d, t.rope[0]->rope_base, t.rope[0]->rope_scale,
                                                         t.rope[0]->rope_proportion);
                 if (rc != AIONHIP_UNSUPPORTED) { *rc_out = wrap(i, st, rc); ++calls_last_execute; return 6; }
+            }
+        }
+    }
+    // The cache side over quantized caches, linear or rings: RoPE1D on q and k -> SequenceAppend of k and of v, four steps from the first of the ropes on
+    if ((fusion & AIONHIP_FUSE_WORKSPACE) && st.tag == AIONHIP_STEP_ROPE1D && i + 3 < count) {
+        const aionhip_step *rope[2] = {nullptr, nullptr}, *app[2] = {nullptr, nullptr};                    // q's, k's; k's, v's
+        int n_rope = 0, n_app = 0;
+        for (size_t j = i; j < i + 4; ++j) {
+            if (steps[j].tag == AIONHIP_STEP_ROPE1D && n_rope < 2) rope[n_rope++] = &steps[j];
+            else if (steps[j].tag == AIONHIP_STEP_SEQUENCE_APPEND && n_app < 2 && is_quant_cache(steps[j].out)) app[n_app++] = &steps[j];
+        }
+        if (n_rope == 2 && n_app == 2) {
+            if (!same_tensor(app[0]->in[0], rope[0]->out) && !same_tensor(app[0]->in[0], rope[1]->out)) std::swap(app[0], app[1]);
+            if (!same_tensor(app[0]->in[0], rope[1]->out)) std::swap(rope[0], rope[1]);
+            const aionhip_tensor_ref &xq = rope[0]->in[0], &xk = rope[1]->in[0], &xv = app[1]->in[0], &qo = rope[0]->out, &ko = rope[1]->out, &kc = app[0]->out, &vc = app[1]->out;
+            const aionhip_tensor_ref &pos = rope[0]->in[1], &end = app[0]->in[1];
+            const size_t d = xq.shape[3];
+            bool ok = same_tensor(app[0]->in[0], ko) && app[0] > rope[1] && is_f32(xv) && pos.handle == rope[1]->in[1].handle && end.handle == app[1]->in[1].handle &&
+                      rope[0]->rope_base == rope[1]->rope_base && rope[0]->rope_scale == rope[1]->rope_scale && rope[0]->rope_proportion == rope[1]->rope_proportion &&
+                      xk.shape[3] == d && xv.shape[3] == d && kc.shape[3] == d && vc.shape[3] == d && xk.shape[0] == xq.shape[0] && xv.shape[0] == xq.shape[0] &&
+                      kc.shape[0] == xq.shape[0] && vc.shape[0] == xq.shape[0] && xk.shape[1] == xq.shape[1] && xv.shape[1] == xq.shape[1] && xv.shape[2] == xk.shape[2] &&
+                      kc.shape[2] == xk.shape[2] && vc.shape[2] == xk.shape[2] && kc.shape[1] == vc.shape[1] && kc.dtype == vc.dtype &&
+                      ((kc.flags ^ vc.flags) & AIONHIP_TENSOR_ROLLING) == 0 && clear_of(ko, {&xq, &xv, &pos, &end}) && !range_of(kc).overlaps(range_of(vc));
+            for (const aionhip_tensor_ref *o : {&qo, &kc, &vc}) ok = ok && clear_of(*o, {&xq, &xk, &xv, &pos, &end, &ko});
+            ok = ok && !range_of(qo).overlaps(range_of(kc)) && !range_of(qo).overlaps(range_of(vc)) && dead_after(ko, i + 3);
+            if (ok) {
+                const int rc = aionhip_step_rope_append_quant(ctx, kc.dtype, qo.handle, xq.handle, xk.handle, xv.handle, kc.handle, vc.handle, pos.handle, end.handle,
+                                                              xq.shape[0], xq.shape[1], kc.shape[1], xq.shape[2], xk.shape[2], d, rope[0]->rope_base, rope[0]->rope_scale,
+                                                              rope[0]->rope_proportion, (kc.flags & AIONHIP_TENSOR_ROLLING) ? 1 : 0);
+                if (rc != AIONHIP_UNSUPPORTED) { *rc_out = wrap(i, st, rc); ++calls_last_execute; return 4; }
             }
         }
     }

@@ -4,7 +4,8 @@ The step sequence is the one aion's graph compiler emits for a decoder (pattern 
 src/bench/models.zig:433-536, trimmed to a plain pre-norm block): Gather -> per layer
 [RMSNorm -> MatMul q,k,v -> RoPE1D(q,k) -> Cast f16 + SequenceAppend(k,v) -> Attention ->
 MatMul o -> add -> RMSNorm -> MatMul gate,up -> gate(gelu) -> MatMul down -> add] ->
-RMSNorm -> MatMul lm_head -> ArgMax. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
+RMSNorm -> MatMul lm_head -> ArgMax. With `cache_dtype` Q8_0 or Q4_0 the keys and values are quantised as they are appended
+(SequenceAppend takes the f32 rows, no Cast) and attention reads the codes. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
 only q4 layout aion has), q8_0 weights are [N,K] quant_axis 1 MatMulNT operands.
 
 Prefill runs the steps eagerly; the single-token decode step is recorded once into a program
@@ -36,6 +37,7 @@ class DecoderConfig:
     eps: float = 1e-6
     rope_base: float = 10000.0
     wdtype: int = be.Q4_0
+    cache_dtype: int = be.F16        # F16, or Q8_0 / Q4_0: keys and values held in 8 or 4 bits (head_dim a multiple of 32)
 
     @property
     def q_dim(self):
@@ -44,6 +46,18 @@ class DecoderConfig:
     @property
     def kv_dim(self):
         return self.kv_heads * self.head_dim
+
+    @property
+    def quant_cache(self):
+        return self.cache_dtype in be.BLOCK_BYTES
+
+    def cache_bytes(self, gpu):
+        """Bytes of one layer's cache of keys (or values)."""
+        if self.quant_cache:
+            return gpu.cache_quant_bytes(self.cache_dtype, 1, self.max_seq, self.kv_heads, self.head_dim)
+        if self.cache_dtype != be.F16:
+            raise ValueError("cache_dtype: F16, Q8_0 or Q4_0")
+        return self.max_seq * self.kv_dim * 2
 
 
 def weight_shapes(cfg):
@@ -118,7 +132,7 @@ class Decoder:
                 on_weight("l%d.norm1" % l, ones)
                 on_weight("l%d.norm2" % l, ones)
             on_weight("norm_f", ones)
-        kv_bytes = cfg.max_seq * cfg.kv_dim * 2
+        kv_bytes = cfg.cache_bytes(gpu)
         self.kc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.vc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.one = gpu.upload(np.ones(1, np.int32))
@@ -128,7 +142,7 @@ class Decoder:
         self.state = {}        # S -> activation buffers
         self.program = None
         self.pos = 0
-        if one_launch:
+        if one_launch and not cfg.quant_cache:               # (the one-launch form reads f16 caches)
             layers = [{"wq": self.w["l%d.wq" % l], "wk": self.w["l%d.wk" % l], "wv": self.w["l%d.wv" % l], "wo": self.w["l%d.wo" % l],
                        "w_gate": self.w["l%d.wgate" % l], "w_up": self.w["l%d.wup" % l], "w_down": self.w["l%d.wdown" % l],
                        "norm1_gamma": self.gamma, "norm2_gamma": self.gamma, "k_cache": self.kc[l], "v_cache": self.vc[l]}
@@ -163,7 +177,13 @@ class Decoder:
         scale = 1.0 / math.sqrt(c.head_dim)
         for l in range(c.layers if not (s == 1 and self.stack is not None) else 0):
             p = "l%d." % l
-            if s == 1 and c.hidden <= 8192 and c.head_dim % 8 == 0:
+            if c.quant_cache:
+                # RMSNorm -> MatMul q, k, v (one call), RoPE1D(q), RoPE1D(k) -> quantized append of k and v (one launch)
+                g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s,
+                                      [b["q"], b["k"], b["v"]], c.eps)
+                g.step_rope_append_quant(c.cache_dtype, b["qr"], b["q"], b["k"], b["v"], self.kc[l], self.vc[l], b["positions"], b["write_index"],
+                                         1, s, c.max_seq, c.heads, c.kv_heads, c.head_dim, base=c.rope_base)
+            elif s == 1 and c.hidden <= 8192 and c.head_dim % 8 == 0:
                 # one new token: RMSNorm -> MatMul q, k, v -> RoPE1D(q), RoPE1D(k) -> f16 -> append, one launch
                 g.step_rmsnorm_qkv_rope_append(self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"], b["x"], self.gamma, c.eps,
                                                b["qr"], self.kc[l], self.vc[l], b["positions"], b["write_index"],
@@ -181,8 +201,8 @@ class Decoder:
             # attention, then MatMul o with beta = 1: x = x + att @ Wo (the residual add rides on the matmul's beta); a prompt's attention leaves
             # its rows as the exact GEMM reads them
             shape = (1, s, c.max_seq, c.heads, c.kv_heads, c.head_dim, c.head_dim)
-            options = {"q_dtype": be.F32, "kv_dtype": be.F16, "window": be.CAUSAL, "query_positions": b["positions"], "kv_lengths": b["kv_len"]}
-            if s == 1 or not g.step_attention_matmul(self.w[p + "wo"], b["qr"], self.kc[l], self.vc[l], shape, scale, b["x"], beta=1.0, **options):
+            options = {"q_dtype": be.F32, "kv_dtype": c.cache_dtype, "window": be.CAUSAL, "query_positions": b["positions"], "kv_lengths": b["kv_len"]}
+            if s == 1 or c.quant_cache or not g.step_attention_matmul(self.w[p + "wo"], b["qr"], self.kc[l], self.vc[l], shape, scale, b["x"], beta=1.0, **options):
                 g.step_attention(b["att"], b["qr"], self.kc[l], self.vc[l], shape, scale, **options)
                 g.step_matmul(self.w[p + "wo"], b["att"], s, b["x"], beta=1.0)
             if s == 1 and c.hidden <= 8192 and c.ffn % 32 == 0:
@@ -335,7 +355,7 @@ class SessionDecoder:
         self.w = {name: gpu.upload(weights.blocks(name)) for name in weight_shapes(cfg)}
         self.embed = gpu.upload(weights.embed())
         self.gamma = gpu.upload(np.ones(cfg.hidden, np.float32))
-        kv_bytes = cfg.max_seq * cfg.kv_dim * 2
+        kv_bytes = cfg.cache_bytes(gpu)
         self.kc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.vc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.one = gpu.upload(np.ones(1, np.int32))
@@ -372,20 +392,24 @@ class SessionDecoder:
         p.gather_rows(ss.tensor(self.embed, be.F32, (c.vocab, c.hidden)), ss.tensor(b["ids"], be.I32, (1, s)), x)
         for l in range(c.layers):
             n = "l%d." % l
-            kc = ss.tensor(self.kc[l], be.F16, (1, c.max_seq, c.kv_heads, c.head_dim))
-            vc = ss.tensor(self.vc[l], be.F16, (1, c.max_seq, c.kv_heads, c.head_dim))
+            kc = ss.tensor(self.kc[l], c.cache_dtype, (1, c.max_seq, c.kv_heads, c.head_dim), quant_cache=c.quant_cache)
+            vc = ss.tensor(self.vc[l], c.cache_dtype, (1, c.max_seq, c.kv_heads, c.head_dim), quant_cache=c.quant_cache)
             p.rmsnorm(x, gamma, None, work("h", 1, s, c.hidden), c.eps)
             mm(p, work("h", 1, s, c.hidden), self._weight(n + "wq"), work("q", 1, s, c.q_dim))
             mm(p, work("h", 1, s, c.hidden), self._weight(n + "wk"), work("k", 1, s, c.kv_dim))
             mm(p, work("h", 1, s, c.hidden), self._weight(n + "wv"), work("v", 1, s, c.kv_dim))
             p.rope1d(work("q", 1, s, c.heads, c.head_dim), pos, work("qr", 1, s, c.heads, c.head_dim), base_frequency=c.rope_base)
             p.rope1d(work("k", 1, s, c.kv_heads, c.head_dim), pos, work("kr", 1, s, c.kv_heads, c.head_dim), base_frequency=c.rope_base)
-            k16 = ss.tensor(b["k16"], be.F16, (1, s, c.kv_heads, c.head_dim), workspace=True)
-            v16 = ss.tensor(b["v16"], be.F16, (1, s, c.kv_heads, c.head_dim), workspace=True)
-            p.cast(work("kr", 1, s, c.kv_heads, c.head_dim), k16)
-            p.sequence_append(kc, k16, widx)
-            p.cast(work("v", 1, s, c.kv_heads, c.head_dim), v16)
-            p.sequence_append(vc, v16, widx)
+            if c.quant_cache:
+                p.sequence_append(kc, work("kr", 1, s, c.kv_heads, c.head_dim), widx)
+                p.sequence_append(vc, work("v", 1, s, c.kv_heads, c.head_dim), widx)
+            else:
+                k16 = ss.tensor(b["k16"], be.F16, (1, s, c.kv_heads, c.head_dim), workspace=True)
+                v16 = ss.tensor(b["v16"], be.F16, (1, s, c.kv_heads, c.head_dim), workspace=True)
+                p.cast(work("kr", 1, s, c.kv_heads, c.head_dim), k16)
+                p.sequence_append(kc, k16, widx)
+                p.cast(work("v", 1, s, c.kv_heads, c.head_dim), v16)
+                p.sequence_append(vc, v16, widx)
             p.attention(work("qr", 1, s, c.heads, c.head_dim), kc, vc, work("att", 1, s, c.heads, c.head_dim), 1.0 / math.sqrt(c.head_dim),
                         query_positions=pos, kv_lengths=kvl)
             mm(p, work("att", 1, s, c.q_dim), self._weight(n + "wo"), work("o", 1, s, c.hidden))

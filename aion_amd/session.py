@@ -21,19 +21,19 @@ ROPE1D, SEQUENCE_APPEND, CAST, MATMUL_NT, TRANSFER = 21, 22, 31, 32, 33
 ADD, SUB, MUL, DIV, GATE = 0, 1, 2, 3, 10
 RELU, GELU, SILU, SIGMOID, TANH, SQRT, LOG = range(7)
 IDENTICAL, SCALAR_A, SCALAR_B, SUFFIX_A, SUFFIX_B, GENERIC = range(6)
-ROLLING, WORKSPACE = 1, 2
+ROLLING, WORKSPACE, QUANT_CACHE = 1, 2, 4
 FUSE_SIBLINGS, FUSE_WORKSPACE = 1, 2
 
 
-def tensor(buf, dtype, shape, rolling=False, workspace=False, offset=0):
-    """A TensorRef for the device buffer `buf` (None: the step has no such operand)."""
+def tensor(buf, dtype, shape, rolling=False, workspace=False, offset=0, quant_cache=False):
+    """A TensorRef for the device buffer `buf` (None: the step has no such operand). quant_cache: a cache held in 8 or 4 bits (`HipBackend.cache_quant_bytes`)."""
     t = TensorRef()
     if buf is None:
         return t
     t.handle = buf.handle + offset
     t.dtype = dtype
     t.rank = len(shape)
-    t.flags = (ROLLING if rolling else 0) | (WORKSPACE if workspace else 0)
+    t.flags = (ROLLING if rolling else 0) | (WORKSPACE if workspace else 0) | (QUANT_CACHE if quant_cache else 0)
     for i, d in enumerate(shape):
         t.shape[i] = d
     return t

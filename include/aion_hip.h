@@ -480,6 +480,7 @@ void aionhip_program_destroy(aionhip_ctx *ctx, aionhip_program *prog);
  * (backend/backend.zig:85-107). */
 #define AIONHIP_MAX_RANK 8
 enum { AIONHIP_TENSOR_ROLLING = 1u,    /* a rolling sequence cache (storage/cache.zig:35-38) */
+       AIONHIP_TENSOR_QUANT_CACHE = 4u, /* [B,T,H,D] of a block type: a cache as aionhip_cache_quant_bytes lays it out, T its capacity */
        AIONHIP_TENSOR_WORKSPACE = 2u   /* lives in a planned workspace slot (graph/program/workspace.zig:1-60): nothing reads
                                           its value after the last step of this list that does */ };
 typedef struct aionhip_tensor_ref {
@@ -509,7 +510,7 @@ enum { AIONHIP_BINARY_GATE = 10 };     /* ElemwiseBinaryOp.gate (backend/types.z
  *   GatherRows           out; table, indices
  *   Gather               out; data, indices                  axis, batch_dims
  *   RoPE1D               out; x, positions                   rope_base, rope_scale, rope_proportion
- *   SequenceAppend       out = cache; new_kv, end_index
+ *   SequenceAppend       out = cache; new_kv, end_index      (a quantized cache takes f32, f16 or bf16 rows, any other rows of its type)
  *   Cast                 out; x                              (the target type is out.dtype)
  *   Transfer             to_host = 1: in[0] = the device tensor, host receives; 0: out = the device tensor, host is read */
 typedef struct aionhip_step {
@@ -545,7 +546,7 @@ int aionhip_session_create(aionhip_ctx *ctx, aionhip_session **out);
  * gate(gelu) -> down MatMul (five steps, aionhip_step_rmsnorm_geglu_matmul); and for any batch and token count the cache
  * side of a block that normalizes its heads: RMSNorm over the head size on q, k, v -> RoPE1D on q and k -> Cast +
  * SequenceAppend of k and of v (nine steps, aionhip_step_headnorm_rope_append), and the same without the norms over linear
- * caches (six steps, aionhip_step_rope_append). A MatMul (beta 0) whose workspace output is
+ * caches (six steps, aionhip_step_rope_append); the latter over quantized caches, which take the rows uncast (four steps, aionhip_step_rope_append_quant). A MatMul (beta 0) whose workspace output is
  * read only by an add right behind it that accumulates in place (x = x + t) writes x itself with beta 1, alone or as the
  * last step of the patterns above: alpha * acc + x is rounded once either way. A pattern whose entry point answers
  * AIONHIP_UNSUPPORTED for the shape runs as the next smaller pattern or as separate steps. aion folds at step level the same
