@@ -329,7 +329,8 @@ int aionhip_step_append_f16(aionhip_ctx *ctx, aionhip_handle cache, aionhip_hand
                             size_t b, size_t s, size_t t_cap, size_t row_elems, int rolling);
 int aionhip_step_cast_f32_f16(aionhip_ctx *ctx, aionhip_handle out_f16, aionhip_handle x_f32, size_t n);
 /* Caches held in 8 or 4 bits (dtype AIONHIP_Q8_0 or AIONHIP_Q4_0), for sequences whose keys and values would not fit, or whose reading bounds a decode
- * step: 34 or 18 bytes to 32 elements instead of 64. aion quantizes weights only; the arithmetic of a block is that of aionhip_quantize_blocks.
+ * step: 34 or 18 bytes to 32 elements instead of 64. aion quantizes weights only; a block's codes are made as aionhip_quantize_blocks makes them,
+ * by a scale of max|x| * (1 / 127) or max|x| * (1 / 7) with the factor rounded to f32.
  * A cache for b sequences of up to t_cap rows of h heads of d elements (d a multiple of 32) is ONE buffer of aionhip_cache_quant_bytes bytes (0: arguments out of
  * range) that begins at a multiple of 16 bytes: codes [B,H,Tp,D * bits / 8] first, Tp = t_cap rounded up to 64, then one f16 scale to every 32 elements,
  * [B,H,D / 32,Tp]. A code is stored with 128 (q8_0) or 8 (q4_0, the even element in the low half of a byte) added, an element is code * scale. Rows

@@ -11,6 +11,25 @@ def padded(t_cap):
     return -(-t_cap // 64) * 64
 
 
+def quantize(dtype, rows):
+    """f32 rows [..., D] -> codes [..., D * bits / 8] as they are stored, scale bits [..., D / 32]. f32 arithmetic, every operation rounded on its own."""
+    f32 = np.float32
+    x = rows.reshape(rows.shape[:-1] + (-1, 32))
+    top = np.abs(x).max(-1, keepdims=True)
+    with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
+        full = np.where(top == 0, f32(1), top * (f32(1) / f32(127 if dtype == be.Q8_0 else 7)))
+        held = full.astype(np.float16).astype(f32)
+        if dtype == be.Q8_0:
+            v = x * np.where((top == 0) | (held == 0), f32(0), f32(1) / held)
+        else:
+            v = x / full
+    v = np.clip(np.copysign(np.floor(np.abs(v).astype(np.float64) + 0.5), v), -OFFSET[dtype], OFFSET[dtype] - 1)      # halves away from zero
+    code = (v + OFFSET[dtype]).astype(np.uint8).reshape(rows.shape)
+    if dtype == be.Q4_0:
+        code = code[..., 0::2] | code[..., 1::2] << 4
+    return code, full.astype(np.float16).view(np.uint16)[..., 0]
+
+
 class QuantCache:
     """Host form of one cache: codes [B, H, Tp, D * bits / 8] and scales [B, H, D / 32, Tp] (f16 bits), views of one byte buffer."""
 
@@ -25,15 +44,9 @@ class QuantCache:
         self.codes = self.bytes[:n_codes].reshape(self.b, self.h, self.tp, -1)
         self.scales = self.bytes[n_codes:].view(np.uint16).reshape(self.b, self.h, self.d // 32, self.tp)
 
-    def put(self, orc, rows, b, row_index):
-        """rows [S, H, D] f32 into rows row_index[i] of sequence b, by the block quantizers of the oracle; a negative index: not written."""
-        s = rows.shape[0]
-        blocks = orc.quantize(self.dtype, np.ascontiguousarray(rows, np.float32).reshape(-1, 32), 1).reshape(s, self.h, self.d // 32, -1)
-        scale = np.ascontiguousarray(blocks[..., :2]).view(np.uint16)[..., 0]
-        code = blocks[..., 2:]
-        if self.dtype == be.Q8_0:
-            code = (code.astype(np.int16) ^ 0x80).astype(np.uint8)               # two's complement -> offset 128
-        code = code.reshape(s, self.h, -1)
+    def put(self, rows, b, row_index):
+        """rows [S, H, D] f32, quantised, into rows row_index[i] of sequence b; a negative index: not written."""
+        code, scale = quantize(self.dtype, np.ascontiguousarray(rows, np.float32))
         for i, r in enumerate(row_index):
             if r >= 0:
                 self.codes[b, :, r] = code[i]
@@ -50,13 +63,13 @@ class QuantCache:
         return x.reshape(self.b, self.h, self.tp, self.d).transpose(0, 2, 1, 3)
 
 
-def filled(orc, rng, dtype, b, t_cap, h, d, sigma=1.0, fill=0xFF, rows=None):
+def filled(rng, dtype, b, t_cap, h, d, sigma=1.0, fill=0xFF, rows=None):
     """A cache whose first `rows` rows (all) hold random numbers; what is behind them is `fill` (0xFF: scales that are NaN)."""
     c = QuantCache(dtype, b, t_cap, h, d, fill)
     n = t_cap if rows is None else rows
     spread = np.exp(0.4 * rng.standard_normal((h, d)))
     for i in range(b):
-        c.put(orc, (rng.standard_normal((n, h, d)) * spread * sigma).astype(np.float32), i, range(n))
+        c.put((rng.standard_normal((n, h, d)) * spread * sigma).astype(np.float32), i, range(n))
     return c
 
 

@@ -66,10 +66,10 @@ def check(gpu, q, kc, vc, t_cap, scale, q_dtype=be.F32, **options):
     return got
 
 
-def case(orc, seed, dtype, bn, l, t_cap, hq, hk, d, dv=None, sigma=1.0, rows=None):
+def case(seed, dtype, bn, l, t_cap, hq, hk, d, dv=None, sigma=1.0, rows=None):
     rng = np.random.default_rng(seed)
     q = rng.standard_normal((bn, l, hq, d)).astype(np.float32)
-    return q, filled(orc, rng, dtype, bn, t_cap, hk, d, sigma, rows=rows), filled(orc, rng, dtype, bn, t_cap, hk, dv or d, 1.0, rows=rows)
+    return q, filled(rng, dtype, bn, t_cap, hk, d, sigma, rows=rows), filled(rng, dtype, bn, t_cap, hk, dv or d, 1.0, rows=rows)
 
 
 BOTH = pytest.mark.parametrize("dtype", [be.Q8_0, be.Q4_0])
@@ -79,19 +79,19 @@ HEADS = [(8, 1, 256), (32, 8, 128), (16, 4, 64), (4, 4, 128), (3, 1, 64), (10, 1
 @BOTH
 @pytest.mark.parametrize("hq,hk,d", HEADS)
 @pytest.mark.parametrize("t", [1, 31, 64, 65, 500])
-def test_one_token(gpu, orc, dtype, hq, hk, d, t):
-    q, kc, vc = case(orc, t + d, dtype, 1, 1, t, hq, hk, d)
+def test_one_token(gpu, dtype, hq, hk, d, t):
+    q, kc, vc = case(t + d, dtype, 1, 1, t, hq, hk, d)
     check(gpu, q, kc, vc, t, 1 / math.sqrt(d), positions=[[t - 1]], kv_lengths=[t])
 
 
 @BOTH
 @pytest.mark.parametrize("q_dtype", [be.F32, be.F16, be.BF16])
 @pytest.mark.parametrize("hq,hk,d", [(8, 1, 256), (32, 8, 128), (16, 4, 64)])
-def test_ragged_batch_with_an_idle_sequence(gpu, orc, dtype, q_dtype, hq, hk, d):
+def test_ragged_batch_with_an_idle_sequence(gpu, dtype, q_dtype, hq, hk, d):
     """Lengths from none to past the capacity (clipped to it); rows behind a sequence's end hold NaN scales."""
     t_cap = 333
     lengths = [333, 0, 1, 64, 200, 5000]
-    q, kc, vc = case(orc, d, dtype, len(lengths), 1, t_cap, hq, hk, d)
+    q, kc, vc = case(d, dtype, len(lengths), 1, t_cap, hq, hk, d)
     for c in (kc, vc):
         for i, n in enumerate(lengths):
             c.scales[i, :, :, n:] = 0x7E00
@@ -102,8 +102,8 @@ def test_ragged_batch_with_an_idle_sequence(gpu, orc, dtype, q_dtype, hq, hk, d)
 @BOTH
 @pytest.mark.parametrize("hq,hk,d", [(8, 2, 256), (32, 8, 128), (6, 2, 64)])
 @pytest.mark.parametrize("l,t", [(2, 70), (5, 301), (9, 64), (17, 400), (40, 130), (130, 130), (200, 777)])
-def test_several_queries(gpu, orc, dtype, hq, hk, d, l, t):
-    q, kc, vc = case(orc, l + t + d, dtype, 2, l, t, hq, hk, d)
+def test_several_queries(gpu, dtype, hq, hk, d, l, t):
+    q, kc, vc = case(l + t + d, dtype, 2, l, t, hq, hk, d)
     pos = np.stack([np.arange(t - l, t), np.arange(0, l)])
     check(gpu, q, kc, vc, t, 1 / math.sqrt(d), positions=pos, kv_lengths=[t, l])
 
@@ -111,17 +111,17 @@ def test_several_queries(gpu, orc, dtype, hq, hk, d, l, t):
 @BOTH
 @pytest.mark.parametrize("l,t", [(1, 600), (7, 600), (150, 600)])
 @pytest.mark.parametrize("window", [be.FULL, (63, 0, 0), (0, 0, 0), (100, 20, 0), (be.UNBOUNDED, 5, 0), (0, 0, 64), (64, 0, 50)])
-def test_windows(gpu, orc, dtype, l, t, window):
-    q, kc, vc = case(orc, l, dtype, 2, l, t, 8, 2, 128)
+def test_windows(gpu, dtype, l, t, window):
+    q, kc, vc = case(l, dtype, 2, l, t, 8, 2, 128)
     pos = np.stack([np.arange(t - l, t), np.arange(100, 100 + l)])
     check(gpu, q, kc, vc, t, 0.1, window=window, positions=pos, kv_lengths=[t, t - 37])
 
 
 @BOTH
 @pytest.mark.parametrize("l", [1, 6, 140])
-def test_rows_that_see_nothing_beside_rows_that_do(gpu, orc, dtype, l):
+def test_rows_that_see_nothing_beside_rows_that_do(gpu, dtype, l):
     """Positions far behind a short sequence and a small window: an empty interval gives zeros, also beside rows of the same tile."""
-    q, kc, vc = case(orc, l, dtype, 2, l, 200, 8, 2, 64)
+    q, kc, vc = case(l, dtype, 2, l, 200, 8, 2, 64)
     pos = np.stack([np.where(np.arange(l) % 2 == 0, 150, 500), np.full(l, 90)])
     got = check(gpu, q, kc, vc, 200, 0.125, window=(40, 0, 0), positions=pos, kv_lengths=[200, 30])
     assert not got[1].any() and (l == 1 or not got[0, 1].any()) and got[0, 0].any()
@@ -130,9 +130,9 @@ def test_rows_that_see_nothing_beside_rows_that_do(gpu, orc, dtype, l):
 @BOTH
 @pytest.mark.parametrize("hq,hk,d", [(8, 1, 256), (16, 4, 64), (32, 8, 128)])
 @pytest.mark.parametrize("t_cap,window", [(1, be.CAUSAL), (63, be.CAUSAL), (64, (30, 0, 0)), (150, be.CAUSAL), (150, (99, 0, 0)), (700, (511, 0, 0)), (700, be.CAUSAL)])
-def test_rings(gpu, orc, dtype, hq, hk, d, t_cap, window):
+def test_rings(gpu, dtype, hq, hk, d, t_cap, window):
     lengths = [t_cap // 2 + 1, t_cap, t_cap + 1, 3 * t_cap + 7, 1000 * t_cap + t_cap // 3, 0]
-    q, kc, vc = case(orc, d + t_cap, dtype, len(lengths), 1, t_cap, hq, hk, d)
+    q, kc, vc = case(d + t_cap, dtype, len(lengths), 1, t_cap, hq, hk, d)
     for c in (kc, vc):
         c.scales[0, :, :, lengths[0]:] = 0x7E00
     check(gpu, q, kc, vc, t_cap, 1 / math.sqrt(d), window=window, positions=[[max(n - 1, 0)] for n in lengths], kv_lengths=lengths, rolling=True)
@@ -140,9 +140,9 @@ def test_rings(gpu, orc, dtype, hq, hk, d, t_cap, window):
 
 @BOTH
 @pytest.mark.parametrize("l", [4, 150])
-def test_rings_and_several_queries(gpu, orc, dtype, l):
+def test_rings_and_several_queries(gpu, dtype, l):
     t_cap = 260
-    q, kc, vc = case(orc, l, dtype, 2, l, t_cap, 8, 2, 128)
+    q, kc, vc = case(l, dtype, 2, l, t_cap, 8, 2, 128)
     lengths = [1000, l + 10]
     pos = np.stack([np.arange(n - l, n) for n in lengths])
     check(gpu, q, kc, vc, t_cap, 0.1, window=(99, 0, 0), positions=pos, kv_lengths=lengths, rolling=True)
@@ -151,23 +151,23 @@ def test_rings_and_several_queries(gpu, orc, dtype, l):
 @BOTH
 @pytest.mark.parametrize("l", [1, 5, 140])
 @pytest.mark.parametrize("soft_cap,scale", [(30.0, 0.2), (5.0, 1.0), (0.0, -0.1), (0.0, 0.0)])
-def test_soft_cap_and_odd_scales(gpu, orc, dtype, l, soft_cap, scale):
-    q, kc, vc = case(orc, l, dtype, 1, l, 300, 8, 2, 64)
+def test_soft_cap_and_odd_scales(gpu, dtype, l, soft_cap, scale):
+    q, kc, vc = case(l, dtype, 1, l, 300, 8, 2, 64)
     check(gpu, q, kc, vc, 300, scale, soft_cap=soft_cap, positions=[np.arange(300 - l, 300)], kv_lengths=[300])
 
 
 @BOTH
 @pytest.mark.parametrize("l", [1, 140])
 @pytest.mark.parametrize("hq,hk,d,dv", [(4, 2, 32, 32), (2, 1, 96, 160), (2, 2, 64, 128), (1, 1, 512, 32)])
-def test_other_head_sizes(gpu, orc, dtype, l, hq, hk, d, dv):
-    q, kc, vc = case(orc, d, dtype, 2, l, 150, hq, hk, d, dv)
+def test_other_head_sizes(gpu, dtype, l, hq, hk, d, dv):
+    q, kc, vc = case(d, dtype, 2, l, 150, hq, hk, d, dv)
     check(gpu, q, kc, vc, 150, 1 / math.sqrt(d), positions=[np.arange(150 - l, 150)] * 2, kv_lengths=[150, 149])
 
 
 @BOTH
 @pytest.mark.parametrize("l", [1, 150])
-def test_no_index_operands(gpu, orc, dtype, l):
-    q, kc, vc = case(orc, l, dtype, 2, l, 200, 8, 2, 128)
+def test_no_index_operands(gpu, dtype, l):
+    q, kc, vc = case(l, dtype, 2, l, 200, 8, 2, 128)
     check(gpu, q, kc, vc, 200, 0.1)
     check(gpu, q, kc, vc, 200, 0.1, window=be.FULL)
 
@@ -175,35 +175,35 @@ def test_no_index_operands(gpu, orc, dtype, l):
 @BOTH
 @pytest.mark.parametrize("l", [1, 150])
 @pytest.mark.parametrize("q_size,k_size,v_size", [(1e4, 1e-4, 1.0), (1e-6, 1e4, 1e-4), (1.0, 1.0, 3e4), (300.0, 1.0, 1.0), (1e30, 1e-4, 1.0)])
-def test_magnitudes(gpu, orc, dtype, l, q_size, k_size, v_size):
+def test_magnitudes(gpu, dtype, l, q_size, k_size, v_size):
     """Queries, keys and values far from one: nothing may leave a half-precision range on the way, and small scales keep their relative accuracy."""
     rng = np.random.default_rng(4)
-    q, kc, vc = case(orc, l, dtype, 1, l, 300, 8, 2, 64)
+    q, kc, vc = case(l, dtype, 1, l, 300, 8, 2, 64)
     for c, size in ((kc, k_size), (vc, v_size)):
         x = rng.standard_normal((300, 2, 64)).astype(np.float32) * np.float32(size)
-        c.put(orc, x, 0, range(300))
+        c.put(x, 0, range(300))
     scale = 0.125 if q_size == 300.0 else 0.3 / (q_size * k_size)
     check(gpu, (q * np.float32(q_size)).astype(np.float32), kc, vc, 300, scale, positions=[np.arange(300 - l, 300)], kv_lengths=[300])
 
 
 @BOTH
 @pytest.mark.parametrize("l", [1, 6])
-def test_values_of_very_different_size_along_the_cache(gpu, orc, dtype, l):
+def test_values_of_very_different_size_along_the_cache(gpu, dtype, l):
     """The scales of the values rise and fall by 2^15 along the cache: the sums follow."""
     rng = np.random.default_rng(6)
-    q, kc, vc = case(orc, l, dtype, 1, l, 1500, 8, 2, 128)
+    q, kc, vc = case(l, dtype, 1, l, 1500, 8, 2, 128)
     size = np.exp2(rng.integers(-10, 6, 1500)).astype(np.float32)
     size[:64], size[700:800] = 2.0 ** -12, 2.0 ** 12
-    vc.put(orc, rng.standard_normal((1500, 2, 128)).astype(np.float32) * size[:, None, None], 0, range(1500))
+    vc.put(rng.standard_normal((1500, 2, 128)).astype(np.float32) * size[:, None, None], 0, range(1500))
     check(gpu, q, kc, vc, 1500, 0.1, positions=[np.arange(1500 - l, 1500)], kv_lengths=[1500])
 
 
 @BOTH
 @pytest.mark.parametrize("l", [1, 5, 150])
-def test_what_is_not_finite_stays_where_it_is_seen(gpu, orc, dtype, l):
+def test_what_is_not_finite_stays_where_it_is_seen(gpu, dtype, l):
     """A NaN key or value is seen by the rows whose interval holds it, and by nobody else; of a value only its block's columns."""
     t = 260
-    q, kc, vc = case(orc, l, dtype, 1, l, t, 4, 2, 64)
+    q, kc, vc = case(l, dtype, 1, l, t, 4, 2, 64)
     pos = 100 + np.arange(l) % 30
     pos[-1] = 250
     check(gpu, q, kc, vc, t, 0.125, positions=[pos], kv_lengths=[t], window=(20, 0, 0))
@@ -223,8 +223,8 @@ def test_what_is_not_finite_stays_where_it_is_seen(gpu, orc, dtype, l):
 
 @BOTH
 @pytest.mark.parametrize("bn,l,hq,hk,d,t", [(1, 1, 8, 1, 256, 5000), (1, 1, 32, 8, 128, 4100), (3, 1, 16, 4, 64, 3000), (1, 40, 8, 2, 128, 4000), (1, 200, 8, 1, 256, 3000)])
-def test_long_caches_are_divided(gpu, orc, dtype, bn, l, hq, hk, d, t):
-    q, kc, vc = case(orc, t, dtype, bn, l, t, hq, hk, d)
+def test_long_caches_are_divided(gpu, dtype, bn, l, hq, hk, d, t):
+    q, kc, vc = case(t, dtype, bn, l, t, hq, hk, d)
     lengths = [t - 700 * i for i in range(bn)]
     check(gpu, q, kc, vc, t, 1 / math.sqrt(d), positions=[np.arange(n - l, n) for n in lengths], kv_lengths=lengths)
 
@@ -259,11 +259,11 @@ def test_refusals(gpu):
 
 
 @BOTH
-def test_a_decode_recorded_and_replayed(gpu, orc, dtype):
+def test_a_decode_recorded_and_replayed(gpu, dtype):
     """Append and attention of one token as a program: token by token, each replay against 64 bits, with eager work between the replays."""
     rng = np.random.default_rng(8)
     b, t_cap, hq, hk, d = 2, 200, 8, 2, 128
-    kc, vc = (filled(orc, rng, dtype, b, t_cap, hk, d, rows=100) for _ in range(2))
+    kc, vc = (filled(rng, dtype, b, t_cap, hk, d, rows=100) for _ in range(2))
     bufs = [gpu.upload(c.bytes) for c in (kc, vc)]
     rows = [gpu.alloc(b * hk * d * 4) for _ in range(2)]
     q, out = gpu.alloc(b * hq * d * 4), gpu.alloc(b * hq * d * 4)
@@ -282,7 +282,7 @@ def test_a_decode_recorded_and_replayed(gpu, orc, dtype):
             gpu.write(buf, x)
         for c, x in zip((kc, vc), new):
             for j in range(b):
-                c.put(orc, x[j], j, [at[j]])
+                c.put(x[j], j, [at[j]])
         if prog is None:
             issue()
             prog = gpu.record_program(issue)

@@ -1,4 +1,4 @@
-"""Rows into caches held in 8 or 4 bits and out again, against the oracle's block quantizers: the codes and scales bit for bit, the rows read back exactly
+"""Rows into caches held in 8 or 4 bits and out again, against the same arithmetic in numpy: the codes and scales bit for bit, the rows read back exactly
 (a code times a scale is exact in f32 and is rounded once)."""
 import numpy as np
 import pytest
@@ -42,7 +42,7 @@ def as_source(x, src):
     (3, 9, 50, 2, 128, [46, 1000003, -4], True, be.F32),       # rings: over the end, long after, before the beginning
     (2, 50, 50, 1, 64, [7, 2147483000], True, be.F16),         # the whole ring, and a step index near 2^31
 ])
-def test_append(gpu, orc, dtype, b, s, t_cap, h, d, starts, rolling, src):
+def test_append(gpu, dtype, b, s, t_cap, h, d, starts, rolling, src):
     rng = np.random.default_rng(b * 1000 + s * 10 + d)
     rows = [(rng.standard_normal((b, s, h, d)) * np.exp(rng.standard_normal((b, s, h, 1)))).astype(np.float32) for _ in range(2)]
     rows[0][0, 0, 0, :32] = 0.0
@@ -53,7 +53,7 @@ def test_append(gpu, orc, dtype, b, s, t_cap, h, d, starts, rolling, src):
         c = QuantCache(dtype, b, t_cap, h, d, FILL)
         bufs.append(put(gpu, c))
         for i in range(b):
-            c.put(orc, exact[i], i, indices(starts[i], s, t_cap, rolling))
+            c.put(exact[i], i, indices(starts[i], s, t_cap, rolling))
         want.append(c)
         srcs.append(gpu.upload(up))
     index = gpu.upload(np.array(starts, np.int32))
@@ -78,7 +78,7 @@ def test_append(gpu, orc, dtype, b, s, t_cap, h, d, starts, rolling, src):
 
 
 @pytest.mark.parametrize("offset", [1, 2, 3])
-def test_rows_at_any_aligned_address(gpu, orc, offset):
+def test_rows_at_any_aligned_address(gpu, offset):
     rng = np.random.default_rng(offset)
     x = rng.standard_normal((1, 3, 2, 64)).astype(np.float32)
     for src, up in ((be.F32, x), (be.F16, x.astype(np.float16))):
@@ -86,7 +86,7 @@ def test_rows_at_any_aligned_address(gpu, orc, offset):
         buf, cache, index, out = gpu.upload(flat), gpu.zeros(gpu.cache_quant_bytes(be.Q8_0, 1, 5, 2, 64)), gpu.upload(np.array([1], np.int32)), gpu.alloc(4 * (x.size + 4))
         gpu.step_append_quant(be.Q8_0, [cache], [buf.view(offset * up.itemsize)], index, (1, 3, 5, 2, 64), src_dtype=src)
         c = QuantCache(be.Q8_0, 1, 5, 2, 64)
-        c.put(orc, up.astype(np.float32)[0], 0, range(1, 4))
+        c.put(up.astype(np.float32)[0], 0, range(1, 4))
         assert np.array_equal(gpu.download(cache, np.uint8, c.bytes.shape), c.bytes)
         gpu.step_cache_read(be.Q8_0, [out.view(4 * offset)], [cache], index, (1, 3, 5, 2, 64))
         assert np.array_equal(gpu.download(out, np.float32, x.shape, offset=4 * offset)[0], c.values()[0, 1:4].astype(np.float32))
@@ -98,9 +98,9 @@ def test_rows_at_any_aligned_address(gpu, orc, offset):
 @pytest.mark.parametrize("out_dtype", [be.F32, be.F16, be.BF16])
 @pytest.mark.parametrize("b,s,t_cap,h,d,starts,rolling", [
     (1, 1, 1, 1, 32, [0], False), (2, 77, 130, 3, 64, [53, -9], False), (3, 64, 64, 2, 256, [0, 60, -64], False), (2, 33, 40, 4, 96, [77, -3], True)])
-def test_read(gpu, orc, dtype, out_dtype, b, s, t_cap, h, d, starts, rolling):
+def test_read(gpu, dtype, out_dtype, b, s, t_cap, h, d, starts, rolling):
     rng = np.random.default_rng(s + d)
-    c = filled(orc, rng, dtype, b, t_cap, h, d)
+    c = filled(rng, dtype, b, t_cap, h, d)
     buf, index = put(gpu, c), gpu.upload(np.array(starts, np.int32))
     size = 4 if out_dtype == be.F32 else 2
     guard = 64
@@ -124,7 +124,7 @@ def test_read(gpu, orc, dtype, out_dtype, b, s, t_cap, h, d, starts, rolling):
 
 
 @pytest.mark.parametrize("dtype", [be.Q8_0, be.Q4_0])
-def test_what_is_not_finite_stays_in_its_block(gpu, orc, dtype):
+def test_what_is_not_finite_stays_in_its_block(gpu, dtype):
     rng = np.random.default_rng(1)
     x = rng.standard_normal((1, 4, 2, 64)).astype(np.float32)
     x[0, 0, 0, 3], x[0, 1, 1, 40], x[0, 2, 0, 63] = np.nan, np.inf, -np.inf
@@ -137,7 +137,7 @@ def test_what_is_not_finite_stays_in_its_block(gpu, orc, dtype):
     gone[0, 0, 0, 0] = gone[0, 1, 1, 1] = gone[0, 2, 0, 1] = True
     assert np.isnan(got[gone]).all()
     c = QuantCache(dtype, 1, 4, 2, 64)
-    c.put(orc, np.where(np.isfinite(x), x, 0)[0], 0, range(4))
+    c.put(np.where(np.isfinite(x), x, 0)[0], 0, range(4))
     assert np.array_equal(got[~gone], c.values()[:, :4].reshape(got.shape)[~gone].astype(np.float32))
     for b in (src, index, cache, out):
         b.free()
@@ -171,10 +171,10 @@ def test_rope_append(gpu, dtype, b, s, t_cap, hq, hk, d, proportion, rolling):
 
 
 @pytest.mark.parametrize("dtype", [be.Q8_0, be.Q4_0])
-def test_growth_by_its_two_parts(gpu, orc, dtype):
+def test_growth_by_its_two_parts(gpu, dtype):
     rng = np.random.default_rng(5)
     b, h, d, old, new = 2, 3, 64, 70, 200
-    c = filled(orc, rng, dtype, b, old, h, d, fill=0)
+    c = filled(rng, dtype, b, old, h, d, fill=0)
     grown = QuantCache(dtype, b, new, h, d)
     grown.codes[:, :, :c.tp], grown.scales[..., :c.tp] = c.codes, c.scales
     src, dst = put(gpu, c), gpu.alloc(grown.bytes.size)
@@ -232,7 +232,7 @@ def test_refusals(gpu):
         buf.free()
 
 
-def test_recorded_append_follows_the_index(gpu, orc):
+def test_recorded_append_follows_the_index(gpu):
     """The write index is read on the device: a recorded append moves with it, replay by replay."""
     rng = np.random.default_rng(2)
     x = rng.standard_normal((1, 1, 2, 64)).astype(np.float32)
@@ -252,8 +252,8 @@ def test_recorded_append_follows_the_index(gpu, orc):
         gpu.write(index, np.array([3 * i], np.int32))
         gpu.program_execute(prog)
         if i == 0:
-            c.put(orc, x[0], 0, [0])
-        c.put(orc, y[0], 0, [3 * i])
+            c.put(x[0], 0, [0])
+        c.put(y[0], 0, [3 * i])
         assert np.array_equal(gpu.download(cache, np.uint8, c.bytes.shape), c.bytes)
         assert np.array_equal(gpu.download(out, np.float32, x.shape)[0, 0], c.values()[0, 3 * i].astype(np.float32))
     gpu.program_destroy(prog)

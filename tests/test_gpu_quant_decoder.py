@@ -120,7 +120,7 @@ SHAPE = dict(layers=2, hidden=256, heads=4, kv_heads=2, head_dim=64, ffn=512, vo
 
 
 @BOTH
-def test_decoders_over_quantized_caches(gpu, orc, dtype):
+def test_decoders_over_quantized_caches(gpu, dtype):
     """The hand-routed decoder and the session over the same step list: the same logits to the bit, prompt and replayed steps; the keys of the first block
     are what the separate steps quantise."""
     cfg = DecoderConfig(cache_dtype=dtype, **SHAPE)
@@ -145,7 +145,7 @@ def test_decoders_over_quantized_caches(gpu, orc, dtype):
         g.step_rmsnorm_matmul([a.w["l0.wk"]], x, a.gamma, n, [k], cfg.eps)
         g.step_rope(kr, k, pos, 1, n, cfg.kv_heads, cfg.head_dim, base=cfg.rope_base)
         want = QuantCache(dtype, 1, cfg.max_seq, cfg.kv_heads, cfg.head_dim)
-        want.put(orc, g.download(kr, np.float32, (n, cfg.kv_heads, cfg.head_dim)), 0, range(n))
+        want.put(g.download(kr, np.float32, (n, cfg.kv_heads, cfg.head_dim)), 0, range(n))
         out = g.alloc(n * cfg.kv_dim * 4)
         g.step_cache_read(dtype, [out], [a.kc[0]], zero, (1, n, cfg.max_seq, cfg.kv_heads, cfg.head_dim))
         assert np.array_equal(g.download(out, np.float32, (n, cfg.kv_heads, cfg.head_dim)), want.values()[0, :n].astype(np.float32))
