@@ -101,22 +101,40 @@ int launch_generic(aionhip_ctx *ctx, const QuantArgs &a) {
 // ---------------------------------------------------------------------------------------------------------------------- few query rows
 using h2 = __attribute__((ext_vector_type(2))) _Float16;
 
+// In registers where the compiler would use a constant: one operand of an instruction may be a scalar, so that a mask and an exponent merge into one
+// instruction only if one of them is a vector register; and a product by one or plus zero is replaced by more instructions than it was.
+struct Constants {
+    unsigned one = 0x64006400u;                      // two f16 1024
+    float zero = 0.f, minus = -1.f;
+    __device__ __forceinline__ Constants() { asm volatile("" : "+v"(one), "+v"(zero), "+v"(minus)); }
+};
 // Codes as the half-precision numbers they are, offset taken off: a code under the mantissa of 1024 is 1024 + code, and the rest is exact.
 // 4 bits: eight codes of a word, in the order 0 4 1 5 2 6 3 7 (a mask takes every fourth nibble of them).
-__device__ __forceinline__ u32x4 halves_q4(unsigned w) {
-    const unsigned m = 0x000F000Fu, one = 0x64006400u, v = w >> 8;
+__device__ __forceinline__ u32x4 halves_q4(const Constants &k, unsigned w) {
+    const unsigned m = 0x000F000Fu, v = w >> 8;
     const h2 low{(_Float16)-1032.f, (_Float16)-1032.f}, high{(_Float16)-72.f, (_Float16)-72.f}, by{(_Float16)0.0625f, (_Float16)0.0625f};
-    const h2 a = __builtin_bit_cast(h2, (w & m) | one) + low, b = __builtin_bit_cast(h2, (w & (m << 4)) | one) * by + high;
-    const h2 c = __builtin_bit_cast(h2, (v & m) | one) + low, d = __builtin_bit_cast(h2, (v & (m << 4)) | one) * by + high;
+    const h2 a = __builtin_bit_cast(h2, (w & m) | k.one) + low, b = __builtin_bit_cast(h2, (w & (m << 4)) | k.one) * by + high;
+    const h2 c = __builtin_bit_cast(h2, (v & m) | k.one) + low, d = __builtin_bit_cast(h2, (v & (m << 4)) | k.one) * by + high;
     return u32x4{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, c), __builtin_bit_cast(unsigned, d)};
 }
 // 8 bits: the eight codes of two words, in order
-__device__ __forceinline__ u32x4 halves_q8(unsigned w0, unsigned w1) {
+__device__ __forceinline__ u32x4 halves_q8(const Constants &k, unsigned w0, unsigned w1) {
     const h2 off{(_Float16)-1152.f, (_Float16)-1152.f};
     auto pair = [&](unsigned w, unsigned sel) {
-        return __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, sel)) + off);
+        return __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, __builtin_amdgcn_perm(k.one, w, sel)) + off);
     };
-    return u32x4{pair(w0, 0x04010400u), pair(w0, 0x04030402u), pair(w1, 0x04010400u), pair(w1, 0x04030402u)};
+    return u32x4{pair(w0, 0x07010700u), pair(w0, 0x07030702u), pair(w1, 0x07010700u), pair(w1, 0x07030702u)};
+}
+// The same for keys under few query rows: the codes as they are stored, under the mantissa of zero, are f16 numbers of 2^-24 a step, which the matrix pipe
+// multiplies exactly, subnormal or not. Two instructions less to a pair; the offset is taken back as -offset * sum(q), with which a product begins.
+// Nibbles 1 3 5 7 stand sixteen times higher, so their elements of the query are a sixteenth (split_query).
+__device__ __forceinline__ u32x4 raw_q4(unsigned w) {
+    const unsigned m = 0x000F000Fu, v = w >> 8;
+    return u32x4{w & m, w & (m << 4), v & m, v & (m << 4)};
+}
+__device__ __forceinline__ u32x4 raw_q8(unsigned w0, unsigned w1) {
+    return u32x4{__builtin_amdgcn_perm(0u, w0, 0x0C010C00u), __builtin_amdgcn_perm(0u, w0, 0x0C030C02u), __builtin_amdgcn_perm(0u, w1, 0x0C010C00u),
+                 __builtin_amdgcn_perm(0u, w1, 0x0C030C02u)};
 }
 // element of a block that lies in slot j of a query operand, and key of eight in slot j of a P operand: the order the codes come out of their words
 template <int DT>
@@ -141,34 +159,56 @@ __device__ __forceinline__ float fma_half(float x, unsigned pair, int k, float y
 }
 // In the body of a rare condition: or the compiler computes what it changes for every tile and selects, and has both forms in registers
 __device__ __forceinline__ void stay_branch() { asm volatile(""); }
-// A zero that the compiler does not know: fma_half with it stays one instruction (a product alone is a conversion and a multiplication)
-__device__ __forceinline__ float opaque_zero() {
-    float z = 0.f;
-    asm volatile("" : "+v"(z));
-    return z;
-}
 __device__ __forceinline__ unsigned pack_half(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 
-// A query row times a power of two that leaves its largest element in [1, 2): shrink = 2^-e, grow = 2^e, both normal floats. A row that holds no finite maximum stays as it is.
+// A query row times a power of two that leaves its largest element in [2^8, 2^9): shrink = 2^(8 - e), grow = 2^(e - 8), both normal floats. A row without a finite
+// maximum stays as it is.
 struct Power2 {
     float shrink, grow;
     __device__ __forceinline__ explicit Power2(float amax) {
-        const unsigned e = amax < INFINITY ? min(max(__float_as_uint(amax) >> 23, 2u), 252u) : 127u;
+        const unsigned e = amax < INFINITY ? min(max(__float_as_uint(amax) >> 23, 10u), 252u) - 8u : 127u;
         shrink = __uint_as_float((254u - e) << 23);
         grow = __uint_as_float(e << 23);
     }
 };
-// eight elements of a block times `by` as the sum of two f16 each, in the order of K's codes
-template <int DT>
-__device__ __forceinline__ void split_query(const float (&q)[8], float by, u32x4 (&op)[2]) {
-    float x[8], y[8];
+// eight elements of each block of a query row, from element `at` of the queries on (any alignment their type allows)
+template <int KK>
+__device__ __forceinline__ void load_query(const QuantArgs &a, size_t at, float (&x)[KK][8]) {
+    if (a.q_dtype == AIONHIP_F32) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) __builtin_memcpy(x[kk], (const float *)a.q + at + kk * 32, 32);
+        return;
+    }
+    unsigned short h[KK][8];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) __builtin_memcpy(h[kk], (const unsigned short *)a.q + at + kk * 32, 16);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(h[kk][j])) : bf16_bits_to_f32(h[kk][j]);
+}
+// Eight elements of a block times `by` as the sum of two f16 each, in the order of K's codes (RAW: for the codes of raw_q4 / raw_q8). Returns the sum of what the operands hold.
+template <int DT, bool RAW>
+__device__ __forceinline__ float split_query(const float (&q)[8], float by, u32x4 (&op)[2]) {
+    float x[8], y[8], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        x[j] = q[element_slot<DT>(j)] * by;
-        y[j] = x[j] - (float)(_Float16)x[j];
+        const bool high_nibble = RAW && DT == AIONHIP_Q4_0 && (j >> 1 & 1);
+        x[j] = q[element_slot<DT>(j)] * (high_nibble ? by * 0.0625f : by);
+        const float high = (float)(_Float16)x[j];
+        y[j] = x[j] - high;
+        sum += (high + (float)(_Float16)y[j]) * (high_nibble ? 16.f : 1.f);
     }
     op[0] = u32x4{pack2<AIONHIP_F16>(x[0], x[1]), pack2<AIONHIP_F16>(x[2], x[3]), pack2<AIONHIP_F16>(x[4], x[5]), pack2<AIONHIP_F16>(x[6], x[7])};
     op[1] = u32x4{pack2<AIONHIP_F16>(y[0], y[1]), pack2<AIONHIP_F16>(y[2], y[3]), pack2<AIONHIP_F16>(y[4], y[5]), pack2<AIONHIP_F16>(y[6], y[7])};
+    return sum;
+}
+// The largest of three (fmaxf multiplies what it cannot see the origin of by one first, to quiet a signalling NaN that none of these can be). Not for what the matrix
+// pipe wrote: the wait for its results is the compiler's, and it does not look in here.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 // cap * tanh(s * by) * log2(e), as 1 - 2 / (e^2x + 1): off by less than 2^-22 of the cap wherever s lies, without a branch
@@ -209,54 +249,72 @@ struct Split {
     int nseg, row_tiles;
 };
 constexpr int NW = 4;                       // wavefronts of a workgroup
-constexpr int MAX_SEG = 256;                // most segments of a row tile (the merge's table of factors)
+constexpr int MAX_SEG = 256;                // most segments of a row tile
 
 template <int D, int REP>
 struct Part {                               // a row tile's sums: o [rows][D], then (reference, sum) of its 16 columns
     static constexpr int ROWS = 16 / REP, FLOATS = ROWS * D + 32;
 };
 
-// Sums of all segments of a row tile -> output rows. The wavefronts derive the segments' factors, a lane to a segment, then every thread adds four
-// columns of a row over the segments in their order. `at(i, n)`: n (2 or 4) floats of the tile's parts from the i-th on.
+// Sums of a row tile's segments -> output rows. A thread has four columns of a row and every `groups`-th run of eight segments, all of a run's loads in
+// flight at once (reference, sum and columns: one memory round trip); the groups meet in LDS. The elements are [first, last) of rows x D / 4.
+// `load(2 or 4, i)`: that many floats of the tile's parts from the i-th on.
+constexpr int RUN = 8;
 template <int D, int REP, class Load, class Store>
-__device__ __forceinline__ void merge_parts(int nseg, int rows, int first, int step, float (*factor)[MAX_SEG], float *total, Load &&load, Store &&store) {
+__device__ __forceinline__ void merge_parts(int nseg, int first, int last, int groups, f32x4 *meet_o, float2 *meet_s, Load &&load, Store &&store) {
     constexpr int ROWS = Part<D, REP>::ROWS, FLOATS = Part<D, REP>::FLOATS;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int c = wave; c < 16; c += NW) {
-        float ref[MAX_SEG / 64], top = REF_NONE, sum = 0.f;
-        float l[MAX_SEG / 64];
-#pragma unroll
-        for (int j = 0; j < MAX_SEG / 64; ++j) {
-            const int s = lane + 64 * j;
-            const u32x2 x = s < nseg ? load(std::integral_constant<int, 2>{}, (size_t)s * FLOATS + ROWS * D + 2 * c) : u32x2{__float_as_uint(REF_NONE), 0u};
-            ref[j] = __uint_as_float(x.x);
-            l[j] = __uint_as_float(x.y);
-            top = fmaxf(top, ref[j]);
-        }
-        top = lanes_max(top);
-#pragma unroll
-        for (int j = 0; j < MAX_SEG / 64; ++j) {
-            const float f = exp2f(ref[j] - top);
-            if (lane + 64 * j < nseg) factor[c][lane + 64 * j] = f;
-            sum += l[j] * f;
-        }
-        sum = lanes_sum(sum);
-        if (lane == 0) total[c] = sum;
-    }
-    __syncthreads();
-    for (int e = first; e < rows * (D / 4); e += step) {
-        const int row = e / (D / 4), col = e % (D / 4) * 4, c = (col / 32) % REP * ROWS + row;
+    const int per = NW * 64 / groups, group = (int)threadIdx.x / per, runs = (nseg + RUN - 1) / RUN;
+    for (int e0 = first; e0 < last; e0 += per) {
+        const int e = min(e0 + (int)threadIdx.x % per, last - 1), row = e / (D / 4), col = e % (D / 4) * 4, c = (col / 32) % REP * ROWS + row;
+        const bool mine = group < groups && e0 + (int)threadIdx.x % per < last;
+        float ref = REF_NONE, l = 0.f;
         f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < nseg; s0 += 8) {
-            u32x4 x[8];
+        for (int run = group; run < runs && mine; run += groups) {
+            u32x2 st[RUN];
+            u32x4 x[RUN];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = load(std::integral_constant<int, 4>{}, (size_t)min(s0 + u, nseg - 1) * FLOATS + row * D + col);
+            for (int u = 0; u < RUN; ++u) {
+                const size_t part = (size_t)min(run * RUN + u, nseg - 1) * FLOATS;
+                st[u] = load(std::integral_constant<int, 2>{}, part + ROWS * D + 2 * c);
+                x[u] = load(std::integral_constant<int, 4>{}, part + row * D + col);
+            }
+            float top = ref;
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < nseg) o += __builtin_bit_cast(f32x4, x[u]) * factor[c][s0 + u];
+            for (int u = 0; u < RUN; ++u) top = fmaxf(top, __uint_as_float(st[u].x));
+            const float keep = __builtin_amdgcn_exp2f(ref - top);
+            o *= keep;
+            l *= keep;
+            ref = top;
+#pragma unroll
+            for (int u = 0; u < RUN; ++u)
+                if (run * RUN + u < nseg) {
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(st[u].x) - top);
+                    l += __uint_as_float(st[u].y) * f;
+                    o += __builtin_bit_cast(f32x4, x[u]) * f;
+                }
         }
-        const float l = total[c];
-        store(row, col, o * (l != 0.f ? 1.f / l : 0.f));
+        if (groups > 1) {
+            __syncthreads();                                                  // (what the threads met in before has been read)
+            if (group < groups) {
+                meet_o[threadIdx.x] = o;
+                meet_s[threadIdx.x] = make_float2(ref, l);
+            }
+            __syncthreads();
+            if (group == 0) {
+                float top = ref;
+                for (int k = 1; k < groups; ++k) top = fmaxf(top, meet_s[threadIdx.x + k * per].x);
+                const float keep = __builtin_amdgcn_exp2f(ref - top);
+                o *= keep;
+                l *= keep;
+                for (int k = 1; k < groups; ++k) {
+                    const float2 st = meet_s[threadIdx.x + k * per];
+                    const float f = __builtin_amdgcn_exp2f(st.x - top);
+                    l += st.y * f;
+                    o += meet_o[threadIdx.x + k * per] * f;
+                }
+            }
+        }
+        if (group == 0 && mine) store(row, col, o * (l != 0.f ? 1.f / l : 0.f));
     }
 }
 
@@ -275,18 +333,19 @@ __device__ __forceinline__ void merge_parts(int nseg, int rows, int first, int s
 // P' is kept where f16 is accurate: a column's reference is its maximum minus a power of two that keeps the largest P' seen (it decays as the maximum grows)
 // between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite.
 // Tiles are 64 keys, 32 at head size 256; there, and where sixteen rows share the columns, the query's operands lie in LDS as well: the registers hold no more.
+constexpr int decode_waves(int d, int rep) { return d > 128 || (d == 128 && rep < 4) ? 2 : d == 128 || rep == 1 ? 3 : 4; }      // to a SIMD
 template <int DT, int D, int REP>
 struct DecodeCfg {
     static constexpr int TK = D > 128 ? 32 : 64, RB = DT == AIONHIP_Q8_0 ? D : D / 2, ROWS = 16 / REP;
-    static constexpr bool Q_LDS = D > 128 || (D == 128 && REP == 1);
+    static constexpr bool Q_LDS = D >= 128;
     static constexpr bool PV_TWICE = D / 32 / REP * (TK / 4) > 32;              // P' is made once for its maximum and again for its use
     static constexpr int Q_BYTES = Q_LDS ? D / 32 * 2 * 1024 : 0, V_BYTES = NW * TK * RB;
-    static constexpr int MEET_BYTES = NW * (ROWS * (D + 4) + 32) * 4, TABLE_BYTES = (16 * MAX_SEG + 16) * 4;
-    static constexpr int MOST = MEET_BYTES > TABLE_BYTES ? MEET_BYTES : TABLE_BYTES;
+    static constexpr int MEET_BYTES = NW * (ROWS * (D + 4) + 32) * 4, MERGE_BYTES = NW * 64 * 24;
+    static constexpr int MOST = MEET_BYTES > MERGE_BYTES ? MEET_BYTES : MERGE_BYTES;
     static constexpr int LDS_BYTES = Q_BYTES + V_BYTES > MOST ? Q_BYTES + V_BYTES : MOST;
 };
 template <int DT, int D, int REP>
-__global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, Split sp) {
+__global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_kernel(QuantArgs a, Split sp) {
     using Cfg = DecodeCfg<DT, D, REP>;
     constexpr int ROWS = 16 / REP, KK = D / 32, MT = D / 16, SETS = KK / REP;
     constexpr int TK = Cfg::TK, H = TK / 16, KG = TK / 4;                                  // keys of a tile; its sub-tiles; keys of a lane
@@ -296,13 +355,13 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int rt = (int)blockIdx.x / sp.nseg, seg = (int)blockIdx.x - rt * sp.nseg, hk = (int)blockIdx.y, b = (int)blockIdx.z;
+    const int rt = sp.row_tiles == 1 ? 0 : (int)blockIdx.x / sp.nseg, seg = (int)blockIdx.x - rt * sp.nseg, hk = (int)blockIdx.y, b = (int)blockIdx.z;
     const int unit = b * a.Hkv + hk, rows_total = a.L * a.groups;
     const int rows = min(ROWS, rows_total - rt * ROWS);
     const int sub = n / ROWS;
 
     // ---- this lane's query row (columns past the last row repeat it) and its visible keys
-    const int r = rt * ROWS + min(n % ROWS, rows - 1), li = r / a.groups, hq = hk * a.groups + (r - li * a.groups);
+    const int r = rt * ROWS + min(n % ROWS, rows - 1), li = a.L == 1 ? 0 : r / a.groups, hq = hk * a.groups + (r - li * a.groups);
     const size_t qbase = (((size_t)b * a.L + li) * a.Hq + hq) * D;
     constexpr int E0G = DT == AIONHIP_Q8_0 || D == 64;                  // where a lane's eight elements of a block begin, by how K is loaded
     const int e0 = E0G ? (g & 1) * 16 + (g >> 1) * 8 : g * 8;
@@ -322,7 +381,7 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         const long span = (long)(p0 % TK) + (uni_hi - uni_lo);
         count = (int)min((long)all_tiles, (span + TK - 1) / TK + (a.ring && (long)p0 + (uni_hi - uni_lo) > a.ring ? 1 : 0));
     }
-    const int per = (count + sp.nseg - 1) / sp.nseg;
+    const int per = sp.nseg == 1 ? count : (count + sp.nseg - 1) / sp.nseg;
     const int t_end = min((seg + 1) * per, count);
     int t = seg * per + wave;
     auto tile_of = [&](int i) { const int x = first_tile + i; return x >= all_tiles ? x - all_tiles : x; };
@@ -380,35 +439,28 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
 
     // ---- Q^T: eight elements of each block, in the order of K's codes, times 2^-e and the sign of the scale, in two parts
     float qx[KK][8], amax = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        if (a.q_dtype == AIONHIP_F32) {
-            __builtin_memcpy(qx[kk], (const float *)a.q + qbase + kk * 32 + e0, 32);
-        } else {
-            unsigned short x[8];
-            __builtin_memcpy(x, (const unsigned short *)a.q + qbase + kk * 32 + e0, 16);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) qx[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(x[j])) : bf16_bits_to_f32(x[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[kk][j]));
-    }
+    load_query<KK>(a, qbase + e0, qx);
     if (t < t_end) {
         load_k(t);
         load_v(t);
     }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[kk][j]));
     const Power2 by(groups4_max(amax));
     const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
-    const float row_scale = fabsf(a.scale) * by.grow;
+    const float row_scale = fabsf(a.scale) * 16777216.f * by.grow;             // (codes are 2^-24 a step)
     const float to_log2 = a.soft_cap > 0.f ? 1.f : fmaxf(row_scale * LOG2E, 1e-30f);          // (not zero: the score of a key that is not seen is minus infinity)
-    const float zero = opaque_zero();
+    const Constants cst;
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
     u32x4 q_op[Cfg::Q_LDS ? 1 : KK][2];
+    float offset[SETS] = {};
     const unsigned q_addr = (unsigned)(size_t)(lds_void *)lds + lane * 16;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
         u32x4 op[2];
-        split_query<DT>(qx[kk], kk % REP == sub ? sign : 0.f, op);
+        offset[kk / REP] += split_query<DT, true>(qx[kk], kk % REP == sub ? sign : 0.f, op);
         if constexpr (Cfg::Q_LDS) {                                           // (every wavefront has the same rows: each stores its share of the blocks)
             if (kk % NW == wave) {
                 asm volatile("ds_write_b128 %0, %1 offset:%3\n\tds_write_b128 %0, %2 offset:%4" ::"v"(q_addr), "v"(op[0]), "v"(op[1]), "n"(kk * 2048), "n"(kk * 2048 + 1024) : "memory");
@@ -418,6 +470,8 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
             q_op[kk][1] = op[1];
         }
     }
+#pragma unroll
+    for (int st = 0; st < SETS; ++st) offset[st] = groups4_sum(offset[st]) * ((DT == AIONHIP_Q8_0 ? -128.f : -8.f) / 16777216.f);
     if constexpr (Cfg::Q_LDS) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (no wait for the loads in flight)
 
     f32x4 acc[MT];
@@ -454,26 +508,28 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         for (int st = 0; st < SETS; ++st) {
             f32x4 d[H];
 #pragma unroll
-            for (int h = 0; h < H; ++h) d[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < H; ++h) d[h] = f32x4{offset[st], offset[st], offset[st], offset[st]};
 #pragma unroll
             for (int u = 0; u < REP; ++u) {
                 const int kk = st * REP + u;
                 if constexpr (Cfg::Q_LDS)
                     if (kk % 2 == 0) read_four(q_addr + kk * 2048, q4);
                 const u32x4 high = Cfg::Q_LDS ? q4[kk % 2 * 2] : q_op[Cfg::Q_LDS ? 0 : kk][0], low = Cfg::Q_LDS ? q4[kk % 2 * 2 + 1] : q_op[Cfg::Q_LDS ? 0 : kk][1];
+                u32x4 k8[H];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const u32x4 k8 = DT == AIONHIP_Q8_0 ? halves_q8(kw[h][2 * kk % KD], kw[h][(2 * kk + 1) % KD]) : halves_q4(kw[h][kk % KD]);
-                    d[h] = mfma16<AIONHIP_F16>(k8, high, d[h]);
-                    d[h] = mfma16<AIONHIP_F16>(k8, low, d[h]);
+                    k8[h] = DT == AIONHIP_Q8_0 ? raw_q8(kw[h][2 * kk % KD], kw[h][(2 * kk + 1) % KD]) : raw_q4(kw[h][kk % KD]);
+                    d[h] = mfma16<AIONHIP_F16>(k8[h], high, d[h]);
                 }
+#pragma unroll
+                for (int h = 0; h < H; ++h) d[h] = mfma16<AIONHIP_F16>(k8[h], low, d[h]);
             }
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int key = h * 4 + j;
-                    s[key] = fma_half(d[h][j], ksc[st][key >> 3][(key & 7) >> 1], key & 1, st ? s[key] : zero);
+                    s[key] = fma_half(d[h][j], ksc[st][key >> 3][(key & 7) >> 1], key & 1, st ? s[key] : cst.zero);
                 }
         }
         if (more) {
@@ -512,9 +568,9 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
                 }
             }
         }
-        float mx = s[0];
+        float mx = max3(s[0], s[1], s[1]);
 #pragma unroll
-        for (int j = 1; j < KG; ++j) mx = fmaxf(mx, s[j]);
+        for (int j = 2; j < KG; j += 2) mx = max3(mx, s[j], s[j + 1]);
         mx = groups4_max(mx);
         const float m_new = fmaxf(m_run, mx * to_log2);
         float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
@@ -524,14 +580,15 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         for (int j = 0; j < KG; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], to_log2, -ref));
         m_run = m_new;
         // -- the largest P' of the column, and the shift that keeps it in range
-        auto times_scale = [&](int st, int j) __attribute__((always_inline)) { return fma_half(p[j], vsc[st][j >> 3][(j & 7) >> 1], j & 1, zero); };
-        float pv[Cfg::PV_TWICE ? 1 : SETS][KG], top = 0.f;
+        auto times_scale = [&](int st, int j) __attribute__((always_inline)) { return fma_half(p[j], vsc[st][j >> 3][(j & 7) >> 1], j & 1, cst.zero); };
+        float pv[Cfg::PV_TWICE ? 1 : SETS][KG], top = 0.f, before = 0.f;
 #pragma unroll
         for (int st = 0; st < SETS; ++st)
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
                 const float x = times_scale(st, j);
-                top = fmaxf(top, x);
+                if (j % 2) top = max3(top, before, x);
+                before = x;
                 if constexpr (!Cfg::PV_TWICE) pv[st][j] = x;
             }
         top = fmaxf(largest * alpha, groups4_max(top));
@@ -579,7 +636,7 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
                     const float x = Cfg::PV_TWICE ? times_scale(st, k0) : pv[Cfg::PV_TWICE ? 0 : st][k0], y = Cfg::PV_TWICE ? times_scale(st, k1) : pv[Cfg::PV_TWICE ? 0 : st][k1];
                     const unsigned high = pack_half(x, y);
                     ph[step][j] = high;
-                    pl[step][j] = pack_half(fma_half(-1.f, high, 0, x), fma_half(-1.f, high, 1, y));
+                    pl[step][j] = pack_half(fma_half(cst.minus, high, 0, x), fma_half(cst.minus, high, 1, y));
                 }
             constexpr int READS = REP * CB * STEPS, N = READS < 8 ? READS : 8;
             static_for<0, READS / N>([&](auto part_c) __attribute__((always_inline)) {
@@ -599,11 +656,11 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
                         const u32x2 w = v[c * STEPS + step];
                         if constexpr (DT == AIONHIP_Q8_0) {
                             f32x4 &o = acc[c0 + c];
-                            const u32x4 x = halves_q8(w.x, w.y);
+                            const u32x4 x = halves_q8(cst, w.x, w.y);
                             o = mfma16<AIONHIP_F16>(x, ph[step], o);
                             o = mfma16<AIONHIP_F16>(x, pl[step], o);
                         } else {                                              // the even columns of the block, and the odd ones
-                            const u32x4 x = halves_q4(w.x), y = halves_q4(w.y);
+                            const u32x4 x = halves_q4(cst, w.x), y = halves_q4(cst, w.y);
                             f32x4 &o = acc[(c0 + c) * 2], &o2 = acc[(c0 + c) * 2 + 1];
                             const u32x4 even{x.x, x.z, y.x, y.z}, odd{x.y, x.w, y.y, y.w};
                             o = mfma16<AIONHIP_F16>(even, ph[step], o);
@@ -658,7 +715,7 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
     [[maybe_unused]] const __amdgpu_buffer_rsrc_t parts_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)parts, 0, (unsigned)(sp.nseg * FLOATS * 4), 0x00027000);
 #endif
     auto store_out = [&](int row, int col, f32x4 v) {
-        const int rr = rt * ROWS + row, l2 = rr / a.groups, g2 = rr - l2 * a.groups;
+        const int rr = rt * ROWS + row, l2 = a.L == 1 ? 0 : rr / a.groups, g2 = rr - l2 * a.groups;
         __builtin_memcpy(a.out + (((size_t)b * a.L + l2) * a.Hq + hk * a.groups + g2) * D + col, &v, 16);
     };
     auto meet = [&](int c, float (&f)[NW], float &ref, float &l) {
@@ -669,7 +726,7 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         for (int w = 0; w < NW; ++w) ref = fmaxf(ref, x[w] = mg[w * WS + ROWS * RS + 2 * c]);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            f[w] = exp2f(x[w] - ref);
+            f[w] = __builtin_amdgcn_exp2f(x[w] - ref);
             l += mg[w * WS + ROWS * RS + 2 * c + 1] * f[w];
         }
     };
@@ -704,8 +761,9 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
     __syncthreads();
     if (mine != sp.nseg - 1) return;
     if (threadIdx.x == 0) __hip_atomic_store(sp.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int elements = rows * (D / 4);
     merge_parts<D, REP>(
-        sp.nseg, rows, (int)threadIdx.x, NW * 64, (float (*)[MAX_SEG])lds, (float *)lds + 16 * MAX_SEG,
+        sp.nseg, 0, elements, max(1, min(NW * 64 / elements, (sp.nseg + RUN - 1) / RUN)), (f32x4 *)lds, (float2 *)(lds + NW * 64 * 16),
         [&](auto count_c, size_t at) __attribute__((always_inline)) {
             if constexpr (decltype(count_c)::value == 2) {
                 u32x2 x = {};
@@ -724,16 +782,17 @@ __global__ __launch_bounds__(NW * 64, 2) void quant_decode_kernel(QuantArgs a, S
         store_out);
 }
 
-// The merge as a launch, for row tiles whose parts are too much for one workgroup: (row tile, share of the rows' columns, unit)
-constexpr int MERGE_SHARES = 16;
+// The merge as a launch, for row tiles whose parts are too much for one workgroup or come from quant_prompt_kernel: (row tile and share of its elements, unit)
 template <int D, int REP>
-__global__ __launch_bounds__(NW * 64) void quant_merge_kernel(QuantArgs a, Split sp) {
-    __shared__ float factor[16][MAX_SEG], total[16];
+__global__ __launch_bounds__(NW * 64) void quant_merge_kernel(QuantArgs a, Split sp, int groups, int shares) {
+    __shared__ f32x4 meet_o[NW * 64];
+    __shared__ float2 meet_s[NW * 64];
     constexpr int ROWS = Part<D, REP>::ROWS, FLOATS = Part<D, REP>::FLOATS;
-    const int rt = blockIdx.x / MERGE_SHARES, share = blockIdx.x % MERGE_SHARES, unit = blockIdx.y, b = unit / a.Hkv, hk = unit % a.Hkv;
+    const int rt = blockIdx.x / shares, share = blockIdx.x % shares, unit = blockIdx.y, b = unit / a.Hkv, hk = unit % a.Hkv, per = NW * 64 / groups;
+    const int elements = min(ROWS, a.L * a.groups - rt * ROWS) * (D / 4);
     const float *parts = sp.parts + ((size_t)unit * sp.row_tiles + rt) * sp.nseg * FLOATS;
     merge_parts<D, REP>(
-        sp.nseg, min(ROWS, a.L * a.groups - rt * ROWS), share * NW * 64 + (int)threadIdx.x, MERGE_SHARES * NW * 64, factor, total,
+        sp.nseg, share * per, min((share + 1) * per, elements), groups, meet_o, meet_s,
         [&](auto count_c, size_t at) __attribute__((always_inline)) {
             if constexpr (decltype(count_c)::value == 2) return *(const u32x2 *)(parts + at);
             else return *(const u32x4 *)(parts + at);
@@ -742,6 +801,12 @@ __global__ __launch_bounds__(NW * 64) void quant_merge_kernel(QuantArgs a, Split
             const int rr = rt * ROWS + row, l2 = rr / a.groups, g2 = rr - l2 * a.groups;
             __builtin_memcpy(a.out + (((size_t)b * a.L + l2) * a.Hq + hk * a.groups + g2) * D + col, &v, 16);
         });
+}
+template <int D, int REP>
+void launch_merge(aionhip_ctx *ctx, const QuantArgs &a, const Split &sp) {
+    const int groups = (sp.nseg + RUN - 1) / RUN, per = NW * 64 / groups, shares = (Part<D, REP>::ROWS * (D / 4) + per - 1) / per;
+    ProfScope scope(ctx, "attn_quant_merge");
+    launch_k(ctx, quant_merge_kernel<D, REP>, dim3((unsigned)(sp.row_tiles * shares), (unsigned)(a.B * a.Hkv)), dim3(NW * 64), 0, a, sp, groups, shares);
 }
 
 template <int DT, int D, int REP>
@@ -756,7 +821,8 @@ int launch_decode(aionhip_ctx *ctx, const QuantArgs &a) {
     long keys = a.T;
     if (a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + Cfg::TK);
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
-    sp.nseg = (int)max(1L, min(min((long)MAX_SEG, 4 * cus / tiles), (key_tiles + NW - 1) / NW));
+    const char *QS = getenv("QSEG");
+    sp.nseg = (int)max(1L, min(min((long)MAX_SEG, (QS ? atoi(QS) : 4) * cus / tiles), (key_tiles + NW - 1) / NW));
     if (sp.nseg > 1) {
         if (const int rc = ensure_scratch2(ctx, (size_t)tiles * sp.nseg * Part<D, REP>::FLOATS * sizeof(float))) return rc;
         sp.parts = (float *)ctx->scratch2;
@@ -772,10 +838,7 @@ int launch_decode(aionhip_ctx *ctx, const QuantArgs &a) {
         ProfScope scope(ctx, "attn_quant_decode");
         launch_k(ctx, quant_decode_kernel<DT, D, REP>, dim3((unsigned)(sp.row_tiles * sp.nseg), (unsigned)a.Hkv, (unsigned)a.B), dim3(NW * 64), LDS, a, sp);
     }
-    if (sp.nseg > 1 && !sp.tickets) {
-        ProfScope scope(ctx, "attn_quant_merge");
-        launch_k(ctx, quant_merge_kernel<D, REP>, dim3((unsigned)(sp.row_tiles * MERGE_SHARES), (unsigned)units), dim3(NW * 64), 0, a, sp);
-    }
+    if (sp.nseg > 1 && !sp.tickets) launch_merge<D, REP>(ctx, a, sp);
     LAUNCH_CHECK(ctx, "attn_quant_decode");
     return AIONHIP_OK;
 }
@@ -868,7 +931,7 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
     const unsigned char *kc = a.k.codes + unit_rows * RB, *vc = a.v.codes + unit_rows * RB;
     const __half *ks = a.k.scales + unit_rows * KK, *vs = a.v.scales + unit_rows * KK;
 
-    const float zero = opaque_zero();
+    const Constants cst;
     // ---- a tile on its way: 512 bytes to an instruction, K in order, V as eight keys x 16 bytes to sixteen lanes
     u32x2 kraw[KI], vraw[KI];
     u32x4 vscale[KI], kscale{};
@@ -896,10 +959,10 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                 const int off = (j * WAVES + wave) * 512 + lane * 8, key = off / RB, piece = off % RB / 8;
                 const int pos = key % KG / 4 * 16 + key / KG * 4 + key % 4;
                 if constexpr (DT == AIONHIP_Q8_0) {
-                    *(u32x4 *)(k_op + (piece * TK + pos) * 16) = halves_q8(kraw[j].x, kraw[j].y);
+                    *(u32x4 *)(k_op + (piece * TK + pos) * 16) = halves_q8(cst, kraw[j].x, kraw[j].y);
                 } else {
-                    *(u32x4 *)(k_op + (piece * 2 * TK + pos) * 16) = halves_q4(kraw[j].x);
-                    *(u32x4 *)(k_op + ((piece * 2 + 1) * TK + pos) * 16) = halves_q4(kraw[j].y);
+                    *(u32x4 *)(k_op + (piece * 2 * TK + pos) * 16) = halves_q4(cst, kraw[j].x);
+                    *(u32x4 *)(k_op + ((piece * 2 + 1) * TK + pos) * 16) = halves_q4(cst, kraw[j].y);
                 }
                 *(u32x2 *)(swap + lane * 8) = vraw[j];
                 v2i w{};
@@ -926,7 +989,7 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                         const unsigned word = x[k >> 1];
                         const h2 pair = __builtin_bit_cast(h2, word);
                         const int key = key_slot<DT>(k);
-                        v[key] = fma_half(k & 1 ? (float)pair.y : (float)pair.x, sc[key >> 1], key & 1, zero);
+                        v[key] = fma_half(k & 1 ? (float)pair.y : (float)pair.x, sc[key >> 1], key & 1, cst.zero);
                     }
                     u32x4 high, low;
 #pragma unroll
@@ -939,9 +1002,9 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                     *(u32x4 *)(o + Cfg::V_BYTES) = low;
                 };
                 if constexpr (DT == AIONHIP_Q8_0) {
-                    store(halves_q8((unsigned)w.x, (unsigned)w.y), v_chunk(j) * 16 + n);
+                    store(halves_q8(cst, (unsigned)w.x, (unsigned)w.y), v_chunk(j) * 16 + n);
                 } else {
-                    const u32x4 x = halves_q4((unsigned)w.x), y = halves_q4((unsigned)w.y);
+                    const u32x4 x = halves_q4(cst, (unsigned)w.x), y = halves_q4(cst, (unsigned)w.y);
                     store(u32x4{x.x, x.z, y.x, y.z}, v_chunk(j) * 32 + n);
                     store(u32x4{x.y, x.w, y.y, y.w}, v_chunk(j) * 32 + 16 + n);
                 }
@@ -957,24 +1020,16 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         float x[KK][8], amax = 0.f;
+        load_query<KK>(a, qbase[ct] + g * 8, x);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            if (a.q_dtype == AIONHIP_F32) {
-                __builtin_memcpy(x[kk], (const float *)a.q + qbase[ct] + kk * 32 + g * 8, 32);
-            } else {
-                unsigned short y[8];
-                __builtin_memcpy(y, (const unsigned short *)a.q + qbase[ct] + kk * 32 + g * 8, 16);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(y[j])) : bf16_bits_to_f32(y[j]);
-            }
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[kk][j]));
-        }
         const Power2 by(groups4_max(amax));
         row_scale[ct] = fabsf(a.scale) * by.grow;
         const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) split_query<DT>(x[kk], sign, q_op[ct][kk]);
+        for (int kk = 0; kk < KK; ++kk) (void)split_query<DT, false>(x[kk], sign, q_op[ct][kk]);
     }
 
     f32x4 acc[CT][MT];
@@ -1025,7 +1080,7 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) s[ct][o * 8 + j] = fma_half(d[ct][j >> 2][j & 3], sc[j >> 1], j & 1, kk ? s[ct][o * 8 + j] : zero);
+                        for (int j = 0; j < 8; ++j) s[ct][o * 8 + j] = fma_half(d[ct][j >> 2][j & 3], sc[j >> 1], j & 1, kk ? s[ct][o * 8 + j] : cst.zero);
                 }
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)                                   // (or the products of the second column group would wait, unscaled, behind the first's softmax)
@@ -1053,9 +1108,9 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
 #pragma unroll
                     for (int j = 0; j < KG; ++j) s[ct][j] = sees(ct, p0 + j) ? s[ct][j] : -INFINITY;
                 }
-                float mx = s[ct][0];
+                float mx = max3(s[ct][0], s[ct][1], s[ct][1]);
 #pragma unroll
-                for (int j = 1; j < KG; ++j) mx = fmaxf(mx, s[ct][j]);
+                for (int j = 2; j < KG; j += 2) mx = max3(mx, s[ct][j], s[ct][j + 1]);
                 mx = groups4_max(mx) * to_log2;
                 // the reference follows the maximum only where that has grown by 2^8: an exponential of up to 2^8 is as exact as one of up to one
                 if (__any(mx > m_ref[ct] + 8.f)) {
@@ -1175,10 +1230,7 @@ int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
         ProfScope scope(ctx, "attn_quant_prompt");
         launch_k(ctx, quant_prompt_kernel<DT, D>, dim3((unsigned)(wgs * sp.nseg)), dim3(Cfg::WAVES * 64), Cfg::LDS_BYTES, a, sp);
     }
-    if (sp.nseg > 1) {
-        ProfScope scope(ctx, "attn_quant_merge");
-        launch_k(ctx, quant_merge_kernel<D, 1>, dim3((unsigned)(sp.row_tiles * MERGE_SHARES), (unsigned)units), dim3(NW * 64), 0, a, sp);
-    }
+    if (sp.nseg > 1) launch_merge<D, 1>(ctx, a, sp);
     LAUNCH_CHECK(ctx, "attn_quant_prompt");
     return AIONHIP_OK;
 }
