@@ -339,7 +339,7 @@ struct DecodeCfg {
     static constexpr int TK = D > 128 ? 32 : 64, RB = DT == AIONHIP_Q8_0 ? D : D / 2, ROWS = 16 / REP;
     static constexpr bool Q_LDS = D >= 128;
     static constexpr bool PV_TWICE = D / 32 / REP * (TK / 4) > 32;              // P' is made once for its maximum and again for its use
-    static constexpr int Q_BYTES = Q_LDS ? D / 32 * 2 * 1024 : 0, V_BYTES = NW * TK * RB;
+    static constexpr int Q_BYTES = Q_LDS ? D / 32 * (2048 + 64) + 256 : 0, V_BYTES = NW * TK * RB;
     static constexpr int MEET_BYTES = NW * (ROWS * (D + 4) + 32) * 4, MERGE_BYTES = NW * 64 * 24;
     static constexpr int MOST = MEET_BYTES > MERGE_BYTES ? MEET_BYTES : MERGE_BYTES;
     static constexpr int LDS_BYTES = Q_BYTES + V_BYTES > MOST ? Q_BYTES + V_BYTES : MOST;
@@ -365,11 +365,22 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
     const size_t qbase = (((size_t)b * a.L + li) * a.Hq + hq) * D;
     constexpr int E0G = DT == AIONHIP_Q8_0 || D == 64;                  // where a lane's eight elements of a block begin, by how K is loaded
     const int e0 = E0G ? (g & 1) * 16 + (g >> 1) * 8 : g * 8;
-    int lo, hi;
+    // (each wavefront has the blocks it makes operands of; all of them where they stay in its registers)
+    constexpr int QB = Cfg::Q_LDS ? KK / NW : KK;
+    const int first_block = Cfg::Q_LDS ? wave * QB : 0;
+    float qx[QB][8];
+    load_query<QB>(a, qbase + first_block * 32 + e0, qx);
+    int lo, hi, uni_lo, uni_hi, full_lo, full_hi;
     visible(a, b, li, lo, hi);
     if (hi <= lo) lo = hi = 0;
+    if (a.L == 1) {                                                          // one token: every row sees the same keys
+        uni_lo = full_lo = __builtin_amdgcn_readfirstlane(lo);
+        uni_hi = full_hi = __builtin_amdgcn_readfirstlane(hi);
+    } else {
+        uni_lo = rows16_min_i(hi > lo ? lo : INT_MAX), uni_hi = rows16_max_i(hi);
+        full_lo = rows16_max_i(lo), full_hi = rows16_min_i(hi);
+    }
     const int kv_end = clip_kv_end(a.ring, a.T, a.kv_lengths ? a.kv_lengths[b] : a.T);
-    const int uni_lo = rows16_min_i(hi > lo ? lo : INT_MAX), uni_hi = rows16_max_i(hi), full_lo = rows16_max_i(lo), full_hi = rows16_min_i(hi);
 
     // ---- the tiles of the segment. A ring is walked by its rows: row p holds step base + p before the row the next step goes to, and a round less from there on.
     const int wrap = a.ring ? kv_end % a.ring : INT_MAX, base = a.ring ? kv_end - wrap : 0;
@@ -437,42 +448,59 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
 #endif
     };
 
-    // ---- Q^T: eight elements of each block, in the order of K's codes, times 2^-e and the sign of the scale, in two parts
-    float qx[KK][8], amax = 0.f;
-    load_query<KK>(a, qbase + e0, qx);
     if (t < t_end) {
         load_k(t);
         load_v(t);
     }
+    // ---- Q^T: eight elements of each block, in the order of K's codes, times a power of two and the sign of the scale, in two parts
+    float amax = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < QB; ++kk)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[kk][j]));
-    const Power2 by(groups4_max(amax));
+        for (int j = 0; j < 8; j += 2) amax = max3(amax, fabsf(qx[kk][j]), fabsf(qx[kk][j + 1]));
+    amax = groups4_max(amax);
+    constexpr int Q_OFFSETS = KK * 2048, Q_MAXIMA = Q_OFFSETS + KK * 64;      // in LDS: the operands, the blocks' offsets by columns, the wavefronts' maxima by columns
+    const unsigned q_addr = (unsigned)(size_t)(lds_void *)lds + lane * 16, n_addr = (unsigned)(size_t)(lds_void *)lds + n * 4;
+    if constexpr (Cfg::Q_LDS) {                                               // (no wait for the loads in flight)
+        asm volatile("ds_write_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"v"(n_addr + Q_MAXIMA + wave * 64), "v"(amax) : "memory");
+        float m0, m1, m2, m3;
+        asm volatile("ds_read_b32 %0, %4 offset:%5\n\tds_read_b32 %1, %4 offset:%6\n\tds_read_b32 %2, %4 offset:%7\n\tds_read_b32 %3, %4 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(m0), "=&v"(m1), "=&v"(m2), "=&v"(m3)
+                     : "v"(n_addr), "n"(Q_MAXIMA), "n"(Q_MAXIMA + 64), "n"(Q_MAXIMA + 128), "n"(Q_MAXIMA + 192) : "memory");
+        amax = max3(max3(m0, m1, m2), m3, m3);
+    }
+    const Power2 by(amax);
     const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
     const float row_scale = fabsf(a.scale) * 16777216.f * by.grow;             // (codes are 2^-24 a step)
     const float to_log2 = a.soft_cap > 0.f ? 1.f : fmaxf(row_scale * LOG2E, 1e-30f);          // (not zero: the score of a key that is not seen is minus infinity)
-    const Constants cst;
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
+    const Constants cst;
+    constexpr float OFFSET = (DT == AIONHIP_Q8_0 ? -128.f : -8.f) / 16777216.f;
     u32x4 q_op[Cfg::Q_LDS ? 1 : KK][2];
     float offset[SETS] = {};
-    const unsigned q_addr = (unsigned)(size_t)(lds_void *)lds + lane * 16;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
+    for (int j = 0; j < QB; ++j) {
+        const int kk = first_block + j;
         u32x4 op[2];
-        offset[kk / REP] += split_query<DT, true>(qx[kk], kk % REP == sub ? sign : 0.f, op);
-        if constexpr (Cfg::Q_LDS) {                                           // (every wavefront has the same rows: each stores its share of the blocks)
-            if (kk % NW == wave) {
-                asm volatile("ds_write_b128 %0, %1 offset:%3\n\tds_write_b128 %0, %2 offset:%4" ::"v"(q_addr), "v"(op[0]), "v"(op[1]), "n"(kk * 2048), "n"(kk * 2048 + 1024) : "memory");
-            }
+        const float sum = split_query<DT, true>(qx[j], kk % REP == sub ? sign : 0.f, op);
+        if constexpr (Cfg::Q_LDS) {
+            asm volatile("ds_write_b128 %0, %2\n\tds_write_b128 %0, %3 offset:1024\n\tds_write_b32 %1, %4" ::"v"(q_addr + kk * 2048),
+                         "v"(n_addr + Q_OFFSETS + kk * 64), "v"(op[0]), "v"(op[1]), "v"(groups4_sum(sum) * OFFSET) : "memory");
         } else {
-            q_op[kk][0] = op[0];
-            q_op[kk][1] = op[1];
+            q_op[j][0] = op[0];
+            q_op[j][1] = op[1];
+            offset[j / REP] += sum;
         }
     }
+    if constexpr (Cfg::Q_LDS) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int st = 0; st < SETS; ++st) offset[st] = groups4_sum(offset[st]) * ((DT == AIONHIP_Q8_0 ? -128.f : -8.f) / 16777216.f);
-    if constexpr (Cfg::Q_LDS) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (no wait for the loads in flight)
+        for (int st = 0; st < SETS; ++st)
+            asm volatile("ds_read_b32 %0, %1 offset:%2\n\ts_waitcnt lgkmcnt(0)" : "=&v"(offset[st]) : "v"(n_addr + sub * 64), "n"(Q_OFFSETS + st * REP * 64) : "memory");
+    } else {
+#pragma unroll
+        for (int st = 0; st < SETS; ++st) offset[st] = groups4_sum(offset[st]) * OFFSET;
+    }
 
     f32x4 acc[MT];
 #pragma unroll
@@ -821,8 +849,9 @@ int launch_decode(aionhip_ctx *ctx, const QuantArgs &a) {
     long keys = a.T;
     if (a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + Cfg::TK);
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
-    const char *QS = getenv("QSEG");
-    sp.nseg = (int)max(1L, min(min((long)MAX_SEG, (QS ? atoi(QS) : 4) * cus / tiles), (key_tiles + NW - 1) / NW));
+    // As many as two workgroups to a CU take, each wavefront with a tile at least. us a step with one / two / four to a CU: 32 sequences of 16384 keys, 8 x 128 in 4
+    // bits, 167 / 139 / 144; 4 x 5 queries over 3001 keys of 32 x 128 20 / 19 / 28; 16 over 9692 of 2 x 256 in 8 bits 34 / 34 / 53; 131072 keys of 8 x 128 50 / 53 / 48.
+    sp.nseg = (int)max(1L, min(min((long)MAX_SEG, 2 * cus / tiles), (key_tiles + NW - 1) / NW));
     if (sp.nseg > 1) {
         if (const int rc = ensure_scratch2(ctx, (size_t)tiles * sp.nseg * Part<D, REP>::FLOATS * sizeof(float))) return rc;
         sp.parts = (float *)ctx->scratch2;
