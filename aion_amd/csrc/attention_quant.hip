@@ -851,7 +851,8 @@ int launch_decode(aionhip_ctx *ctx, const QuantArgs &a) {
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
     // As many as two workgroups to a CU take, each wavefront with a tile at least. us a step with one / two / four to a CU: 32 sequences of 16384 keys, 8 x 128 in 4
     // bits, 167 / 139 / 144; 4 x 5 queries over 3001 keys of 32 x 128 20 / 19 / 28; 16 over 9692 of 2 x 256 in 8 bits 34 / 34 / 53; 131072 keys of 8 x 128 50 / 53 / 48.
-    sp.nseg = (int)max(1L, min(min((long)MAX_SEG, 2 * cus / tiles), (key_tiles + NW - 1) / NW));
+    // Up to two tiles to a wavefront are not worth a meeting: one token over 256 keys of one head of 256 10.4 in two segments, 8.6 in one; 512 keys 10.3 in four, 12.1.
+    sp.nseg = key_tiles <= 2 * NW ? 1 : (int)max(1L, min(min((long)MAX_SEG, 2 * cus / tiles), (key_tiles + NW - 1) / NW));
     if (sp.nseg > 1) {
         if (const int rc = ensure_scratch2(ctx, (size_t)tiles * sp.nseg * Part<D, REP>::FLOATS * sizeof(float))) return rc;
         sp.parts = (float *)ctx->scratch2;
@@ -882,12 +883,17 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 
 // --------------------------------------------------------------------------------------------------------------------- many query rows
 // A workgroup has ROWS query rows, 32 to a wavefront (16 at head size 256), and walks its keys a tile at a time. What bounds it is the arithmetic, so the
-// conversions are made once for all of its rows: eight wavefronts turn a tile's codes into operands in LDS while they multiply the tile before it
-// (two stages, one barrier a tile).
+// conversions are made once for all of its rows: eight wavefronts turn a tile's codes into operands in LDS around their products of the tile before it
+// (two stages, one barrier a tile; four convert first and four last, so that of the two wavefronts of a SIMD one converts while the other multiplies). The
+// tile after that is asked for between the softmax and P V, when the scores' registers are free.
 //   K: the codes as f16, exact, [block][lane group][row of a sub-tile] of 16 bytes: an operand is one read, and its scale goes onto the product (a block long).
 //     The query row is the sum of two f16, as in quant_decode_kernel.
 //   V: here the scale can go onto the value, which many rows share: code * scale (19 bits) as the sum of two bf16 (whose exponents hold any of them),
 //     P as well, and of the four products the smallest is left out, 2^-18. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
+// Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 374 us, 370 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
+// at 9000 keys, 8 heads on 2 of 256, q4_0: 219 us. It is bound by issue: a wavefront's tile is 160 matrix instructions and 590 others (128 scales onto products, 180
+// conversions, the softmax 280). Asking for a tile a whole round ahead cost the products their registers (428 us before), four wavefronts' operands read one product
+// ahead and higher wave priority around the products gave the rest.
 // A scale that is not finite would reach rows that do not see its key (0 * NaN): such a value is taken as zero and the rows that do see it get their NaN by hand.
 template <int DT, int D>
 struct PromptCfg {
@@ -899,6 +905,10 @@ struct PromptCfg {
 };
 typedef __attribute__((ext_vector_type(2))) int v2i;
 typedef __attribute__((address_space(3))) v2i lds_v2i;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
 
 template <int DT, int D>
 __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split sp) {
@@ -964,19 +974,24 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
     // ---- a tile on its way: 512 bytes to an instruction, K in order, V as eight keys x 16 bytes to sixteen lanes
     u32x2 kraw[KI], vraw[KI];
     u32x4 vscale[KI], kscale{};
-    auto v_octet = [&](int j) { return ((j * WAVES + wave) * 4 + g) / CH; };
-    auto v_chunk = [&](int j) { return ((j * WAVES + wave) * 4 + g) % CH; };
+    static_assert(32 % CH == 0, "a load's chunk is its lane's");
+    const int octet0 = (wave * 4 + g) / CH, chunk = (wave * 4 + g) % CH;     // of V, the lane's; each further load 32 / CH octets on
+    auto v_octet = [&](int j) { return j * (32 / CH) + octet0; };
+    const int k_lane = wave * 512 + lane * 8, v_lane = (octet0 * 8 + (n >> 1)) * RB + chunk * 16 + (n & 1) * 8;
+    const __half *vs_lane = vs + (size_t)(DT == AIONHIP_Q8_0 ? chunk / 2 : chunk) * a.Tp + octet0 * 8;
+    const __half *ks_lane = ks + (size_t)(threadIdx.x / (TK / 8)) * a.Tp + (threadIdx.x % (TK / 8)) * 8;
     auto request = [&](int i) __attribute__((always_inline)) {
         const int row0 = row0_of(i);
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(kc + (size_t)row0 * RB), 0, TK * RB, 0x00027000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(vc + (size_t)row0 * RB), 0, TK * RB, 0x00027000);
 #pragma unroll
         for (int j = 0; j < KI; ++j)
             if (K_ALL % WAVES == 0 || j * WAVES + wave < K_ALL) {
-                kraw[j] = *(const u32x2 *)(kc + (size_t)row0 * RB + (j * WAVES + wave) * 512 + lane * 8);
-                const int key = row0 + v_octet(j) * 8;
-                vraw[j] = *(const u32x2 *)(vc + (size_t)(key + (n >> 1)) * RB + v_chunk(j) * 16 + (n & 1) * 8);
-                vscale[j] = *(const u32x4 *)(vs + (size_t)(DT == AIONHIP_Q8_0 ? v_chunk(j) / 2 : v_chunk(j)) * a.Tp + key);
+                kraw[j] = __builtin_amdgcn_raw_buffer_load_b64(rk, k_lane, j * WAVES * 512, 0);
+                vraw[j] = __builtin_amdgcn_raw_buffer_load_b64(rv, v_lane, j * WAVES * 512, 0);
+                vscale[j] = *(const u32x4 *)(vs_lane + row0 + j * (256 / CH));
             }
-        if (threadIdx.x < KK * TK / 8) kscale = *(const u32x4 *)(ks + (size_t)(threadIdx.x / (TK / 8)) * a.Tp + row0 + (int)(threadIdx.x % (TK / 8)) * 8);
+        if (threadIdx.x < KK * TK / 8) kscale = *(const u32x4 *)(ks_lane + row0);
     };
     auto convert = [&](int i, int stage) __attribute__((always_inline)) {
         unsigned char *k_op = lds + stage * Cfg::STAGE, *v_op = k_op + Cfg::K_BYTES, *s_op = v_op + 2 * Cfg::V_BYTES, *swap = lds + 2 * Cfg::STAGE + wave * 512;
@@ -999,9 +1014,9 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(lds_void *)(swap + lane * 8));
 #endif
                 u32x4 sc = vscale[j];
-                bool bad = false;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bad |= (sc[k] & 0x7C00u) == 0x7C00u || (sc[k] & 0x7C000000u) == 0x7C000000u;
+                // (an infinity's or NaN's 15 bits plus 2^10 carry into the 16th)
+                const unsigned most = max_u16x2(max_u16x2(sc.x & 0x7FFF7FFFu, sc.y & 0x7FFF7FFFu), max_u16x2(sc.z & 0x7FFF7FFFu, sc.w & 0x7FFF7FFFu));
+                const bool bad = ((most + 0x04000400u) & 0x80008000u) != 0;
                 if (__any(bad)) {
                     odd = true;
 #pragma unroll
@@ -1031,11 +1046,11 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                     *(u32x4 *)(o + Cfg::V_BYTES) = low;
                 };
                 if constexpr (DT == AIONHIP_Q8_0) {
-                    store(halves_q8(cst, (unsigned)w.x, (unsigned)w.y), v_chunk(j) * 16 + n);
+                    store(halves_q8(cst, (unsigned)w.x, (unsigned)w.y), chunk * 16 + n);
                 } else {
                     const u32x4 x = halves_q4(cst, (unsigned)w.x), y = halves_q4(cst, (unsigned)w.y);
-                    store(u32x4{x.x, x.z, y.x, y.z}, v_chunk(j) * 32 + n);
-                    store(u32x4{x.y, x.w, y.y, y.w}, v_chunk(j) * 32 + 16 + n);
+                    store(u32x4{x.x, x.z, y.x, y.z}, chunk * 32 + n);
+                    store(u32x4{x.y, x.w, y.y, y.w}, chunk * 32 + 16 + n);
                 }
             }
         if (odd && lane == 0) meet_lds[2 + stage] = i + 1;
@@ -1071,51 +1086,68 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
         for (int mt = 0; mt < MT; ++mt) acc[ct][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    const bool early = wave < WAVES / 2;
     if (t0 < t_end) {
         convert(t0, 0);
-        if (t0 + 1 < t_end) request(t0 + 1);
+        if (early && t0 + 1 < t_end) request(t0 + 1);
     }
     __syncthreads();
     for (int i = t0; i < t_end; ++i) {
         const int stage = (i - t0) & 1, row0 = row0_of(i);
-        if (i + 1 < t_end) {
-            convert(i + 1, stage ^ 1);
-            if (i + 2 < t_end) request(i + 2);
-        }
+        if (early && i + 1 < t_end) convert(i + 1, stage ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         const unsigned char *k_op = lds + stage * Cfg::STAGE, *v_op = k_op + Cfg::K_BYTES, *s_op = v_op + 2 * Cfg::V_BYTES;
         // keys of the tile: `first` the first row's, one after the other but where a ring begins again
         const int first = row0 < wrap ? base + row0 : base + row0 - a.ring;
+        auto ask = [&]() __attribute__((always_inline)) {
+            const int ahead = i + (early ? 2 : 1);
+            if (ahead < t_end) request(ahead);
+        };
         const bool plain = row0 + TK <= a.T && !(row0 < wrap && row0 + TK > wrap);
         if (!plain || (first < uni_hi && first + TK > uni_lo)) {
             float s[CT][KG];
+            // Products of a sub-tile and a block at a time: the scales meet one's while the matrix cores work on the next's, whose operands have been on their way for
+            // three. (Two sub-tiles share their scales' load.)
+            constexpr int UNITS = H * KK;
+            u32x4 k_at[4], sc_at[2];
+            f32x4 d[2][CT];
+            auto k_load = [&](int x) __attribute__((always_inline)) {
+                k_at[x & 3] = *(const u32x4 *)(k_op + ((x / 2 % KK * 4 + g) * TK + (x / (2 * KK) * 2 + (x & 1)) * 16 + n) * 16);
+            };
+            auto s_load = [&](int x) __attribute__((always_inline)) {
+                if ((x & 1) == 0) sc_at[x / 2 & 1] = *(const u32x4 *)(s_op + (x / 2 % KK * TK + g * KG + x / (2 * KK) * 8) * 2);
+            };
+            auto scaled = [&](int x) __attribute__((always_inline)) {
+                const int kk = x / 2 % KK, at = x / (2 * KK) * 8 + (x & 1) * 4;
 #pragma unroll
-            for (int o = 0; o < H / 2; ++o)                                   // two sub-tiles: four products (two) on their way
+                for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    u32x4 k8[2];
+                    for (int j = 0; j < 4; ++j) s[ct][at + j] = fma_half(d[x & 1][ct][j], sc_at[x / 2 & 1][(x & 1) * 2 + (j >> 1)], j & 1, kk ? s[ct][at + j] : cst.zero);
+            };
+            __builtin_amdgcn_s_setprio(1);
+            k_load(0);
+            k_load(1);
+            k_load(2);
+            s_load(0);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) k8[h] = *(const u32x4 *)(k_op + ((kk * 4 + g) * TK + (o * 2 + h) * 16 + n) * 16);
-                    const u32x4 sc = *(const u32x4 *)(s_op + (kk * TK + g * KG + o * 8) * 2);
-                    f32x4 d[CT][2];
+            for (int x = 0; x <= UNITS; ++x) {
+                if (x < UNITS) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int part = 0; part < 2; ++part)
 #pragma unroll
-                        for (int ct = 0; ct < CT; ++ct) d[ct][h] = mfma16<AIONHIP_F16>(k8[h], q_op[ct][kk][0], f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int ct = 0; ct < CT; ++ct) d[ct][h] = mfma16<AIONHIP_F16>(k8[h], q_op[ct][kk][1], d[ct][h]);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) s[ct][o * 8 + j] = fma_half(d[ct][j >> 2][j & 3], sc[j >> 1], j & 1, kk ? s[ct][o * 8 + j] : cst.zero);
+                        for (int ct = 0; ct < CT; ++ct) d[x & 1][ct] = mfma16<AIONHIP_F16>(k_at[x & 3], q_op[ct][x / 2 % KK][part], part ? d[x & 1][ct] : f32x4{0.f, 0.f, 0.f, 0.f});
                 }
+                if (x > 0) scaled(x - 1);
+                if (x + 2 < UNITS) s_load(x + 2);
+                if (x + 3 < UNITS) k_load(x + 3);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct)                                   // (or the products of the second column group would wait, unscaled, behind the first's softmax)
 #pragma unroll
                 for (int j = 0; j < KG; ++j) asm volatile("" : "+v"(s[ct][j]));
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             const bool whole = plain && first >= full_lo && first + TK <= full_hi;
             u32x4 ph[CT][STEPS], pl[CT][STEPS];
             auto sees = [&](int ct, int p) __attribute__((always_inline)) {
@@ -1170,20 +1202,29 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
+            ask();
+            u32x4 v_at[2][2];                                                 // the operands of a product and of the next
+            auto v_load = [&](int x) __attribute__((always_inline)) {
+                const unsigned char *o = v_op + ((g * STEPS + x % STEPS) * D + x / STEPS * 16 + n) * 16;
+                v_at[x & 1][0] = *(const u32x4 *)o;
+                v_at[x & 1][1] = *(const u32x4 *)(o + Cfg::V_BYTES);
+            };
+            __builtin_amdgcn_s_setprio(1);
+            v_load(0);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int x = 0; x < MT * STEPS; ++x) {
+                const int mt = x / STEPS, step = x % STEPS;
+                if (x + 1 < MT * STEPS) v_load(x + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int step = 0; step < STEPS; ++step) {
-                    const unsigned char *o = v_op + ((g * STEPS + step) * D + mt * 16 + n) * 16;
-                    const u32x4 vh = *(const u32x4 *)o, vl = *(const u32x4 *)(o + Cfg::V_BYTES);
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][0], ph[ct][step], acc[ct][mt]);
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vh, ph[ct][step], acc[ct][mt]);
-                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vh, pl[ct][step], acc[ct][mt]);
-                        acc[ct][mt] = mfma16<AIONHIP_BF16>(vl, ph[ct][step], acc[ct][mt]);
-                    }
-                    if (mt % 2 == 1 && step == STEPS - 1) __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][0], pl[ct][step], acc[ct][mt]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][1], ph[ct][step], acc[ct][mt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
             if (meet_lds[2 + stage] == i + 1) {
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk)
@@ -1198,7 +1239,10 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                         if (groups4_max(gone) > 0.f) acc[ct][2 * kk] = acc[ct][2 * kk + 1] = f32x4{NAN, NAN, NAN, NAN};
                     }
             }
+        } else {
+            ask();
         }
+        if (!early && i + 1 < t_end) convert(i + 1, stage ^ 1);
         __syncthreads();
     }
 
@@ -1247,7 +1291,10 @@ int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
     long keys = a.T;
     if (a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + Cfg::TK);
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
-    sp.nseg = (int)max(1L, min(min((long)cus / wgs, 16L), key_tiles / 4));
+    // One workgroup per CU. Two where the rows see half the keys on average (a prompt on its own), so that short workgroups follow long ones - but for prompts whose
+    // parts take longer to merge: with 256 tiles of rows 4096 keys at D = 64 go from 187 to 142 us, 2048 at D = 128 from 158 to 151, twice 1024 from 89 to 99.
+    const long want = 2 * (long)a.L > keys && key_tiles >= 32 ? 2L * cus : cus;
+    sp.nseg = (int)max(1L, min(min(want / wgs, 16L), key_tiles / 4));
     if (wgs * sp.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
     if (sp.nseg > 1) {
         if (const int rc = ensure_scratch2(ctx, (size_t)units * sp.row_tiles * sp.nseg * Part<D, 1>::FLOATS * sizeof(float))) return rc;
