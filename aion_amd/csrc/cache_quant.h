@@ -60,11 +60,23 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], unsigned (&word)[
             word[i >> 2] |= (unsigned)q << (8 * (i & 3));
         }
     } else {
+        // the quotient by the reciprocal, within 2e-6: it rounds as the exact one does but beside a half, and there (3 elements in 100 000) and where the reciprocal
+        // may leave f32's range the divisions are made
+        float c[8];
+        const float inv = __builtin_amdgcn_rcpf(full);
+        bool near = !(full > 1e-36f && full < 1e36f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int q = (int)fminf(7.f, fmaxf(-8.f, roundf(x[i] / full))) + 8;
-            word[0] |= (unsigned)q << (4 * i);
+            const float t = x[i] * inv;
+            c[i] = rintf(t);
+            near |= fabsf(t - c[i]) > 0.49999f;
         }
+        if (__any(near)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = roundf(x[i] / full);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word[0] |= (unsigned)((int)fminf(7.f, fmaxf(-8.f, c[i])) + 8) << (4 * i);
     }
 }
 

@@ -77,6 +77,46 @@ def test_append(gpu, dtype, b, s, t_cap, h, d, starts, rolling, src):
         x.free()
 
 
+@pytest.mark.parametrize("dtype", [be.Q8_0, be.Q4_0])
+@pytest.mark.parametrize("exponent", [-146, -126, -120, -30, -3, 0, 9, 100, 122])
+def test_codes_beside_halves(gpu, dtype, exponent):
+    """quotients at, just under and just over the halves between two codes, at scales from f32's smallest to its largest"""
+    rng = np.random.default_rng(exponent + 200)
+    s, h, d = 40, 2, 64
+    levels = 127 if dtype == be.Q8_0 else 7
+    top = np.ldexp(rng.uniform(1, 2, (1, s, h, d // 32, 1)), exponent).astype(np.float32)
+    x = top * ((rng.integers(-levels, levels, (1, s, h, d // 32, 32)) + 0.5) / levels).astype(np.float32)
+    for _ in range(2):
+        x = np.where(rng.integers(0, 2, x.shape) == 0, x, np.nextafter(x, np.where(rng.integers(0, 2, x.shape) == 0, np.float32(-np.inf), np.float32(np.inf))))
+    x[..., 7:8] = top
+    x = np.clip(x, -top, top).astype(np.float32).reshape(1, s, h, d)
+    want = QuantCache(dtype, 1, s, h, d, FILL)
+    buf = put(gpu, want)
+    with np.errstate(over="ignore"):
+        want.put(x[0], 0, np.arange(s))
+    gpu.step_append_quant(dtype, [buf], [gpu.upload(x)], gpu.upload(np.zeros(1, np.int32)), (1, s, s, h, d))
+    assert np.array_equal(gpu.download(buf, np.uint8, want.bytes.shape), want.bytes)
+
+
+@pytest.mark.parametrize("dtype", [be.Q8_0, be.Q4_0])
+@pytest.mark.parametrize("s,h,d", [(1, 1, 2048), (5, 2, 2080), (3, 1, 4128), (11, 3, 1056), (9, 2, 672)])
+def test_long_heads(gpu, dtype, s, h, d):
+    """heads of more pieces than a workgroup has threads, and such as do not divide it"""
+    rng = np.random.default_rng(d)
+    x = rng.standard_normal((2, s, h, d)).astype(np.float32)
+    want = QuantCache(dtype, 2, 80, h, d, FILL)
+    buf = put(gpu, want)
+    for i in range(2):
+        want.put(x[i], i, np.arange(60 * i, 60 * i + s))
+    index = gpu.upload(np.array([0, 60], np.int32))
+    gpu.step_append_quant(dtype, [buf], [gpu.upload(x)], index, (2, s, 80, h, d))
+    assert np.array_equal(gpu.download(buf, np.uint8, want.bytes.shape), want.bytes)
+    out = gpu.alloc(x.nbytes)
+    gpu.step_cache_read(dtype, [out], [buf], index, (2, s, 80, h, d))
+    for i in range(2):
+        assert np.array_equal(gpu.download(out, np.float32, x.shape)[i], want.values()[i, 60 * i:60 * i + s])
+
+
 @pytest.mark.parametrize("offset", [1, 2, 3])
 def test_rows_at_any_aligned_address(gpu, offset):
     rng = np.random.default_rng(offset)
