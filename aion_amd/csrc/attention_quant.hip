@@ -2,6 +2,8 @@
 //   S[r,t] = scale * sum_j sk[t,j] * (q[r,j] . ck[t,j]),   P = softmax(S),   O[r,j] = sum_t P[r,t] * sv[t,j] * cv[t,j]
 // with codes c and scales s as they are stored. Sums, the running maximum and the scales are f32 throughout.
 //
+// quant_decode_kernel - up to 64 or 128 query rows of a key head, head sizes 64, 128, 256: bound by memory over long caches, by latency over short ones.
+// quant_prompt_kernel - more rows: bound by instruction issue.
 // quant_generic_kernel - any head size: one wavefront per query row, keys 64 at a time, in f32. Slow; it exists so that every shape the
 //   step allows has a path.
 #include "attention_common.h"
@@ -55,11 +57,12 @@ __global__ __launch_bounds__(256) void quant_generic_kernel(QuantArgs a) {
     for (int j = lane; j < a.d_k; j += 64) qs[j] = load_scalar(a.q, a.q_dtype, row * a.d_k + j);
     for (int j = lane; j < a.d_v; j += 64) acc[j] = 0.f;
     float m = -INFINITY, l = 0.f;
-    for (int t0 = lo; t0 < hi; t0 += 64) {
+    const int keys = hi - lo;                                                // (counted from the first: a ring's keys may end where int does)
+    for (int t0 = 0; t0 < keys; t0 += 64) {
         const int t = t0 + lane;
         float s = -INFINITY;
-        if (t < hi) {
-            const size_t r = (size_t)phys_key(a.ring, t);
+        if (t < keys) {
+            const size_t r = (size_t)phys_key(a.ring, lo + t);
             s = 0.f;
             for (int j = 0; j < a.d_k / 32; ++j) {
                 float dot = 0.f;
@@ -71,14 +74,14 @@ __global__ __launch_bounds__(256) void quant_generic_kernel(QuantArgs a) {
         }
         const float m_new = fmaxf(m, wave_max(s));
         const float shrink = m > -INFINITY ? exp2f((m - m_new) * LOG2E) : 0.f;
-        const float p = t < hi && s != -INFINITY ? exp2f((s - m_new) * LOG2E) : 0.f;
+        const float p = t < keys && s != -INFINITY ? exp2f((s - m_new) * LOG2E) : 0.f;
         l = l * shrink + wave_sum(p);
         m = m_new;
         for (int j0 = 0; j0 < a.d_v; j0 += 64) {
             const int j = min(j0 + lane, a.d_v - 1);                         // (every lane hands its probability on, also where there is no column for it)
             float o = acc[j] * shrink;
-            for (int i = 0; i < min(64, hi - t0); ++i) {
-                const size_t r = (size_t)phys_key(a.ring, t0 + i);
+            for (int i = 0; i < min(64, keys - t0); ++i) {
+                const size_t r = (size_t)phys_key(a.ring, lo + t0 + i);
                 o = fmaf(__shfl(p, i, 64), code_at<DT>(vc + r * rb_v, j) * __half2float(vs[(size_t)(j / 32) * a.Tp + r]), o);
             }
             if (j0 + lane < a.d_v) acc[j] = o;
@@ -332,6 +335,8 @@ __device__ __forceinline__ void merge_parts(int nseg, int first, int last, int g
 // scales are one load or two. V goes to LDS as it is and comes back transposed, eight keys of a byte at a time: of two value columns where a byte holds two.
 // P' is kept where f16 is accurate: a column's reference is its maximum minus a power of two that keeps the largest P' seen (it decays as the maximum grows)
 // between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite.
+// Measured (32 query heads on 8 of 128): one token over 131072 keys in 8 bits 62 us, 4.6 TB/s of the 5.1 that a copy reaches; 32 tokens over 16384 keys each
+// in 4 bits 90 us, 4.9 TB/s; one token over 531 keys of one head of 256 10.5 us, of which 4 are the launch and 3 the meeting of its segments.
 // Tiles are 64 keys, 32 at head size 256; there, and where sixteen rows share the columns, the query's operands lie in LDS as well: the registers hold no more.
 constexpr int decode_waves(int d, int rep) { return d > 128 || (d == 128 && rep < 4) ? 2 : d == 128 || rep == 1 ? 3 : 4; }      // to a SIMD
 template <int DT, int D, int REP>
@@ -579,14 +584,14 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
         // -- which keys this row sees; whole tiles that every row sees need no mask
         bool whole = row0 + TK <= a.T;
         {
-            const int first = row0 < wrap ? base + row0 : base + row0 - a.ring;
-            whole = whole && !(row0 < wrap && row0 + TK > wrap) && first >= full_lo && first + TK <= full_hi;
+            const int first = row0 < wrap ? base + row0 : base - a.ring + row0;
+            whole = whole && !(row0 < wrap && row0 + TK > wrap) && first >= full_lo && first <= full_hi - TK;
         }
         if (!whole) {
             stay_branch();                                                    // a key that is not seen: no score, and a scale of zero (what is there may be anything)
 #pragma unroll
             for (int j = 0; j < KG; ++j) {
-                const int p = row0 + g * KG + j, key = p < wrap ? base + p : base + p - a.ring;
+                const int p = row0 + g * KG + j, key = p < wrap ? base + p : base - a.ring + p;
                 const bool ok = p < a.T && key >= lo && key < hi;
                 s[j] = ok ? s[j] : -INFINITY;
 #pragma unroll
@@ -1098,13 +1103,13 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
         __builtin_amdgcn_sched_barrier(0);
         const unsigned char *k_op = lds + stage * Cfg::STAGE, *v_op = k_op + Cfg::K_BYTES, *s_op = v_op + 2 * Cfg::V_BYTES;
         // keys of the tile: `first` the first row's, one after the other but where a ring begins again
-        const int first = row0 < wrap ? base + row0 : base + row0 - a.ring;
+        const int first = row0 < wrap ? base + row0 : base - a.ring + row0;
         auto ask = [&]() __attribute__((always_inline)) {
             const int ahead = i + (early ? 2 : 1);
             if (ahead < t_end) request(ahead);
         };
         const bool plain = row0 + TK <= a.T && !(row0 < wrap && row0 + TK > wrap);
-        if (!plain || (first < uni_hi && first + TK > uni_lo)) {
+        if (!plain || (first < uni_hi && uni_lo - TK < first)) {
             float s[CT][KG];
             // Products of a sub-tile and a block at a time: the scales meet one's while the matrix cores work on the next's, whose operands have been on their way for
             // three. (Two sub-tiles share their scales' load.)
@@ -1148,10 +1153,10 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                 for (int j = 0; j < KG; ++j) asm volatile("" : "+v"(s[ct][j]));
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(0);
-            const bool whole = plain && first >= full_lo && first + TK <= full_hi;
+            const bool whole = plain && first >= full_lo && first <= full_hi - TK;
             u32x4 ph[CT][STEPS], pl[CT][STEPS];
             auto sees = [&](int ct, int p) __attribute__((always_inline)) {
-                const int key = p < wrap ? base + p : base + p - a.ring;
+                const int key = p < wrap ? base + p : base - a.ring + p;
                 return p < a.T && key >= lo[ct] && key < hi[ct];
             };
 #pragma unroll
@@ -1313,7 +1318,9 @@ int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
 
 template <int DT, int D>
 int launch_rows(aionhip_ctx *ctx, const QuantArgs &a) {
-    if ((long)a.L * a.groups > 64) return launch_prompt<DT, D>(ctx, a);
+    // Few rows are cheaper tile by tile. us, rows a tile / many rows: 96 rows of 8 x 128 in 8 bits over 4000 keys 23 / 37, eight sequences of them 80 / 109, 192 rows
+    // 29 / 41 and 142 / 111; 96 rows of 4 x 64 over 3000 keys, four sequences, 15 / 27; 64 rows of 256 in 4 bits over 5000 keys 38 / 41, 96 rows over 3000 38 / 35.
+    if ((long)a.L * a.groups > (D > 128 ? 64 : 128)) return launch_prompt<DT, D>(ctx, a);
     return launch_decode_rows<DT, D>(ctx, a);
 }
 

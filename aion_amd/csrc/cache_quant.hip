@@ -204,6 +204,7 @@ int tiles_of(aionhip_ctx *ctx, const char *who, size_t b, size_t s, size_t h, si
     *grid = (unsigned)(b * h * wgs);
     return AIONHIP_OK;
 }
+bool overlap(aionhip_handle a, size_t a_bytes, aionhip_handle b, size_t b_bytes) { return a && b && a < b + b_bytes && b < a + a_bytes; }
 int check_cache(aionhip_ctx *ctx, const char *who, aionhip_handle c) {
     return c & 15 ? set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: a cache begins at a multiple of 16 bytes", who) : AIONHIP_OK;
 }
@@ -225,10 +226,11 @@ int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cach
     if (!k_cache || !k || !write_index || !v_cache != !v) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: null operand");
     if (src_dtype != AIONHIP_F32 && src_dtype != AIONHIP_F16 && src_dtype != AIONHIP_BF16)
         return set_err(ctx, AIONHIP_UNSUPPORTED, "append_quant: rows are f32, f16 or bf16, not dtype %d", src_dtype);
-    if (k_cache == v_cache) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: keys and values in one cache");
     int rc = check_shape(ctx, "append_quant", dtype, b, s, t_cap, h, d);
     if (!rc) rc = check_cache(ctx, "append_quant", k_cache | v_cache);
     if (rc || !b || !s || !h || !d) return rc;
+    const size_t bytes = aionhip_cache_quant_bytes(dtype, b, t_cap, h, d);
+    if (overlap(k_cache, bytes, v_cache, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: the caches of keys and values overlap");
     Tiles tiles;
     unsigned grid;
     if ((rc = tiles_of(ctx, "append_quant", b, s, h, d, &tiles, &grid))) return rc;
@@ -248,15 +250,18 @@ int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q
     if (!q_out || !q || !k || !v || !k_cache || !v_cache || !positions || !write_index) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: null operand");
     if (!(base_frequency > 0.f) || !(base_frequency < INFINITY) || !(scale_factor > 0.f) || !(scale_factor < INFINITY) || !(rope_proportion >= 0.f && rope_proportion <= 1.f))
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: base/scale must be positive and finite, proportion in [0,1]");
-    if (k_cache == v_cache) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: keys and values in one cache");
-    if (q_out == q) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: q is read again while q_out is written");
     int rc = check_shape(ctx, "rope_append_quant", dtype, b, s, t_cap, h_kv, d);
     if (!rc) rc = check_cache(ctx, "rope_append_quant", k_cache | v_cache);
     if (rc || !b || !s || !h_q || !h_kv || !d) return rc;
     if (h_q > MAX_HEADS) return set_err(ctx, AIONHIP_UNSUPPORTED, "rope_append_quant: dimension too large");
+    const size_t bytes = aionhip_cache_quant_bytes(dtype, b, t_cap, h_kv, d);
+    if (overlap(k_cache, bytes, v_cache, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: the caches of keys and values overlap");
     const size_t half = d / 2, slots = (h_q + 2 * h_kv) * (d / 8);
     if (b > 0x7FFFFFFF / s || b * s > 0xFFFFFF00u / slots) return set_err(ctx, AIONHIP_UNSUPPORTED, "rope_append_quant: too many rows for one launch");
     const unsigned total = (unsigned)(b * s * slots), grid = (total + 255) / 256;
+    const size_t q_bytes = b * s * h_q * d * sizeof(float), kv_bytes = b * s * h_kv * d * sizeof(float);
+    if (overlap(q_out, q_bytes, q, q_bytes) || overlap(q_out, q_bytes, k, kv_bytes) || overlap(q_out, q_bytes, v, kv_bytes))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: q, k and v are still read while q_out is written");
     size_t rope_pairs = (size_t)floorf(rope_proportion * (float)half);
     if (rope_pairs > half) rope_pairs = half;
     const float freq_step = (float)pow((double)base_frequency, (double)(-2.0f / (float)d));
@@ -280,6 +285,8 @@ int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_
     int rc = check_shape(ctx, "cache_read", dtype, b, s, t_cap, h, d);
     if (!rc) rc = check_cache(ctx, "cache_read", k_cache | v_cache);
     if (rc || !b || !s || !h || !d) return rc;
+    const size_t out_bytes = b * s * h * d * (out_dtype == AIONHIP_F32 ? 4 : 2);
+    if (overlap(k_out, out_bytes, v_out, out_bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "cache_read: the rows of keys and values overlap");
     Tiles tiles;
     unsigned grid;
     if ((rc = tiles_of(ctx, "cache_read", b, s, h, d, &tiles, &grid))) return rc;

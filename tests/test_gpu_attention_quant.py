@@ -149,6 +149,14 @@ def test_rings_and_several_queries(gpu, dtype, l):
 
 
 @BOTH
+@pytest.mark.parametrize("l,d", [(1, 128), (1, 96), (5, 64), (150, 128), (90, 256), (4, 96)])
+def test_rings_as_far_as_an_index_goes(gpu, dtype, l, d):
+    q, kc, vc = case(77 + l, dtype, 2, l, 170, 4, 2, d)
+    lengths = [2147483647, 2147483647 - 40]
+    check(gpu, q, kc, vc, 170, 0.1, window=(120, 0, 0), positions=[list(range(n - l, n)) for n in lengths], kv_lengths=lengths, rolling=True)
+
+
+@BOTH
 @pytest.mark.parametrize("l", [1, 5, 140])
 @pytest.mark.parametrize("soft_cap,scale", [(30.0, 0.2), (5.0, 1.0), (0.0, -0.1), (0.0, 0.0)])
 def test_soft_cap_and_odd_scales(gpu, dtype, l, soft_cap, scale):

@@ -253,13 +253,17 @@ def test_refusals(gpu):
     refused(bad, append, be.Q8_0, [a.view(8)], [x], i, shape)
     refused(bad, read, be.Q8_0, [x], [a.view(8)], i, shape)
     refused(bad, append, be.Q8_0, [a, a], [x, x], i, shape)
+    refused(bad, append, be.Q8_0, [a, a.view(size - 16)], [x, x], i, shape)     # one in the other's end
+    refused(bad, read, be.Q8_0, [x, x.view(1020)], [a, b], i, shape)
     refused(no, append, be.Q8_0, [a], [x], i, shape, src_dtype=be.I32)
     refused(no, read, be.Q8_0, [x], [a], i, shape, out_dtype=be.Q8_0)
     rope = gpu.step_rope_append_quant
     ok = (be.Q8_0, x.view(2048), x, x, x, a, b, i, i, 1, 2, 64, 2, 2, 64)
     refused(bad, rope, be.F32, *ok[1:])
     refused(bad, rope, *ok[:1], x, *ok[2:])                                     # in place
+    refused(bad, rope, *ok[:1], x.view(1020), *ok[2:])                          # nearly
     refused(bad, rope, *ok[:6], a, *ok[7:])
+    refused(bad, rope, *ok[:6], a.view(size - 16), *ok[7:])
     refused(bad, rope, *ok, proportion=1.5)
     refused(bad, rope, *ok, base=0.0)
     for e in (0, 1, 3, 4):                                                      # nothing to do is no error
