@@ -129,11 +129,13 @@ __device__ __forceinline__ u32x4 halves_q8(const Constants &k, unsigned w0, unsi
     return u32x4{pair(w0, 0x07010700u), pair(w0, 0x07030702u), pair(w1, 0x07010700u), pair(w1, 0x07030702u)};
 }
 // The same for keys under few query rows: the codes as they are stored, under the mantissa of zero, are f16 numbers of 2^-24 a step, which the matrix pipe
-// multiplies exactly, subnormal or not. Two instructions less to a pair; the offset is taken back as -offset * sum(q), with which a product begins.
-// Nibbles 1 3 5 7 stand sixteen times higher, so their elements of the query are a sixteenth (split_query).
+// multiplies exactly, subnormal or not. Fewer instructions to a pair; the offset is taken back as -offset * sum(q), with which a product begins. The pipe lines products
+// up by their exponents and a subnormal number's leading zeros are lost below: a nibble stands sixteen times higher, 2^-20 a step (relative error 3e-7; 2.5e-6
+// with every other one in the lowest four bits).
+constexpr float raw_step(int dt) { return dt == AIONHIP_Q8_0 ? 1.f / 16777216.f : 1.f / 1048576.f; }
 __device__ __forceinline__ u32x4 raw_q4(unsigned w) {
-    const unsigned m = 0x000F000Fu, v = w >> 8;
-    return u32x4{w & m, w & (m << 4), v & m, v & (m << 4)};
+    const unsigned m = 0x00F000F0u;
+    return u32x4{(w << 4) & m, w & m, (w >> 4) & m, (w >> 8) & m};
 }
 __device__ __forceinline__ u32x4 raw_q8(unsigned w0, unsigned w1) {
     return u32x4{__builtin_amdgcn_perm(0u, w0, 0x0C010C00u), __builtin_amdgcn_perm(0u, w0, 0x0C030C02u), __builtin_amdgcn_perm(0u, w1, 0x0C010C00u),
@@ -190,17 +192,16 @@ __device__ __forceinline__ void load_query(const QuantArgs &a, size_t at, float 
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(h[kk][j])) : bf16_bits_to_f32(h[kk][j]);
 }
-// Eight elements of a block times `by` as the sum of two f16 each, in the order of K's codes (RAW: for the codes of raw_q4 / raw_q8). Returns the sum of what the operands hold.
-template <int DT, bool RAW>
+// Eight elements of a block times `by` as the sum of two f16 each, in the order of K's codes. Returns the sum of what the operands hold.
+template <int DT>
 __device__ __forceinline__ float split_query(const float (&q)[8], float by, u32x4 (&op)[2]) {
     float x[8], y[8], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const bool high_nibble = RAW && DT == AIONHIP_Q4_0 && (j >> 1 & 1);
-        x[j] = q[element_slot<DT>(j)] * (high_nibble ? by * 0.0625f : by);
+        x[j] = q[element_slot<DT>(j)] * by;
         const float high = (float)(_Float16)x[j];
         y[j] = x[j] - high;
-        sum += (high + (float)(_Float16)y[j]) * (high_nibble ? 16.f : 1.f);
+        sum += high + (float)(_Float16)y[j];
     }
     op[0] = u32x4{pack2<AIONHIP_F16>(x[0], x[1]), pack2<AIONHIP_F16>(x[2], x[3]), pack2<AIONHIP_F16>(x[4], x[5]), pack2<AIONHIP_F16>(x[6], x[7])};
     op[1] = u32x4{pack2<AIONHIP_F16>(y[0], y[1]), pack2<AIONHIP_F16>(y[2], y[3]), pack2<AIONHIP_F16>(y[4], y[5]), pack2<AIONHIP_F16>(y[6], y[7])};
@@ -476,18 +477,18 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
     }
     const Power2 by(amax);
     const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
-    const float row_scale = fabsf(a.scale) * 16777216.f * by.grow;             // (codes are 2^-24 a step)
+    const float row_scale = fabsf(a.scale) * (1.f / raw_step(DT)) * by.grow;
     const float to_log2 = a.soft_cap > 0.f ? 1.f : fmaxf(row_scale * LOG2E, 1e-30f);          // (not zero: the score of a key that is not seen is minus infinity)
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
     const Constants cst;
-    constexpr float OFFSET = (DT == AIONHIP_Q8_0 ? -128.f : -8.f) / 16777216.f;
+    constexpr float OFFSET = (DT == AIONHIP_Q8_0 ? -128.f : -8.f) * raw_step(DT);
     u32x4 q_op[Cfg::Q_LDS ? 1 : KK][2];
     float offset[SETS] = {};
 #pragma unroll
     for (int j = 0; j < QB; ++j) {
         const int kk = first_block + j;
         u32x4 op[2];
-        const float sum = split_query<DT, true>(qx[j], kk % REP == sub ? sign : 0.f, op);
+        const float sum = split_query<DT>(qx[j], kk % REP == sub ? sign : 0.f, op);
         if constexpr (Cfg::Q_LDS) {
             asm volatile("ds_write_b128 %0, %2\n\tds_write_b128 %0, %3 offset:1024\n\tds_write_b32 %1, %4" ::"v"(q_addr + kk * 2048),
                          "v"(n_addr + Q_OFFSETS + kk * 64), "v"(op[0]), "v"(op[1]), "v"(groups4_sum(sum) * OFFSET) : "memory");
@@ -1078,7 +1079,7 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
         row_scale[ct] = fabsf(a.scale) * by.grow;
         const float sign = a.scale < 0.f ? -by.shrink : by.shrink;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) (void)split_query<DT, false>(x[kk], sign, q_op[ct][kk]);
+        for (int kk = 0; kk < KK; ++kk) (void)split_query<DT>(x[kk], sign, q_op[ct][kk]);
     }
 
     f32x4 acc[CT][MT];
