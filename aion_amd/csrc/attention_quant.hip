@@ -894,13 +894,16 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 // tile after that is asked for between the softmax and P V, when the scores' registers are free.
 //   K: the codes as f16, exact, [block][lane group][row of a sub-tile] of 16 bytes: an operand is one read, and its scale goes onto the product (a block long).
 //     The query row is the sum of two f16, as in quant_decode_kernel.
-//   V: here the scale can go onto the value, which many rows share: code * scale (19 bits) as the sum of two bf16 (whose exponents hold any of them),
-//     P as well, and of the four products the smallest is left out, 2^-18. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
+//   V: here the scale can go onto the value, which many rows share: code * scale (19 bits) times a power of two as the sum of two f16, exact down to 2^-18 of the
+//     largest that the workgroup's rows see in that block of columns, and good to 2^-40 of it (two bf16, which need no power, were off by 2^-17: 3e-6 of
+//     an output where this is 3e-7). The largest is found first, from the scales alone, 1/32 to 1/16 of V. P is the sum of two f16 too, and of the four products
+//     the smallest, 2^-22, is left out. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
 // Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 374 us, 370 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
 // at 9000 keys, 8 heads on 2 of 256, q4_0: 219 us. It is bound by issue: a wavefront's tile is 160 matrix instructions and 590 others (128 scales onto products, 180
 // conversions, the softmax 280). Asking for a tile a whole round ahead cost the products their registers (428 us before), four wavefronts' operands read one product
 // ahead and higher wave priority around the products gave the rest.
-// A scale that is not finite would reach rows that do not see its key (0 * NaN): such a value is taken as zero and the rows that do see it get their NaN by hand.
+// A scale that is not finite would reach rows that do not see its key (0 * NaN), as would one that none of the rows sees and that the power of two takes past f16:
+// such a value is taken as zero, and the rows that see one that is not finite get their NaN by hand.
 template <int DT, int D>
 struct PromptCfg {
     static constexpr int WAVES = 8, TK = D > 128 ? 32 : 64, CT = D > 128 ? 1 : 2, ROWS = WAVES * 16 * CT;
@@ -951,6 +954,7 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
         meet_lds[0] = INT_MAX;
         meet_lds[1] = 0;
         meet_lds[2] = meet_lds[3] = 0;                                       // one more than the last tile with a value whose scale is not finite, by stages
+        for (int kk = 0; kk < KK; ++kk) meet_lds[4 + kk] = 0;                // the blocks' largest scales
     }
     __syncthreads();
     if (lane == 0) {
@@ -981,6 +985,12 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
     u32x2 kraw[KI], vraw[KI];
     u32x4 vscale[KI], kscale{};
     static_assert(32 % CH == 0, "a load's chunk is its lane's");
+    auto seen = [&](int p) __attribute__((always_inline)) {                  // by a row of the workgroup
+        const int key = p < wrap ? base + p : base - a.ring + p;
+        return p < a.T && key >= wg_lo && key < wg_hi;
+    };
+    unsigned limit = 0;                                                      // of the scales of the lane's block of V, and what brings it below 2^8
+    float grow = 1.f;
     const int octet0 = (wave * 4 + g) / CH, chunk = (wave * 4 + g) % CH;     // of V, the lane's; each further load 32 / CH octets on
     auto v_octet = [&](int j) { return j * (32 / CH) + octet0; };
     const int k_lane = wave * 512 + lane * 8, v_lane = (octet0 * 8 + (n >> 1)) * RB + chunk * 16 + (n & 1) * 8;
@@ -1020,32 +1030,30 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(lds_void *)(swap + lane * 8));
 #endif
                 u32x4 sc = vscale[j];
-                // (an infinity's or NaN's 15 bits plus 2^10 carry into the 16th)
                 const unsigned most = max_u16x2(max_u16x2(sc.x & 0x7FFF7FFFu, sc.y & 0x7FFF7FFFu), max_u16x2(sc.z & 0x7FFF7FFFu, sc.w & 0x7FFF7FFFu));
-                const bool bad = ((most + 0x04000400u) & 0x80008000u) != 0;
-                if (__any(bad)) {
-                    odd = true;
+                if (__any(max(most >> 16, most & 0xFFFFu) > limit)) {                  // not finite, or of no key that the workgroup's rows see
+                    stay_branch();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if ((sc[k] & 0x7C00u) == 0x7C00u) sc[k] &= 0xFFFF0000u;
-                        if ((sc[k] & 0x7C000000u) == 0x7C000000u) sc[k] &= 0xFFFFu;
+                    for (int k = 0; k < 8; ++k) {
+                        const unsigned half = sc[k >> 1] >> (16 * (k & 1)) & 0x7FFFu;
+                        const int p = row0_of(i) + v_octet(j) * 8 + k;
+                        odd |= half >= 0x7C00u && seen(p);
+                        if (half > limit) sc[k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
                     }
                 }
+                float by[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) by[k] = fma_half(grow, sc[k >> 1], k & 1, cst.zero);
                 // x: pairs of codes of the keys ka, kb; stored at column `col` of the octet
                 auto store = [&](const u32x4 &x, int col) __attribute__((always_inline)) {
                     float v[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const unsigned word = x[k >> 1];
-                        const h2 pair = __builtin_bit_cast(h2, word);
-                        const int key = key_slot<DT>(k);
-                        v[key] = fma_half(k & 1 ? (float)pair.y : (float)pair.x, sc[key >> 1], key & 1, cst.zero);
-                    }
+                    for (int k = 0; k < 8; ++k) v[key_slot<DT>(k)] = fma_half(by[key_slot<DT>(k)], x[k >> 1], k & 1, cst.zero);
                     u32x4 high, low;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        high[k] = pack2<AIONHIP_BF16>(v[2 * k], v[2 * k + 1]);
-                        low[k] = pack2<AIONHIP_BF16>(v[2 * k] - __uint_as_float(high[k] << 16), v[2 * k + 1] - __uint_as_float(high[k] & 0xFFFF0000u));
+                        high[k] = pack_half(v[2 * k], v[2 * k + 1]);
+                        low[k] = pack_half(fma_half(cst.minus, high[k], 0, v[2 * k]), fma_half(cst.minus, high[k], 1, v[2 * k + 1]));
                     }
                     unsigned char *o = v_op + (v_octet(j) * D + col) * 16;
                     *(u32x4 *)o = high;
@@ -1059,10 +1067,30 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                     store(u32x4{x.y, x.w, y.y, y.w}, chunk * 32 + 16 + n);
                 }
             }
-        if (odd && lane == 0) meet_lds[2 + stage] = i + 1;
+        if (__any(odd) && lane == 0) meet_lds[2 + stage] = i + 1;
     };
 
     if (t0 < t_end) request(t0);
+    // ---- the largest scale of each block of V that a row of the workgroup sees, in the tiles it is about to walk
+    constexpr int LOADS = KK * TK / 8;                                       // of a tile's scales
+    {
+        const int slot = threadIdx.x % LOADS, kk = slot / (TK / 8), at = slot % (TK / 8) * 8;
+        unsigned most = 0;
+#pragma unroll 4
+        for (int i = t0 + (int)threadIdx.x / LOADS; i < t_end; i += WAVES * 64 / LOADS) {
+            const int row = row0_of(i) + at;
+            const u32x4 sc = *(const u32x4 *)(vs + (size_t)kk * a.Tp + row);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const unsigned half = sc[k >> 1] >> (16 * (k & 1)) & 0x7FFFu;
+                most = max(most, half < 0x7C00u && seen(row + k) ? half : 0u);
+            }
+        }
+        atomicMax(&meet_lds[4 + kk], (int)most);
+        __syncthreads();
+        limit = (unsigned)meet_lds[4 + (DT == AIONHIP_Q8_0 ? chunk / 2 : chunk)];
+        grow = __uint_as_float((149u - max(limit >> 10, 1u)) << 23);
+    }
     // ---- Q^T, two parts of eight elements of each block
     const float inv_cap = a.soft_cap > 0.f ? 1.f / a.soft_cap : 0.f;
     u32x4 q_op[CT][KK][2];
@@ -1179,10 +1207,11 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
 #pragma unroll
                 for (int j = 2; j < KG; j += 2) mx = max3(mx, s[ct][j], s[ct][j + 1]);
                 mx = groups4_max(mx) * to_log2;
-                // the reference follows the maximum only where that has grown by 2^8: an exponential of up to 2^8 is as exact as one of up to one
-                if (__any(mx > m_ref[ct] + 8.f)) {
+                // the reference is the maximum less 7, and follows it only where that has grown by another 8: exponentials of up to 2^15, whose two f16 end 2^-32 below
+                // the largest
+                if (__any(mx > m_ref[ct] + 15.f)) {
                     stay_branch();
-                    const float m_new = mx > m_ref[ct] + 8.f ? mx : m_ref[ct];
+                    const float m_new = mx > m_ref[ct] + 15.f ? mx - 7.f : m_ref[ct];
                     const float alpha = __builtin_amdgcn_exp2f(m_ref[ct] - m_new);
                     m_ref[ct] = m_new;
                     l_run[ct] *= alpha;
@@ -1202,9 +1231,9 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float x = s[ct][step * 8 + 2 * k], y = s[ct][step * 8 + 2 * k + 1];
-                        const unsigned high = pack2<AIONHIP_BF16>(x, y);
+                        const unsigned high = pack_half(x, y);
                         ph[ct][step][k] = high;
-                        pl[ct][step][k] = pack2<AIONHIP_BF16>(x - __uint_as_float(high << 16), y - __uint_as_float(high & 0xFFFF0000u));
+                        pl[ct][step][k] = pack_half(fma_half(cst.minus, high, 0, x), fma_half(cst.minus, high, 1, y));
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -1223,11 +1252,11 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
                 if (x + 1 < MT * STEPS) v_load(x + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][0], ph[ct][step], acc[ct][mt]);
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_F16>(v_at[x & 1][0], ph[ct][step], acc[ct][mt]);
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][0], pl[ct][step], acc[ct][mt]);
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_F16>(v_at[x & 1][0], pl[ct][step], acc[ct][mt]);
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_BF16>(v_at[x & 1][1], ph[ct][step], acc[ct][mt]);
+                for (int ct = 0; ct < CT; ++ct) acc[ct][mt] = mfma16<AIONHIP_F16>(v_at[x & 1][1], ph[ct][step], acc[ct][mt]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
@@ -1273,7 +1302,8 @@ __global__ __launch_bounds__(512, 2) void quant_prompt_kernel(QuantArgs a, Split
         }
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
-            const f32x4 x = acc[ct][2 * kk] * inv, y = acc[ct][2 * kk + 1] * inv;
+            const float back = inv * __uint_as_float((105u + max((unsigned)meet_lds[4 + kk] >> 10, 1u)) << 23);
+            const f32x4 x = acc[ct][2 * kk] * back, y = acc[ct][2 * kk + 1] * back;
             f32x4 first4, second4;
             int at, next;
             if constexpr (DT == AIONHIP_Q8_0) {

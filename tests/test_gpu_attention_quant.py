@@ -207,6 +207,36 @@ def test_values_of_very_different_size_along_the_cache(gpu, dtype, l):
 
 
 @BOTH
+@pytest.mark.parametrize("fill", [0x7B, 0xFB, 0x7C])
+@pytest.mark.parametrize("l,d", [(1, 128), (5, 64), (150, 128), (90, 256), (300, 64)])
+def test_large_scales_of_rows_nobody_sees(gpu, dtype, l, d, fill):
+    """Behind the last row, and before a window, lie scales near f16's largest, of either sign, or NaN."""
+    rng = np.random.default_rng(fill + l)
+    t, rows = 700, 470
+    q = rng.standard_normal((2, l, 4, d)).astype(np.float32)
+    kc, vc = (filled(rng, dtype, 2, t, 2, d, 1.0, fill=fill, rows=rows) for _ in range(2))
+    small = rng.standard_normal((rows, 2, d)).astype(np.float32) * np.float32(1e-3)
+    for b in range(2):
+        vc.put(small, b, range(rows))
+    first = rows - l - 60
+    for c in (kc, vc):
+        c.scales[:, :, :, :first] = fill * 257
+    pos = [np.arange(rows - l, rows)] * 2
+    check(gpu, q, kc, vc, t, 0.1, positions=pos, kv_lengths=[rows, rows], window=(59, 0, 0))
+
+
+@BOTH
+@pytest.mark.parametrize("l", [1, 150])
+def test_columns_of_very_different_size(gpu, dtype, l):
+    """The blocks of the values lie 2^30 apart; each column is as exact as its own size asks for."""
+    rng = np.random.default_rng(l)
+    q, kc, vc = case(l, dtype, 1, l, 333, 4, 2, 128)
+    size = np.repeat(np.float32([2.0 ** 12, 2.0 ** -16, 1.0, 2.0 ** -18]), 32)
+    vc.put(rng.standard_normal((333, 2, 128)).astype(np.float32) * size, 0, range(333))
+    check(gpu, q, kc, vc, 333, 0.1, positions=[np.arange(333 - l, 333)], kv_lengths=[333])
+
+
+@BOTH
 @pytest.mark.parametrize("l", [1, 5, 150])
 def test_what_is_not_finite_stays_where_it_is_seen(gpu, dtype, l):
     """A NaN key or value is seen by the rows whose interval holds it, and by nobody else; of a value only its block's columns."""
