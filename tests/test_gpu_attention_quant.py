@@ -334,3 +334,50 @@ def test_a_decode_recorded_and_replayed(gpu, dtype):
     gpu.program_destroy(prog)
     for x in bufs + rows + [q, out, index, lens, pos]:
         x.free()
+
+
+@BOTH
+def test_two_programs_of_one_context(gpu, dtype):
+    """A chunk of a prompt and a token as programs that share the context's work buffers, replayed in turn: appended rows, attention, rows read back."""
+    rng = np.random.default_rng(9)
+    t_cap, hq, hk, d = 1500, 8, 2, 128
+    kc, vc = (filled(rng, dtype, 1, t_cap, hk, d, rows=900) for _ in range(2))
+    bufs = [gpu.upload(c.bytes) for c in (kc, vc)]
+    index, lens = (gpu.upload(np.zeros(1, np.int32)) for _ in range(2))
+    calls = {}
+    for s in (150, 1):
+        rows, back = [[gpu.alloc(s * hk * d * 4) for _ in range(2)] for _ in range(2)]
+        q, out, pos = gpu.alloc(s * hq * d * 4), gpu.alloc(s * hq * d * 4), gpu.alloc(s * 4)
+
+        def issue(s=s, rows=rows, back=back, q=q, out=out, pos=pos):
+            gpu.step_append_quant(dtype, bufs, rows, index, (1, s, t_cap, hk, d))
+            gpu.step_attention(out, q, *bufs, (1, s, t_cap, hq, hk, d, d), 0.1, kv_dtype=dtype, query_positions=pos, kv_lengths=lens)
+            gpu.step_cache_read(dtype, back, bufs, index, (1, s, t_cap, hk, d))
+        calls[s] = (issue, rows, back, q, out, pos)
+        issue()
+    for c, buf in zip((kc, vc), bufs):
+        gpu.write(buf, c.bytes)
+    progs = {s: gpu.record_program(calls[s][0]) for s in calls}
+    at = 900
+    for s in (150, 1, 1, 150, 1):
+        _, rows, back, q, out, pos = calls[s]
+        new = [rng.standard_normal((1, s, hk, d)).astype(np.float32) for _ in range(2)]
+        qv = rng.standard_normal((1, s, hq, d)).astype(np.float32)
+        steps = np.arange(at, at + s, dtype=np.int32)
+        for buf, x in zip(rows + [q, index, lens, pos], new + [qv, steps[:1], steps[-1:] + 1, steps]):
+            gpu.write(buf, x)
+        for c, x in zip((kc, vc), new):
+            c.put(x[0], 0, steps)
+        gpu.program_execute(progs[s])
+        got = gpu.download(out, np.float32, qv.shape)
+        want, near = attention_f64(qv, kc.values(), vc.values(), 0.1, t_cap, positions=[steps], kv_lengths=[at + s])
+        inside = bool((np.abs(got - want) <= bound_of(near)).all())
+        assert inside, (at, s)
+        for c, buf, o in zip((kc, vc), bufs, back):
+            assert np.array_equal(gpu.download(buf, np.uint8, c.bytes.shape), c.bytes)
+            assert np.array_equal(gpu.download(o, np.float32, (s, hk, d)), c.values()[0, steps].astype(np.float32))
+        at += s
+    for p in progs.values():
+        gpu.program_destroy(p)
+    for x in bufs + [index, lens] + [y for _, rows, back, q, out, pos in calls.values() for y in rows + back + [q, out, pos]]:
+        x.free()
