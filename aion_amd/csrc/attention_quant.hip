@@ -241,8 +241,8 @@ __device__ __forceinline__ void read_transposed(const unsigned (&at)[N], u32x2 (
 }
 // sixteen bytes from each of four places, complete when the statement is
 __device__ __forceinline__ void read_four(unsigned at, u32x4 (&r)[4]) {
-    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\tds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]) : "v"(at) : "memory");
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\tds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]) : "v"(at), "n"(1024), "n"(2 * 1024), "n"(3 * 1024) : "memory");
 }
 
 // Key segments: every workgroup of a row tile takes a share of its sequence's 64-key tiles and leaves sums over them; `parts` holds those, `tickets`
@@ -336,8 +336,8 @@ __device__ __forceinline__ void merge_parts(int nseg, int first, int last, int g
 // scales are one load or two. V goes to LDS as it is and comes back transposed, eight keys of a byte at a time: of two value columns where a byte holds two.
 // P' is kept where f16 is accurate: a column's reference is its maximum minus a power of two that keeps the largest P' seen (it decays as the maximum grows)
 // between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite.
-// Measured (32 query heads on 8 of 128): one token over 131072 keys in 8 bits 62 us, 4.6 TB/s of the 5.1 that a copy reaches; 32 tokens over 16384 keys each
-// in 4 bits 90 us, 4.9 TB/s; one token over 531 keys of one head of 256 10.5 us, of which 4 are the launch and 3 the meeting of its segments.
+// Measured (32 query heads on 8 of 128): one token over 131072 keys in 8 bits 57 us, 5.0 TB/s (a copy reaches 5.1, a read 6.8); 32 tokens over 16384 keys
+// each in 4 bits 85 us, 5.2 TB/s; one token over 531 keys of one head of 256 10.5 us, of which 4 are the launch and 3 the meeting of its segments.
 // Tiles are 64 keys, 32 at head size 256; there, and where sixteen rows share the columns, the query's operands lie in LDS as well: the registers hold no more.
 constexpr int decode_waves(int d, int rep) { return d > 128 || (d == 128 && rep < 4) ? 2 : d == 128 || rep == 1 ? 3 : 4; }      // to a SIMD
 template <int DT, int D, int REP>
@@ -412,19 +412,22 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
     unsigned kw[H][KD];
     u32x4 ksc[SETS][KG / 8], vsc[SETS][KG / 8];
     const unsigned k_lane = (unsigned)(((n >> 2) * KG + (n & 3)) * RB + g * (KD == 2 ? 8 : 16));
+    // Up to eight rows are one row tile, which reads every code once: past the caches (32 sequences of 16384 keys in 4 bits 91 -> 85 us). The row tiles of more rows read
+    // a key together (8 sequences of 96 rows over 4000 keys in 8 bits: 82 us, past the caches 104).
+    constexpr bool ONCE = REP > 1;
     auto load_k = [&](int i) __attribute__((always_inline)) {
         const int row0 = tile_of(i) * TK;
         const unsigned char *p = kc + (size_t)row0 * RB + k_lane;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             if constexpr (KD == 2) {
-                const u32x2 x = *(const u32x2 *)(p + h * 4 * RB);
+                const u32x2 x = ONCE ? __builtin_nontemporal_load((const u32x2 *)(p + h * 4 * RB)) : *(const u32x2 *)(p + h * 4 * RB);
                 kw[h][0] = x.x;
                 kw[h][1] = x.y;
             } else {
 #pragma unroll
                 for (int c = 0; c < KD / 4; ++c) {
-                    const u32x4 x = *(const u32x4 *)(p + h * 4 * RB + c * 64);
+                    const u32x4 *from = (const u32x4 *)(p + h * 4 * RB + c * 64), x = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) kw[h][c * 4 + j] = x[j];
                 }
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(vc + (size_t)row0 * RB), 0, TK * RB, 0x00027000);
 #pragma unroll
         for (int j = 0; j < NVI; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(v_lds + j * 1024), 16, (int)(v_lane ^ (unsigned)(((4 * j) & (CH - 1)) << 4)), j * 1024, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(v_lds + j * 1024), 16, (int)(v_lane ^ (unsigned)(((4 * j) & (CH - 1)) << 4)), j * 1024, 0, ONCE ? 2 : 0);
 #endif
     };
 

@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace {
 using namespace cq;
@@ -52,13 +53,14 @@ struct Pair {
 };
 
 // How append_quant_kernel and cache_read_kernel share the rows out: a workgroup has ROWS_EACH * `rows` tokens of one head, so that what it touches of the cache is
-// one run of codes and a run of each block's scales; a thread has eight elements of each ROWS_EACH-th of them, all asked for before the first is used.
+// one run of codes and a run of each block's scales; a thread has the same few
+// elements of ROWS_EACH of them, all asked for before the first is used.
 constexpr int ROWS_EACH = 2;
 struct Tiles {
     unsigned per, rows, wgs;     // threads to a row, rows side by side, workgroups of a head
 };
 struct Place {
-    unsigned unit, first, piece;      // sequence and head; the thread's first token (past every length: none) and its eight elements
+    unsigned unit, first, piece;      // sequence and head; the thread's first token (past every length: none) and its elements
 };
 __device__ __forceinline__ Place place_of(const Tiles &t) {
     const unsigned unit = blockIdx.x / t.wgs, row = threadIdx.x / min(t.per, 256u);
@@ -66,7 +68,7 @@ __device__ __forceinline__ Place place_of(const Tiles &t) {
 }
 
 // SequenceAppend with the quantization in it: four threads hold a block. 8000 tokens of 8 heads of 128, k and v, f32 to
-// q4_0: 16.7 us, 4.5 TB/s of 5.1 that a copy reaches (17.3 with one token to a thread, 19.0 with four).
+// q4_0: 16.0 us, 4.7 TB/s of 5.1 that a copy reaches (one token to a thread 17.3, four 19.0).
 template <int DT>
 __global__ __launch_bounds__(256) void append_quant_kernel(Pair p, const int *write_index, int src_dtype, int s_len, int t_cap, int tp, int h, int d, int rolling, Tiles tiles) {
     const Place at = place_of(tiles);
@@ -139,50 +141,57 @@ struct ReadPair {
 };
 
 // Rows first[b] .. first[b] + s_len - 1 as numbers; a row that the cache does not hold is zeros. The product of a code and a scale is exact in f32 and rounded once.
-// 4 x 16000 tokens of 8 heads of 128, q4_0 to f16: 40.9 us, 4.1 TB/s (45.7 with one token to a thread, 58 with the threads in the result's order: a workgroup
-// then has two bytes of each scale line).
+// A thread has sixteen bytes of the result, so that a wavefront's store is whole lines, which pass the caches by: they would push out what is read.
+// 4 x 16000 tokens of 8 heads of 128, q4_0 to f16: 28.3 us, 5.9 TB/s (41.5 through the caches; there 45.7 with one token to a thread, and 58 with the threads in the
+// result's order, where a workgroup has two bytes of each scale line). 8000 tokens of k and v, q4_0 to f32: 14.9 us, 4.9 TB/s (32 bytes a thread: 16.7, and 28 past the
+// caches, half lines at a time).
+constexpr int read_each(int out) { return out == AIONHIP_F32 ? 4 : 8; }      // elements of a thread
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void cache_read_kernel(ReadPair p, const int *first, int s_len, int t_cap, int tp, int h, int d, int rolling, Tiles tiles) {
+    constexpr int E = read_each(OUT), BYTES = DT == AIONHIP_Q8_0 ? E : E / 2;
+    using Codes = std::conditional_t<BYTES == 8, unsigned long, std::conditional_t<BYTES == 4, unsigned, unsigned short>>;
+    typedef unsigned u32x4u __attribute__((ext_vector_type(4), aligned(2)));
     const Place at = place_of(tiles);
     const unsigned b = at.unit / (unsigned)h, head = at.unit - b * (unsigned)h;
     const int which = blockIdx.y, index = first[b];
     for (unsigned piece = at.piece; piece < tiles.per; piece += 256) {
-        uint2 w[ROWS_EACH];
+        Codes w[ROWS_EACH];
         float scale[ROWS_EACH];
 #pragma unroll
         for (int r = 0; r < ROWS_EACH; ++r) {
             const unsigned s = at.first + r * tiles.rows;
             const long row = s < (unsigned)s_len ? row_of((long)index + s, t_cap, rolling) : -1;
-            w[r] = DT == AIONHIP_Q8_0 ? make_uint2(0x80808080u, 0x80808080u) : make_uint2(0x88888888u, 0u);
+            w[r] = DT == AIONHIP_Q8_0 ? (Codes)0x8080808080808080ul : (Codes)0x88888888u;
             scale[r] = 0.f;
             if (row >= 0) {
-                scale[r] = __half2float(p.scales[which][((size_t)at.unit * (d / 32) + piece / 4) * tp + (size_t)row]);
-                const unsigned char *c = p.codes[which] + ((size_t)at.unit * tp + (size_t)row) * (DT == AIONHIP_Q8_0 ? d : d / 2) + piece * (DT == AIONHIP_Q8_0 ? 8 : 4);
-                if constexpr (DT == AIONHIP_Q8_0) w[r] = *(const uint2 *)c;
-                else w[r].x = *(const unsigned *)c;
+                scale[r] = __half2float(p.scales[which][((size_t)at.unit * (d / 32) + piece / (32 / E)) * tp + (size_t)row]);
+                w[r] = *(const Codes *)(p.codes[which] + ((size_t)at.unit * tp + (size_t)row) * (DT == AIONHIP_Q8_0 ? d : d / 2) + piece * BYTES);
             }
         }
 #pragma unroll
         for (int r = 0; r < ROWS_EACH; ++r) {
             const unsigned s = at.first + r * tiles.rows;
             if (s >= (unsigned)s_len) continue;
-            const size_t o_at = (((size_t)b * s_len + s) * h + head) * d + piece * 8;
-            float x[8];
+            const size_t o_at = (((size_t)b * s_len + s) * h + head) * d + piece * E;
+            float x[E];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (DT == AIONHIP_Q8_0) x[i] = (float)((int)((i < 4 ? w[r].x : w[r].y) >> (8 * (i & 3)) & 255u) - 128) * scale[r];
-                else x[i] = (float)((int)(w[r].x >> (4 * i) & 15u) - 8) * scale[r];
+            for (int i = 0; i < E; ++i) {
+                if constexpr (DT == AIONHIP_Q8_0) x[i] = (float)((int)(w[r] >> (8 * i) & 255u) - 128) * scale[r];
+                else x[i] = (float)((int)(w[r] >> (4 * i) & 15u) - 8) * scale[r];
             }
+            u32x4u o;
             if constexpr (OUT == AIONHIP_F32) {
-                __builtin_memcpy((float *)p.out[which] + o_at, x, 32);
+                __builtin_memcpy(&o, x, 16);
+                __builtin_nontemporal_store(o, (u32x4u *)((float *)p.out[which] + o_at));
             } else {
-                unsigned short o[8];
+                unsigned short half[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if (OUT == AIONHIP_F16) o[i] = __half_as_ushort(__float2half_rn(x[i]));
-                    else o[i] = __builtin_bit_cast(unsigned short, (__bf16)x[i]);
+                    if (OUT == AIONHIP_F16) half[i] = __half_as_ushort(__float2half_rn(x[i]));
+                    else half[i] = __builtin_bit_cast(unsigned short, (__bf16)x[i]);
                 }
-                __builtin_memcpy((unsigned short *)p.out[which] + o_at, o, 16);
+                __builtin_memcpy(&o, half, 16);
+                __builtin_nontemporal_store(o, (u32x4u *)((unsigned short *)p.out[which] + o_at));
             }
         }
     }
@@ -196,9 +205,9 @@ int check_shape(aionhip_ctx *ctx, const char *who, int dtype, size_t b, size_t s
     if (b && h && d && t_cap && !aionhip_cache_quant_bytes(dtype, b, t_cap, h, d)) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: size overflow", who);
     return AIONHIP_OK;
 }
-// the workgroups of `b` sequences' `h` heads with `s` rows each
-int tiles_of(aionhip_ctx *ctx, const char *who, size_t b, size_t s, size_t h, size_t d, Tiles *tiles, unsigned *grid) {
-    const size_t per = d / 8, rows = per < 256 ? 256 / per : 1, wgs = (s + rows * ROWS_EACH - 1) / (rows * ROWS_EACH);
+// the workgroups of `b` sequences' `h` heads with `s` rows of `per` threads each
+int tiles_of(aionhip_ctx *ctx, const char *who, size_t b, size_t s, size_t h, size_t per, Tiles *tiles, unsigned *grid) {
+    const size_t rows = per < 256 ? 256 / per : 1, wgs = (s + rows * ROWS_EACH - 1) / (rows * ROWS_EACH);
     if (b > 0x7FFFFFFF / h || b * h > 0x7FFFFFFF / wgs) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
     *tiles = Tiles{(unsigned)per, (unsigned)rows, (unsigned)wgs};
     *grid = (unsigned)(b * h * wgs);
@@ -233,7 +242,7 @@ int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cach
     if (overlap(k_cache, bytes, v_cache, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "append_quant: the caches of keys and values overlap");
     Tiles tiles;
     unsigned grid;
-    if ((rc = tiles_of(ctx, "append_quant", b, s, h, d, &tiles, &grid))) return rc;
+    if ((rc = tiles_of(ctx, "append_quant", b, s, h, d / 8, &tiles, &grid))) return rc;
     const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
     const Pair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k), dp<void>(v)}};
     ProfScope scope(ctx, "append_quant");
@@ -289,7 +298,7 @@ int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_
     if (overlap(k_out, out_bytes, v_out, out_bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "cache_read: the rows of keys and values overlap");
     Tiles tiles;
     unsigned grid;
-    if ((rc = tiles_of(ctx, "cache_read", b, s, h, d, &tiles, &grid))) return rc;
+    if ((rc = tiles_of(ctx, "cache_read", b, s, h, d / read_each(out_dtype), &tiles, &grid))) return rc;
     const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
     const ReadPair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k_out), dp<void>(v_out)}};
     const auto kernel = dtype == AIONHIP_Q8_0 ? (out_dtype == AIONHIP_F32 ? cache_read_kernel<AIONHIP_Q8_0, AIONHIP_F32>
