@@ -1332,11 +1332,14 @@ int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
     // One workgroup per CU. Two where the rows see half the keys on average (a prompt on its own), so that short workgroups follow long ones - but for prompts whose
     // parts take longer to merge: with 256 tiles of rows 4096 keys at D = 64 go from 187 to 142 us, 2048 at D = 128 from 158 to 151, twice 1024 from 89 to 99.
-    const long want = 2 * (long)a.L > keys && key_tiles >= 32 ? 2L * cus : cus;
-    sp.nseg = (int)max(1L, min(min(want / wgs, 16L), key_tiles / 4));
+    // Never more than the scratch memory that a recording finds there (aionhip_program_begin), so that a step has the same segments recorded or not: the 2048 keys
+    // stay in one.
+    const size_t part_bytes = (size_t)units * sp.row_tiles * Part<D, 1>::FLOATS * sizeof(float);
+    const long want = 2 * (long)a.L > keys && key_tiles >= 32 ? 2L * cus : cus, fit = (long)(prefill_added_scratch(cus) / part_bytes);
+    sp.nseg = (int)max(1L, min(min(min(want / wgs, fit), 16L), key_tiles / 4));
     if (wgs * sp.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
     if (sp.nseg > 1) {
-        if (const int rc = ensure_scratch2(ctx, (size_t)units * sp.row_tiles * sp.nseg * Part<D, 1>::FLOATS * sizeof(float))) return rc;
+        if (const int rc = ensure_scratch2(ctx, sp.nseg * part_bytes)) return rc;
         sp.parts = (float *)ctx->scratch2;
     }
     static std::atomic<uint64_t> attr{0};

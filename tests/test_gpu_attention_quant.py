@@ -381,3 +381,28 @@ def test_two_programs_of_one_context(gpu, dtype):
         gpu.program_destroy(p)
     for x in bufs + [index, lens] + [y for _, rows, back, q, out, pos in calls.values() for y in rows + back + [q, out, pos]]:
         x.free()
+
+
+@BOTH
+@pytest.mark.parametrize("l,t,hq,hk,d", [(1, 4000, 8, 1, 256), (300, 1000, 16, 8, 128), (1100, 2200, 16, 4, 64), (40, 600, 4, 4, 96)])
+def test_recorded_without_having_run(dtype, l, t, hq, hk, d):
+    fresh = be.HipBackend(0)
+    q, kc, vc = case(3, dtype, 1, l, t, hq, hk, d)
+    bufs = [fresh.upload(x) for x in (q, kc.bytes, vc.bytes)]
+    pos, lens, out = fresh.upload(np.arange(t - l, t, dtype=np.int32)), fresh.upload(np.array([t], np.int32)), fresh.zeros(q.nbytes)
+
+    def issue():
+        fresh.step_attention(out, *bufs, (1, l, t, hq, hk, d, d), 0.1, kv_dtype=dtype, query_positions=pos, kv_lengths=lens)
+
+    prog = fresh.record_program(issue)
+    want, near = attention_f64(q, kc.values(), vc.values(), 0.1, t, positions=[np.arange(t - l, t)], kv_lengths=[t])
+    for _ in range(3):
+        fresh.write(out, np.full(q.shape, np.nan, np.float32))
+        fresh.program_execute(prog)
+        got = fresh.download(out, np.float32, q.shape)
+        inside = bool((np.abs(got - want) <= bound_of(near)).all())
+        assert inside
+    issue()
+    assert np.array_equal(fresh.download(out, np.float32, q.shape), got)
+    fresh.program_destroy(prog)
+    fresh.close()
