@@ -893,7 +893,7 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 // --------------------------------------------------------------------------------------------------------------------- many query rows
 // A workgroup has ROWS query rows, 32 to a wavefront (16 at head size 256), and walks its keys a tile at a time. What bounds it is the arithmetic, so the
 // conversions are made once for all of its rows: eight wavefronts turn a tile's codes into operands in LDS around their products of the tile before it
-// (two stages, one barrier a tile; four convert first and four last, so that of the two wavefronts of a SIMD one converts while the other multiplies). The
+// (two stages, one barrier a tile; four convert first and four last, of which each SIMD has one: 377 us below against 379 and 398 where all do so first or last). The
 // tile after that is asked for between the softmax and P V, when the scores' registers are free.
 //   K: the codes as f16, exact, [block][lane group][row of a sub-tile] of 16 bytes: an operand is one read, and its scale goes onto the product (a block long).
 //     The query row is the sum of two f16, as in quant_decode_kernel.
@@ -901,7 +901,7 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 //     largest that the workgroup's rows see in that block of columns, and good to 2^-40 of it (two bf16, which need no power, were off by 2^-17: 3e-6 of
 //     an output where this is 3e-7). The largest is found first, from the scales alone, 1/32 to 1/16 of V. P is the sum of two f16 too, and of the four products
 //     the smallest, 2^-22, is left out. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
-// Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 374 us, 370 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
+// Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 377 us, 365 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
 // at 9000 keys, 8 heads on 2 of 256, q4_0: 219 us. It is bound by issue: a wavefront's tile is 160 matrix instructions and 590 others (128 scales onto products, 180
 // conversions, the softmax 280). Asking for a tile a whole round ahead cost the products their registers (428 us before), four wavefronts' operands read one product
 // ahead and higher wave priority around the products gave the rest.

@@ -18,7 +18,7 @@ import numpy as np
 import pytest
 
 from aion_amd import backend as be
-from quant_cases import attention_f64, filled
+from quant_cases import QuantCache, attention_f64, filled
 from test_gpu_attention import to_bf16
 
 pytestmark = pytest.mark.gpu
@@ -406,3 +406,38 @@ def test_recorded_without_having_run(dtype, l, t, hq, hk, d):
     assert np.array_equal(fresh.download(out, np.float32, q.shape), got)
     fresh.program_destroy(prog)
     fresh.close()
+
+
+@BOTH
+@pytest.mark.parametrize("d", [256, 128, 96])
+def test_offsets_beyond_32_bits(gpu, dtype, d):
+    """The last rows of caches of more than 4 GiB of codes: appended, read back, attended to; against the same rows in a small cache."""
+    rng = np.random.default_rng(d)
+    hq, hk, s, tail = 4, 2, 260, 300
+    t_cap = (1 << 32) // (d if dtype == be.Q8_0 else d // 2) // hk + 40000
+    size = gpu.cache_quant_bytes(dtype, 1, t_cap, hk, d)
+    bufs = [gpu.alloc(size) for _ in range(2)]
+    new = [rng.standard_normal((1, s, hk, d)).astype(np.float32) for _ in range(2)]
+    small = [QuantCache(dtype, 1, tail, hk, d) for _ in range(2)]
+    for c, x in zip(small, new):
+        c.put(x[0], 0, np.arange(tail - s, tail))
+    rows = [gpu.upload(x) for x in new]
+    index = gpu.upload(np.array([t_cap - s], np.int32))
+    gpu.step_append_quant(dtype, bufs, rows, index, (1, s, t_cap, hk, d))
+    backs = [gpu.alloc(x.nbytes) for x in new]
+    gpu.step_cache_read(dtype, backs, bufs, index, (1, s, t_cap, hk, d))
+    for o, c in zip(backs, small):
+        assert np.array_equal(gpu.download(o, np.float32, (s, hk, d)), c.values()[0, tail - s:tail].astype(np.float32))
+    for l in (1, 9, 150):
+        q = rng.standard_normal((1, l, hq, d)).astype(np.float32)
+        pos = np.arange(tail - l, tail)
+        want, near = attention_f64(q, small[0].values(), small[1].values(), 0.1, tail, window=(100, 0, 0), positions=[pos], kv_lengths=[tail])
+        up, out = gpu.upload(q), gpu.alloc(q.nbytes)
+        at, length = gpu.upload((pos + t_cap - tail).astype(np.int32)), gpu.upload(np.array([t_cap], np.int32))
+        gpu.step_attention(out, up, *bufs, (1, l, t_cap, hq, hk, d, d), 0.1, kv_dtype=dtype, window=(100, 0, 0), query_positions=at, kv_lengths=length)
+        inside = bool((np.abs(gpu.download(out, np.float32, q.shape) - want) <= bound_of(near)).all())
+        assert inside, l
+        for x in (up, out, at, length):
+            x.free()
+    for x in bufs + rows + backs + [index]:
+        x.free()
