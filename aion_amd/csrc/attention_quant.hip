@@ -335,10 +335,14 @@ __device__ __forceinline__ void merge_parts(int nseg, int first, int last, int g
 // Keys of a tile of TK: sub-tile h, row m holds key TK / 4 * (m / 4) + 4 h + m % 4, which gives the lanes 16 g .. of a result neighbouring keys, whose
 // scales are one load or two. V goes to LDS as it is and comes back transposed, eight keys of a byte at a time: of two value columns where a byte holds two.
 // P' is kept where f16 is accurate: a column's reference is its maximum minus a power of two that keeps the largest P' seen (it decays as the maximum grows)
-// between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite.
+// between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite. The shift has an end, 2^MOST_BIAS: where the keys with
+// the highest scores have values of zero (a block that f16 holds no scale of, a row of zeros), P' comes from keys far below them, and P itself, whose largest is
+// 2^bias, is what leaves f32's range first. Beyond the end P' keeps an absolute 2^-24, which is 2^-104 of the normalizer; and P, its sum and what
+// a merge takes one by the other stay finite with room (P' at most 2^96, a part that a merge loses below 2^-42 of the whole).
 // Measured (32 query heads on 8 of 128): one token over 131072 keys in 8 bits 57 us, 5.0 TB/s (a copy reaches 5.1, a read 6.8); 32 tokens over 16384 keys
 // each in 4 bits 85 us, 5.2 TB/s; one token over 531 keys of one head of 256 10.5 us, of which 4 are the launch and 3 the meeting of its segments.
 // Tiles are 64 keys, 32 at head size 256; there, and where sixteen rows share the columns, the query's operands lie in LDS as well: the registers hold no more.
+constexpr float MOST_BIAS = 80.f;
 constexpr int decode_waves(int d, int rep) { return d > 128 || (d == 128 && rep < 4) ? 2 : d == 128 || rep == 1 ? 3 : 4; }      // to a SIMD
 template <int DT, int D, int REP>
 struct DecodeCfg {
@@ -631,7 +635,7 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
         top = fmaxf(largest * alpha, groups4_max(top));
         if (__any(top > 32768.f || top < 512.f)) {
             const bool move = top > 0.f && top < INFINITY && (top > 32768.f || top < 512.f);
-            const float by = move ? (float)(139 - (int)(__float_as_uint(top) >> 23)) : 0.f;      // to 2^12 .. 2^13
+            const float by = move ? fminf((float)(139 - (int)(__float_as_uint(top) >> 23)), MOST_BIAS - bias) : 0.f;      // to 2^12 .. 2^13
             const float f = __builtin_amdgcn_exp2f(by);
             bias += by;
             top *= f;
