@@ -335,7 +335,7 @@ __device__ __forceinline__ void merge_parts(int nseg, int first, int last, int g
 // Keys of a tile of TK: sub-tile h, row m holds key TK / 4 * (m / 4) + 4 h + m % 4, which gives the lanes 16 g .. of a result neighbouring keys, whose
 // scales are one load or two. V goes to LDS as it is and comes back transposed, eight keys of a byte at a time: of two value columns where a byte holds two.
 // P' is kept where f16 is accurate: a column's reference is its maximum minus a power of two that keeps the largest P' seen (it decays as the maximum grows)
-// between 2^9 and 2^15; the low part then ends 2^-34 below it. No shift is made for a value that is not finite. The shift has an end, 2^MOST_BIAS: where the keys with
+// between 2^9 and 2^15; the low part then ends 2^-34 below it. A value that is not finite has no part in it. The shift has an end, 2^MOST_BIAS: where the keys with
 // the highest scores have values of zero (a block that f16 holds no scale of, a row of zeros), P' comes from keys far below them, and P itself, whose largest is
 // 2^bias, is what leaves f32's range first. Beyond the end P' keeps an absolute 2^-24, which is 2^-104 of the normalizer; and P, its sum and what
 // a merge takes one by the other stay finite with room (P' at most 2^96, a part that a merge loses below 2^-42 of the whole).
@@ -622,17 +622,45 @@ __global__ __launch_bounds__(NW * 64, decode_waves(D, REP)) void quant_decode_ke
         m_run = m_new;
         // -- the largest P' of the column, and the shift that keeps it in range
         auto times_scale = [&](int st, int j) __attribute__((always_inline)) { return fma_half(p[j], vsc[st][j >> 3][(j & 7) >> 1], j & 1, cst.zero); };
-        float pv[Cfg::PV_TWICE ? 1 : SETS][KG], top = 0.f, before = 0.f;
+        float pv[Cfg::PV_TWICE ? 1 : SETS][KG], top = 0.f;
+        // An infinite scale has no range to keep, the column's other blocks do: the largest is taken again without it. Where the products are not kept, after the
+        // scale has become a NaN, which no maximum takes; by the same code at head size 256 (20 rows over 9000 keys 46 us, 49 with code of its own,
+        // for want of registers).
+        constexpr int PASSES = Cfg::PV_TWICE && SETS > 1 ? 2 : 1;
+#pragma unroll D > 128 ? 1 : 2
+        for (int pass = 0; pass < PASSES; ++pass) {
+            float before = 0.f;
+            top = 0.f;
 #pragma unroll
-        for (int st = 0; st < SETS; ++st)
+            for (int st = 0; st < SETS; ++st)
 #pragma unroll
-            for (int j = 0; j < KG; ++j) {
-                const float x = times_scale(st, j);
-                if (j % 2) top = max3(top, before, x);
-                before = x;
-                if constexpr (!Cfg::PV_TWICE) pv[st][j] = x;
+                for (int j = 0; j < KG; ++j) {
+                    const float x = times_scale(st, j);
+                    if (j % 2) top = max3(top, before, x);
+                    before = x;
+                    if constexpr (!Cfg::PV_TWICE) pv[st][j] = x;
+                }
+            top = fmaxf(largest * alpha, groups4_max(top));
+            if (pass + 1 == PASSES || !__any(top == INFINITY)) break;
+#pragma unroll
+            for (int st = 0; st < SETS; ++st)
+#pragma unroll
+                for (int j = 0; j < KG; j += 2) {
+                    const unsigned w = vsc[st][j >> 3][(j & 7) >> 1];
+                    vsc[st][j >> 3][(j & 7) >> 1] = w | ((w & 0x7FFFu) == 0x7C00u ? 0x200u : 0u) | ((w >> 16 & 0x7FFFu) == 0x7C00u ? 0x2000000u : 0u);
+                }
+        }
+        if constexpr (!Cfg::PV_TWICE && SETS > 1) {
+            if (__any(top == INFINITY)) {
+                stay_branch();
+                int most = 1 << 23;                                           // bits of the largest finite one plus 2^23: what is not finite is negative or less
+#pragma unroll
+                for (int st = 0; st < SETS; ++st)
+#pragma unroll
+                    for (int j = 0; j < KG; ++j) most = max(most, (int)(__float_as_uint(pv[st][j]) + (1u << 23)));
+                top = fmaxf(largest * alpha, groups4_max(__int_as_float(most - (1 << 23))));
             }
-        top = fmaxf(largest * alpha, groups4_max(top));
+        }
         if (__any(top > 32768.f || top < 512.f)) {
             const bool move = top > 0.f && top < INFINITY && (top > 32768.f || top < 512.f);
             const float by = move ? fminf((float)(139 - (int)(__float_as_uint(top) >> 23)), MOST_BIAS - bias) : 0.f;      // to 2^12 .. 2^13

@@ -49,3 +49,27 @@ def test_the_best_key_has_no_values(gpu, dtype, d, l, t, best, second):
             want, near = attention_f64(q, kc.values(), values, d ** -0.5, t, window=be.FULL)
             inside = bool((np.abs(got - want) <= bound_of(near) + lost).all())
             assert inside, (gap, gpu.last_kernel(), float(np.abs(got - want).max()), bool(np.isfinite(got).all()))
+
+
+@BOTH
+@pytest.mark.parametrize("size", [1.0, 300.0, 1e4])
+@pytest.mark.parametrize("what", [0x7C00, 0x7E00])
+@pytest.mark.parametrize("l,d", [(1, 64), (1, 128), (1, 256), (3, 128), (3, 256), (6, 64), (7, 128), (30, 128), (30, 256), (150, 128), (150, 256), (5, 96)])
+def test_a_block_that_is_not_finite_leaves_the_others_their_range(gpu, dtype, l, d, what, size):
+    """A value that every row sees has no finite scale in one block, at the first key or at a later one; the other blocks' scales are below and above one."""
+    rng = np.random.default_rng(l + d)
+    t, hq, hk, blocks = 400, 4, 2, d // 32
+    q = rng.standard_normal((1, l, hq, d)).astype(np.float32)
+    kc, vc = filled(rng, dtype, 1, t, hk, d), filled(rng, dtype, 1, t, hk, d, size)
+    want, near = attention_f64(q, kc.values(), vc.values(), 0.1, t, window=be.FULL)
+    assert np.isfinite(want).all()                                # (scales that f16 holds)
+    for key in (0, 130):
+        for block in (0, blocks - 1):
+            held = vc.scales[0, :, block, key].copy()
+            vc.scales[0, :, block, key] = what
+            got = step(gpu, q, kc, vc, t, 0.1, window=be.FULL).reshape(1, l, hq, blocks, 32)
+            vc.scales[0, :, block, key] = held
+            others = [j for j in range(blocks) if j != block]
+            gone = not np.isfinite(got[..., block, :]).any()
+            near_enough = (np.abs(got.reshape(want.shape) - want) <= bound_of(near)).reshape(got.shape)[..., others, :].all()
+            assert gone and near_enough, (key, block, gone, gpu.last_kernel())
