@@ -28,6 +28,11 @@ size_t elems(const aionhip_tensor_ref &t) {
     return n;
 }
 bool is_quant_cache(const aionhip_tensor_ref &t) { return (t.flags & AIONHIP_TENSOR_QUANT_CACHE) && t.rank == 4 && cq::is_quant(t.dtype); }
+// neither a quantized cache, or two whose codes and scales lie at the same places
+bool same_layout(const aionhip_tensor_ref &a, const aionhip_tensor_ref &b) {
+    if (!is_quant_cache(a) || !is_quant_cache(b)) return !is_quant_cache(a) && !is_quant_cache(b);
+    return a.shape[0] == b.shape[0] && cq::padded(a.shape[1]) == cq::padded(b.shape[1]) && a.shape[2] == b.shape[2] && a.shape[3] == b.shape[3];
+}
 // bytes of a tensor as aion stores it: 34 / 18 bytes per 32 elements for the block formats (backend/types.zig:41-59), and of a quantized cache
 size_t bytes_of(const aionhip_tensor_ref &t) {
     const size_t n = elems(t);
@@ -194,6 +199,14 @@ int aionhip_session::check(size_t i, const aionhip_step &st) {
     if (st.out.rank > AIONHIP_MAX_RANK) return bad("rank above 8");
     for (int j = 0; j < 5; ++j)
         if (st.in[j].rank > AIONHIP_MAX_RANK) return bad("rank above 8");
+    // a quantized cache has a layout of its own: what expects aion's blocks would read codes as scales
+    for (int j = -1; j < 5; ++j) {
+        const aionhip_tensor_ref &t = j < 0 ? st.out : st.in[j];
+        if (!t.handle || !(t.flags & AIONHIP_TENSOR_QUANT_CACHE)) continue;
+        if (!is_quant_cache(t)) return bad("a quantized cache is [B, T, H, D] of q8_0 or q4_0");
+        const bool held = st.tag == AIONHIP_STEP_ATTENTION ? j == 1 || j == 2 : st.tag == AIONHIP_STEP_SEQUENCE_APPEND ? j < 0 : st.tag == AIONHIP_STEP_COPY || st.tag == AIONHIP_STEP_TRANSFER;
+        if (!held) return bad("a quantized cache is the cache of an Attention or a SequenceAppend, or copied or transferred whole");
+    }
     switch (st.tag) {
     case AIONHIP_STEP_MATMUL:
     case AIONHIP_STEP_MATMUL_NT: {
@@ -274,6 +287,7 @@ int aionhip_session::check(size_t i, const aionhip_step &st) {
     case AIONHIP_STEP_COPY:
         if (bytes_of(st.out) == 0 && elems(st.out) != 0) return unsupported("Copy: an element type this device does not hold");
         if (!st.in[0].handle || !st.out.handle || bytes_of(st.in[0]) != bytes_of(st.out) || st.in[0].dtype != st.out.dtype) return bad("Copy: src and dst of one type and size");
+        if (!same_layout(st.in[0], st.out)) return bad("Copy: a quantized cache goes to one of the same shape");
         return AIONHIP_OK;
     case AIONHIP_STEP_GATHER:
         if (st.axis != 0 || st.batch_dims != 0) return unsupported("Gather: axis 0 without batch dims");

@@ -483,7 +483,8 @@ void aionhip_program_destroy(aionhip_ctx *ctx, aionhip_program *prog);
  * (backend/backend.zig:85-107). */
 #define AIONHIP_MAX_RANK 8
 enum { AIONHIP_TENSOR_ROLLING = 1u,    /* a rolling sequence cache (storage/cache.zig:35-38) */
-       AIONHIP_TENSOR_QUANT_CACHE = 4u, /* [B,T,H,D] of a block type: a cache as aionhip_cache_quant_bytes lays it out, T its capacity */
+       AIONHIP_TENSOR_QUANT_CACHE = 4u, /* [B,T,H,D] of a block type: a cache as aionhip_cache_quant_bytes lays it out, T its capacity. An operand of
+                                          Attention (k, v) and SequenceAppend (out), or of a Copy (both sides, one shape) or Transfer; refused elsewhere */
        AIONHIP_TENSOR_WORKSPACE = 2u   /* lives in a planned workspace slot (graph/program/workspace.zig:1-60): nothing reads
                                           its value after the last step of this list that does */ };
 typedef struct aionhip_tensor_ref {
