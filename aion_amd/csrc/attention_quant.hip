@@ -1410,8 +1410,11 @@ int run_attention_quant(aionhip_ctx *ctx, const aionhip_attention *p) {
     if (p->d_k % 32 != 0 || p->d_v % 32 != 0) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: head sizes over a quantized cache are multiples of 32");
     if (p->d_k > GENERIC_HEAD || p->d_v > GENERIC_HEAD) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: head sizes above %d over a quantized cache", GENERIC_HEAD);
     if ((p->k | p->v) & 15) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: a quantized cache begins at a multiple of 16 bytes");
-    if (p->t_kv && (!aionhip_cache_quant_bytes(p->kv_dtype, p->batch, p->t_kv, p->h_kv, p->d_k) || !aionhip_cache_quant_bytes(p->kv_dtype, p->batch, p->t_kv, p->h_kv, p->d_v)))
-        return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
+    const size_t k_bytes = aionhip_cache_quant_bytes(p->kv_dtype, p->batch, p->t_kv, p->h_kv, p->d_k), v_bytes = aionhip_cache_quant_bytes(p->kv_dtype, p->batch, p->t_kv, p->h_kv, p->d_v);
+    if (!k_bytes || !v_bytes) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention: dimension too large");
+    const aionhip_handle out_end = p->out + p->batch * p->l_q * p->h_q * p->d_v * sizeof(float);
+    if ((p->out < p->k + k_bytes && p->k < out_end) || (p->out < p->v + v_bytes && p->v < out_end))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention: the output lies in a quantized cache of the call");
     QuantArgs a{};
     a.q = (const void *)(uintptr_t)p->q;
     a.out = (float *)(uintptr_t)p->out;

@@ -4,7 +4,9 @@
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 namespace {
 using namespace cq;
@@ -214,6 +216,13 @@ int tiles_of(aionhip_ctx *ctx, const char *who, size_t b, size_t s, size_t h, si
     return AIONHIP_OK;
 }
 bool overlap(aionhip_handle a, size_t a_bytes, aionhip_handle b, size_t b_bytes) { return a && b && a < b + b_bytes && b < a + a_bytes; }
+// rows that are read or written while the caches are written or read lie outside of both
+int check_rows(aionhip_ctx *ctx, const char *who, std::initializer_list<std::pair<aionhip_handle, size_t>> rows, aionhip_handle k_cache, aionhip_handle v_cache, size_t cache_bytes) {
+    for (const auto &r : rows)
+        if (overlap(r.first, r.second, k_cache, cache_bytes) || overlap(r.first, r.second, v_cache, cache_bytes))
+            return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: rows lie in a cache of the call", who);
+    return AIONHIP_OK;
+}
 int check_cache(aionhip_ctx *ctx, const char *who, aionhip_handle c) {
     return c & 15 ? set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: a cache begins at a multiple of 16 bytes", who) : AIONHIP_OK;
 }
@@ -243,6 +252,8 @@ int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cach
     Tiles tiles;
     unsigned grid;
     if ((rc = tiles_of(ctx, "append_quant", b, s, h, d / 8, &tiles, &grid))) return rc;
+    const size_t row_bytes = b * s * h * d * (src_dtype == AIONHIP_F32 ? 4 : 2);
+    if ((rc = check_rows(ctx, "append_quant", {{k, row_bytes}, {v, row_bytes}}, k_cache, v_cache, bytes))) return rc;
     const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
     const Pair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k), dp<void>(v)}};
     ProfScope scope(ctx, "append_quant");
@@ -271,6 +282,7 @@ int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q
     const size_t q_bytes = b * s * h_q * d * sizeof(float), kv_bytes = b * s * h_kv * d * sizeof(float);
     if (overlap(q_out, q_bytes, q, q_bytes) || overlap(q_out, q_bytes, k, kv_bytes) || overlap(q_out, q_bytes, v, kv_bytes))
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rope_append_quant: q, k and v are still read while q_out is written");
+    if ((rc = check_rows(ctx, "rope_append_quant", {{q_out, q_bytes}, {q, q_bytes}, {k, kv_bytes}, {v, kv_bytes}}, k_cache, v_cache, bytes))) return rc;
     size_t rope_pairs = (size_t)floorf(rope_proportion * (float)half);
     if (rope_pairs > half) rope_pairs = half;
     const float freq_step = (float)pow((double)base_frequency, (double)(-2.0f / (float)d));
@@ -299,6 +311,7 @@ int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_
     Tiles tiles;
     unsigned grid;
     if ((rc = tiles_of(ctx, "cache_read", b, s, h, d / read_each(out_dtype), &tiles, &grid))) return rc;
+    if ((rc = check_rows(ctx, "cache_read", {{k_out, out_bytes}, {v_out, out_bytes}}, k_cache, v_cache, aionhip_cache_quant_bytes(dtype, b, t_cap, h, d)))) return rc;
     const Cache kc = view(k_cache, dtype, b, t_cap, h, d), vc = v_cache ? view(v_cache, dtype, b, t_cap, h, d) : kc;
     const ReadPair p{{kc.codes, vc.codes}, {kc.scales, vc.scales}, {dp<void>(k_out), dp<void>(v_out)}};
     const auto kernel = dtype == AIONHIP_Q8_0 ? (out_dtype == AIONHIP_F32 ? cache_read_kernel<AIONHIP_Q8_0, AIONHIP_F32>

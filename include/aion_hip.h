@@ -341,16 +341,17 @@ size_t aionhip_cache_quant_bytes(int dtype, size_t b, size_t t_cap, size_t h, si
 /* StepSequenceAppend into such caches, the quantization included: rows k (and v; v_cache and v may both be 0) [B,S,H,D] of src_dtype F32, F16 or BF16 go to
  * token index write_index[b] .. +S (i32 [B] on device) as aionhip_step_append_f16 places them: rolling = 1 to row t % t_cap; a row outside of a linear cache
  * is not written. An infinity or a NaN makes its block of 32 read back as NaN; a block whose scale f16 does not hold (values past 65504 * 127 or * 7) reads back
- * as not finite either. The two caches do not overlap. */
+ * as not finite either. The two caches do not overlap, and no rows lie in them. */
 int aionhip_step_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle k_cache, aionhip_handle k, aionhip_handle v_cache, aionhip_handle v, int src_dtype,
                               aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling);
 /* aionhip_step_rope_append over such caches (rolling = 1: rings): RoPE1D on q and k, quantization and append of k and v as one launch, the
- * bits of aionhip_step_rope followed by aionhip_step_append_quant. q_out overlaps none of q, k and v. */
+ * bits of aionhip_step_rope followed by aionhip_step_append_quant. q_out overlaps none of q, k and v, and none of the four lies in a cache. */
 int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q_out, aionhip_handle q, aionhip_handle k, aionhip_handle v, aionhip_handle k_cache,
                                    aionhip_handle v_cache, aionhip_handle positions, aionhip_handle write_index, size_t b, size_t s, size_t t_cap, size_t h_q, size_t h_kv,
                                    size_t d, float base_frequency, float scale_factor, float rope_proportion, int rolling);
 /* Rows back out of such caches: out [B,S,H,D] of out_dtype F32, F16 or BF16 = the elements of steps first[b] .. +S (i32 [B] on device), of k_cache and, unless v_out
- * and v_cache are both 0, of v_cache; rolling = 1: step t is in row t % t_cap. Steps before the first, or past the end of a linear cache, read as zeros. */
+ * and v_cache are both 0, of v_cache; rolling = 1: step t is in row t % t_cap. Steps before the first, or past the end of a linear cache, read as zeros. The rows
+ * do not lie in the caches. */
 int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_handle k_out, aionhip_handle k_cache, aionhip_handle v_out, aionhip_handle v_cache,
                             aionhip_handle first, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling);
 /* StepSequenceAppend as the step itself (runtime/executable.zig:193-206, cpu/exec/sequence_append.zig:12-104): cache
