@@ -340,7 +340,7 @@ __device__ __forceinline__ void merge_parts(int nseg, int first, int last, int g
 // 2^bias, is what leaves f32's range first. Beyond the end P' keeps an absolute 2^-24, which is 2^-104 of the normalizer; and P, its sum and what
 // a merge takes one by the other stay finite with room (P' at most 2^96, a part that a merge loses below 2^-42 of the whole).
 // Measured (32 query heads on 8 of 128): one token over 131072 keys in 8 bits 57 us, 5.0 TB/s (a copy reaches 5.1, a read 6.8); 32 tokens over 16384 keys
-// each in 4 bits 85 us, 5.2 TB/s; one token over 531 keys of one head of 256 10.5 us, of which 4 are the launch and 3 the meeting of its segments.
+// each in 4 bits 85 us, 5.2 TB/s; one token over 531 keys of one head of 256 11.1 us, of which 4 are the launch and 3 the meeting of its segments.
 // Tiles are 64 keys, 32 at head size 256; there, and where sixteen rows share the columns, the query's operands lie in LDS as well: the registers hold no more.
 constexpr float MOST_BIAS = 80.f;
 constexpr int decode_waves(int d, int rep) { return d > 128 || (d == 128 && rep < 4) ? 2 : d == 128 || rep == 1 ? 3 : 4; }      // to a SIMD
@@ -925,7 +925,7 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 // --------------------------------------------------------------------------------------------------------------------- many query rows
 // A workgroup has ROWS query rows, 32 to a wavefront (16 at head size 256), and walks its keys a tile at a time. What bounds it is the arithmetic, so the
 // conversions are made once for all of its rows: eight wavefronts turn a tile's codes into operands in LDS around their products of the tile before it
-// (two stages, one barrier a tile; four convert first and four last, of which each SIMD has one: 377 us below against 379 and 398 where all do so first or last). The
+// (two stages, one barrier a tile; four convert first and four last, of which each SIMD has one: 377 us against 379 and 398 where all do so first or last). The
 // tile after that is asked for between the softmax and P V, when the scores' registers are free.
 //   K: the codes as f16, exact, [block][lane group][row of a sub-tile] of 16 bytes: an operand is one read, and its scale goes onto the product (a block long).
 //     The query row is the sum of two f16, as in quant_decode_kernel.
@@ -933,8 +933,9 @@ int launch_decode_rows(aionhip_ctx *ctx, const QuantArgs &a) {
 //     largest that the workgroup's rows see in that block of columns, and good to 2^-40 of it (two bf16, which need no power, were off by 2^-17: 3e-6 of
 //     an output where this is 3e-7). The largest is found first, from the scales alone, 1/32 to 1/16 of V. P is the sum of two f16 too, and of the four products
 //     the smallest, 2^-22, is left out. Eight keys of a byte come by a transposing read; the exchange is a wavefront's own.
-// Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 377 us, 365 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
-// at 9000 keys, 8 heads on 2 of 256, q4_0: 219 us. It is bound by issue: a wavefront's tile is 160 matrix instructions and 590 others (128 scales onto products, 180
+// Measured: 4096 tokens, 32 heads on 8 of 128, q8_0: 333 us, 413 TFLOP/s (of the products as formulas write them; the matrix cores make five for two); 2 x 500 tokens
+// at 9000 keys, 8 heads on 2 of 256, q4_0: 191 us and 8.5 for the merge. (After 0.3 s of passes. The forms compared here had twenty passes each, with the clock
+// still rising: 377 us as it is.) It is bound by issue: a wavefront's tile is 160 matrix instructions and 590 others (128 scales onto products, 180
 // conversions, the softmax 280). Asking for a tile a whole round ahead cost the products their registers (428 us before), four wavefronts' operands read one product
 // ahead and higher wave priority around the products gave the rest.
 // A scale that is not finite would reach rows that do not see its key (0 * NaN), as would one that none of the rows sees and that the power of two takes past f16:
@@ -1363,9 +1364,9 @@ int launch_prompt(aionhip_ctx *ctx, const QuantArgs &a) {
     if (a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + Cfg::TK);
     const long key_tiles = (keys + Cfg::TK - 1) / Cfg::TK;
     // One workgroup per CU. Two where the rows see half the keys on average (a prompt on its own), so that short workgroups follow long ones - but for prompts whose
-    // parts take longer to merge: with 256 tiles of rows 4096 keys at D = 64 go from 187 to 142 us, 2048 at D = 128 from 158 to 151, twice 1024 from 89 to 99.
-    // Never more than the scratch memory that a recording finds there (aionhip_program_begin), so that a step has the same segments recorded or not: the 2048 keys
-    // stay in one.
+    // parts take longer to merge: with 256 tiles of rows 4096 keys at D = 64 go from 187 to 142 us, twice 1024 at D = 128 would go from 89 to 99.
+    // Never more than the scratch memory that a recording finds there (aionhip_program_begin), so that a step has the same segments recorded or not. That keeps 2048
+    // keys at D = 128 in one segment, 158 us, where two took 151.
     const size_t part_bytes = (size_t)units * sp.row_tiles * Part<D, 1>::FLOATS * sizeof(float);
     const long want = 2 * (long)a.L > keys && key_tiles >= 32 ? 2L * cus : cus, fit = (long)(prefill_added_scratch(cus) / part_bytes);
     sp.nseg = (int)max(1L, min(min(min(want / wgs, fit), 16L), key_tiles / 4));

@@ -30,7 +30,7 @@ inline Cache view(aionhip_handle cache, int dtype, size_t b, size_t t_cap, size_
 }
 
 // Eight elements of a block held by each of four neighbouring lanes. The arithmetic is the block quantizers' (quant.hip) but for one step: the scale is the
-// maximum times the f32 nearest to 1 / 127 (1 / 7), a product in place of a quotient, which may differ in its last f32 bit and so, once in some thousand blocks, by the
+// maximum times the f32 nearest to 1 / 127 (1 / 7), a product in place of a quotient, which may differ in its last f32 bit and so, in one block of 15 000 (q4_0) or 3 million (q8_0), by the
 // last bit of the f16. q8_0 codes go by the scale as it is stored, q4_0 codes by the scale before it is rounded, halves are rounded away from zero. A block that holds an infinity or a NaN gets
 // a NaN as its scale, so that reading it back says so: a maximum alone would drop the NaN and store a number in its place.
 template <int DT>

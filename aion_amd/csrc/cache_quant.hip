@@ -70,7 +70,7 @@ __device__ __forceinline__ Place place_of(const Tiles &t) {
 }
 
 // SequenceAppend with the quantization in it: four threads hold a block. 8000 tokens of 8 heads of 128, k and v, f32 to
-// q4_0: 16.0 us, 4.7 TB/s of 5.1 that a copy reaches (one token to a thread 17.3, four 19.0).
+// q4_0: 15.7 us, 4.8 TB/s of 5.1 that a copy reaches (twenty passes from rest 16.7; one token to a thread 17.3, four 19.0).
 template <int DT>
 __global__ __launch_bounds__(256) void append_quant_kernel(Pair p, const int *write_index, int src_dtype, int s_len, int t_cap, int tp, int h, int d, int rolling, Tiles tiles) {
     const Place at = place_of(tiles);
@@ -93,6 +93,7 @@ __global__ __launch_bounds__(256) void append_quant_kernel(Pair p, const int *wr
 
 // RoPE1D on q and k, and the append of k and v, for the tokens of one step: a thread holds eight elements of one head of one token. What it rotates
 // with lies half a head away, in another thread, and is read a second time rather than exchanged. The bits of aionhip_step_rope and aionhip_step_append_quant.
+// 4096 tokens, 32 + 8 + 8 heads of 128, q4_0: 39.9 us, 4.3 TB/s, the second reading not counted; one token 3.9 us, the launch and two loads that wait for each other.
 template <int DT>
 __global__ __launch_bounds__(256) void rope_append_quant_kernel(float *q_out, const float *q, const float *k, const float *v, Cache kc, Cache vc, const int *positions,
                                                                 const int *write_index, int s_len, int t_cap, int tp, int h_q, int h_kv, int d, int rope_pairs,
@@ -144,9 +145,9 @@ struct ReadPair {
 
 // Rows first[b] .. first[b] + s_len - 1 as numbers; a row that the cache does not hold is zeros. The product of a code and a scale is exact in f32 and rounded once.
 // A thread has sixteen bytes of the result, so that a wavefront's store is whole lines, which pass the caches by: they would push out what is read.
-// 4 x 16000 tokens of 8 heads of 128, q4_0 to f16: 28.3 us, 5.9 TB/s (41.5 through the caches; there 45.7 with one token to a thread, and 58 with the threads in the
-// result's order, where a workgroup has two bytes of each scale line). 8000 tokens of k and v, q4_0 to f32: 14.9 us, 4.9 TB/s (32 bytes a thread: 16.7, and 28 past the
-// caches, half lines at a time).
+// 4 x 16000 tokens of 8 heads of 128, q4_0 to f16: 25.8 us, 6.5 TB/s (twenty passes from rest 28.3; 41.5 through the caches; there 45.7 with one token to a thread, and 58
+// with the threads in the result's order, where a workgroup has two bytes of each scale line). 8000 tokens of k and v, q4_0 to f32: 14.8 us, 5.1 TB/s (32 bytes a thread:
+// 16.7, and 28 past the caches, half lines at a time).
 constexpr int read_each(int out) { return out == AIONHIP_F32 ? 4 : 8; }      // elements of a thread
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void cache_read_kernel(ReadPair p, const int *first, int s_len, int t_cap, int tp, int h, int d, int rolling, Tiles tiles) {
