@@ -256,9 +256,9 @@ typedef struct aionhip_attention {
     int q_dtype;   /* F32 | F16 | BF16 */
     int kv_dtype;  /* F32 | F16 | BF16, or Q8_0 | Q4_0: caches as aionhip_cache_quant_bytes describes them (t_kv = their capacity,
                     * head sizes multiples of 32 up to 1024). Such a step keeps f32 accuracy (about 1e-6, and 5e-8 of a soft cap), whatever
-                   * aionhip_set_attention_precise says. What a row gets from keys whose probabilities lie far below its largest one, which shows where
-                   * the keys before them have values of zero, is held to 2^-104 of the largest (long prompts: 2^-31); in long prompts values below 2^-20 of
-                   * the largest that up to 256 neighbouring rows see in the same 32 columns keep fewer bits, down to 2^-40 of it. */
+                    * aionhip_set_attention_precise says. What a row gets from keys whose probabilities lie far below its largest one, which shows where
+                    * the keys above them have values of zero, is held to 2^-104 of that one (long prompts: 2^-31); in long prompts values below 2^-20 of
+                    * the largest that up to 256 neighbouring rows see in the same 32 columns keep fewer bits, down to 2^-40 of it. */
     float scale, attn_logits_soft_cap;
     uint32_t window_left, window_right, window_chunk;
     /* 1: k and v are rolling caches (storage/cache.zig:35-38, 202-207): logical key t lives in row t % T,
