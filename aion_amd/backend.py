@@ -15,6 +15,7 @@ from .hip import (BF16, F16, F32, GEMM_BF16_MFMA, GEMM_BF16_MFMA_ALWAYS, GEMM_EX
                   AionHipError)
 
 BLOCK_BYTES = {Q4_0: 18, Q8_0: 34}
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BANDS, ROTARY_RAMP = range(4)
 CAUSAL = (UNBOUNDED, 0, 0)
 FULL = (UNBOUNDED, UNBOUNDED, 0)
 
@@ -40,6 +41,21 @@ def _pair(buffers):
     if not 1 <= len(buffers) <= 2:
         raise AionHipError(hip.INVALID_ARGUMENT, "%d buffers: one of keys, or one of keys and one of values" % len(buffers))
     return buffers[0].handle, buffers[1].handle if len(buffers) == 2 else 0
+
+
+def Rotary(dims, base=10000.0, interleaved=False, scaling=ROTARY_PLAIN, factor=1.0, original_length=0.0, low=0.0, high=0.0, magnitude=1.0):
+    """How rows turn with their positions (aionhip_rotary): made once, handed to the steps."""
+    return hip.Rotary(dims, 1 if interleaved else 0, scaling, base, factor, original_length, low, high, magnitude)
+
+
+class PagedCache:
+    """A cache in pages (aionhip_paged_cache): two pools, a page table, and their shape. The buffers stay the caller's."""
+
+    def __init__(self, k_pages, v_pages, page_table, pages, batch, width, page_rows, h_kv, d, dtype):
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.desc = hip.PagedCache(k_pages.handle, v_pages.handle, page_table.handle, pages, batch, width, page_rows, h_kv, d, dtype)
+        self.ref = C.byref(self.desc)
+        self.capacity = width * page_rows
 
 
 class DeviceBuffer:
@@ -453,6 +469,42 @@ class HipBackend:
         """Steps first[b] .. +s of one or two quantised caches (lists of buffers) as rows [b, s, h, d]; shape = (b, s, t_cap, h, d)."""
         (ko, vo), (kc, vc) = _pair(outs), _pair(caches)
         self._check(self._lib.aionhip_step_cache_read(self._ctx, dtype, out_dtype, ko, kc, vo, vc, first.handle, *shape, 1 if rolling else 0))
+
+    def paged_cache(self, k_pages, v_pages, page_table, pages, batch, width, page_rows, h_kv, d, dtype=F16):
+        """Pools [pages, h_kv, page_rows, d] of keys and values and a table i32 [batch, width] as one cache."""
+        return PagedCache(k_pages, v_pages, page_table, pages, batch, width, page_rows, h_kv, d, dtype)
+
+    def step_rotary(self, out, x, positions, b, t, h, d, rotary, dtype=F32):
+        """Rows [b, t, h, d] turned by their positions (i32 [b, t]); out may be x."""
+        self._check(self._lib.aionhip_step_rotary(self._ctx, out.handle, x.handle, positions.handle, dtype, b, t, h, d, C.byref(rotary)))
+
+    def step_append_paged(self, cache, k, v, write_index, s, src_dtype=F32):
+        """Rows k, v [b, s, h_kv, d] to steps write_index[b] .. +s of their sequences' pages."""
+        self._check(self._lib.aionhip_step_append_paged(self._ctx, cache.ref, k.handle, v.handle, src_dtype, write_index.handle, s))
+
+    def step_rotary_append_paged(self, cache, rotary, q_out, q, k, v, positions, write_index, s, h_q, dtype=F32):
+        """step_rotary on q and k and step_append_paged of k and v, one launch."""
+        self._check(self._lib.aionhip_step_rotary_append_paged(self._ctx, cache.ref, C.byref(rotary), q_out.handle, q.handle, k.handle, v.handle, dtype, positions.handle,
+                                                               write_index.handle, s, h_q))
+
+    def step_read_paged(self, cache, k_out, v_out, first, s, out_dtype=F32):
+        """Steps first[b] .. +s of a cache in pages as rows [b, s, h_kv, d]."""
+        self._check(self._lib.aionhip_step_read_paged(self._ctx, cache.ref, k_out.handle, v_out.handle, out_dtype, first.handle, s))
+
+    def step_attention_paged(self, out, q, cache, l_q, h_q, scale, q_dtype=F32, window=CAUSAL, soft_cap=0.0, query_positions=None, kv_lengths=None, weights=None, weights_before=None):
+        """step_attention over pages. weights f32 [b, h_kv, capacity] = weights_before (None: zeros; may be the same buffer) + what each key's probabilities add up to."""
+        c = cache.desc
+        p = hip.Attention(out.handle, q.handle, 0, 0, query_positions.handle if query_positions is not None else 0, kv_lengths.handle if kv_lengths is not None else 0,
+                          c.batch, l_q, cache.capacity, h_q, c.h_kv, c.d, c.d, q_dtype, c.dtype, scale, soft_cap, window[0], window[1], window[2], 0)
+        self._check(self._lib.aionhip_step_attention_paged(self._ctx, C.byref(p), cache.ref, weights_before.handle if weights_before is not None else 0,
+                                                           weights.handle if weights is not None else 0))
+
+    def step_evict_paged(self, cache, weights, kv_lengths, weights_out, lengths_out, keep, limit=None, first=0, recent=0, table_out=None, width_out=0, kept=None):
+        """Sequences of more than `limit` (None: keep) rows keep `keep` of them: the `first` oldest, the `recent` newest, the ones of greatest weight between. table_out
+        None: in place; else the kept rows are copied to its pages. kept i32 [b, h_kv, limit]: the steps they were."""
+        e = hip.Eviction(weights.handle, kv_lengths.handle, weights_out.handle, lengths_out.handle, table_out.handle if table_out is not None else 0,
+                         kept.handle if kept is not None else 0, width_out, keep if limit is None else limit, keep, first, recent)
+        self._check(self._lib.aionhip_step_evict_paged(self._ctx, cache.ref, C.byref(e)))
 
     def cache_grow(self, dst, src, outer, old_run_bytes, new_run_bytes):
         """dst [outer, new_run_bytes] <- the runs of src [outer, old_run_bytes], zero elsewhere (storage/manager/grow.zig:37-78)."""

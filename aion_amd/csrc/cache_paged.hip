@@ -1,0 +1,376 @@
+// Rows turned by their positions, written to caches in pages and read back (the layout: cache_paged.h). One pass over the data each; what a call
+// of a few rows costs is its launch, what one of many rows costs is memory.
+#include "cache_paged.h"
+
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+namespace {
+using namespace paged;
+
+template <typename T> T *dp(aionhip_handle h) { return reinterpret_cast<T *>((uintptr_t)h); }
+
+template <int DT> struct Elem { using T = unsigned short; };
+template <> struct Elem<AIONHIP_F32> { using T = float; };
+
+template <int DT>
+__device__ __forceinline__ float to_f32(typename Elem<DT>::T x) {
+    if constexpr (DT == AIONHIP_F32) return x;
+    else if constexpr (DT == AIONHIP_F16) return __half2float(__ushort_as_half(x));
+    else return __uint_as_float((unsigned)x << 16);
+}
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T from_f32(float x) {
+    if constexpr (DT == AIONHIP_F32) return x;
+    else if constexpr (DT == AIONHIP_F16) return __half_as_ushort(__float2half_rn(x));
+    else return __builtin_bit_cast(unsigned short, (__bf16)x);
+}
+// N neighbouring elements, n of them there, of any alignment their type allows (global memory takes wide accesses at any address)
+template <int DT, int N>
+__device__ __forceinline__ void load_n(const void *src, size_t i, int n, float (&x)[N]) {
+    typename Elem<DT>::T h[N];
+    const auto *p = (const typename Elem<DT>::T *)src + i;
+    if (n == N) {
+        __builtin_memcpy(h, p, sizeof h);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = j < n ? p[j] : typename Elem<DT>::T(0);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = to_f32<DT>(h[j]);
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_n(void *dst, size_t i, int n, const float (&x)[N]) {
+    typename Elem<DT>::T h[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) h[j] = from_f32<DT>(x[j]);
+    auto *p = (typename Elem<DT>::T *)dst + i;
+    if (n == N) {
+        __builtin_memcpy(p, h, sizeof h);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < n) p[j] = h[j];
+    }
+}
+
+// Sine and cosine of an angle given as a fraction of a turn, 2^64 to the whole: the nearest quarter turn is taken off in integers, what is left, up to an eighth
+// of a turn, is exact to 2^-32 and goes into the two power series (cut where the next term is below 2e-9).
+__device__ __forceinline__ void sincos_turn(unsigned long turn, float &sn, float &cs) {
+    const unsigned t = (unsigned)(turn >> 32), quarter = (t + 0x20000000u) >> 30;
+    const float x = (float)(int)(t - (quarter << 30)) * 1.4629180792671596e-9f;            // 2 pi / 2^32
+    const float z = x * x;
+    const float s = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
+    const float c = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+    const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+    sn = quarter & 2 ? -a : a;
+    cs = (quarter + 1) & 2 ? -b : b;
+}
+
+// A thread has E pairs, or 2 E elements that stay, of HEADS heads of one token: the angles are computed once for all of them. A head's elements are dealt out as
+// `turning` pieces of pairs, then pieces of those that stay; the threads of a workgroup lie over pieces, then heads.
+struct Rotate {
+    void *q_out;
+    const void *q, *k, *v;
+    const int *positions, *write_index;
+    const unsigned long *turns;           // a pair's fraction of a turn a position
+    float magnitude;
+    int dims, interleaved, d, h_q, h_kv, s_len;
+    int pieces, turning, heads_wg;        // of a head; of those that turn; heads side by side in a workgroup
+    Table table;
+    unsigned char *k_pages, *v_pages;
+};
+constexpr int pairs_each(int dt) { return dt == AIONHIP_F32 ? 4 : 8; }
+
+template <int DT, int CT, int HEADS>
+__global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
+    constexpr int E = pairs_each(DT);
+    const int slot0 = (int)threadIdx.x / a.pieces, piece = (int)threadIdx.x - slot0 * a.pieces;
+    if (slot0 >= a.heads_wg) return;
+    const size_t tok = blockIdx.x;
+    const int slots = a.h_q + 2 * a.h_kv, first = (int)blockIdx.y * a.heads_wg * HEADS + slot0;
+    const int half = a.dims >> 1;
+    const bool turns = piece < a.turning;
+    // the thread's two runs of elements of a head
+    int lo, hi, n_lo, n_hi;
+    if (turns && !a.interleaved) {
+        lo = piece * E, hi = half + lo;
+        n_lo = n_hi = min(E, half - lo);
+    } else {
+        const int end = turns ? a.dims : a.d;
+        lo = turns ? piece * 2 * E : a.dims + (piece - a.turning) * 2 * E, hi = lo + E;
+        n_lo = min(E, end - lo), n_hi = max(0, min(E, end - hi));
+    }
+    // what the heads need is asked for before the first of them is used
+    float x[HEADS][2][E];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int slot = first + i * a.heads_wg;
+        if (slot >= slots) break;
+        const bool is_q = slot < a.h_q, is_v = slot >= a.h_q + a.h_kv;
+        const void *src = is_q ? a.q : is_v ? a.v : a.k;
+        const size_t at = is_q ? (tok * a.h_q + slot) * a.d : (tok * a.h_kv + (slot - a.h_q - (is_v ? a.h_kv : 0))) * a.d;
+        load_n<DT, E>(src, at + lo, n_lo, x[i][0]);
+        load_n<DT, E>(src, at + hi, n_hi, x[i][1]);
+    }
+    float sn[E], cs[E];
+    if (turns) {
+        const int pos = a.positions[tok], pair0 = piece * E;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            sincos_turn(a.turns[min(pair0 + j, half - 1)] * (unsigned long)(long)pos, sn[j], cs[j]);
+            sn[j] *= a.magnitude;
+            cs[j] *= a.magnitude;
+        }
+    }
+    int page = -1, row = 0;
+    size_t seq = 0;
+    if (a.write_index) {
+        seq = tok / (unsigned)a.s_len;
+        const long step = (long)a.write_index[seq] + (long)(tok - seq * (unsigned)a.s_len);
+        page = step >= 0 && step < (long)MAX_ROWS ? page_of(a.table, seq, (int)step) : -1;
+        row = (int)step & ((1 << a.table.shift) - 1);
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        const int slot = first + i * a.heads_wg;
+        if (slot >= slots) break;
+        const bool is_q = slot < a.h_q, is_v = slot >= a.h_q + a.h_kv;
+        float(&l)[E] = x[i][0], (&h)[E] = x[i][1];
+        if (turns && !is_v) {
+            if (a.interleaved) {
+                float y[2 * E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) y[j] = l[j], y[E + j] = h[j];
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const float p = y[2 * j], r = y[2 * j + 1];
+                    y[2 * j] = p * cs[j] - r * sn[j];
+                    y[2 * j + 1] = p * sn[j] + r * cs[j];
+                }
+#pragma unroll
+                for (int j = 0; j < E; ++j) l[j] = y[j], h[j] = y[E + j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const float p = l[j], r = h[j];
+                    l[j] = p * cs[j] - r * sn[j];
+                    h[j] = p * sn[j] + r * cs[j];
+                }
+            }
+        }
+        if (is_q) {
+            const size_t at = (tok * a.h_q + slot) * a.d;
+            store_n<DT, E>(a.q_out, at + lo, n_lo, l);
+            store_n<DT, E>(a.q_out, at + hi, n_hi, h);
+        } else if (page >= 0) {
+            const int head = slot - a.h_q - (is_v ? a.h_kv : 0);
+            const size_t at = ((((size_t)page * a.h_kv + head) << a.table.shift) + row) * a.d;
+            store_n<CT, E>(is_v ? a.v_pages : a.k_pages, at + lo, n_lo, l);
+            store_n<CT, E>(is_v ? a.v_pages : a.k_pages, at + hi, n_hi, h);
+        }
+    }
+}
+
+struct ReadArgs {
+    const unsigned char *pages[2];
+    void *out[2];
+    const int *first;
+    Table table;
+    int s_len, h, d;
+};
+// Rows back as numbers: a thread has eight elements of a row.
+template <int CT, int OUT>
+__global__ __launch_bounds__(256) void read_paged_kernel(ReadArgs a, size_t total) {
+    const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (gid >= total) return;
+    const unsigned per = (unsigned)a.d / 8;
+    const size_t row = gid / per, tok = row / (unsigned)a.h, seq = tok / (unsigned)a.s_len;
+    const int piece = (int)(gid - row * per), head = (int)(row - tok * (unsigned)a.h);
+    const long step = (long)a.first[seq] + (long)(tok - seq * (unsigned)a.s_len);
+    const int page = step >= 0 && step < (long)MAX_ROWS ? page_of(a.table, seq, (int)step) : -1;
+    float x[8] = {};
+    if (page >= 0) load_n<CT, 8>(a.pages[blockIdx.y], ((((size_t)page * a.h + head) << a.table.shift) + ((int)step & ((1 << a.table.shift) - 1))) * a.d + piece * 8, 8, x);
+    store_n<OUT, 8>(a.out[blockIdx.y], row * a.d + piece * 8, 8, x);
+}
+
+bool row_type(int dt) { return dt == AIONHIP_F32 || dt == AIONHIP_F16 || dt == AIONHIP_BF16; }
+size_t size_of(int dt) { return dt == AIONHIP_F32 ? 4 : 2; }
+
+int check_rotary(aionhip_ctx *ctx, const char *who, const aionhip_rotary *r, size_t d) {
+    if (!r) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: no rotary", who);
+    auto positive = [](float x) { return x > 0.f && x < INFINITY; };
+    if (r->dims % 2 != 0 || r->dims > d) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: %u turning elements of a head of %zu (an even number of them)", who, r->dims, d);
+    if (r->scaling < AIONHIP_ROTARY_PLAIN || r->scaling > AIONHIP_ROTARY_RAMP) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: unknown scaling %d", who, r->scaling);
+    if (!positive(r->base) || !(fabsf(r->magnitude) < INFINITY)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: base must be positive and finite, magnitude finite", who);
+    if (r->scaling != AIONHIP_ROTARY_PLAIN && !positive(r->factor)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: factor must be positive and finite", who);
+    if (r->scaling >= AIONHIP_ROTARY_BANDS && (!positive(r->original_length) || !positive(r->low) || !positive(r->high) || !(r->low < r->high)))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: original_length, low and high must be positive and finite, low below high", who);
+    if (r->scaling == AIONHIP_ROTARY_RAMP && !(r->base > 1.f)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: a ramp needs a base above one", who);
+    return AIONHIP_OK;
+}
+
+// each pair's fraction of a turn a position, 2^64 to the whole; one table per kind of turning, kept by the context as RoPE's are
+int turn_table(aionhip_ctx *ctx, const aionhip_rotary *r, const unsigned long **out) {
+    aionhip_rotary key{};
+    key.dims = r->dims, key.scaling = r->scaling, key.base = r->base;
+    if (r->scaling != AIONHIP_ROTARY_PLAIN) key.factor = r->factor;
+    if (r->scaling >= AIONHIP_ROTARY_BANDS) key.original_length = r->original_length, key.low = r->low, key.high = r->high;
+    for (const auto &t : ctx->turn_tables)
+        if (std::memcmp(&t.key, &key, sizeof key) == 0) {
+            *out = (const unsigned long *)t.turns;
+            return AIONHIP_OK;
+        }
+    if (ctx->capturing)
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "a table of rotary turns cannot be built while a program is being recorded: run the steps once before recording");
+    const long double two_pi = 6.283185307179586476925286766559L, base = r->base, dims = r->dims;
+    std::vector<unsigned long> host(r->dims / 2);
+    long double a = 0, b = 0;
+    if (r->scaling == AIONHIP_ROTARY_RAMP) {
+        auto at = [&](long double turns) { return dims * logl((long double)r->original_length / (turns * two_pi)) / (2 * logl(base)); };
+        a = fmaxl(floorl(at(r->high)), 0);
+        b = fminl(ceill(at(r->low)), dims - 1);
+    }
+    for (uint32_t i = 0; i < r->dims / 2; ++i) {
+        long double f = powl(base, -2.0L * i / dims), kept = 1;
+        if (r->scaling == AIONHIP_ROTARY_LINEAR) kept = 0;
+        else if (r->scaling == AIONHIP_ROTARY_BANDS)
+            kept = ((long double)r->original_length * f / two_pi - r->low) / ((long double)r->high - r->low);
+        else if (r->scaling == AIONHIP_ROTARY_RAMP)
+            kept = 1 - (i - a) / fmaxl(b - a, 0.001L);
+        kept = fminl(fmaxl(kept, 0), 1);
+        f *= kept + (1 - kept) / (r->scaling == AIONHIP_ROTARY_PLAIN ? 1.0L : (long double)r->factor);
+        const long double turn = f / two_pi;
+        host[i] = (unsigned long)ldexpl(turn - floorl(turn), 64);          // (a base below one may turn more than once a position: whole turns are none)
+    }
+    void *dev = nullptr;
+    if (const int rc = dev_malloc(ctx, &dev, host.size() * sizeof(host[0]), "a table of rotary turns")) return rc;
+    hipError_t e = hipMemcpyAsync(dev, host.data(), host.size() * sizeof(host[0]), hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(dev);
+        return set_err(ctx, AIONHIP_EXECUTION_FAILED, "upload of a table of rotary turns: %s", hipGetErrorString(e));
+    }
+    ctx->turn_tables.push_back({key, dev});
+    *out = (const unsigned long *)dev;
+    return AIONHIP_OK;
+}
+
+// the launch of `tokens` rows; `rotary` null or of no pairs: nothing turns
+int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rotary *rotary, size_t tokens, int dtype, int cache_dtype) {
+    if (rotary && rotary->dims) {
+        if (const int rc = turn_table(ctx, rotary, &a.turns)) return rc;
+        a.dims = (int)rotary->dims;
+        a.interleaved = rotary->interleaved ? 1 : 0;
+        a.magnitude = rotary->magnitude;
+    }
+    if (tokens > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
+    const int each = pairs_each(dtype);
+    a.turning = (a.dims / 2 + each - 1) / each;
+    a.pieces = a.turning + (a.d - a.dims + 2 * each - 1) / (2 * each);
+    const int slots = a.h_q + 2 * a.h_kv;
+    a.heads_wg = min(256 / a.pieces, slots);                             // (heads of up to 1024 have 129 pieces at most)
+    // Few tokens are a chain of latencies, spread thin; many have the angles of each computed once for four heads (measured at the kernel).
+    const bool many = tokens >= 1024;
+    const dim3 grid((unsigned)tokens, (unsigned)((slots + a.heads_wg * (many ? 4 : 1) - 1) / (a.heads_wg * (many ? 4 : 1))));
+    const unsigned threads = (unsigned)((a.heads_wg * a.pieces + 63) / 64 * 64);
+    ProfScope scope(ctx, who);
+    auto go = [&](auto dt, auto ct) {
+        if (many) launch_k(ctx, rotary_kernel<decltype(dt)::value, decltype(ct)::value, 4>, grid, dim3(threads), 0, a);
+        else launch_k(ctx, rotary_kernel<decltype(dt)::value, decltype(ct)::value, 1>, grid, dim3(threads), 0, a);
+    };
+    auto types = [&](auto dt) {
+        if (cache_dtype == AIONHIP_F16) go(dt, std::integral_constant<int, AIONHIP_F16>{});
+        else go(dt, std::integral_constant<int, AIONHIP_BF16>{});
+    };
+    if (dtype == AIONHIP_F32) types(std::integral_constant<int, AIONHIP_F32>{});
+    else if (dtype == AIONHIP_F16) types(std::integral_constant<int, AIONHIP_F16>{});
+    else types(std::integral_constant<int, AIONHIP_BF16>{});
+    LAUNCH_CHECK(ctx, who);
+    return AIONHIP_OK;
+}
+
+int append(aionhip_ctx *ctx, const char *who, const aionhip_paged_cache *c, const aionhip_rotary *rotary, aionhip_handle q_out, aionhip_handle q, aionhip_handle k, aionhip_handle v,
+           int dtype, aionhip_handle positions, aionhip_handle write_index, size_t s, size_t h_q) {
+    int rc = check_cache(ctx, who, c);
+    if (rc) return rc;
+    if (!k || !v || !write_index) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: null operand", who);
+    if (!row_type(dtype)) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: rows are f32, f16 or bf16, not dtype %d", who, dtype);
+    if (s > capacity(c)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: %zu rows exceed the capacity %zu", who, s, capacity(c));
+    if (h_q > 65535) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: dimension too large", who);
+    if (!c->batch || !s) return AIONHIP_OK;
+    const size_t tokens = c->batch * s, q_bytes = tokens * h_q * c->d * size_of(dtype), kv_bytes = tokens * c->h_kv * c->d * size_of(dtype);
+    if (in_cache(c, q, q_bytes) || in_cache(c, q_out, q_bytes) || in_cache(c, k, kv_bytes) || in_cache(c, v, kv_bytes))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: rows lie in the cache", who);
+    if ((q_out != q && overlap(q_out, q_bytes, q, q_bytes)) || overlap(q_out, q_bytes, k, kv_bytes) || overlap(q_out, q_bytes, v, kv_bytes))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: q, k and v are still read while q_out is written", who);
+    Rotate a{};
+    a.q_out = dp<void>(q_out), a.q = dp<const void>(q), a.k = dp<const void>(k), a.v = dp<const void>(v);
+    a.positions = dp<const int>(positions), a.write_index = dp<const int>(write_index);
+    a.d = (int)c->d, a.h_q = (int)h_q, a.h_kv = (int)c->h_kv, a.s_len = (int)s;
+    a.table = table_of(c);
+    a.k_pages = dp<unsigned char>(c->k_pages), a.v_pages = dp<unsigned char>(c->v_pages);
+    return launch_rotary(ctx, who, a, rotary, tokens, dtype, c->dtype);
+}
+
+}  // namespace
+
+extern "C" {
+
+int aionhip_step_rotary(aionhip_ctx *ctx, aionhip_handle out, aionhip_handle x, aionhip_handle positions, int dtype, size_t b, size_t t, size_t h, size_t d,
+                        const aionhip_rotary *rotary) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (!out || !x || !positions) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rotary: null operand");
+    if (!row_type(dtype)) return set_err(ctx, AIONHIP_UNSUPPORTED, "rotary: rows are f32, f16 or bf16, not dtype %d", dtype);
+    if (const int rc = check_rotary(ctx, "rotary", rotary, d)) return rc;
+    if (d > MAX_HEAD || h > 65535 || b > 0x7FFFFFFF || t > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "rotary: dimension too large");
+    if (!b || !t || !h || !d) return AIONHIP_OK;
+    if (b > 0x7FFFFFFF / t) return set_err(ctx, AIONHIP_UNSUPPORTED, "rotary: too many rows for one launch");
+    const size_t bytes = b * t * h * d * size_of(dtype);
+    if ((out != x && overlap(out, bytes, x, bytes)) || overlap(out, bytes, positions, b * t * 4))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rotary: x and the positions are still read while out is written");
+    Rotate a{};
+    a.q_out = dp<void>(out), a.q = dp<const void>(x), a.positions = dp<const int>(positions);
+    a.d = (int)d, a.h_q = (int)h;
+    return launch_rotary(ctx, "rotary", a, rotary, b * t, dtype, AIONHIP_F16);
+}
+
+int aionhip_step_append_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, aionhip_handle k, aionhip_handle v, int src_dtype, aionhip_handle write_index, size_t s) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    return append(ctx, "append_paged", cache, nullptr, 0, 0, k, v, src_dtype, 0, write_index, s, 0);
+}
+
+int aionhip_step_rotary_append_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, const aionhip_rotary *rotary, aionhip_handle q_out, aionhip_handle q,
+                                     aionhip_handle k, aionhip_handle v, int dtype, aionhip_handle positions, aionhip_handle write_index, size_t s, size_t h_q) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (!q_out || !q || !positions) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "rotary_append_paged: null operand");
+    if (const int rc = check_cache(ctx, "rotary_append_paged", cache)) return rc;
+    if (const int rc = check_rotary(ctx, "rotary_append_paged", rotary, cache->d)) return rc;
+    return append(ctx, "rotary_append_paged", cache, rotary, q_out, q, k, v, dtype, positions, write_index, s, h_q);
+}
+
+int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *c, aionhip_handle k_out, aionhip_handle v_out, int out_dtype, aionhip_handle first, size_t s) {
+    if (!ctx) return AIONHIP_INVALID_ARGUMENT;
+    if (const int rc = check_cache(ctx, "read_paged", c)) return rc;
+    if (!k_out || !v_out || !first) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: null operand");
+    if (!row_type(out_dtype)) return set_err(ctx, AIONHIP_UNSUPPORTED, "read_paged: rows are f32, f16 or bf16, not dtype %d", out_dtype);
+    if (s > capacity(c)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: %zu rows exceed the capacity %zu", s, capacity(c));
+    if (!c->batch || !s) return AIONHIP_OK;
+    const size_t rows = c->batch * s * c->h_kv, bytes = rows * c->d * size_of(out_dtype), total = rows * (c->d / 8);
+    if (overlap(k_out, bytes, v_out, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: the rows of keys and values overlap");
+    if (in_cache(c, k_out, bytes) || in_cache(c, v_out, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: rows lie in the cache");
+    if ((total + 255) / 256 > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "read_paged: too many rows for one launch");
+    const ReadArgs a{{dp<const unsigned char>(c->k_pages), dp<const unsigned char>(c->v_pages)}, {dp<void>(k_out), dp<void>(v_out)}, dp<const int>(first), table_of(c), (int)s, (int)c->h_kv,
+                     (int)c->d};
+    const bool f16 = c->dtype == AIONHIP_F16;
+    const auto kernel = out_dtype == AIONHIP_F32   ? (f16 ? read_paged_kernel<AIONHIP_F16, AIONHIP_F32> : read_paged_kernel<AIONHIP_BF16, AIONHIP_F32>)
+                        : out_dtype == AIONHIP_F16 ? (f16 ? read_paged_kernel<AIONHIP_F16, AIONHIP_F16> : read_paged_kernel<AIONHIP_BF16, AIONHIP_F16>)
+                                                   : (f16 ? read_paged_kernel<AIONHIP_F16, AIONHIP_BF16> : read_paged_kernel<AIONHIP_BF16, AIONHIP_BF16>);
+    ProfScope scope(ctx, "read_paged");
+    launch_k(ctx, kernel, dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, a, total);
+    LAUNCH_CHECK(ctx, "read_paged");
+    return AIONHIP_OK;
+}
+
+}  // extern "C"

@@ -81,6 +81,12 @@ struct aionhip_ctx {
         float *freq;
     };
     std::vector<RopeTable> rope_tables;
+    // rotary turns (fractions of a turn a position, u64), one table per kind of turning (cache_paged.hip)
+    struct TurnTable {
+        aionhip_rotary key;
+        void *turns;
+    };
+    std::vector<TurnTable> turn_tables;
     // true between aionhip_program_begin/end: launches are captured, nothing may synchronise or allocate
     bool capturing = false;
     // per-launch timing, off by default

@@ -39,6 +39,21 @@ class DecoderStackDesc(C.Structure):
                [("window_left", C.c_uint32), ("window_right", C.c_uint32), ("window_chunk", C.c_uint32), ("rolling", C.c_int)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("k_pages", "v_pages", "page_table")] + \
+               [(n, C.c_size_t) for n in ("pages", "batch", "table_width", "page_rows", "h_kv", "d")] + [("dtype", C.c_int)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("dims", C.c_uint32), ("interleaved", C.c_uint32), ("scaling", C.c_int)] + \
+               [(n, C.c_float) for n in ("base", "factor", "original_length", "low", "high", "magnitude")]
+
+
+class Eviction(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("weights", "kv_lengths", "weights_out", "lengths_out", "table_out", "kept")] + \
+               [(n, C.c_size_t) for n in ("width_out", "limit", "keep", "first", "recent")]
+
+
 MAX_RANK = 8
 
 
@@ -142,6 +157,12 @@ _SIGS = {
     "aionhip_step_append_quant": (C.c_int, [C.c_void_p, C.c_int] + [C.c_uint64] * 4 + [C.c_int, C.c_uint64] + [C.c_size_t] * 5 + [C.c_int]),
     "aionhip_step_rope_append_quant": (C.c_int, [C.c_void_p, C.c_int] + [C.c_uint64] * 8 + [C.c_size_t] * 6 + [C.c_float] * 3 + [C.c_int]),
     "aionhip_step_cache_read": (C.c_int, [C.c_void_p, C.c_int, C.c_int] + [C.c_uint64] * 5 + [C.c_size_t] * 5 + [C.c_int]),
+    "aionhip_step_rotary": (C.c_int, [C.c_void_p] + [C.c_uint64] * 3 + [C.c_int] + [C.c_size_t] * 4 + [C.POINTER(Rotary)]),
+    "aionhip_step_append_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCache), C.c_uint64, C.c_uint64, C.c_int, C.c_uint64, C.c_size_t]),
+    "aionhip_step_rotary_append_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCache), C.POINTER(Rotary)] + [C.c_uint64] * 4 + [C.c_int] + [C.c_uint64] * 2 + [C.c_size_t] * 2),
+    "aionhip_step_read_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCache), C.c_uint64, C.c_uint64, C.c_int, C.c_uint64, C.c_size_t]),
+    "aionhip_step_attention_paged": (C.c_int, [C.c_void_p, C.POINTER(Attention), C.POINTER(PagedCache), C.c_uint64, C.c_uint64]),
+    "aionhip_step_evict_paged": (C.c_int, [C.c_void_p, C.POINTER(PagedCache), C.POINTER(Eviction)]),
     "aionhip_step_cast_f32_f16": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_size_t]),
     "aionhip_step_headnorm_rope_append": (C.c_int, [C.c_void_p] + [C.c_uint64] * 10 + [C.c_float] + [C.c_uint64] * 4 + [C.c_size_t] * 6 +
                                           [C.c_float] * 3 + [C.c_int]),

@@ -355,6 +355,75 @@ int aionhip_step_rope_append_quant(aionhip_ctx *ctx, int dtype, aionhip_handle q
  * do not lie in the caches. */
 int aionhip_step_cache_read(aionhip_ctx *ctx, int dtype, int out_dtype, aionhip_handle k_out, aionhip_handle k_cache, aionhip_handle v_out, aionhip_handle v_cache,
                             aionhip_handle first, size_t b, size_t s, size_t t_cap, size_t h, size_t d, int rolling);
+/* ---- caches in pages -------------------------------------------------------------------------
+ * For programs that hold many sequences, or long ones, whose lengths are not known beforehand: memory is handed out a page at a time, and sequences may share
+ * pages (a common beginning). aion's caches are one buffer a sequence; this is an option of a binding, as quantized caches are.
+ * Two pools [pages, H, P, D] of dtype F16 or BF16, keys and values (each begins at a multiple of 16 bytes), P = page_rows a power of two from 16 to 1024, D a multiple
+ * of 8 up to 1024, and a table i32 [batch, table_width] on the device: step t of sequence b is row t % P of page page_table[b, t / P]. The capacity of a sequence is
+ * table_width * P. An entry outside [0, pages) is no page: its keys are invisible, its rows are not written and read as zeros. Which page belongs to whom is
+ * the caller's: a page that a step writes belongs to one sequence. Rows that were never written may hold anything, as long as no step is told to read them. */
+typedef struct aionhip_paged_cache {
+    aionhip_handle k_pages, v_pages, page_table;
+    size_t pages, batch, table_width, page_rows, h_kv, d;
+    int dtype;                           /* F16 | BF16 */
+} aionhip_paged_cache;
+
+/* How rows turn with their positions. Of a head's d elements the first `dims` (even) turn, in dims / 2 pairs, the others stay. Pair i is the elements i and i +
+ * dims / 2, or with interleaved = 1 the elements 2i and 2i + 1; it turns by position * f_i, f_i = base^(-2 i / dims) radians, changed by `scaling`:
+ *   PLAIN   f_i
+ *   LINEAR  f_i / factor
+ *   BANDS   f_i (k + (1 - k) / factor), k = clamp((original_length f_i / 2 pi - low) / (high - low), 0, 1): by how often a pair turns in original_length positions
+ *   RAMP    the same, k = 1 - clamp((i - a) / max(b - a, 0.001), 0, 1), a = max(floor(at(high)), 0), b = min(ceil(at(low)), dims - 1), at(turns) =
+ *           dims ln(original_length / (2 pi turns)) / (2 ln base): a ramp over pair numbers, between those that turn `high` and `low` times
+ * and the turned elements are multiplied by `magnitude`. The angle is position * f_i to 2^-32 of a turn at any position (the frequencies are held to 2^-60 of a
+ * turn and multiplied in 64-bit fixed point), where aionhip_step_rope multiplies in f32 as aion does and is off by 0.06 radians at a million. Fields that a kind of
+ * scaling does not name are not looked at. */
+enum { AIONHIP_ROTARY_PLAIN = 0, AIONHIP_ROTARY_LINEAR = 1, AIONHIP_ROTARY_BANDS = 2, AIONHIP_ROTARY_RAMP = 3 };
+typedef struct aionhip_rotary {
+    uint32_t dims, interleaved;
+    int scaling;
+    float base, factor, original_length, low, high, magnitude;
+} aionhip_rotary;
+/* x, out [B,T,H,D] of dtype F32, F16 or BF16 (D up to 1024), positions i32 [B,T]; f32 arithmetic, rounded once. out may be x. */
+int aionhip_step_rotary(aionhip_ctx *ctx, aionhip_handle out, aionhip_handle x, aionhip_handle positions, int dtype, size_t b, size_t t, size_t h, size_t d,
+                        const aionhip_rotary *rotary);
+/* SequenceAppend into pages: rows k, v [B,S,H,D] of src_dtype F32, F16 or BF16 go to steps write_index[b] .. +S (i32 [B] on the device). A row before the first
+ * step, past the capacity or on an entry that is no page is not written. No rows lie in the pools. */
+int aionhip_step_append_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, aionhip_handle k, aionhip_handle v, int src_dtype, aionhip_handle write_index, size_t s);
+/* aionhip_step_rotary on q [B,S,h_q,D] (to q_out, which may be q) and k, and aionhip_step_append_paged of k and v, as one launch; all rows of one dtype, positions
+ * i32 [B,S]. Keys are rounded once, from the turned f32 value. */
+int aionhip_step_rotary_append_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, const aionhip_rotary *rotary, aionhip_handle q_out, aionhip_handle q,
+                                     aionhip_handle k, aionhip_handle v, int dtype, aionhip_handle positions, aionhip_handle write_index, size_t s, size_t h_q);
+/* Steps first[b] .. +S (i32 [B] on the device) as rows k_out, v_out [B,S,H,D] of out_dtype F32, F16 or BF16: to hand a prefix to a linear cache, or to read it. Steps that
+ * the cache does not hold are zeros. The rows do not lie in the pools and do not overlap. */
+int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, aionhip_handle k_out, aionhip_handle v_out, int out_dtype, aionhip_handle first, size_t s);
+/* aionhip_step_attention over pages: out, q, batch, l_q, h_q, q_dtype, scale, soft cap and window as there; k and v are 0, t_kv is the capacity, h_kv, d_k = d_v and kv_dtype
+ * are the cache's, rolling is 0. kv_lengths 0: every sequence fills its capacity; a length past it counts as the capacity. query_positions 0: the queries are the last
+ * l_q steps, kv_lengths[b] - l_q + i (one before the first step sees nothing) - and so a position is the row in the cache, which after an eviction is no longer the position that
+ * the row was turned by. f32 accuracy (about 1e-6) whatever aionhip_set_attention_precise says. A query that sees no key, or only scores of minus infinity, gets zeros; what is not
+ * finite reaches the queries that see it and no others. Head sizes 64, 128 and 256 run on the matrix pipe, others on a slow kernel. Made for one to a few tokens: of more
+ * query rows to a KV head than sixteen, every sixteen walk the keys on their own.
+ * weights (0: none), f32 [batch, h_kv, capacity]: weights = weights_before (the same shape, the same buffer or 0, which counts as zeros) + the probability of
+ * each key, summed over the queries and the query heads of its KV head. What aionhip_step_evict_paged goes by. AIONHIP_UNSUPPORTED where the scores (4 bytes a
+ * query row and key of the capacity) would take more than 4 GiB of scratch memory: ask with the last queries of a long prompt alone. */
+int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_attention *p, const aionhip_paged_cache *cache, aionhip_handle weights_before, aionhip_handle weights);
+/* Eviction: of each sequence longer than `limit` every KV head keeps `keep` rows (first + recent <= keep <= limit): the `first` oldest, the `recent` newest, and of
+ * those between them the ones of greatest weight, of equal weights the oldest (a NaN is the greatest, -0 equals 0). A head's rows keep their order and become steps 0 .. keep - 1;
+ * which steps remain differs from head to head, how many does not. A sequence of up to `limit` rows keeps all. Decided on the device: a recorded
+ * program may hold the step and run it every token.
+ *   weights  f32 [batch, h_kv, capacity], kv_lengths i32 [batch]
+ *   table_out 0: in place. The rows move within the cache's own pages (none of them shared with another sequence), a sequence of up to `limit` rows is left alone;
+ *     weights_out may be weights, lengths_out kv_lengths. Pages past the new length are then the caller's again.
+ *   table_out i32 [batch, width_out]: the rows of every sequence are copied to these pages of the same pools, which are none of the source's; nothing else of the cache changes, so
+ *     that sequences may share what they began with. width_out * page_rows >= limit; weights_out is not weights. A row that falls on no page is not written.
+ *   weights_out f32 [batch, h_kv, C], C = the capacity, or width_out * page_rows: the kept rows' weights, then zeros. lengths_out i32 [batch].
+ *   kept (may be 0) i32 [batch, h_kv, limit]: the step each row was, -1 behind them.
+ * Operands that are written overlap nothing else but as said. */
+typedef struct aionhip_eviction {
+    aionhip_handle weights, kv_lengths, weights_out, lengths_out, table_out, kept;
+    size_t width_out, limit, keep, first, recent;
+} aionhip_eviction;
+int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, const aionhip_eviction *e);
 /* StepSequenceAppend as the step itself (runtime/executable.zig:193-206, cpu/exec/sequence_append.zig:12-104): cache
  * [B,T,H,D] and new_kv [B,S,H,D] of the same element type `dtype` (AIONHIP_F16 or AIONHIP_F32), end_index i32 [B] on the
  * device; rows go to token index end_index[b] .. +S (rolling = 1: to row t % T). A row that would fall outside a linear
