@@ -6,7 +6,8 @@
 //   K goes from the pages to registers in the order the matrix instruction wants it, V through LDS, where it is read transposed. Sixteen keys lie in one page, so a
 //   page number is a scalar to each half tile: a lane fetches one of the next 64, and they become addresses without a load in between.
 //   Accuracy: q and P enter the products as sums of halves (two f16, three bf16; q that comes in the cache's type as it is), K and V are exact, sums are f32.
-// paged_merge_kernel - adds the segments of a row, and forms the keys' weights from the scores that the first kernel left.
+//   The workgroup that ends last adds the segments of its rows.
+// paged_weights_kernel - what the keys draw, from the scores that the first kernel left.
 // paged_generic_kernel - other head sizes: a wavefront a key at a time, f32. It is there so that every shape has a path.
 #include "attention_common.h"
 #include "cache_paged.h"
@@ -21,15 +22,14 @@ constexpr float MASKED = -INFINITY;
 // Probabilities are held as 2^(s - ref + HEAD_ROOM), the reference being raised only when a score passes it by more than SLACK: 2^14 at most fits f16, and what f16
 // pairs round away lies 2^-31 below the largest.
 constexpr float HEAD_ROOM = 6.f, SLACK = 8.f;
-// A number becomes a sum of halves that all have its sign and are not zero, each but the last taken from slightly less than what is left: an infinite key or value then
-// has products of one sign, and no zero times infinity, as the number itself has.
 template <int KV> constexpr float LESS = KV == AIONHIP_F16 ? 1.f - 0x1p-11f : 1.f - 0x1p-8f;
 
 struct PagedArgs {
     float *out, *partial, *scores;
     const float *weights_before;
     float *weights;
-    float2 *stats;            // [unit][padded rows][nseg] reference (log2) and sum
+    float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
+    unsigned *tickets;
     Table table;
     int T, tpad, L, Hkv, groups, rows_total, row_tiles, nseg;
     int d, q_dtype, kv_dtype;
@@ -50,132 +50,139 @@ __device__ __forceinline__ void row_keys(const PagedArgs &a, int b, int li, int 
     if (hi < lo) hi = lo;
 }
 
+constexpr int MOST_SEGMENTS = 256;      // of a row tile
 template <int D>
 struct Cfg {
-    static constexpr int NW = D == 256 ? 4 : 8;
+    static constexpr int NW = D == 256 ? 8 : 4;                  // wavefronts of a workgroup
     static constexpr int ROW = D * 2, TILE = TILE_KEYS * ROW;
-    static constexpr int SLOT = 16 * (D + 4) + 32;               // a wavefront's results in the merge: [16][D + 4], 16 references, 16 sums
-    static constexpr int MERGE = NW * SLOT * 4, LDS = NW * TILE > MERGE ? NW * TILE : MERGE;
+    static constexpr int SLOT = 16 * (D + 4) + 32;               // a wavefront's results where they meet: [16][D + 4], 16 references, 16 sums
+    static constexpr int PART = 16 * D + 32;                     // a segment's results in memory: [16][D], [16] (reference, sum)
+    static constexpr int MOST = MOST_SEGMENTS;
+    static constexpr int MEET = NW * SLOT * 4, JOIN = (16 * MOST + 64) * 4 + NW * 64 * 16;          // LDS where wavefronts, where segments meet
+    static constexpr int MAIN = NW * TILE > MEET ? (NW * TILE > JOIN ? NW * TILE : JOIN) : MEET > JOIN ? MEET : JOIN;
 };
-// tiles of a segment: the tiles are dealt out evenly, no fewer than one to a wavefront
-__device__ __forceinline__ int tiles_each(int tiles, int nseg, int nw) { return max(nw, (tiles + nseg - 1) / nseg); }
+// 16 bytes of LDS by address, not waited for (as a builtin the compiler would wait for every load in flight into LDS first)
+template <int OFF>
+__device__ __forceinline__ u32x4 lds_read(unsigned addr) {
+    u32x4 x;
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(x) : "v"(addr), "n"(OFF) : "memory");
+    return x;
+}
 
-// Q parts: how many halves a query element is the sum of
-template <int KV, int D, int QP, bool WEIGH>
-__global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a) {
+// QP: how many halves a query element is the sum of. MULTI: several queries a sequence, whose keys may differ (of one query all rows see the same). ONCE: keys and values
+// go past the caches. The leading arguments, 14 words, arrive in SGPRs with the wavefront. heads: KV heads, query heads of each << 16;
+// form: segments, log2 of a page's rows << 12, query type << 16, rows of the queries in LDS << 24.
+template <int KV, int D, int QP, bool MULTI, bool ONCE>
+__global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
+                                                                     unsigned heads, unsigned form, PagedArgs tail) {
     using C = Cfg<D>;
     constexpr int NW = C::NW, KK = D / 32, MT = D / 16;
     constexpr int PP = KV == AIONHIP_F16 ? 2 : 3;                // parts of a probability
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    PagedArgs a = tail;
+    const int L = MULTI ? queries : 1;
+    a.kv_lengths = kv_lengths, a.q = q, a.table.pages = table, a.T = T, a.L = L;
+    a.Hkv = (int)(heads & 0xFFFFu), a.groups = (int)(heads >> 16);
+    a.nseg = (int)(form & 0xFFFu), a.table.shift = (int)(form >> 12 & 0xFu), a.q_dtype = (int)(form >> 16 & 0xFFu);
+    a.table.width = T >> a.table.shift;
+    const int q_rows = D == 256 ? (int)(form >> 24) : 16;        // 8 or 16
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int rt = blockIdx.x / a.nseg, seg = blockIdx.x - rt * a.nseg, hk = blockIdx.y, b = blockIdx.z;
+    const int rows_total = L * a.groups;
+    const int rt = rows_total <= 16 ? 0 : blockIdx.x / a.nseg, seg = blockIdx.x - rt * a.nseg, hk = blockIdx.y, b = blockIdx.z;
     const int unit = b * a.Hkv + hk;
-    const int r = rt * 16 + n;
-    const bool row_ok = r < a.rows_total;
-    const int li = row_ok ? r / a.groups : 0, gi = row_ok ? r - li * a.groups : 0;
-    int lo, hi;
-    row_keys(a, b, li, a.kv_lengths ? a.kv_lengths[b] : 0, a.positions ? a.positions[(size_t)b * a.L + li] : 0, lo, hi);
-    if (!row_ok) lo = hi = 0;
-    const bool some = hi > lo;
-    const int uni_lo = rows16_min_i(some ? lo : INT_MAX), uni_hi = rows16_max_i(some ? hi : 0);
-    // keys that every row sees
-    const int all_lo = rows16_max_i(row_ok ? (some ? lo : INT_MAX) : 0), all_hi = rows16_min_i(row_ok ? (some ? hi : 0) : INT_MAX);
+    const int len_raw = kv_lengths ? kv_lengths[b] : 0;
 
-    // ---- the queries
-    const size_t qbase = (((size_t)b * a.L + li) * (a.Hkv * a.groups) + hk * a.groups + gi) * D;
-    u32x4 qf[QP][KK];
-    float to_score = 1.f;                                        // a product's sum times this is q . k
-    if constexpr (QP == 1) {
+    // ---- the pages of this wavefront's first tiles are asked for beside the length: the segments take a sequence's tiles in turn, their first wavefronts first, so that
+    // which are whose does not depend on how many there are (behind a window they begin later, and are asked for again)
+    const int *pages = table + (size_t)b * a.table.width;
+    const int stride = a.nseg * NW;
+    int t_begin = wave * a.nseg + seg;
+    // the pages of the half tiles of 32 steps, one to a lane; -1: none
+    auto fetch_pages = [&](int step0) __attribute__((always_inline)) {
+        const int e = (int)((unsigned)((t_begin + (step0 + (lane >> 1)) * stride) * TILE_KEYS + (lane & 1) * 16) >> a.table.shift);
+        return e >= 0 && e < a.table.width ? pages[e] : -1;
+    };
+    int ids = fetch_pages(0);
+
+    // ---- the queries: a thread asks for eight elements of one row (of two, at head size 256) before anything is waited for
+    constexpr int QT = D / 8, QROWS = NW * 64 / QT, QSETS = QROWS >= 16 ? 1 : 16 / QROWS;
+    const int q_row = (int)threadIdx.x / QT, q_col = (int)threadIdx.x % QT * 8;
+    float qx[QSETS][8];
+    u32x4 qh[QSETS];
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            __builtin_memcpy(&qf[0][kk], (const unsigned short *)a.q + qbase + kk * 32 + g * 8, 16);
-            if (!row_ok) qf[0][kk] = u32x4{0u, 0u, 0u, 0u};
-        }
-    } else {
-        float x[KK][8];
-        float top = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const size_t at = qbase + kk * 32 + g * 8;
+    for (int i = 0; i < QSETS; ++i) {
+        const int r = rt * 16 + q_row + i * QROWS;
+        const bool there = q_row + i * QROWS < 16 && r < rows_total;
+        const int l2 = L > 1 && there ? r / a.groups : 0, g2 = there ? r - l2 * a.groups : 0;
+        const size_t at = (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + q_col;
+        if constexpr (QP == 1) {
+            __builtin_memcpy(&qh[i], (const unsigned short *)q + at, 16);
+            if (!there) qh[i] = u32x4{0u, 0u, 0u, 0u};
+        } else {
             if (a.q_dtype == AIONHIP_F32) {
-                __builtin_memcpy(x[kk], (const float *)a.q + at, 32);
+                __builtin_memcpy(qx[i], (const float *)q + at, 32);
             } else {
                 unsigned short h[8];
-                __builtin_memcpy(h, (const unsigned short *)a.q + at, 16);
+                __builtin_memcpy(h, (const unsigned short *)q + at, 16);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[kk][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(h[j])) : bf16_bits_to_f32(h[j]);
+                for (int j = 0; j < 8; ++j) qx[i][j] = a.q_dtype == AIONHIP_F16 ? __half2float(__ushort_as_half(h[j])) : bf16_bits_to_f32(h[j]);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (!row_ok) x[kk][j] = 0.f;
-                top = fmaxf(top, fabsf(x[kk][j]));
-            }
+            for (int j = 0; j < 8; ++j) qx[i][j] = there ? qx[i][j] : 0.f;
         }
-        float factor = 1.f;
-        if constexpr (KV == AIONHIP_F16) {
-            // a row goes into f16's range by a power of two that takes its largest element to 2^10: what the second half rounds away then lies 2^-35 below that
-            top = groups4_max(top);
-            const int e = (int)(__float_as_uint(top) >> 23);
-            const int f = e == 255 ? 127 : max(1, min(264 - e, 253));
-            factor = __uint_as_float((unsigned)f << 23);
-            to_score = __uint_as_float((unsigned)(254 - f) << 23);
-        }
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float u = x[kk][j] * factor, w = x[kk][j + 1] * factor;
-#pragma unroll
-                for (int p = 0; p < QP; ++p) {
-                    const unsigned both = p + 1 < QP ? pack2<KV>(u * LESS<KV>, w * LESS<KV>) : pack2<KV>(u, w);
-                    qf[p][kk][j / 2] = both;
-                    // (an infinite element has no rest)
-                    const float ru = u - from_half_bits<KV>((unsigned short)both), rw = w - from_half_bits<KV>((unsigned short)(both >> 16));
-                    u = fabsf(ru) < INFINITY ? ru : u;
-                    w = fabsf(rw) < INFINITY ? rw : w;
-                }
-            }
     }
-    const float to_log2 = a.soft_cap > 0.f ? to_score * (a.scale / a.soft_cap) : to_score * (a.scale * LOG2E), cap_log2 = a.soft_cap * LOG2E;
+
+    // ---- what this lane's row sees
+    const int r = rt * 16 + n;
+    const bool row_ok = r < rows_total;
+    const int li = MULTI && row_ok ? r / a.groups : 0;
+    int lo, hi;
+    row_keys(a, b, li, len_raw, a.positions ? a.positions[(size_t)b * L + li] : 0, lo, hi);
+    int uni_lo, uni_hi, all_lo, all_hi;                          // of any row's keys, of those that every row sees
+    if constexpr (MULTI) {
+        if (!row_ok) lo = hi = 0;
+        const bool some = hi > lo;
+        uni_lo = rows16_min_i(some ? lo : INT_MAX), uni_hi = rows16_max_i(some ? hi : 0);
+        all_lo = rows16_max_i(row_ok ? (some ? lo : INT_MAX) : 0), all_hi = rows16_min_i(row_ok ? (some ? hi : 0) : INT_MAX);
+    } else {
+        lo = uni_lo = all_lo = __builtin_amdgcn_readfirstlane(lo);
+        hi = uni_hi = all_hi = __builtin_amdgcn_readfirstlane(hi);
+    }
 
     // ---- this wavefront's tiles
-    int t_begin = 0, t_end = 0;
-    if (uni_hi > uni_lo) {
-        const int tb = uni_lo / TILE_KEYS, te = (uni_hi + TILE_KEYS - 1) / TILE_KEYS, per = tiles_each(te - tb, a.nseg, NW);
-        t_begin = tb + seg * per;
-        t_end = min(t_begin + per, te);
+    int tb = 0, te = 0;
+    if (uni_hi > uni_lo) tb = uni_lo / TILE_KEYS, te = (uni_hi + TILE_KEYS - 1) / TILE_KEYS;
+    const int live = min(a.nseg, te - tb);                       // segments that have tiles
+    if (seg >= max(live, 1)) return;
+    if (tb > 0) {
+        t_begin += tb;
+        ids = fetch_pages(0);
     }
-    if (t_begin >= t_end && (seg > 0 || a.nseg > 1)) return;     // (the merge counts the segments that have tiles)
-    t_begin += wave;
-    const int steps = t_begin < t_end ? (t_end - t_begin + NW - 1) / NW : 0;
+    const int steps = t_begin < te ? (te - t_begin + stride - 1) / stride : 0;
 
     unsigned char *vs = lds + wave * C::TILE;
     const size_t page_bytes = ((size_t)a.Hkv << a.table.shift) * C::ROW, head_bytes = ((size_t)hk << a.table.shift) * C::ROW;
-    const unsigned char *kp = a.k + head_bytes, *vp = a.v + head_bytes;
+    const unsigned char *kp = k + head_bytes, *vp = v + head_bytes;
     const int row_mask = (1 << a.table.shift) - 1;
-    const int *pages = a.table.pages + (size_t)b * a.table.width;
-    // the pages of the half tiles of 32 steps, one to a lane; -1: none
-    auto fetch_pages = [&](int step0) __attribute__((always_inline)) {
-        const int tile = t_begin + (step0 + (lane >> 1)) * NW, e = (tile * TILE_KEYS + (lane & 1) * 16) >> a.table.shift;
-        int id = -1;
-        if (tile < t_end && e < a.table.width) id = pages[e];
-        return (unsigned)id < (unsigned)a.table.count ? id : -1;
-    };
     u32x4 kf[2][KK];
     auto load_k = [&](int t, int id0, int id1) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const unsigned char *at = kp + (size_t)(unsigned)max(h ? id1 : id0, 0) * page_bytes + (size_t)((t * TILE_KEYS + h * 16) & row_mask) * C::ROW;
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) kf[h][kk] = *(const u32x4 *)(at + (unsigned)(n * C::ROW + g * 16) + kk * 64);
+            for (int kk = 0; kk < KK; ++kk) {
+                const u32x4 *from = (const u32x4 *)(at + (unsigned)(n * C::ROW + g * 16) + kk * 64);
+                kf[h][kk] = ONCE ? __builtin_nontemporal_load(from) : *from;
+            }
         }
     };
     // V: 1 KiB an instruction, straight into LDS. 16-byte chunk c of key k lies at slot c ^ (2 * ((k >> 2) & 3)) ^ (8 * (k & 1)) of its row (the last term for rows
     // of 256 bytes and more), so that the sixteen keys of a transposing read fall on distinct banks.
     constexpr int NVI = C::TILE / 1024, KEYS_PER_VI = 1024 / C::ROW;
     const int v_key_in = (lane * 16) / C::ROW, v_slot = ((lane * 16) % C::ROW) / 16;
-    (void)v_key_in; (void)v_slot; (void)vp; (void)NVI; (void)KEYS_PER_VI;
+    constexpr int NON_TEMPORAL = 2;                              // the nt bit of a buffer access
+    (void)v_slot; (void)vp; (void)NON_TEMPORAL;
     auto load_v = [&](int t, int id0, int id1) __attribute__((always_inline)) {
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
@@ -186,39 +193,140 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a
             for (int i = 0; i < NVI / 2; ++i) {
                 const int key = i * KEYS_PER_VI + v_key_in;
                 const int chunk = v_slot ^ (2 * ((key >> 2) & 3)) ^ (D >= 128 ? 8 * (key & 1) : 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(vs + (h * (NVI / 2) + i) * 1024), 16, key * C::ROW + chunk * 16, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(vs + (h * (NVI / 2) + i) * 1024), 16, key * C::ROW + chunk * 16, 0, 0, ONCE ? NON_TEMPORAL : 0);
             }
         }
 #endif
     };
+    // a lane's page number as a scalar, -1: none
+    auto page_at = [&](int l) __attribute__((always_inline)) {
+        const int id = __builtin_amdgcn_readlane(ids, l);
+        return (unsigned)id < (unsigned)a.table.count ? id : -1;
+    };
+    int id0 = -1, id1 = -1;
+    auto begin = [&]() __attribute__((always_inline)) {
+        id0 = page_at(0), id1 = page_at(1);
+        load_k(t_begin, id0, id1);
+        load_v(t_begin, id0, id1);
+    };
+    if (steps > 0) begin();
+
+    // ---- the queries as operands in LDS, under the first tile's way: [part][k-step][16-byte piece of 4][row]
+    unsigned char *qs = lds + C::MAIN;
+    float *q_scale = (float *)(qs + QP * q_rows * C::ROW);       // what brings a row's products back to q . k
+    const int q_shift = q_rows == 16 ? 4 : 3;
+#pragma unroll
+    for (int i = 0; i < QSETS; ++i) {
+        const int row = q_row + i * QROWS;
+        const unsigned at = (unsigned)(((q_col / 8) << q_shift) + row) * 16;
+        if constexpr (QP == 1) {
+            if (row < q_rows) *(u32x4 *)(qs + at) = qh[i];
+            if (row < q_rows && q_col == 0) q_scale[row] = 1.f;
+        } else {
+            float factor = 1.f, back = 1.f;
+            if constexpr (KV == AIONHIP_F16) {
+                // a row goes into f16's range by a power of two that takes its largest element to 2^10: what the second half rounds away then lies 2^-35 below that
+                float top = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(qx[i][j]));
+                top = fmaxf(top, dpp_f<DPP_QUAD_XOR1>(top));
+                top = fmaxf(top, dpp_f<DPP_QUAD_XOR2>(top));
+                top = fmaxf(top, dpp_f<DPP_ROW_HALF_MIRROR>(top));
+                if constexpr (QT > 8) top = fmaxf(top, dpp_f<DPP_ROW_MIRROR>(top));
+                if constexpr (QT > 16) {
+                    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                    top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                }
+                const int e = (int)(__float_as_uint(top) >> 23);
+                const int f = e == 255 ? 127 : max(1, min(264 - e, 253));
+                factor = __uint_as_float((unsigned)f << 23);
+                back = __uint_as_float((unsigned)(254 - f) << 23);
+            }
+            u32x4 part[QP];
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                float u = qx[i][j] * factor, w = qx[i][j + 1] * factor;
+#pragma unroll
+                for (int p = 0; p < QP; ++p) {
+                    const unsigned both = pack2<KV>(u, w);
+                    part[p][j / 2] = both;
+                    // (an infinite element has no rest)
+                    const float ru = u - from_half_bits<KV>((unsigned short)both), rw = w - from_half_bits<KV>((unsigned short)(both >> 16));
+                    u = fabsf(ru) < INFINITY ? ru : 0.f;
+                    w = fabsf(rw) < INFINITY ? rw : 0.f;
+                }
+            }
+            if (row < q_rows) {
+#pragma unroll
+                for (int p = 0; p < QP; ++p) *(u32x4 *)(qs + p * q_rows * C::ROW + at) = part[p];
+                if (q_col == 0) q_scale[row] = back;
+            }
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");       // (no wait for the K and V loads in flight)
+    const int q_mine = n & (q_rows - 1);                         // (of eight rows, the upper eight columns are the lower once more, and nobody's)
+    const unsigned q_addr = (unsigned)(size_t)(lds_void *)qs + (unsigned)(((g << q_shift) + q_mine) * 16), q_part = (unsigned)(q_rows * C::ROW), q_step = 64u << q_shift;
+    float to_log2;
+    {
+        u32x2 x;
+        asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x.x) : "v"((unsigned)(size_t)(lds_void *)q_scale + (unsigned)q_mine * 4) : "memory");
+        const float back = __uint_as_float(x.x);
+        to_log2 = a.soft_cap > 0.f ? back * (a.scale / a.soft_cap) : back * (a.scale * LOG2E);
+    }
+    const float cap_log2 = a.soft_cap * LOG2E;
+
     const int tr_r = (lane >> 2) & 3, tr_q = lane & 3;
     const unsigned v_rowaddr = (unsigned)(size_t)(lds_void *)vs + (unsigned)((4 * g + tr_r) * C::ROW + (tr_q & 1) * 8);
     const unsigned v_slot_l = (unsigned)(((tr_q >> 1) ^ (2 * g) ^ (D >= 128 ? 8 * (tr_r & 1) : 0)) << 4);
-    auto v_operand = [&](auto mt_c) __attribute__((always_inline)) {
+    auto v_operand = [&](unsigned vr, unsigned vl, auto mt_c) __attribute__((always_inline)) {
         constexpr int mt = decltype(mt_c)::value;
-        const unsigned addr = v_rowaddr + (v_slot_l ^ (unsigned)(mt << 5));
+        const unsigned addr = vr + (vl ^ (unsigned)(mt << 5));
         u32x2 a0, a1;
         asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3" : "=&v"(a0), "=&v"(a1) : "v"(addr), "n"(16 * C::ROW) : "memory");
         return u32x4{a0.x, a0.y, a1.x, a1.y};
     };
 
     f32x4 acc[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref = MASKED, l_run = 0.f;                             // l_run: of this lane's keys
-    float *scores = WEIGH ? a.scores + ((size_t)unit * a.rows_total + r) * a.tpad : nullptr;
+    float *scores = a.scores + ((size_t)unit * rows_total + r) * a.tpad;
+    // A sum of halves times something infinite is no number where a half is zero or of the other sign. A wavefront that ends with such walks its tiles again with care: scores
+    // that are no numbers are the first halves' then, and every half of a probability but the last is taken from slightly less than what is left, so that all are above zero.
+    bool care = false;
 
     // MORE: another tile of this wavefront follows (two copies of the body, so that every path requests K and V in the same order and the count of loads in flight holds)
     auto tile = [&](int t, bool ok0, bool ok1, int next0, int next1, auto more_c) __attribute__((always_inline)) {
         constexpr bool more = decltype(more_c)::value;
         const int key0 = t * TILE_KEYS;
         f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        // (the operands' addresses are made anew for each tile: kept, they would take the registers of two wavefronts' worth of keys in flight)
+        unsigned qa = q_addr, vr = v_rowaddr, vl = v_slot_l;
+        asm volatile("" : "+v"(qa), "+v"(vr), "+v"(vl));
+        constexpr int QA = KK * QP < 4 ? KK * QP : 4;            // operands requested ahead
+        u32x4 qf[QA];
+        auto q_operand = [&](auto ic) __attribute__((always_inline)) {
+            constexpr int i = decltype(ic)::value;
+            return lds_read<0>(qa + (unsigned)(i / QP) * q_step + (unsigned)(i % QP) * q_part);
+        };
+        static_for<0, QA>([&](auto ic) __attribute__((always_inline)) { qf[decltype(ic)::value] = q_operand(ic); });
+        static_for<0, KK * QP>([&](auto ic) __attribute__((always_inline)) {
+            constexpr int i = decltype(ic)::value, later = KK * QP - 1 - i < QA - 1 ? KK * QP - 1 - i : QA - 1;
+            asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(qf[i % QA]) : "n"(later));
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+            for (int h = 0; h < 2; ++h) s[h] = mfma16<KV>(kf[h][i / QP], qf[i % QA], s[h]);
+            if constexpr (i + QA < KK * QP) qf[i % QA] = q_operand(std::integral_constant<int, i + QA>{});
+        });
+        if (QP > 1 && care) {
+            f32x4 first[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+            static_for<0, KK>([&](auto ic) __attribute__((always_inline)) {
+                constexpr int kk = decltype(ic)::value;
+                u32x4 x = q_operand(std::integral_constant<int, kk * QP>{});
+                asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x));
 #pragma unroll
-            for (int p = 0; p < QP; ++p)
+                for (int h = 0; h < 2; ++h) first[h] = mfma16<KV>(kf[h][kk], x, first[h]);
+            });
 #pragma unroll
-                for (int h = 0; h < 2; ++h) s[h] = mfma16<KV>(kf[h][kk], qf[p][kk], s[h]);
+            for (int j = 0; j < 8; ++j) s[j >> 2][j & 3] = s[j >> 2][j & 3] != s[j >> 2][j & 3] ? first[j >> 2][j & 3] : s[j >> 2][j & 3];
+        }
         const bool full = key0 >= all_lo && key0 + TILE_KEYS <= all_hi && ok0 && ok1;      // every row sees every key
         // lane: keys key0 + h * 16 + g * 4 + i of row n
         float p[8];
@@ -239,14 +347,14 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a
                 seen |= see ? 1u << j : 0u;
             }
         }
-        if constexpr (WEIGH) {
+        if (a.scores) {
             if (row_ok) {
                 *(f32x4 *)(scores + key0 + g * 4) = f32x4{p[0], p[1], p[2], p[3]};
                 *(f32x4 *)(scores + key0 + 16 + g * 4) = f32x4{p[4], p[5], p[6], p[7]};
             }
         }
         if (more) {
-            load_k(t + NW, next0, next1);
+            load_k(t + stride, next0, next1);
             asm volatile("" ::: "memory");         // requested here, ahead of the counted wait for V below
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
@@ -260,7 +368,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a
                 ref = ref_new;
             }
         }
-        const float base = (ref > MASKED ? ref : 0.f) - HEAD_ROOM;
+        const float base = (ref > MASKED ? ref : 0.f) - HEAD_ROOM, less = care ? LESS<KV> : 1.f;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -274,7 +382,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a
             float u = p[j], w = p[j + 1];
 #pragma unroll
             for (int part = 0; part < PP; ++part) {
-                const unsigned both = part + 1 < PP ? pack2<KV>(u * LESS<KV>, w * LESS<KV>) : pack2<KV>(u, w);
+                const unsigned both = part + 1 < PP ? pack2<KV>(u * less, w * less) : pack2<KV>(u, w);
                 pf[part][j / 2] = both;
                 u -= from_half_bits<KV>((unsigned short)both);
                 w -= from_half_bits<KV>((unsigned short)(both >> 16));
@@ -288,193 +396,269 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64) void paged_attn_kernel(PagedArgs a
         if (!full) {
             // Rows that no query sees count as zeros (they may hold anything, and zero times that need not be zero). Where a row is seen by some and not finite, the
             // queries are taken one by one below.
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < NVI; ++i) {
                 const int key = key0 + i * KEYS_PER_VI + v_key_in;
                 u32x4 *at = (u32x4 *)(vs + i * 1024 + lane * 16);
                 if (key < uni_lo || key >= uni_hi || !(i < NVI / 2 ? ok0 : ok1)) {
                     *at = u32x4{0u, 0u, 0u, 0u};
-                } else {
+                } else if constexpr (MULTI) {
                     constexpr unsigned EXP = KV == AIONHIP_F16 ? 0x7C00u : 0x7F80u;
                     const u32x4 x = *at;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) odd |= (x[j] & EXP) == EXP || (x[j] >> 16 & EXP) == EXP;
                 }
             }
-            odd = __any(odd);
+            if constexpr (MULTI) odd = __any(odd);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        if (!odd) {
+        if (!MULTI || !odd) {
             constexpr int VA = MT < 4 ? MT : 4;                  // operands requested ahead
             u32x4 vop[VA];
-            static_for<0, VA>([&](auto mc) __attribute__((always_inline)) { vop[decltype(mc)::value] = v_operand(mc); });
+            static_for<0, VA>([&](auto mc) __attribute__((always_inline)) { vop[decltype(mc)::value] = v_operand(vr, vl, mc); });
             static_for<0, MT>([&](auto mc) __attribute__((always_inline)) {
                 constexpr int mt = decltype(mc)::value;
                 constexpr int later = MT - 1 - mt < VA - 1 ? MT - 1 - mt : VA - 1;
                 asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(vop[mt % VA]) : "n"(2 * later));
 #pragma unroll
                 for (int part = 0; part < PP; ++part) acc[mt] = mfma16<KV>(vop[mt % VA], pf[part], acc[mt]);
-                if constexpr (mt + VA < MT) vop[mt % VA] = v_operand(std::integral_constant<int, mt + VA>{});
+                if constexpr (mt + VA < MT) vop[mt % VA] = v_operand(vr, vl, std::integral_constant<int, mt + VA>{});
             });
-        } else {
+        } else if constexpr (MULTI) {
             // a query at a time, with zeros for the keys that it does not see, into that query's sums alone
-            for (int q = 0; q < 16; ++q) {
-                const unsigned mine = (unsigned)__shfl((int)seen, (lane & 48) + q, 64);
+            for (int i = 0; i < 16; ++i) {
+                const unsigned mine = (unsigned)__shfl((int)seen, (lane & 48) + i, 64);
                 static_for<0, MT>([&](auto mc) __attribute__((always_inline)) {
                     constexpr int mt = decltype(mc)::value;
-                    u32x4 v = v_operand(mc);
-                    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v));
+                    u32x4 x = v_operand(vr, vl, mc);
+                    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] &= (mine >> (2 * j) & 1u ? 0xFFFFu : 0u) | (mine >> (2 * j + 1) & 1u ? 0xFFFF0000u : 0u);
+                    for (int j = 0; j < 4; ++j) x[j] &= (mine >> (2 * j) & 1u ? 0xFFFFu : 0u) | (mine >> (2 * j + 1) & 1u ? 0xFFFF0000u : 0u);
                     f32x4 c = acc[mt];
 #pragma unroll
-                    for (int part = 0; part < PP; ++part) c = mfma16<KV>(v, pf[part], c);
-                    if (n == q) acc[mt] = c;
+                    for (int part = 0; part < PP; ++part) c = mfma16<KV>(x, pf[part], c);
+                    if (n == i) acc[mt] = c;
                 });
             }
         }
         if (more) {
             asm volatile("" ::: "memory");         // the operand reads above are complete: each was waited for before its product
-            load_v(t + NW, next0, next1);
+            load_v(t + stride, next0, next1);
         }
     };
-    if (steps > 0) {
-        int ids = fetch_pages(0);
-        int id0 = __builtin_amdgcn_readlane(ids, 0), id1 = __builtin_amdgcn_readlane(ids, 1);
-        load_k(t_begin, id0, id1);
-        load_v(t_begin, id0, id1);
+    for (;;) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        ref = MASKED, l_run = 0.f;
+        if (steps == 0) break;
         int t = t_begin;
-        for (int i = 1; i < steps; ++i, t += NW) {
+        for (int i = 1; i < steps; ++i, t += stride) {
             if ((i & 31) == 0) ids = fetch_pages(i);
-            const int next0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31)), next1 = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + 1);
+            const int next0 = page_at(2 * (i & 31)), next1 = page_at(2 * (i & 31) + 1);
             tile(t, id0 >= 0, id1 >= 0, next0, next1, std::true_type{});
             id0 = next0, id1 = next1;
         }
         tile(t, id0 >= 0, id1 >= 0, 0, 0, std::false_type{});
+        bool none = l_run != l_run;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) none |= acc[mt][j] != acc[mt][j];
+        if (care || !__any(none)) break;
+        care = true;
+        if (steps > 32) ids = fetch_pages(0);
+        begin();
     }
     l_run = groups4_sum(l_run);
 
-    // ---- the wavefronts meet in LDS
-    __syncthreads();
-    float *mg = (float *)lds;
-    {
-        float *w = mg + wave * C::SLOT;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) *(f32x4 *)(w + n * (D + 4) + mt * 16 + g * 4) = acc[mt];
-        if (g == 0) { w[16 * (D + 4) + n] = ref; w[16 * (D + 4) + 16 + n] = l_run; }
-    }
-    __syncthreads();
-    const bool alone = !WEIGH && a.nseg == 1;
-    for (int e = threadIdx.x; e < 16 * D / 4; e += NW * 64) {
-        const int row = e / (D / 4), col = (e % (D / 4)) * 4, rr = rt * 16 + row;
-        if (rr >= a.rows_total) break;
-        float top = MASKED, l = 0.f;
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) top = fmaxf(top, mg[w * C::SLOT + 16 * (D + 4) + row]);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float rw = mg[w * C::SLOT + 16 * (D + 4) + row];
-            // (a wavefront without a reference has seen nothing, or what is not a number: its sums then say so)
-            const float f = rw > MASKED ? __builtin_amdgcn_exp2f(rw - top) : 1.f;
-            l += mg[w * C::SLOT + 16 * (D + 4) + 16 + row] * f;
-            o += *(const f32x4 *)(mg + w * C::SLOT + row * (D + 4) + col) * f;
-        }
-        if (alone) {
-            const int l2 = rr / a.groups, g2 = rr - l2 * a.groups;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            *(f32x4 *)(a.out + (((size_t)b * a.L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + col) = o * inv;
-        } else {
-            *(f32x4 *)(a.partial + (((size_t)(unit * a.row_tiles + rt) * a.nseg + seg) * 16 + row) * D + col) = o;
-            if (col == 0) a.stats[((size_t)unit * a.rows_total + rr) * a.nseg + seg] = float2{top, l};
-        }
-    }
-}
-
-// How many segments of a row's tile have tiles; every row of the tile agrees on it.
-__device__ __forceinline__ int segments_of(const PagedArgs &a, int b, int rt, int nw) {
-    int uni_lo = INT_MAX, uni_hi = 0;
-    const int len = a.kv_lengths ? a.kv_lengths[b] : 0;
-    for (int i = 0; i < 16; ++i) {
-        const int r = rt * 16 + i;
-        if (r >= a.rows_total) break;
-        int lo, hi;
-        const int li = r / a.groups;
-        row_keys(a, b, li, len, a.positions ? a.positions[(size_t)b * a.L + li] : 0, lo, hi);
-        if (hi > lo) uni_lo = min(uni_lo, lo), uni_hi = max(uni_hi, hi);
-    }
-    if (uni_hi <= uni_lo) return 0;
-    const int tiles = (uni_hi + TILE_KEYS - 1) / TILE_KEYS - uni_lo / TILE_KEYS, per = tiles_each(tiles, a.nseg, nw);
-    return (tiles + per - 1) / per;
-}
-
-// The first merge_rows workgroups of a unit add the segments of a row each, the others (where weights are asked for) have 1024 keys each.
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a, int nw, int merge_rows) {
-    __shared__ float red[256];
-    __shared__ __attribute__((aligned(16))) f32x4 s_o[256];
-    const int hk = blockIdx.y, b = blockIdx.z, unit = b * a.Hkv + hk, tid = threadIdx.x;
-    if ((int)blockIdx.x < merge_rows) {
-        const int r = blockIdx.x, rt = r >> 4, nseg = segments_of(a, b, rt, nw);
-        const float2 *st = a.stats + ((size_t)unit * a.rows_total + r) * a.nseg;
-        const int per = a.d / 4, sets = 256 / per, set = tid / per, col = (tid - set * per) * 4;
-        float top = MASKED;
-        for (int s = 0; s < nseg; ++s) top = fmaxf(top, st[s].x);
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
-        for (int s = set; s < nseg; s += sets) {
-            const float f = st[s].x > MASKED ? __builtin_amdgcn_exp2f(st[s].x - top) : 1.f;
-            l += st[s].y * f;
-            o += *(const f32x4 *)(a.partial + (((size_t)(unit * a.row_tiles + rt) * a.nseg + s) * 16 + (r & 15)) * a.d + col) * f;
-        }
-        s_o[tid] = o;
-        red[tid] = l;
-        __syncthreads();
-        if (set > 0) return;
-        for (int i = 1; i < sets; ++i) o += s_o[i * per + tid], l += red[i * per + tid];
-        const int l2 = r / a.groups, g2 = r - l2 * a.groups;
+    const int rows = min(16, rows_total - rt * 16);
+    auto put = [&](int row, int col, f32x4 o, float top, float l) __attribute__((always_inline)) {
+        const int rr = rt * 16 + row, l2 = L > 1 ? rr / a.groups : 0, g2 = rr - l2 * a.groups;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        *(f32x4 *)(a.out + (((size_t)b * a.L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * a.d + col) = o * inv;
-        return;
-    }
-    const int key = ((int)blockIdx.x - merge_rows) * 1024 + tid * 4;
-    __shared__ float s_top[16], s_inv[16];
-    __shared__ int s_lo[16], s_hi[16];
-    f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int rt = 0; rt < (a.rows_total + 15) / 16; ++rt) {
-        const int nseg = segments_of(a, b, rt, nw);
+        *(f32x4 *)(a.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + col) = o * inv;
+        if (a.stats && col == 0) a.stats[(size_t)unit * rows_total + rr] = float2{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
+    };
+    // Device-scope accesses: written through, read at the point where the XCDs' caches agree.
+    constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access
+    (void)DEVICE_SCOPE;
+    const int meeting = unit * a.row_tiles + rt;
+    [[maybe_unused]] float *const slots = a.partial + (size_t)meeting * a.nseg * C::PART;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const __amdgpu_buffer_rsrc_t slots_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)slots, 0, (unsigned)(a.nseg * C::PART * 4), 0x00027000);
+#endif
+    auto publish = [&](int row, int col, f32x4 o, float top, float l) __attribute__((always_inline)) {
+        if (live <= 1) {
+            put(row, col, o, top, l);
+            return;
+        }
+#if defined(__HIP_DEVICE_COMPILE__)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), slots_rsrc, (seg * C::PART + row * D + col) * 4, 0, DEVICE_SCOPE);
+        if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(l)}, slots_rsrc, (seg * C::PART + 16 * D + row * 2) * 4, 0, DEVICE_SCOPE);
+#endif
+    };
+    if (te - tb <= a.nseg) {                                     // the first wavefront has all there is
+        if (wave == 0 && row_ok) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) publish(n, mt * 16 + g * 4, acc[mt], ref, l_run);
+        }
+    } else {
+        // ---- the wavefronts meet in LDS
         __syncthreads();
-        if (tid < 16) {
-            const int r = rt * 16 + tid;
-            int lo = 0, hi = 0;
-            float top = MASKED, l = 0.f;
-            if (r < a.rows_total) {
-                const int li = r / a.groups;
-                row_keys(a, b, li, a.kv_lengths ? a.kv_lengths[b] : 0, a.positions ? a.positions[(size_t)b * a.L + li] : 0, lo, hi);
-                const float2 *st = a.stats + ((size_t)unit * a.rows_total + r) * a.nseg;
-                for (int s = 0; s < nseg; ++s) top = fmaxf(top, st[s].x);
-                for (int s = 0; s < nseg; ++s) l += st[s].y * (st[s].x > MASKED ? __builtin_amdgcn_exp2f(st[s].x - top) : 1.f);
+        float *mg = (float *)lds;
+        if (row_ok) {
+            float *w = mg + wave * C::SLOT;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) *(f32x4 *)(w + n * (D + 4) + mt * 16 + g * 4) = acc[mt];
+            if (g == 0) { w[16 * (D + 4) + n] = ref; w[16 * (D + 4) + 16 + n] = l_run; }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * (D / 4); e += NW * 64) {
+            const int row = e / (D / 4), col = (e % (D / 4)) * 4;
+            float rw[NW], lw[NW], top = MASKED, l = 0.f;
+            f32x4 ow[NW], o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                rw[w] = mg[w * C::SLOT + 16 * (D + 4) + row];
+                lw[w] = mg[w * C::SLOT + 16 * (D + 4) + 16 + row];
+                ow[w] = *(const f32x4 *)(mg + w * C::SLOT + row * (D + 4) + col);
+                top = fmaxf(top, rw[w]);
             }
-            s_lo[tid] = lo, s_hi[tid] = hi;
-            s_top[tid] = (top > MASKED ? top : 0.f) - HEAD_ROOM;
-            s_inv[tid] = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                // (a wavefront without a reference has seen nothing, or what is not a number: its sums then say so)
+                const float f = rw[w] > MASKED ? __builtin_amdgcn_exp2f(rw[w] - top) : 1.f;
+                l += lw[w] * f;
+                o += ow[w] * f;
+            }
+            publish(row, col, o, top, l);
+        }
+    }
+    if (live <= 1) return;
+
+    // ---- the workgroup that ends last adds the segments: each publishes its part, waits until the stores have been acknowledged and takes a ticket; whoever draws the
+    // last one finds all of them. Nobody waits for anybody.
+    __syncthreads();
+    int *s_ticket = (int *)lds;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) *s_ticket = (int)__hip_atomic_fetch_add(a.tickets + meeting * MEET_TICKET_WORDS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*s_ticket != live - 1) return;
+    if (threadIdx.x == 0) __hip_atomic_store(a.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    float *s_f = (float *)lds, *s_top = s_f + 16 * C::MOST, *s_l = s_top + 16;      // factors of the segments of each row
+    f32x4 *s_o = (f32x4 *)(lds + (16 * C::MOST + 64) * 4);
+    // A wavefront derives the segments' factors for every NW-th row, a lane to a segment; all are asked for at once.
+    constexpr int EACH = 16 / NW;
+    u32x2 st[EACH][C::MOST / 64];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+#pragma unroll
+        for (int j = 0; j < C::MOST / 64; ++j) {
+            st[i][j] = u32x2{__float_as_uint(MASKED), 0u};
+#if defined(__HIP_DEVICE_COMPILE__)
+            if (wave + i * NW < rows && lane + 64 * j < live)
+                st[i][j] = __builtin_amdgcn_raw_buffer_load_b64(slots_rsrc, ((lane + 64 * j) * C::PART + 16 * D + (wave + i * NW) * 2) * 4, 0, DEVICE_SCOPE);
+#endif
+        }
+    // A thread has four columns of a row; where there are more threads than that, several share the segments. Eight parts at a time, the next eight asked for ahead.
+    const int pieces = rows * (D / 4), sets = max(1, NW * 64 / pieces), set = (int)threadIdx.x / pieces;
+    const bool mine = set < sets;
+    int e = (int)threadIdx.x - set * pieces, s0 = set;
+    u32x4 x[2][8];
+    auto ask = [&](u32x4 (&to)[8], int e, int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            [[maybe_unused]] const int s = s0 + j * sets;        // (past the last segment: past the buffer's end, which reads as zeros)
+            to[j] = u32x4{0u, 0u, 0u, 0u};
+#if defined(__HIP_DEVICE_COMPILE__)
+            to[j] = __builtin_amdgcn_raw_buffer_load_b128(slots_rsrc, s < live && e < pieces ? (s * C::PART + e / (D / 4) * D + e % (D / 4) * 4) * 4 : 0x7FFFFFF0, 0, DEVICE_SCOPE);
+#endif
+        }
+    };
+    ask(x[0], e, s0);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int row = wave + i * NW;
+        if (row >= rows) break;
+        float top = MASKED, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::MOST / 64; ++j) top = fmaxf(top, __uint_as_float(st[i][j].x));
+        top = lanes_max(top);
+#pragma unroll
+        for (int j = 0; j < C::MOST / 64; ++j) {
+            const float sr = __uint_as_float(st[i][j].x), f = sr > MASKED ? __builtin_amdgcn_exp2f(sr - top) : 1.f;
+            s_f[row * C::MOST + lane + 64 * j] = lane + 64 * j < live ? f : 0.f;
+            sum += __uint_as_float(st[i][j].y) * f;
+        }
+        sum = lanes_sum(sum);
+        if (lane == 0) s_top[row] = top, s_l[row] = sum;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    // one round: eight parts added, and the piece written with its last ones; false: none are left
+    auto round = [&](u32x4 (&now)[8], u32x4 (&next)[8]) __attribute__((always_inline)) {
+        const bool last = s0 + 8 * sets - set >= live;           // (the same for all threads)
+        const int e2 = last ? e + NW * 64 : e, s2 = last ? set : s0 + 8 * sets;
+        const bool more = !last || (sets == 1 && e2 - (int)threadIdx.x < pieces);
+        if (more) ask(next, e2, s2);
+        const int row = min(e / (D / 4), 15);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o += __builtin_bit_cast(f32x4, now[j]) * (s0 + j * sets < live ? s_f[row * C::MOST + s0 + j * sets] : 0.f);
+        if (last) {
+            if (sets > 1) {
+                s_o[threadIdx.x] = o;
+                __syncthreads();
+                if (set == 0)
+                    for (int i = 1; i < sets; ++i) o += s_o[i * pieces + threadIdx.x];
+            }
+            if (mine && set == 0 && e < pieces) put(row, e % (D / 4) * 4, o, s_top[row], s_l[row]);
+            o = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        e = e2, s0 = s2;
+        return more;
+    };
+    while (round(x[0], x[1]) && round(x[1], x[0])) {}
+}
+
+// What the keys draw: a thread has four of them, of 1024 to a workgroup, and adds the rows' probabilities in order. stats: a row's reference and the reciprocal of its sum.
+constexpr int WEIGH_ROWS = 64;
+__global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
+    __shared__ float2 s_stat[WEIGH_ROWS];
+    __shared__ int2 s_keys[WEIGH_ROWS];
+    const int hk = blockIdx.y, b = blockIdx.z, unit = b * a.Hkv + hk, tid = threadIdx.x, key = (int)blockIdx.x * 1024 + tid * 4;
+    const size_t at = (size_t)unit * a.T + key;
+    f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int len = a.kv_lengths ? a.kv_lengths[b] : 0;
+    for (int r0 = 0; r0 < a.rows_total; r0 += WEIGH_ROWS) {
+        const int rows = min(WEIGH_ROWS, a.rows_total - r0);
+        if (r0) __syncthreads();
+        if (tid < rows) {
+            const int r = r0 + tid, li = a.L > 1 ? r / a.groups : 0;
+            int lo, hi;
+            row_keys(a, b, li, len, a.positions ? a.positions[(size_t)b * a.L + li] : 0, lo, hi);
+            s_keys[tid] = int2{lo, hi};
+            s_stat[tid] = a.stats[(size_t)unit * a.rows_total + r];
         }
         __syncthreads();
         if (key < a.T)
-            for (int i = 0; i < 16 && rt * 16 + i < a.rows_total; ++i) {
-                if (key >= s_hi[i] || key + 4 <= s_lo[i]) continue;
-                const f32x4 s = *(const f32x4 *)(a.scores + ((size_t)unit * a.rows_total + rt * 16 + i) * a.tpad + key);
+            for (int i = 0; i < rows; ++i) {
+                const int2 see = s_keys[i];
+                if (key >= see.y || key + 4 <= see.x) continue;
+                const f32x4 s = *(const f32x4 *)(a.scores + ((size_t)unit * a.rows_total + r0 + i) * a.tpad + key);
+                const float2 st = s_stat[i];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (key + j >= s_lo[i] && key + j < s_hi[i]) w[j] += __builtin_amdgcn_exp2f(s[j] - s_top[i]) * s_inv[i];
+                    if (key + j >= see.x && key + j < see.y) w[j] += __builtin_amdgcn_exp2f(s[j] - st.x) * st.y;
             }
     }
     if (key < a.T) {                             // (a capacity is a multiple of sixteen)
-        const size_t at = (size_t)unit * a.T + key;
-        if (a.weights_before)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] += a.weights_before[at + j];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a.weights[at + j] = w[j];
+        if (a.weights_before) {
+            f32x4 before;
+            __builtin_memcpy(&before, a.weights_before + at, 16);
+            w += before;
+        }
+        __builtin_memcpy(a.weights + at, &w, 16);
     }
 }
 
@@ -531,32 +715,41 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int c = threadIdx.x; c < a.d; c += 256) a.out[qbase + c] = (s_o[0][c] * f[0] + s_o[1][c] * f[1] + s_o[2][c] * f[2] + s_o[3][c] * f[3]) * inv;
-    if (a.stats && threadIdx.x == 0) a.stats[(size_t)unit * a.rows_total + r] = float2{top, sum * __builtin_amdgcn_exp2f(HEAD_ROOM)};
+    if (a.stats && threadIdx.x == 0) a.stats[(size_t)unit * a.rows_total + r] = float2{top > MASKED ? top : 0.f, inv};
 }
 
-template <int KV, int D, int QP>
+template <int KV, int D, int QP, bool MULTI, bool ONCE>
 int launch(aionhip_ctx *ctx, const PagedArgs &a, int batch) {
+    const auto kernel = paged_attn_kernel<KV, D, QP, MULTI, ONCE>;
+    const int q_rows = D == 256 && a.rows_total <= 8 ? 8 : 16;
+    const size_t lds = Cfg<D>::MAIN + QP * q_rows * Cfg<D>::ROW + 64;
+    static std::atomic<uint64_t> attr{0};
+    if (const int rc = allow_lds(ctx, attr, (const void *)kernel, Cfg<D>::MAIN + QP * 16 * Cfg<D>::ROW + 64)) return rc;
     ProfScope scope(ctx, "paged_attn");
-    const dim3 grid((unsigned)(a.row_tiles * a.nseg), (unsigned)a.Hkv, (unsigned)batch), block(Cfg<D>::NW * 64);
-    static std::atomic<uint64_t> attr[2];
-    const void *fn = a.weights ? (const void *)paged_attn_kernel<KV, D, QP, true> : (const void *)paged_attn_kernel<KV, D, QP, false>;
-    if (const int rc = allow_lds(ctx, attr[a.weights ? 1 : 0], fn, Cfg<D>::LDS)) return rc;
-    if (a.weights) launch_k(ctx, paged_attn_kernel<KV, D, QP, true>, grid, block, Cfg<D>::LDS, a);
-    else launch_k(ctx, paged_attn_kernel<KV, D, QP, false>, grid, block, Cfg<D>::LDS, a);
+    launch_k(ctx, kernel, dim3((unsigned)(a.row_tiles * a.nseg), (unsigned)a.Hkv, (unsigned)batch), dim3(Cfg<D>::NW * 64), lds, a.kv_lengths, a.q, a.table.pages, a.k, a.v, a.T, a.L,
+             (unsigned)a.Hkv | (unsigned)a.groups << 16, (unsigned)a.nseg | (unsigned)a.table.shift << 12 | (unsigned)a.q_dtype << 16 | (unsigned)q_rows << 24, a);
     LAUNCH_CHECK(ctx, "paged_attn");
     return AIONHIP_OK;
 }
+template <int KV, int D, int QP>
+int launch_form(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
+    if (a.L > 1) return launch<KV, D, QP, true, false>(ctx, a, batch);
+    return once ? launch<KV, D, QP, false, true>(ctx, a, batch) : launch<KV, D, QP, false, false>(ctx, a, batch);
+}
 template <int KV, int D>
-int launch_parts(aionhip_ctx *ctx, const PagedArgs &a, int batch) {
-    if (a.q_dtype == KV) return launch<KV, D, 1>(ctx, a, batch);
-    return launch<KV, D, KV == AIONHIP_F16 ? 2 : 3>(ctx, a, batch);
+int launch_parts(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
+    if (a.q_dtype == KV) return launch_form<KV, D, 1>(ctx, a, batch, once);
+    return launch_form<KV, D, KV == AIONHIP_F16 ? 2 : 3>(ctx, a, batch, once);
 }
 template <int KV>
-int launch_head(aionhip_ctx *ctx, const PagedArgs &a, int batch) {
-    if (a.d == 64) return launch_parts<KV, 64>(ctx, a, batch);
-    if (a.d == 128) return launch_parts<KV, 128>(ctx, a, batch);
-    return launch_parts<KV, 256>(ctx, a, batch);
+int launch_head(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
+    if (a.d == 64) return launch_parts<KV, 64>(ctx, a, batch, once);
+    if (a.d == 128) return launch_parts<KV, 128>(ctx, a, batch, once);
+    return launch_parts<KV, 256>(ctx, a, batch, once);
 }
+
+// keys and values of this many bytes go past the caches (see the launcher)
+constexpr size_t ONCE_BYTES = (size_t)192 << 20;
 
 }  // namespace
 
@@ -596,38 +789,42 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     a.scale = p->scale, a.soft_cap = p->attn_logits_soft_cap;
     a.win_left = p->window_left, a.win_right = p->window_right, a.win_chunk = p->window_chunk;
     const bool fast = (c->d == 64 || c->d == 128 || c->d == 256) && (p->out & 15) == 0;
-    const int nw = c->d == 256 ? 4 : 8;
     a.nseg = 1;
+    bool once = false;
     if (fast) {
         // Behind a window there are no more keys than it shows to the call's consecutive queries.
         long keys = a.T;
         if (!a.positions && a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + TILE_KEYS);
-        const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles;
-        a.nseg = (int)max(1L, min(min((4 * cus + wgs - 1) / wgs, (keys + nw * TILE_KEYS - 1) / (nw * TILE_KEYS)), 256L));
+        const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
+        const long per_cu = (c->d == 256 ? 1 : 2) * (wgs >= cus ? 2 : 1);
+        a.nseg = (int)max(1L, min(min((per_cu * cus + wgs - 1) / wgs, tiles), (long)MOST_SEGMENTS));
+        once = (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
     if ((size_t)a.row_tiles * a.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
-    const bool merge = fast && (a.nseg > 1 || weights);
-    const size_t partial_bytes = merge ? units * a.row_tiles * a.nseg * 16 * c->d * 4 : 0, stats_bytes = merge || weights ? (units * rows * a.nseg * 8 + 255) / 256 * 256 : 0;
     if (weights && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take more than 4 GiB; ask for weights with fewer queries", units * rows, T);
-    const size_t scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
+    const size_t meetings = a.nseg > 1 ? units * a.row_tiles : 0, partial_bytes = meetings * a.nseg * (16 * c->d + 32) * 4;
+    const size_t stats_bytes = weights ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
     if (const int rc = ensure_scratch2(ctx, partial_bytes + stats_bytes + scores_bytes)) return rc;
-    if (merge || weights) {
-        a.stats = (float2 *)ctx->scratch2;
-        a.partial = (float *)((char *)ctx->scratch2 + stats_bytes);
-        a.scores = weights ? (float *)((char *)ctx->scratch2 + stats_bytes + partial_bytes) : nullptr;
+    if (meetings) {
+        if (const int rc = ensure_tickets(ctx, meetings * MEET_TICKET_WORDS * sizeof(unsigned))) return rc;
+        a.tickets = (unsigned *)ctx->tickets;
+        a.partial = (float *)ctx->scratch2;
+    }
+    if (weights) {
+        a.stats = (float2 *)((char *)ctx->scratch2 + partial_bytes);
+        a.scores = (float *)((char *)ctx->scratch2 + partial_bytes + stats_bytes);
     }
     if (fast) {
-        if (const int rc = c->dtype == AIONHIP_F16 ? launch_head<AIONHIP_F16>(ctx, a, (int)p->batch) : launch_head<AIONHIP_BF16>(ctx, a, (int)p->batch)) return rc;
+        if (const int rc = c->dtype == AIONHIP_F16 ? launch_head<AIONHIP_F16>(ctx, a, (int)p->batch, once) : launch_head<AIONHIP_BF16>(ctx, a, (int)p->batch, once)) return rc;
     } else {
         ProfScope scope(ctx, "paged_generic");
         launch_k(ctx, paged_generic_kernel, dim3((unsigned)rows, (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
         LAUNCH_CHECK(ctx, "paged_generic");
     }
-    if (merge || weights) {
-        ProfScope scope(ctx, "paged_merge");
-        const unsigned merge_rows = fast ? (unsigned)rows : 0, chunks = weights ? (unsigned)((T + 1023) / 1024) : 0;
-        launch_k(ctx, paged_merge_kernel, dim3(merge_rows + chunks, (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a, nw, (int)merge_rows);
+    if (weights) {
+        ProfScope scope(ctx, "paged_weights");
+        launch_k(ctx, paged_weights_kernel, dim3((unsigned)((T + 1023) / 1024), (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
         LAUNCH_CHECK(ctx, fast ? "paged_attn" : "paged_generic");
     }
     return AIONHIP_OK;
