@@ -11,9 +11,9 @@ template <typename T> T *dp(aionhip_handle h) { return reinterpret_cast<T *>((ui
 
 // a weight's place in the order that the greatest is taken from, as a number: a NaN above all, -0 as 0
 __device__ __forceinline__ unsigned rank_of(float w) {
-    if (w != w) return 0xFFFFFFFFu;
     const unsigned u = __float_as_uint(w + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const unsigned r = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+    return w != w ? 0xFFFFFFFFu : r;
 }
 
 struct Select {
@@ -24,24 +24,32 @@ struct Select {
     int h, cap, cap_out, limit, keep, first, recent;
     int in_place, tell;           // tell: what an uncut sequence keeps is asked for, or copied
 };
-constexpr int SELECT_THREADS = 1024, DIGIT = 256;
+constexpr int SELECT_EACH = 8;        // neighbouring rows of a thread in a chunk
+constexpr int HELD = 4;               // chunks of weights that a workgroup keeps in registers; longer sequences read the others again in every round
+constexpr int DIGITS = 2048;
 
-// sums of v over the threads before this one, and over all of them; red: 17 ints of LDS
-__device__ __forceinline__ int scan_1024(int v, int *red, int &total) {
+// sum over the lanes up to this one: shifts within rows of sixteen, then the last of a row (of half a wavefront) added to the rows behind it
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);      // row_bcast 31 into rows 2 and 3
+    return v;
+}
+// sums of v over the threads before this one, and over all of them; red: an int of LDS to each wavefront
+template <int THREADS>
+__device__ __forceinline__ int scan_all(int v, int *red, int &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += up;
-    }
+    const int sum = wave_scan(v);
     __syncthreads();
     if (lane == 63) red[wave] = sum;
     __syncthreads();
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < SELECT_THREADS / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         const int x = red[w];
         before += w < wave ? x : 0;
         total += x;
@@ -49,9 +57,15 @@ __device__ __forceinline__ int scan_1024(int v, int *red, int &total) {
     return before + sum - v;
 }
 
-// The m-th greatest rank of a head's middle rows by four rounds over its digits, greatest digit first, then one pass that numbers what stays.
-__global__ __launch_bounds__(SELECT_THREADS) void select_kernel(Select a) {
-    __shared__ int hist[DIGIT], red[SELECT_THREADS / 64], s_digit, s_above;
+// The m-th greatest rank of a head's middle rows by three rounds over its digits (11, 11 and 10 bits, greatest first), each of which counts the digits of what the rounds
+// before left; then one pass that numbers what stays. A thread has eight neighbouring rows of a chunk, so that the places of what stays are one sum over the
+// workgroup to a chunk; a digit's count has copies, as sums of probabilities share their exponents. What bounds it is one CU's instruction issue (long sequences: of 23 us for
+// 32768 rows 6 are the first round, 9 the last pass) and the barriers (short ones: 7 us for 1280 rows). Tried and not kept: what stays gathered in LDS and written side by side
+// (25.5), ranks instead of weights in registers (the same), 64 neighbouring rows to a wavefront, with masks and counts of bits in place of sums (30).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
+    constexpr int CHUNK = THREADS * SELECT_EACH, COPIES = THREADS / 256, OWN = DIGITS / THREADS;
+    __shared__ int hist[DIGITS * COPIES], red[THREADS / 64], s_digit, s_above;
     const int b = blockIdx.y, head = blockIdx.x, tid = threadIdx.x;
     const size_t unit = (size_t)b * a.h + head;
     const int n = max(0, min(a.lengths[b], a.cap));
@@ -63,69 +77,112 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_kernel(Select a) {
     int *kept = a.kept + unit * a.limit;
     if (!cut) {
         if (a.tell)
-            for (int i = tid; i < a.limit; i += SELECT_THREADS) kept[i] = i < n ? i : -1;
+            for (int i = tid; i < a.limit; i += THREADS) kept[i] = i < n ? i : -1;
         if (out != w)                             // (in place an uncut sequence costs nothing but the look at its length)
-            for (int i = tid; i < a.cap_out; i += SELECT_THREADS) out[i] = i < n ? w[i] : 0.f;
+            for (int i = tid; i < a.cap_out; i += THREADS) out[i] = i < n ? w[i] : 0.f;
         return;
     }
     const int lo = a.first, hi = n - a.recent;
+    auto load = [&](int chunk, float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+        const int i = chunk * CHUNK + tid * SELECT_EACH;
+        if (i + SELECT_EACH <= n) {
+            __builtin_memcpy(x, w + i, sizeof x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < SELECT_EACH; ++j) x[j] = i + j < n ? w[i + j] : 0.f;
+        }
+    };
+    float held[HELD][SELECT_EACH];
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+        if (c * CHUNK < n) load(c, held[c]);
     int want = a.keep - a.first - a.recent;
     unsigned prefix = 0;
-    bool none = want == 0;
+    const bool none = want == 0;
     if (!none) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < DIGIT) hist[tid] = 0;
+#pragma unroll 1
+        for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift - 10) {
+            const int bits = shift == 0 ? 10 : 11;
+            for (int i = tid; i < DIGITS * COPIES; i += THREADS) hist[i] = 0;
             __syncthreads();
-            for (int i = lo + tid; i < hi; i += SELECT_THREADS) {
-                const unsigned r = rank_of(w[i]);
-                if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[r >> shift & 255u], 1);
+            auto add = [&](int chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+                const int i = chunk * CHUNK + tid * SELECT_EACH;
+#pragma unroll
+                for (int j = 0; j < SELECT_EACH; ++j) {
+                    const unsigned r = rank_of(x[j]);
+                    if (i + j >= lo && i + j < hi && (shift == 21 || r >> (shift + bits) == prefix >> (shift + bits)))
+                        atomicAdd(&hist[(r >> shift & (DIGITS - 1u) >> (11 - bits)) * COPIES + (tid & (COPIES - 1))], 1);
+                }
+            };
+#pragma unroll
+            for (int c = 0; c < HELD; ++c)
+                if (c * CHUNK < n) add(c, held[c]);
+            for (int c = HELD; c * CHUNK < n; ++c) {
+                float x[SELECT_EACH];
+                load(c, x);
+                add(c, x);
             }
             __syncthreads();
-            if (tid < 64) {                       // one wavefront: four digits a lane, counted from the top
-                int c[4], sum = 0;
+            int c[OWN], sum = 0, all;             // a thread's digits, counted from the top
 #pragma unroll
-                for (int j = 0; j < 4; ++j) c[j] = hist[255 - (tid * 4 + j)], sum += c[j];
-                int upto = sum;
+            for (int j = 0; j < OWN; ++j) {
+                c[j] = 0;
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int up = __shfl_up(upto, o, 64);
-                    if (tid >= o) upto += up;
-                }
-                int above = upto - sum;
+                for (int k = 0; k < COPIES; ++k) c[j] += hist[(DIGITS - 1 - OWN * tid - j) * COPIES + k];
+                sum += c[j];
+            }
+            int above = scan_all<THREADS>(sum, red, all);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (above < want && above + c[j] >= want) s_digit = 255 - (tid * 4 + j), s_above = above;
-                    above += c[j];
-                }
+            for (int j = 0; j < OWN; ++j) {
+                if (above < want && above + c[j] >= want) s_digit = DIGITS - 1 - OWN * tid - j, s_above = above;
+                above += c[j];
             }
             __syncthreads();
             prefix |= (unsigned)s_digit << shift;
             want -= s_above;
-            __syncthreads();
         }
     }
-    // `want` of the rows whose rank is `prefix` stay, the oldest of them. Chunks in order: what is read of a chunk lies behind everything written so far, so that weights may move in place.
-    int at = 0, equal = 0;
-    for (int base = 0; base < n; base += SELECT_THREADS) {
-        const int i = base + tid;
-        const float x = i < n ? w[i] : 0.f;
-        const bool middle = i >= lo && i < hi;
-        const unsigned r = rank_of(x);
-        const bool same = middle && !none && r == prefix;
-        int total;
-        const int eq = equal + scan_1024(same ? 1 : 0, red, total);
-        equal += total;
-        const bool stays = i < n && (!middle || (!none && (r > prefix || (same && eq < want))));
-        const int to = at + scan_1024(stays ? 1 : 0, red, total);
-        at += total;
-        if (stays) {
-            kept[to] = i;
-            out[to] = x;
+    // `want` of the rows whose rank is `prefix` stay, the oldest of them. Chunks in order: what is read of a chunk lies behind everything written so far, and its ranks have been
+    // taken when the workgroup meets, so that weights may move in place.
+    int sure = 0, equal = 0;                      // rows before the chunk that stay whatever `want` is, and of that rank
+    auto place = [&](int chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+        const int i = chunk * CHUNK + tid * SELECT_EACH;
+        unsigned stays = 0, same = 0;
+#pragma unroll
+        for (int j = 0; j < SELECT_EACH; ++j) {
+            const unsigned r = rank_of(x[j]);
+            const bool middle = i + j >= lo && i + j < hi;
+            stays |= (i + j < n && (!middle || (!none && r > prefix)) ? 1u : 0u) << j;
+            same |= (middle && !none && r == prefix ? 1u : 0u) << j;
         }
+        int total;
+        const int before = scan_all<THREADS>(__popc(stays) | __popc(same) << 16, red, total);
+        int s = sure + (before & 0xFFFF), e = equal + (int)((unsigned)before >> 16);
+#pragma unroll
+        for (int j = 0; j < SELECT_EACH; ++j) {
+            const bool mine = stays >> j & 1u, alike = same >> j & 1u;
+            if (mine || (alike && e < want)) {
+                const int to = s + min(e, want);
+                kept[to] = i + j;
+                out[to] = x[j];
+            }
+            s += mine ? 1 : 0;
+            e += alike ? 1 : 0;
+        }
+        sure += total & 0xFFFF;
+        equal += (int)((unsigned)total >> 16);
+    };
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+        if (c * CHUNK < n) place(c, held[c]);
+    for (int c = HELD; c * CHUNK < n; ++c) {
+        float x[SELECT_EACH];
+        load(c, x);
+        place(c, x);
     }
     __syncthreads();
-    for (int i = a.keep + tid; i < a.limit; i += SELECT_THREADS) kept[i] = -1;
-    for (int i = a.keep + tid; i < a.cap_out; i += SELECT_THREADS) out[i] = 0.f;
+    for (int i = a.keep + tid; i < a.limit; i += THREADS) kept[i] = -1;
+    for (int i = a.keep + tid; i < a.cap_out; i += THREADS) out[i] = 0.f;
 }
 
 struct Move {
@@ -138,43 +195,48 @@ struct Move {
     int lanes;                    // 16-byte columns of a row that a workgroup moves
     int slices, parts;            // workgroups over the columns, over the rows
 };
-// Rows in their order, so many at a time that every thread has EACH 16-byte pieces in flight. In place a workgroup moves all rows of its columns: a
-// chunk is read before it is written, its rows come from at or behind where they go, and the next chunk's from behind that.
-constexpr int MOVE_EACH = 4;
+// Rows in their order, keys and values together, so many at a time that every thread has 2 * EACH 16-byte pieces in flight. In place a workgroup moves all rows of its
+// columns: a chunk is read before it is written, its rows come from at or behind where they go, and the next chunk's from behind that.
+template <int EACH>
 __global__ __launch_bounds__(256) void move_kernel(Move a) {
-    const int b = blockIdx.z, head = blockIdx.y % a.h, which = blockIdx.y / a.h;
+    const int b = blockIdx.z, head = blockIdx.y;
     const int slice = blockIdx.x % a.slices, part = blockIdx.x / a.slices;
     const int count = a.counts[b];
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lengths_out[b] = count >= 0 ? count : max(0, min(a.lengths[b], a.cap));
     if (count <= 0) return;
     const int rows = 256 / a.lanes, row = threadIdx.x / a.lanes, col = slice * a.lanes + threadIdx.x % a.lanes;
     const bool live = row < rows && col < a.d / 8;
-    const int chunk = rows * MOVE_EACH;
+    const int chunk = rows * EACH;
     const int chunks = (count + chunk - 1) / chunk, per = (chunks + a.parts - 1) / a.parts;
     const int *kept = a.kept + ((size_t)b * a.h + head) * a.limit;
-    unsigned char *pages = a.pages[which];
     const int mask = (1 << a.from.shift) - 1;
     for (int c = part * per; c < min((part + 1) * per, chunks); ++c) {
-        u32x4 x[MOVE_EACH];
-        int target[MOVE_EACH];
+        u32x4 x[EACH][2];
+        int target[EACH];
 #pragma unroll
-        for (int j = 0; j < MOVE_EACH; ++j) {
+        for (int j = 0; j < EACH; ++j) {
             const int to = c * chunk + j * rows + row;
             target[j] = -1;
             if (live && to < count) {
                 const int from = kept[to], source = page_of(a.from, b, from);
                 if (source >= 0) {
                     target[j] = page_of(a.to, b, to);
-                    x[j] = *(const u32x4 *)(pages + (((((size_t)source * a.h + head) << a.from.shift) + (from & mask)) * a.d + col * 8) * 2);
+                    const size_t at = (((((size_t)source * a.h + head) << a.from.shift) + (from & mask)) * a.d + col * 8) * 2;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) x[j][i] = __builtin_nontemporal_load((const u32x4 *)(a.pages[i] + at));
                 }
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < MOVE_EACH; ++j) {
+        for (int j = 0; j < EACH; ++j) {
             const int to = c * chunk + j * rows + row;
-            if (target[j] >= 0) *(u32x4 *)(pages + (((((size_t)target[j] * a.h + head) << a.from.shift) + (to & mask)) * a.d + col * 8) * 2) = x[j];
+            const size_t at = (((((size_t)max(target[j], 0) * a.h + head) << a.from.shift) + (to & mask)) * a.d + col * 8) * 2;
+            if (target[j] >= 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) __builtin_nontemporal_store(x[j][i], (u32x4 *)(a.pages[i] + at));
+            }
         }
         __syncthreads();
     }
@@ -195,7 +257,7 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
     if (!c->batch) return AIONHIP_OK;
     const size_t cap_out = e->table_out ? e->width_out * c->page_rows : cap, units = c->batch * c->h_kv;
     const size_t limit = min(e->limit, cap), kept_bytes = units * e->limit * 4;
-    if (units > 0x7FFFFFFF || 2 * c->h_kv > 65535) return set_err(ctx, AIONHIP_UNSUPPORTED, "evict_paged: dimension too large");
+    if (units > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "evict_paged: dimension too large");
     const size_t w_bytes = units * cap * 4, wo_bytes = units * cap_out * 4, l_bytes = c->batch * 4, t_bytes = c->batch * e->width_out * 4;
     const bool same_w = e->weights_out == e->weights, same_l = e->lengths_out == e->kv_lengths;
     if ((same_w && e->table_out) || (!same_w && overlap(e->weights_out, wo_bytes, e->weights, w_bytes)) || (!same_l && overlap(e->lengths_out, l_bytes, e->kv_lengths, l_bytes)) ||
@@ -212,7 +274,9 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
                    (int)e->first, (int)e->recent, e->table_out ? 0 : 1, e->table_out || e->kept ? 1 : 0};
     {
         ProfScope scope(ctx, "evict_select");
-        launch_k(ctx, select_kernel, dim3((unsigned)c->h_kv, (unsigned)c->batch), dim3(SELECT_THREADS), 0, s);
+        // (what a short sequence costs is the barriers between the rounds, and those the wavefronts that meet there)
+        if (cap <= 8192) launch_k(ctx, select_kernel<256>, dim3((unsigned)c->h_kv, (unsigned)c->batch), dim3(256), 0, s);
+        else launch_k(ctx, select_kernel<1024>, dim3((unsigned)c->h_kv, (unsigned)c->batch), dim3(1024), 0, s);
         LAUNCH_CHECK(ctx, "evict_select");
     }
     Move m{{dp<unsigned char>(c->k_pages), dp<unsigned char>(c->v_pages)}, kept, counts, dp<int>(e->lengths_out), dp<const int>(e->kv_lengths), table_of(c), table_of(c), (int)c->h_kv, (int)c->d,
@@ -223,7 +287,7 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
         m.to.width = (int)e->width_out;
         m.lanes = min(cols, 256);
         m.slices = 1;
-        const int chunk = 256 / m.lanes * MOVE_EACH;
+        const int chunk = 256 / m.lanes;
         m.parts = (int)max((size_t)1, min((limit + chunk - 1) / chunk, (size_t)65536));
     } else {
         m.lanes = min(cols, 4);
@@ -231,7 +295,7 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
         m.parts = 1;
     }
     ProfScope scope(ctx, "evict_move");
-    launch_k(ctx, move_kernel, dim3((unsigned)(m.slices * m.parts), (unsigned)(2 * c->h_kv), (unsigned)c->batch), dim3(256), 0, m);
+    launch_k(ctx, e->table_out ? move_kernel<1> : move_kernel<4>, dim3((unsigned)(m.slices * m.parts), (unsigned)c->h_kv, (unsigned)c->batch), dim3(256), 0, m);
     LAUNCH_CHECK(ctx, "evict_move");
     return AIONHIP_OK;
 }

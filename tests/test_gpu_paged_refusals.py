@@ -125,7 +125,6 @@ def refusals(lib, ctx, at):
                    dict(weights=at(11)), dict(kv_lengths=at(10)), dict(table_out=0, width_out=0, weights_out=at(9) + 4), dict(lengths_out=at(2)), dict(weights=at(1)), dict(table_out=at(10)),
                    dict(table_out=at(11)), dict(recent=2 ** 64 - 1), dict(first=2 ** 64 - 1)):
         say(("evict", str(change)), evict(good, **change), INV)
-    say(("evict", "heads"), evict(cache(at, h_kv=40000, k_pages=1 << 45, v_pages=1 << 46)), UNS)
     return out
 
 
