@@ -14,6 +14,11 @@ template <typename T> T *dp(aionhip_handle h) { return reinterpret_cast<T *>((ui
 template <int DT> struct Elem { using T = unsigned short; };
 template <> struct Elem<AIONHIP_F32> { using T = float; };
 
+template <int ALIGN> struct Wide;
+template <> struct Wide<2> { typedef unsigned T __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Wide<4> { typedef unsigned T __attribute__((ext_vector_type(4), aligned(4))); };
+template <size_t ALIGN> using u32x4u = typename Wide<(int)ALIGN>::T;
+
 template <int DT>
 __device__ __forceinline__ float to_f32(typename Elem<DT>::T x) {
     if constexpr (DT == AIONHIP_F32) return x;
@@ -27,12 +32,17 @@ __device__ __forceinline__ typename Elem<DT>::T from_f32(float x) {
     else return __builtin_bit_cast(unsigned short, (__bf16)x);
 }
 // N neighbouring elements, n of them there, of any alignment their type allows (global memory takes wide accesses at any address)
-template <int DT, int N>
+template <int DT, int N, bool ONCE = false>
 __device__ __forceinline__ void load_n(const void *src, size_t i, int n, float (&x)[N]) {
     typename Elem<DT>::T h[N];
     const auto *p = (const typename Elem<DT>::T *)src + i;
     if (n == N) {
-        __builtin_memcpy(h, p, sizeof h);
+        if constexpr (ONCE && sizeof h == 16) {
+            const u32x4 w = __builtin_nontemporal_load((const u32x4u<sizeof h[0]> *)p);
+            __builtin_memcpy(h, &w, sizeof h);
+        } else {
+            __builtin_memcpy(h, p, sizeof h);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) h[j] = j < n ? p[j] : typename Elem<DT>::T(0);
@@ -40,14 +50,20 @@ __device__ __forceinline__ void load_n(const void *src, size_t i, int n, float (
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = to_f32<DT>(h[j]);
 }
-template <int DT, int N>
+template <int DT, int N, bool ONCE = false>
 __device__ __forceinline__ void store_n(void *dst, size_t i, int n, const float (&x)[N]) {
     typename Elem<DT>::T h[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) h[j] = from_f32<DT>(x[j]);
     auto *p = (typename Elem<DT>::T *)dst + i;
     if (n == N) {
-        __builtin_memcpy(p, h, sizeof h);
+        if constexpr (ONCE && sizeof h == 16) {
+            u32x4u<sizeof h[0]> w;
+            __builtin_memcpy(&w, h, sizeof h);
+            __builtin_nontemporal_store(w, (u32x4u<sizeof h[0]> *)p);
+        } else {
+            __builtin_memcpy(p, h, sizeof h);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -56,20 +72,25 @@ __device__ __forceinline__ void store_n(void *dst, size_t i, int n, const float 
 }
 
 // Sine and cosine of an angle given as a fraction of a turn, 2^64 to the whole: the nearest quarter turn is taken off in integers, what is left, up to an eighth
-// of a turn, is exact to 2^-32 and goes into the two power series (cut where the next term is below 2e-9).
+// of a turn, is exact to 2^-32 and goes into the two power series (cut where the next term is below 2e-9). Every step is written out, here and in the rotation: left to itself
+// the compiler fuses differently from kernel to kernel, and a row would have other bits alone than in front of an append.
 __device__ __forceinline__ void sincos_turn(unsigned long turn, float &sn, float &cs) {
+#pragma clang fp contract(off)
     const unsigned t = (unsigned)(turn >> 32), quarter = (t + 0x20000000u) >> 30;
     const float x = (float)(int)(t - (quarter << 30)) * 1.4629180792671596e-9f;            // 2 pi / 2^32
     const float z = x * x;
-    const float s = x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
-    const float c = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+    const float s = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
     const float a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
     sn = quarter & 2 ? -a : a;
     cs = (quarter + 1) & 2 ? -b : b;
 }
 
-// A thread has E pairs, or 2 E elements that stay, of HEADS heads of one token: the angles are computed once for all of them. A head's elements are dealt out as
-// `turning` pieces of pairs, then pieces of those that stay; the threads of a workgroup lie over pieces, then heads.
+// A thread has E pairs, or 2 E elements that stay, of HEADS heads of one token: the angles, and the token's place in the pages, are found once for all of them. A head's
+// elements are dealt out as `turning` pieces of pairs, then pieces of those that stay; the threads of a workgroup lie over pieces, then heads. One token, 32 + 8 + 8 heads of
+// 128: 4.0 us, the launch and two loads. 8000 tokens of these, f32 to f16 pages: 60 us, 6.0 TB/s, with four heads to a thread (69 with one) and past the caches (71 through
+// them: what is read and written here is more than they hold). 18000 rows of 32 heads of 128, f32, 96 elements turning: 110 us, 5.4 TB/s, with one head (120 with
+// two or four), 138 through the caches.
 struct Rotate {
     void *q_out;
     const void *q, *k, *v;
@@ -83,7 +104,7 @@ struct Rotate {
 };
 constexpr int pairs_each(int dt) { return dt == AIONHIP_F32 ? 4 : 8; }
 
-template <int DT, int CT, int HEADS>
+template <int DT, int CT, int HEADS, bool ONCE>
 __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
     constexpr int E = pairs_each(DT);
     const int slot0 = (int)threadIdx.x / a.pieces, piece = (int)threadIdx.x - slot0 * a.pieces;
@@ -111,8 +132,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
         const bool is_q = slot < a.h_q, is_v = slot >= a.h_q + a.h_kv;
         const void *src = is_q ? a.q : is_v ? a.v : a.k;
         const size_t at = is_q ? (tok * a.h_q + slot) * a.d : (tok * a.h_kv + (slot - a.h_q - (is_v ? a.h_kv : 0))) * a.d;
-        load_n<DT, E>(src, at + lo, n_lo, x[i][0]);
-        load_n<DT, E>(src, at + hi, n_hi, x[i][1]);
+        load_n<DT, E, ONCE>(src, at + lo, n_lo, x[i][0]);
+        load_n<DT, E, ONCE>(src, at + hi, n_hi, x[i][1]);
     }
     float sn[E], cs[E];
     if (turns) {
@@ -127,7 +148,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
     int page = -1, row = 0;
     size_t seq = 0;
     if (a.write_index) {
-        seq = tok / (unsigned)a.s_len;
+        seq = (unsigned)tok / (unsigned)a.s_len;
         const long step = (long)a.write_index[seq] + (long)(tok - seq * (unsigned)a.s_len);
         page = step >= 0 && step < (long)MAX_ROWS ? page_of(a.table, seq, (int)step) : -1;
         row = (int)step & ((1 << a.table.shift) - 1);
@@ -146,8 +167,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     const float p = y[2 * j], r = y[2 * j + 1];
-                    y[2 * j] = p * cs[j] - r * sn[j];
-                    y[2 * j + 1] = p * sn[j] + r * cs[j];
+                    rope_rotate(p, r, sn[j], cs[j], y[2 * j], y[2 * j + 1]);
                 }
 #pragma unroll
                 for (int j = 0; j < E; ++j) l[j] = y[j], h[j] = y[E + j];
@@ -155,15 +175,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     const float p = l[j], r = h[j];
-                    l[j] = p * cs[j] - r * sn[j];
-                    h[j] = p * sn[j] + r * cs[j];
+                    rope_rotate(p, r, sn[j], cs[j], l[j], h[j]);
                 }
             }
         }
         if (is_q) {
             const size_t at = (tok * a.h_q + slot) * a.d;
-            store_n<DT, E>(a.q_out, at + lo, n_lo, l);
-            store_n<DT, E>(a.q_out, at + hi, n_hi, h);
+            store_n<DT, E, ONCE>(a.q_out, at + lo, n_lo, l);
+            store_n<DT, E, ONCE>(a.q_out, at + hi, n_hi, h);
         } else if (page >= 0) {
             const int head = slot - a.h_q - (is_v ? a.h_kv : 0);
             const size_t at = ((((size_t)page * a.h_kv + head) << a.table.shift) + row) * a.d;
@@ -186,7 +205,7 @@ __global__ __launch_bounds__(256) void read_paged_kernel(ReadArgs a, size_t tota
     const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (gid >= total) return;
     const unsigned per = (unsigned)a.d / 8;
-    const size_t row = gid / per, tok = row / (unsigned)a.h, seq = tok / (unsigned)a.s_len;
+    const size_t row = gid / per, tok = row / (unsigned)a.h, seq = (unsigned)tok / (unsigned)a.s_len;
     const int piece = (int)(gid - row * per), head = (int)(row - tok * (unsigned)a.h);
     const long step = (long)a.first[seq] + (long)(tok - seq * (unsigned)a.s_len);
     const int page = step >= 0 && step < (long)MAX_ROWS ? page_of(a.table, seq, (int)step) : -1;
@@ -257,6 +276,9 @@ int turn_table(aionhip_ctx *ctx, const aionhip_rotary *r, const unsigned long **
     return AIONHIP_OK;
 }
 
+// rows that take this many bytes, read and written, go past the caches (see the kernel)
+constexpr size_t ONCE_BYTES = (size_t)128 << 20;
+
 // the launch of `tokens` rows; `rotary` null or of no pairs: nothing turns
 int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rotary *rotary, size_t tokens, int dtype, int cache_dtype) {
     if (rotary && rotary->dims) {
@@ -271,14 +293,16 @@ int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rot
     a.pieces = a.turning + (a.d - a.dims + 2 * each - 1) / (2 * each);
     const int slots = a.h_q + 2 * a.h_kv;
     a.heads_wg = min(256 / a.pieces, slots);                             // (heads of up to 1024 have 129 pieces at most)
-    // Few tokens are a chain of latencies, spread thin; many have the angles of each computed once for four heads (measured at the kernel).
-    const bool many = tokens >= 1024;
-    const dim3 grid((unsigned)tokens, (unsigned)((slots + a.heads_wg * (many ? 4 : 1) - 1) / (a.heads_wg * (many ? 4 : 1))));
+    // (measured at the kernel)
+    const int heads = tokens >= 1024 && a.h_kv ? 4 : 1;
+    const bool once = tokens * slots * a.d * (dtype == AIONHIP_F32 ? 8 : 4) >= ONCE_BYTES;
+    const dim3 grid((unsigned)tokens, (unsigned)((slots + a.heads_wg * heads - 1) / (a.heads_wg * heads)));
     const unsigned threads = (unsigned)((a.heads_wg * a.pieces + 63) / 64 * 64);
     ProfScope scope(ctx, who);
     auto go = [&](auto dt, auto ct) {
-        if (many) launch_k(ctx, rotary_kernel<decltype(dt)::value, decltype(ct)::value, 4>, grid, dim3(threads), 0, a);
-        else launch_k(ctx, rotary_kernel<decltype(dt)::value, decltype(ct)::value, 1>, grid, dim3(threads), 0, a);
+        constexpr int DT = decltype(dt)::value, CT = decltype(ct)::value;
+        if (heads == 1) launch_k(ctx, once ? rotary_kernel<DT, CT, 1, true> : rotary_kernel<DT, CT, 1, false>, grid, dim3(threads), 0, a);
+        else launch_k(ctx, once ? rotary_kernel<DT, CT, 4, true> : rotary_kernel<DT, CT, 4, false>, grid, dim3(threads), 0, a);
     };
     auto types = [&](auto dt) {
         if (cache_dtype == AIONHIP_F16) go(dt, std::integral_constant<int, AIONHIP_F16>{});
