@@ -113,14 +113,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
     const int slots = a.h_q + 2 * a.h_kv, first = (int)blockIdx.y * a.heads_wg * HEADS + slot0;
     const int half = a.dims >> 1;
     const bool turns = piece < a.turning;
-    // the thread's two runs of elements of a head
+    // the thread's two runs of elements of a head: the two sides of its pairs, or a piece from either half of what lies side by side
     int lo, hi, n_lo, n_hi;
     if (turns && !a.interleaved) {
         lo = piece * E, hi = half + lo;
         n_lo = n_hi = min(E, half - lo);
     } else {
-        const int end = turns ? a.dims : a.d;
-        lo = turns ? piece * 2 * E : a.dims + (piece - a.turning) * 2 * E, hi = lo + E;
+        const int begin = turns ? 0 : a.dims, end = turns ? a.dims : a.d, count = turns ? a.turning : a.pieces - a.turning, at = turns ? piece : piece - a.turning;
+        lo = begin + at * E, hi = begin + (count + at) * E;
         n_lo = min(E, end - lo), n_hi = max(0, min(E, end - hi));
     }
     // what the heads need is asked for before the first of them is used
@@ -137,10 +137,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
     }
     float sn[E], cs[E];
     if (turns) {
-        const int pos = a.positions[tok], pair0 = piece * E;
+        const int pos = a.positions[tok];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            sincos_turn(a.turns[min(pair0 + j, half - 1)] * (unsigned long)(long)pos, sn[j], cs[j]);
+            const int pair = !a.interleaved ? lo + j : j < E / 2 ? lo / 2 + j : hi / 2 + j - E / 2;
+            sincos_turn(a.turns[min(pair, half - 1)] * (unsigned long)(long)pos, sn[j], cs[j]);
             sn[j] *= a.magnitude;
             cs[j] *= a.magnitude;
         }
@@ -161,16 +162,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
         float(&l)[E] = x[i][0], (&h)[E] = x[i][1];
         if (turns && !is_v) {
             if (a.interleaved) {
-                float y[2 * E];
 #pragma unroll
-                for (int j = 0; j < E; ++j) y[j] = l[j], y[E + j] = h[j];
-#pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const float p = y[2 * j], r = y[2 * j + 1];
-                    rope_rotate(p, r, sn[j], cs[j], y[2 * j], y[2 * j + 1]);
+                for (int j = 0; j < E / 2; ++j) {
+                    const float p = l[2 * j], r = l[2 * j + 1], u = h[2 * j], v = h[2 * j + 1];
+                    rope_rotate(p, r, sn[j], cs[j], l[2 * j], l[2 * j + 1]);
+                    rope_rotate(u, v, sn[E / 2 + j], cs[E / 2 + j], h[2 * j], h[2 * j + 1]);
                 }
-#pragma unroll
-                for (int j = 0; j < E; ++j) l[j] = y[j], h[j] = y[E + j];
             } else {
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
