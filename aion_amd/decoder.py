@@ -5,7 +5,9 @@ src/bench/models.zig:433-536, trimmed to a plain pre-norm block): Gather -> per 
 [RMSNorm -> MatMul q,k,v -> RoPE1D(q,k) -> Cast f16 + SequenceAppend(k,v) -> Attention ->
 MatMul o -> add -> RMSNorm -> MatMul gate,up -> gate(gelu) -> MatMul down -> add] ->
 RMSNorm -> MatMul lm_head -> ArgMax. With `cache_dtype` Q8_0 or Q4_0 the keys and values are quantised as they are appended
-(SequenceAppend takes the f32 rows, no Cast) and attention reads the codes. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
+(SequenceAppend takes the f32 rows, no Cast) and attention reads the codes. With `page_rows` the caches are pools of pages under one
+page table; q and k turn as `rotary` says, and with `evict_keep` a sequence that passes `evict_limit` rows keeps that many of them, the ones
+whose keys have drawn the most attention, decided on the device at every step: the text may then be longer than the caches. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
 only q4 layout aion has), q8_0 weights are [N,K] quant_axis 1 MatMulNT operands.
 
 Prefill runs the steps eagerly; the single-token decode step is recorded once into a program
@@ -37,7 +39,13 @@ class DecoderConfig:
     eps: float = 1e-6
     rope_base: float = 10000.0
     wdtype: int = be.Q4_0
-    cache_dtype: int = be.F16        # F16, or Q8_0 / Q4_0: keys and values held in 8 or 4 bits (head_dim a multiple of 32)
+    cache_dtype: int = be.F16        # F16, or Q8_0 / Q4_0: keys and values held in 8 or 4 bits (head_dim a multiple of 32); in pages F16 or BF16
+    page_rows: int = 0               # 0: linear caches; else caches in pages of that many rows (a power of two, 16 to 1024)
+    rotary: object = None            # caches in pages: how q and k turn (backend.Rotary); None: the whole head, in halves, by rope_base
+    evict_keep: int = 0              # caches in pages: rows that a sequence keeps when it passes evict_limit; 0: no eviction
+    evict_limit: int = 0             # 0: max_seq - 1
+    evict_first: int = 4             # of those, the oldest and the newest that stay in any case
+    evict_recent: int = 0            # 0: a quarter of evict_keep
 
     @property
     def q_dim(self):
@@ -51,8 +59,29 @@ class DecoderConfig:
     def quant_cache(self):
         return self.cache_dtype in be.BLOCK_BYTES
 
+    @property
+    def pages(self):
+        return -(-self.max_seq // self.page_rows)
+
+    def eviction(self):
+        """(keep, limit, first, recent), or None"""
+        if not self.evict_keep:
+            return None
+        if not self.page_rows:
+            raise ValueError("evict_keep: eviction is from caches in pages (page_rows)")
+        limit = self.evict_limit or self.max_seq - 1
+        first = min(self.evict_first, self.evict_keep)
+        recent = min(self.evict_recent or self.evict_keep // 4, self.evict_keep - first)
+        if not self.evict_keep <= limit < self.max_seq:
+            raise ValueError("evict_keep %d <= evict_limit %d < max_seq %d must hold" % (self.evict_keep, limit, self.max_seq))
+        return self.evict_keep, limit, first, recent
+
     def cache_bytes(self, gpu):
         """Bytes of one layer's cache of keys (or values)."""
+        if self.page_rows:
+            if self.cache_dtype not in (be.F16, be.BF16):
+                raise ValueError("cache_dtype: caches in pages are F16 or BF16")
+            return self.pages * self.page_rows * self.kv_dim * 2
         if self.quant_cache:
             return gpu.cache_quant_bytes(self.cache_dtype, 1, self.max_seq, self.kv_heads, self.head_dim)
         if self.cache_dtype != be.F16:
@@ -135,14 +164,24 @@ class Decoder:
         kv_bytes = cfg.cache_bytes(gpu)
         self.kc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.vc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
+        self.eviction = cfg.eviction()
+        self.rotary = cfg.rotary or be.Rotary(cfg.head_dim, base=cfg.rope_base)
+        self.page_table, self.caches, self.drawn = None, [], []
+        if cfg.page_rows:
+            self.page_table = gpu.upload(np.arange(cfg.pages, dtype=np.int32))
+            self.caches = [gpu.paged_cache(k, v, self.page_table, cfg.pages, 1, cfg.pages, cfg.page_rows, cfg.kv_heads, cfg.head_dim, cfg.cache_dtype)
+                           for k, v in zip(self.kc, self.vc)]
+        if self.eviction:
+            self.drawn = [gpu.zeros(cfg.kv_heads * self.caches[0].capacity * 4) for _ in range(cfg.layers)]      # what each key has drawn
         self.one = gpu.upload(np.ones(1, np.int32))
         self.logits = gpu.alloc(cfg.vocab * 4)
         self.token = gpu.alloc(4)
-        self.history = gpu.alloc(cfg.max_seq * 4)       # token produced at each position (decode program's log)
+        self.log_capacity = cfg.max_seq if not self.eviction else max(cfg.max_seq, 1 << 16)
+        self.history = gpu.alloc(self.log_capacity * 4)  # token produced at each position (decode program's log)
         self.state = {}        # S -> activation buffers
         self.program = None
-        self.pos = 0
-        if one_launch and not cfg.quant_cache:               # (the one-launch form reads f16 caches)
+        self.pos = self.rows = 0                         # tokens of the text, rows of the caches (fewer, once rows have been evicted)
+        if one_launch and not cfg.quant_cache and not cfg.page_rows:               # (the one-launch form reads linear f16 caches)
             layers = [{"wq": self.w["l%d.wq" % l], "wk": self.w["l%d.wk" % l], "wv": self.w["l%d.wv" % l], "wo": self.w["l%d.wo" % l],
                        "w_gate": self.w["l%d.wgate" % l], "w_up": self.w["l%d.wup" % l], "w_down": self.w["l%d.wdown" % l],
                        "norm1_gamma": self.gamma, "norm2_gamma": self.gamma, "k_cache": self.kc[l], "v_cache": self.vc[l]}
@@ -160,7 +199,7 @@ class Decoder:
         c, g = self.cfg, self.gpu
         f = 4 * s
         b = {
-            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4),
+            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4), "kept_len": g.alloc(4),
             "x": g.alloc(f * c.hidden), "h": g.alloc(f * c.hidden), "o": g.alloc(f * c.hidden),
             "q": g.alloc(f * c.q_dim), "qr": g.alloc(f * c.q_dim), "att": g.alloc(f * c.q_dim),
             "k": g.alloc(f * c.kv_dim), "kr": g.alloc(f * c.kv_dim), "v": g.alloc(f * c.kv_dim),
@@ -177,7 +216,9 @@ class Decoder:
         scale = 1.0 / math.sqrt(c.head_dim)
         for l in range(c.layers if not (s == 1 and self.stack is not None) else 0):
             p = "l%d." % l
-            if c.quant_cache:
+            if c.page_rows:
+                self._paged_block(l, s, b, scale)
+            elif c.quant_cache:
                 # RMSNorm -> MatMul q, k, v (one call), RoPE1D(q), RoPE1D(k) -> quantized append of k and v (one launch)
                 g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s,
                                       [b["q"], b["k"], b["v"]], c.eps)
@@ -202,7 +243,9 @@ class Decoder:
             # its rows as the exact GEMM reads them
             shape = (1, s, c.max_seq, c.heads, c.kv_heads, c.head_dim, c.head_dim)
             options = {"q_dtype": be.F32, "kv_dtype": c.cache_dtype, "window": be.CAUSAL, "query_positions": b["positions"], "kv_lengths": b["kv_len"]}
-            if s == 1 or c.quant_cache or not g.step_attention_matmul(self.w[p + "wo"], b["qr"], self.kc[l], self.vc[l], shape, scale, b["x"], beta=1.0, **options):
+            if c.page_rows:
+                g.step_matmul(self.w[p + "wo"], b["att"], s, b["x"], beta=1.0)
+            elif s == 1 or c.quant_cache or not g.step_attention_matmul(self.w[p + "wo"], b["qr"], self.kc[l], self.vc[l], shape, scale, b["x"], beta=1.0, **options):
                 g.step_attention(b["att"], b["qr"], self.kc[l], self.vc[l], shape, scale, **options)
                 g.step_matmul(self.w[p + "wo"], b["att"], s, b["x"], beta=1.0)
             if s == 1 and c.hidden <= 8192 and c.ffn % 32 == 0:
@@ -221,23 +264,49 @@ class Decoder:
         g.step_rmsnorm_matmul([self.w["lm_head"]], last, self.gamma, 1, [self.logits], c.eps)
         g.step_argmax(self.token, self.logits, 1, c.vocab)
 
+    def _paged_block(self, l, s, b, scale):
+        """The input side and the attention of one block over caches in pages; b["kept_len"]: the rows that stay."""
+        c, g, p, cache = self.cfg, self.gpu, "l%d." % l, self.caches[l]
+        g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s, [b["q"], b["k"], b["v"]], c.eps)
+        g.step_rotary_append_paged(cache, self.rotary, b["qr"], b["q"], b["k"], b["v"], b["positions"], b["write_index"], s, c.heads)
+        if not self.eviction:
+            g.step_attention_paged(b["att"], b["qr"], cache, s, c.heads, scale, kv_lengths=b["kv_len"])
+            return
+        # of a long prompt the last queries alone say what the keys draw
+        asked = min(s, 64)
+        if asked < s:
+            g.step_attention_paged(b["att"], b["qr"], cache, s, c.heads, scale, kv_lengths=b["kv_len"])
+        last = (s - asked) * c.q_dim * 4
+        g.step_attention_paged(b["att"].view(last), b["qr"].view(last), cache, asked, c.heads, scale, kv_lengths=b["kv_len"], weights=self.drawn[l], weights_before=self.drawn[l])
+        keep, limit, first, recent = self.eviction
+        g.step_evict_paged(cache, self.drawn[l], b["kv_len"], self.drawn[l], b["kept_len"], keep, limit=limit, first=first, recent=recent)
+
+    def _advanced(self, s):
+        """The text and the caches are s tokens further."""
+        self.pos += s
+        self.rows += s
+        if self.eviction and self.rows > self.eviction[1]:
+            self.rows = self.eviction[0]
+
     def reset(self):
-        self.pos = 0
+        self.pos = self.rows = 0
+        for w in self.drawn:
+            self.gpu.write(w, np.zeros(w.nbytes // 4, np.float32))
 
     def prefill(self, tokens):
         """Runs the prompt (positions pos .. pos+len-1); returns the greedy next token."""
         t = np.ascontiguousarray(tokens, np.int32)
         s = t.size
-        if self.pos + s > self.cfg.max_seq:
+        if self.rows + s > self.cfg.max_seq:
             raise ValueError("prompt exceeds the cache capacity")
         b = self._buffers(s)
         g = self.gpu
         g.write(b["ids"], t)
         g.write(b["positions"], np.arange(self.pos, self.pos + s, dtype=np.int32))
-        g.write(b["write_index"], np.array([self.pos], np.int32))
-        g.write(b["kv_len"], np.array([self.pos + s], np.int32))
+        g.write(b["write_index"], np.array([self.rows], np.int32))
+        g.write(b["kv_len"], np.array([self.rows + s], np.int32))
         self._forward(s, b)
-        self.pos += s
+        self._advanced(s)
         return int(g.download(self.token, np.int32, (1,))[0])
 
     def logits_host(self):
@@ -248,7 +317,7 @@ class Decoder:
         eagerly first so that every scratch buffer has its final size; it is then rolled back)."""
         g = self.gpu
         b = self._buffers(1)
-        self._set_decode_state(b, first_token, self.pos)
+        self._set_decode_state(b, first_token)
         if self.program is not None and not g.program_is_current(self.program):
             # a longer prompt since the recording made the context replace a work buffer the program's launches address
             g.program_destroy(self.program)
@@ -257,24 +326,29 @@ class Decoder:
             self._decode_buffers = b                 # one launch per step already: nothing to record
             return
         if self.program is None:
+            if self.eviction:                        # (of no keys: nothing draws weight, and no row is evicted)
+                g.write(b["kv_len"], np.zeros(1, np.int32))
             self._forward(1, b)                      # eager warm-up at the current position
             g.sync()
-            self._set_decode_state(b, first_token, self.pos)
+            self._set_decode_state(b, first_token)
 
             def issue():
                 self._forward(1, b)
+                if self.eviction:                    # the next row goes behind those that stay
+                    g.copy(b["write_index"], b["kept_len"], 4)
+                    g.copy(b["kv_len"], b["kept_len"], 4)
                 # advance the device-resident loop state: next id = argmax, positions/write index/kv length += 1; the token
                 # is also logged at the position it was produced at, so that a run of steps needs no read-back per step
-                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["write_index"], b["kv_len"]],
-                                     log=self.history, log_index=b["positions"], log_capacity=self.cfg.max_seq)
+                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["kv_len"]] + ([] if self.eviction else [b["write_index"]]),
+                                     log=self.history, log_index=b["positions"], log_capacity=self.log_capacity)
             self.program = g.record_program(issue)
 
-    def _set_decode_state(self, b, token, pos):
+    def _set_decode_state(self, b, token):
         g = self.gpu
         g.write(b["ids"], np.array([token], np.int32))
-        g.write(b["positions"], np.array([pos], np.int32))
-        g.write(b["write_index"], np.array([pos], np.int32))
-        g.write(b["kv_len"], np.array([pos + 1], np.int32))
+        g.write(b["positions"], np.array([self.pos], np.int32))
+        g.write(b["write_index"], np.array([self.rows], np.int32))
+        g.write(b["kv_len"], np.array([self.rows + 1], np.int32))
 
     def _step_on_device(self):
         """One decode step whose loop state stays on the device: the recorded program, or with the one-launch stack the five
@@ -289,10 +363,10 @@ class Decoder:
 
     def decode_step(self, read_token=True):
         """One decode step on the device-resident state; returns the token it produced (a 4-byte read-back)."""
-        if self.pos + 1 > self.cfg.max_seq:
+        if not self.eviction and self.pos + 1 > self.cfg.max_seq:
             raise ValueError("cache capacity exhausted")
         self._step_on_device()
-        self.pos += 1
+        self._advanced(1)
         if read_token:
             return int(self.gpu.download(self.token, np.int32, (1,))[0])
         return None
@@ -300,12 +374,12 @@ class Decoder:
     def decode_run(self, n):
         """Replays the decode program n times back to back (nothing is read back in between: the loop state and the token
         log live on the device) and returns the n tokens."""
-        if self.pos + n > self.cfg.max_seq:
-            raise ValueError("cache capacity exhausted")
+        if self.pos + n > self.log_capacity:
+            raise ValueError("token log exhausted" if self.eviction else "cache capacity exhausted")
         start = self.pos
         for _ in range(n):
             self._step_on_device()
-        self.pos += n
+            self._advanced(1)
         tokens = self.gpu.download(self.history, np.int32, (n,), offset=start * 4)
         if self.stack is not None:
             self.gpu.decoder_stack_status(self.stack)      # raises if a launch gave up waiting (its tokens would be invalid)
@@ -314,9 +388,9 @@ class Decoder:
     def decode_step_eager(self, token):
         """The same step without a program (used by tests to check the replayed graph)."""
         b = self._buffers(1)
-        self._set_decode_state(b, token, self.pos)
+        self._set_decode_state(b, token)
         self._forward(1, b)
-        self.pos += 1
+        self._advanced(1)
         return int(self.gpu.download(self.token, np.int32, (1,))[0])
 
     def close(self):
@@ -334,7 +408,7 @@ class Decoder:
         for bufs in self.state.values():
             for t in bufs.values():
                 t.free()
-        for t in (self.embed, self.gamma, self.one, self.logits, self.token, self.history):
+        for t in [self.embed, self.gamma, self.one, self.logits, self.token, self.history] + self.drawn + ([self.page_table] if self.page_table else []):
             t.free()
 
 
@@ -347,6 +421,8 @@ class SessionDecoder:
 
     def __init__(self, gpu, cfg, weights, fusion=None):
         from . import session as ss
+        if cfg.page_rows:
+            raise ValueError("page_rows: aion's step list has no caches in pages")
         self.ss, self.gpu, self.cfg = ss, gpu, cfg
         self.sess = ss.Session(gpu)
         if fusion is not None:
