@@ -22,7 +22,6 @@ constexpr float MASKED = -INFINITY;
 // Probabilities are held as 2^(s - ref + HEAD_ROOM), the reference being raised only when a score passes it by more than SLACK: 2^14 at most fits f16, and what f16
 // pairs round away lies 2^-31 below the largest.
 constexpr float HEAD_ROOM = 6.f, SLACK = 8.f;
-template <int KV> constexpr float LESS = KV == AIONHIP_F16 ? 1.f - 0x1p-11f : 1.f - 0x1p-8f;
 
 struct PagedArgs {
     float *out, *partial, *scores;
@@ -69,11 +68,48 @@ __device__ __forceinline__ u32x4 lds_read(unsigned addr) {
     return x;
 }
 
+// One row's share of one wavefront, a key at a time: what its lanes have of the sums (columns lane, lane + 64, ..), its reference and its sum. See paged_attn_kernel.
+template <int D>
+__device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, int r, int rows_total, int L, int lo, int hi, int t_begin, int steps, int stride, float (&o)[D / 64],
+                                                     float &top_out, float &sum_out) {
+    const int lane = threadIdx.x & 63, li = r / a.groups, gi = r - li * a.groups;
+    const size_t qbase = (((size_t)b * L + li) * (a.Hkv * a.groups) + hk * a.groups + gi) * D;
+    float q[D / 64], ref = MASKED, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        q[j] = load_scalar(a.q, a.q_dtype, qbase + lane + 64 * j);
+        o[j] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i)
+#pragma unroll 1
+        for (int k = 0; k < TILE_KEYS; ++k) {
+            const int key = (t_begin + i * stride) * TILE_KEYS + k;
+            if (key < lo || key >= hi) continue;
+            const int page = paged::page_of(a.table, b, key);
+            if (page < 0) continue;
+            const size_t at = ((((size_t)page * a.Hkv + hk) << a.table.shift) + (key & ((1 << a.table.shift) - 1))) * D;
+            float dot = 0.f;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) dot += q[j] * load_scalar(a.k, a.kv_dtype, at + lane + 64 * j);
+            dot = lanes_sum(dot);
+            const float s = a.soft_cap > 0.f ? a.soft_cap * LOG2E * tanhf(dot * (a.scale / a.soft_cap)) : dot * (a.scale * LOG2E);
+            if (a.scores && lane == 0) a.scores[((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key] = s;
+            const float top = fmaxf(ref, s), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + HEAD_ROOM);
+            l = l * alpha + p;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) o[j] = o[j] * alpha + p * load_scalar(a.v, a.kv_dtype, at + lane + 64 * j);
+            ref = top;
+        }
+    top_out = ref;
+    sum_out = l;
+}
+
 // QP: how many halves a query element is the sum of. MULTI: several queries a sequence, whose keys may differ (of one query all rows see the same). ONCE: keys and values
 // go past the caches. The leading arguments, 14 words, arrive in SGPRs with the wavefront. heads: KV heads, query heads of each << 16;
 // form: segments, log2 of a page's rows << 12, query type << 16, rows of the queries in LDS << 24.
 template <int KV, int D, int QP, bool MULTI, bool ONCE>
-__global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
+__global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
                                                                      unsigned heads, unsigned form, PagedArgs tail) {
     using C = Cfg<D>;
     constexpr int NW = C::NW, KK = D / 32, MT = D / 16;
@@ -85,6 +121,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
     a.Hkv = (int)(heads & 0xFFFFu), a.groups = (int)(heads >> 16);
     a.nseg = (int)(form & 0xFFFu), a.table.shift = (int)(form >> 12 & 0xFu), a.q_dtype = (int)(form >> 16 & 0xFFu);
     a.table.width = T >> a.table.shift;
+    a.k = k, a.v = v, a.kv_dtype = KV;
     const int q_rows = D == 256 ? (int)(form >> 24) : 16;        // 8 or 16
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -289,10 +326,6 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
     f32x4 acc[MT];
     float ref = MASKED, l_run = 0.f;                             // l_run: of this lane's keys
     float *scores = a.scores + ((size_t)unit * rows_total + r) * a.tpad;
-    // A sum of halves times something infinite is no number where a half is zero or of the other sign. A wavefront that ends with such walks its tiles again with care: scores
-    // that are no numbers are the first halves' then, and every half of a probability but the last is taken from slightly less than what is left, so that all are above zero.
-    bool care = false;
-
     // MORE: another tile of this wavefront follows (two copies of the body, so that every path requests K and V in the same order and the count of loads in flight holds)
     auto tile = [&](int t, bool ok0, bool ok1, int next0, int next1, auto more_c) __attribute__((always_inline)) {
         constexpr bool more = decltype(more_c)::value;
@@ -315,18 +348,6 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
             for (int h = 0; h < 2; ++h) s[h] = mfma16<KV>(kf[h][i / QP], qf[i % QA], s[h]);
             if constexpr (i + QA < KK * QP) qf[i % QA] = q_operand(std::integral_constant<int, i + QA>{});
         });
-        if (QP > 1 && care) {
-            f32x4 first[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-            static_for<0, KK>([&](auto ic) __attribute__((always_inline)) {
-                constexpr int kk = decltype(ic)::value;
-                u32x4 x = q_operand(std::integral_constant<int, kk * QP>{});
-                asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) first[h] = mfma16<KV>(kf[h][kk], x, first[h]);
-            });
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j >> 2][j & 3] = s[j >> 2][j & 3] != s[j >> 2][j & 3] ? first[j >> 2][j & 3] : s[j >> 2][j & 3];
-        }
         const bool full = key0 >= all_lo && key0 + TILE_KEYS <= all_hi && ok0 && ok1;      // every row sees every key
         // lane: keys key0 + h * 16 + g * 4 + i of row n
         float p[8];
@@ -336,15 +357,11 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] = cap_log2 * tanhf(p[j]);
         }
-        unsigned seen = 0xFF;
         if (!full) {
-            seen = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key = key0 + (j >> 2) * 16 + g * 4 + (j & 3);
-                const bool see = key >= lo && key < hi && (j < 4 ? ok0 : ok1);
-                p[j] = see ? p[j] : MASKED;
-                seen |= see ? 1u << j : 0u;
+                p[j] = key >= lo && key < hi && (j < 4 ? ok0 : ok1) ? p[j] : MASKED;
             }
         }
         if (a.scores) {
@@ -368,7 +385,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
                 ref = ref_new;
             }
         }
-        const float base = (ref > MASKED ? ref : 0.f) - HEAD_ROOM, less = care ? LESS<KV> : 1.f;
+        const float base = (ref > MASKED ? ref : 0.f) - HEAD_ROOM;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -382,7 +399,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
             float u = p[j], w = p[j + 1];
 #pragma unroll
             for (int part = 0; part < PP; ++part) {
-                const unsigned both = part + 1 < PP ? pack2<KV>(u * less, w * less) : pack2<KV>(u, w);
+                const unsigned both = pack2<KV>(u, w);
                 pf[part][j / 2] = both;
                 u -= from_half_bits<KV>((unsigned short)both);
                 w -= from_half_bits<KV>((unsigned short)(both >> 16));
@@ -392,65 +409,34 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
         if (more) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * KK));
         else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         asm volatile("" ::: "memory");
-        bool odd = false;
         if (!full) {
-            // Rows that no query sees count as zeros (they may hold anything, and zero times that need not be zero). Where a row is seen by some and not finite, the
-            // queries are taken one by one below.
+            // rows that no query sees count as zeros: they may hold anything, and zero times that need not be zero
 #pragma unroll 1
             for (int i = 0; i < NVI; ++i) {
                 const int key = key0 + i * KEYS_PER_VI + v_key_in;
-                u32x4 *at = (u32x4 *)(vs + i * 1024 + lane * 16);
-                if (key < uni_lo || key >= uni_hi || !(i < NVI / 2 ? ok0 : ok1)) {
-                    *at = u32x4{0u, 0u, 0u, 0u};
-                } else if constexpr (MULTI) {
-                    constexpr unsigned EXP = KV == AIONHIP_F16 ? 0x7C00u : 0x7F80u;
-                    const u32x4 x = *at;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) odd |= (x[j] & EXP) == EXP || (x[j] >> 16 & EXP) == EXP;
-                }
+                if (key < uni_lo || key >= uni_hi || !(i < NVI / 2 ? ok0 : ok1)) *(u32x4 *)(vs + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
             }
-            if constexpr (MULTI) odd = __any(odd);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        if (!MULTI || !odd) {
-            constexpr int VA = MT < 4 ? MT : 4;                  // operands requested ahead
-            u32x4 vop[VA];
-            static_for<0, VA>([&](auto mc) __attribute__((always_inline)) { vop[decltype(mc)::value] = v_operand(vr, vl, mc); });
-            static_for<0, MT>([&](auto mc) __attribute__((always_inline)) {
-                constexpr int mt = decltype(mc)::value;
-                constexpr int later = MT - 1 - mt < VA - 1 ? MT - 1 - mt : VA - 1;
-                asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(vop[mt % VA]) : "n"(2 * later));
+        constexpr int VA = MT < 4 ? MT : 4;                  // operands requested ahead
+        u32x4 vop[VA];
+        static_for<0, VA>([&](auto mc) __attribute__((always_inline)) { vop[decltype(mc)::value] = v_operand(vr, vl, mc); });
+        static_for<0, MT>([&](auto mc) __attribute__((always_inline)) {
+            constexpr int mt = decltype(mc)::value;
+            constexpr int later = MT - 1 - mt < VA - 1 ? MT - 1 - mt : VA - 1;
+            asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(vop[mt % VA]) : "n"(2 * later));
 #pragma unroll
-                for (int part = 0; part < PP; ++part) acc[mt] = mfma16<KV>(vop[mt % VA], pf[part], acc[mt]);
-                if constexpr (mt + VA < MT) vop[mt % VA] = v_operand(vr, vl, std::integral_constant<int, mt + VA>{});
-            });
-        } else if constexpr (MULTI) {
-            // a query at a time, with zeros for the keys that it does not see, into that query's sums alone
-            for (int i = 0; i < 16; ++i) {
-                const unsigned mine = (unsigned)__shfl((int)seen, (lane & 48) + i, 64);
-                static_for<0, MT>([&](auto mc) __attribute__((always_inline)) {
-                    constexpr int mt = decltype(mc)::value;
-                    u32x4 x = v_operand(vr, vl, mc);
-                    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] &= (mine >> (2 * j) & 1u ? 0xFFFFu : 0u) | (mine >> (2 * j + 1) & 1u ? 0xFFFF0000u : 0u);
-                    f32x4 c = acc[mt];
-#pragma unroll
-                    for (int part = 0; part < PP; ++part) c = mfma16<KV>(x, pf[part], c);
-                    if (n == i) acc[mt] = c;
-                });
-            }
-        }
+            for (int part = 0; part < PP; ++part) acc[mt] = mfma16<KV>(vop[mt % VA], pf[part], acc[mt]);
+            if constexpr (mt + VA < MT) vop[mt % VA] = v_operand(vr, vl, std::integral_constant<int, mt + VA>{});
+        });
         if (more) {
             asm volatile("" ::: "memory");         // the operand reads above are complete: each was waited for before its product
             load_v(t + stride, next0, next1);
         }
     };
-    for (;;) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        ref = MASKED, l_run = 0.f;
-        if (steps == 0) break;
+    for (int mt = 0; mt < MT; ++mt) acc[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (steps > 0) {
         int t = t_begin;
         for (int i = 1; i < steps; ++i, t += stride) {
             if ((i & 31) == 0) ids = fetch_pages(i);
@@ -459,15 +445,32 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, MULTI || D == 256 ? 2 : 3) void pa
             id0 = next0, id1 = next1;
         }
         tile(t, id0 >= 0, id1 >= 0, 0, 0, std::false_type{});
+        // What is infinite or no number may have spoilt a row that does not see it (zero times it is no number), or that does (so is a sum of halves times infinity): rows that end
+        // as no number are walked again, a key at a time and in f32, which has what they see and nothing else.
         bool none = l_run != l_run;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) none |= acc[mt][j] != acc[mt][j];
-        if (care || !__any(none)) break;
-        care = true;
-        if (steps > 32) ids = fetch_pages(0);
-        begin();
+        const uint64_t spoilt = __ballot(none && row_ok);
+        if (spoilt) {
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+                if (!(spoilt >> i & 0x0001000100010001ull)) continue;
+                float o[D / 64], top, sum;
+                walk_again<D>(a, b, hk, rt * 16 + i, rows_total, L, __builtin_amdgcn_readlane(lo, i), __builtin_amdgcn_readlane(hi, i), t_begin, steps, stride, o, top, sum);
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) ((float *)vs)[lane + 64 * j] = o[j];
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (n == i) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) acc[mt] = *(const f32x4 *)((const float *)vs + mt * 16 + g * 4);
+                    ref = top;
+                    l_run = g == 0 ? sum : 0.f;
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        }
     }
     l_run = groups4_sum(l_run);
 
@@ -748,7 +751,28 @@ int launch_head(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
     return launch_parts<KV, 256>(ctx, a, batch, once);
 }
 
-// keys and values of this many bytes go past the caches (see the launcher)
+// Key segments of a row tile. As many as give each CU two workgroups at once (one of head size 256, whose LDS does not hold two), or four (two) in turn where the sequences alone
+// fill the CUs, since these are of uneven lengths: 32 sequences of up to 16384 keys, 8 heads of 128, 253 us in four segments, 263 in two, 277 in one. Fewer where joining them
+// costs more than they save, by what both take, us: a tile of a wavefront, its bytes through the CU's L1 (64 a clock), the wavefronts' meeting, and the workgroup that
+// joins, NW * 8 KiB of parts to a memory round trip. One token over 4015 keys, one head of 256 for 8, 126 segments 18.4 us, 16 15.3.
+int segments(long wgs, long tiles, int rows, int d, long cus) {
+    const long at_once = d == 256 ? 1 : 2;
+    const int nw = d == 256 ? Cfg<256>::NW : Cfg<128>::NW;
+    const long room = wgs >= cus ? (2 * at_once * cus + wgs - 1) / wgs : max(1L, at_once * cus / wgs);
+    const float tile_us = 0.8f + 1.2f * d / 256, fill_us = 0.22f * d / 256, part_bytes = (float)rows * d * 4;
+    long best = max(1L, min(min(room, tiles), (long)MOST_SEGMENTS));
+    float least = INFINITY;
+    for (long n = best;; n = (n + 1) / 2) {
+        const float joins = n > 1 ? 0.7f * ceilf(n * part_bytes / (nw * 8192)) : 0.f;
+        const float us = tile_us * ((tiles + n * nw - 1) / (n * nw)) + fill_us * ((tiles + n - 1) / n) + (tiles > n ? 1.f : 0.f) + joins;
+        if (us < least) least = us, best = n;
+        if (n == 1) break;
+    }
+    return (int)best;
+}
+
+// keys and values of this many bytes go past the caches: what is read once a step would push out what is read again. One token over 131072 keys, 8 heads of 128 (512 MiB),
+// 101 -> 91 us; 55 MB, which the memory-side cache holds from step to step, 14.2 us, and 16.9 past it.
 constexpr size_t ONCE_BYTES = (size_t)192 << 20;
 
 }  // namespace
@@ -796,8 +820,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         long keys = a.T;
         if (!a.positions && a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + TILE_KEYS);
         const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
-        const long per_cu = (c->d == 256 ? 1 : 2) * (wgs >= cus ? 2 : 1);
-        a.nseg = (int)max(1L, min(min((per_cu * cus + wgs - 1) / wgs, tiles), (long)MOST_SEGMENTS));
+        a.nseg = segments(wgs, tiles, min(a.rows_total, 16), a.d, cus);
         once = (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
     if ((size_t)a.row_tiles * a.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
