@@ -795,7 +795,9 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     const size_t w_bytes = weights ? units * T * 4 : 0;
     if (paged::in_cache(c, p->out, out_bytes) || paged::in_cache(c, weights, w_bytes) || paged::overlap(p->out, out_bytes, p->q, q_bytes) ||
         paged::overlap(weights, w_bytes, p->out, out_bytes) || paged::overlap(weights, w_bytes, p->q, q_bytes) ||
-        (weights_before != weights && paged::overlap(weights, w_bytes, weights_before, w_bytes)) || paged::overlap(p->out, out_bytes, weights_before, w_bytes))
+        (weights_before != weights && paged::overlap(weights, w_bytes, weights_before, w_bytes)) || paged::overlap(p->out, out_bytes, weights_before, w_bytes) ||
+        paged::overlap(p->out, out_bytes, p->kv_lengths, p->batch * 4) || paged::overlap(weights, w_bytes, p->kv_lengths, p->batch * 4) ||
+        paged::overlap(p->out, out_bytes, p->query_positions, p->batch * p->l_q * 4) || paged::overlap(weights, w_bytes, p->query_positions, p->batch * p->l_q * 4))
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention_paged: an operand that is written overlaps another");
     PagedArgs a{};
     a.out = (float *)(uintptr_t)p->out;

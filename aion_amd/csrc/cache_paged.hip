@@ -322,10 +322,12 @@ int append(aionhip_ctx *ctx, const char *who, const aionhip_paged_cache *c, cons
     if (h_q > 65535) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: dimension too large", who);
     if (!c->batch || !s) return AIONHIP_OK;
     const size_t tokens = c->batch * s, q_bytes = tokens * h_q * c->d * size_of(dtype), kv_bytes = tokens * c->h_kv * c->d * size_of(dtype);
-    if (in_cache(c, q, q_bytes) || in_cache(c, q_out, q_bytes) || in_cache(c, k, kv_bytes) || in_cache(c, v, kv_bytes))
-        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: rows lie in the cache", who);
-    if ((q_out != q && overlap(q_out, q_bytes, q, q_bytes)) || overlap(q_out, q_bytes, k, kv_bytes) || overlap(q_out, q_bytes, v, kv_bytes))
-        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: q, k and v are still read while q_out is written", who);
+    if (in_cache(c, q, q_bytes) || in_cache(c, q_out, q_bytes) || in_cache(c, k, kv_bytes) || in_cache(c, v, kv_bytes) || in_cache(c, positions, tokens * 4) ||
+        in_cache(c, write_index, c->batch * 4))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: rows or indices lie in the cache", who);
+    if ((q_out != q && overlap(q_out, q_bytes, q, q_bytes)) || overlap(q_out, q_bytes, k, kv_bytes) || overlap(q_out, q_bytes, v, kv_bytes) ||
+        overlap(q_out, q_bytes, positions, tokens * 4) || overlap(q_out, q_bytes, write_index, c->batch * 4))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "%s: q, k, v and the indices are still read while q_out is written", who);
     Rotate a{};
     a.q_out = dp<void>(q_out), a.q = dp<const void>(q), a.k = dp<const void>(k), a.v = dp<const void>(v);
     a.positions = dp<const int>(positions), a.write_index = dp<const int>(write_index);
@@ -379,7 +381,8 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *c, aion
     if (s > capacity(c)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: %zu rows exceed the capacity %zu", s, capacity(c));
     if (!c->batch || !s) return AIONHIP_OK;
     const size_t rows = c->batch * s * c->h_kv, bytes = rows * c->d * size_of(out_dtype), total = rows * (c->d / 8);
-    if (overlap(k_out, bytes, v_out, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: the rows of keys and values overlap");
+    if (overlap(k_out, bytes, v_out, bytes) || overlap(k_out, bytes, first, c->batch * 4) || overlap(v_out, bytes, first, c->batch * 4))
+        return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: the rows of keys and values overlap each other or the indices");
     if (in_cache(c, k_out, bytes) || in_cache(c, v_out, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: rows lie in the cache");
     if ((total + 255) / 256 > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "read_paged: too many rows for one launch");
     const ReadArgs a{{dp<const unsigned char>(c->k_pages), dp<const unsigned char>(c->v_pages)}, {dp<void>(k_out), dp<void>(v_out)}, dp<const int>(first), table_of(c), (int)s, (int)c->h_kv,

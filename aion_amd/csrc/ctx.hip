@@ -93,7 +93,7 @@ int grow_work_buffer(aionhip_ctx *ctx, void **buf, size_t *have, size_t bytes, b
 int ensure_scratch(aionhip_ctx *ctx, size_t bytes) { return grow_work_buffer(ctx, &ctx->scratch, &ctx->scratch_bytes, bytes, false, "scratch"); }
 int ensure_scratch2(aionhip_ctx *ctx, size_t bytes) { return grow_work_buffer(ctx, &ctx->scratch2, &ctx->scratch2_bytes, bytes, false, "GEMM staging"); }
 int ensure_tickets(aionhip_ctx *ctx, size_t bytes) {
-    const size_t attention = (size_t)(ctx->cu_count > 0 ? ctx->cu_count : 256) * MEET_TICKET_WORDS * sizeof(unsigned);
+    const size_t attention = 4 * (size_t)(ctx->cu_count > 0 ? ctx->cu_count : 256) * MEET_TICKET_WORDS * sizeof(unsigned);
     return grow_work_buffer(ctx, &ctx->tickets, &ctx->tickets_bytes, bytes > attention ? bytes : attention, true, "the tickets");
 }
 

@@ -166,7 +166,7 @@ class Decoder:
         self.vc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.eviction = cfg.eviction()
         self.rotary = cfg.rotary or be.Rotary(cfg.head_dim, base=cfg.rope_base)
-        self.page_table, self.caches, self.drawn = None, [], []
+        self.page_table, self.caches, self.drawn, self.linear = None, [], [], None
         if cfg.page_rows:
             self.page_table = gpu.upload(np.arange(cfg.pages, dtype=np.int32))
             self.caches = [gpu.paged_cache(k, v, self.page_table, cfg.pages, 1, cfg.pages, cfg.page_rows, cfg.kv_heads, cfg.head_dim, cfg.cache_dtype)
@@ -179,7 +179,7 @@ class Decoder:
         self.log_capacity = cfg.max_seq if not self.eviction else max(cfg.max_seq, 1 << 16)
         self.history = gpu.alloc(self.log_capacity * 4)  # token produced at each position (decode program's log)
         self.state = {}        # S -> activation buffers
-        self.program = None
+        self.program = self.cut_program = None
         self.pos = self.rows = 0                         # tokens of the text, rows of the caches (fewer, once rows have been evicted)
         if one_launch and not cfg.quant_cache and not cfg.page_rows:               # (the one-launch form reads linear f16 caches)
             layers = [{"wq": self.w["l%d.wq" % l], "wk": self.w["l%d.wk" % l], "wv": self.w["l%d.wv" % l], "wo": self.w["l%d.wo" % l],
@@ -199,25 +199,25 @@ class Decoder:
         c, g = self.cfg, self.gpu
         f = 4 * s
         b = {
-            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4), "kept_len": g.alloc(4),
+            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4), "kept_len": g.alloc(4), "row_positions": g.alloc(4 * s),
             "x": g.alloc(f * c.hidden), "h": g.alloc(f * c.hidden), "o": g.alloc(f * c.hidden),
             "q": g.alloc(f * c.q_dim), "qr": g.alloc(f * c.q_dim), "att": g.alloc(f * c.q_dim),
             "k": g.alloc(f * c.kv_dim), "kr": g.alloc(f * c.kv_dim), "v": g.alloc(f * c.kv_dim),
             "gate": g.alloc(f * c.ffn), "up": g.alloc(f * c.ffn), "act": g.alloc(f * c.ffn),
-            "hl": g.alloc(4 * c.hidden),
+            "hl": g.alloc(4 * c.hidden), "tail": g.alloc(4 * min(s, 64) * c.q_dim),
         }
         self.state[s] = b
         return b
 
-    def _forward(self, s, b):
-        """Launches every step of one forward pass over `s` tokens (eagerly, or into an open recording)."""
+    def _forward(self, s, b, cut=None):
+        """Launches every step of one forward pass over `s` tokens (eagerly, or into an open recording). cut: with the eviction behind each block (None: where it is due)."""
         c, g = self.cfg, self.gpu
         g.step_gather_rows(be.F32, b["x"], self.embed, b["ids"], s, c.hidden, c.vocab)
         scale = 1.0 / math.sqrt(c.head_dim)
         for l in range(c.layers if not (s == 1 and self.stack is not None) else 0):
             p = "l%d." % l
             if c.page_rows:
-                self._paged_block(l, s, b, scale)
+                self._paged_block(l, s, b, scale, self._due(s) if cut is None else cut)
             elif c.quant_cache:
                 # RMSNorm -> MatMul q, k, v (one call), RoPE1D(q), RoPE1D(k) -> quantized append of k and v (one launch)
                 g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s,
@@ -264,29 +264,41 @@ class Decoder:
         g.step_rmsnorm_matmul([self.w["lm_head"]], last, self.gamma, 1, [self.logits], c.eps)
         g.step_argmax(self.token, self.logits, 1, c.vocab)
 
-    def _paged_block(self, l, s, b, scale):
-        """The input side and the attention of one block over caches in pages; b["kept_len"]: the rows that stay."""
+    def _paged_block(self, l, s, b, scale, cut):
+        """The input side and the attention of one block over caches in pages, and with `cut` the eviction; b["kept_len"]: the rows that stay."""
         c, g, p, cache = self.cfg, self.gpu, "l%d." % l, self.caches[l]
         g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s, [b["q"], b["k"], b["v"]], c.eps)
         g.step_rotary_append_paged(cache, self.rotary, b["qr"], b["q"], b["k"], b["v"], b["positions"], b["write_index"], s, c.heads)
-        if not self.eviction:
-            g.step_attention_paged(b["att"], b["qr"], cache, s, c.heads, scale, kv_lengths=b["kv_len"])
-            return
-        # of a long prompt the last queries alone say what the keys draw
         asked = min(s, 64)
         if asked < s:
+            # a prompt: its keys and values in order, for the kernel that shares them among many rows
+            n = self.rows + s
+            if self.linear is None:
+                self.linear = [g.alloc(c.cache_bytes(g)) for _ in range(2)] + [g.upload(np.zeros(1, np.int32))]
+            g.step_read_paged(cache, self.linear[0], self.linear[1], self.linear[2], n, out_dtype=c.cache_dtype)
+            g.step_attention(b["att"], b["qr"], self.linear[0], self.linear[1], (1, s, n, c.heads, c.kv_heads, c.head_dim, c.head_dim), scale, kv_dtype=c.cache_dtype,
+                             query_positions=b["row_positions"])
+        elif not self.eviction:
             g.step_attention_paged(b["att"], b["qr"], cache, s, c.heads, scale, kv_lengths=b["kv_len"])
-        last = (s - asked) * c.q_dim * 4
-        g.step_attention_paged(b["att"].view(last), b["qr"].view(last), cache, asked, c.heads, scale, kv_lengths=b["kv_len"], weights=self.drawn[l], weights_before=self.drawn[l])
+        if not self.eviction:
+            return
+        # (of a prompt the last queries alone say what the keys draw; their rows are there already)
+        out = b["att"] if asked == s else b["tail"]
+        g.step_attention_paged(out, b["qr"].view((s - asked) * c.q_dim * 4), cache, asked, c.heads, scale, kv_lengths=b["kv_len"], weights=self.drawn[l], weights_before=self.drawn[l])
+        if not cut:
+            return
         keep, limit, first, recent = self.eviction
         g.step_evict_paged(cache, self.drawn[l], b["kv_len"], self.drawn[l], b["kept_len"], keep, limit=limit, first=first, recent=recent)
 
+    def _due(self, s):
+        """Whether s tokens more take the caches past their limit: how many rows there are is known here, which ones stay is not."""
+        return bool(self.eviction) and self.rows + s > self.eviction[1]
+
     def _advanced(self, s):
         """The text and the caches are s tokens further."""
+        due = self._due(s)
         self.pos += s
-        self.rows += s
-        if self.eviction and self.rows > self.eviction[1]:
-            self.rows = self.eviction[0]
+        self.rows = self.eviction[0] if due else self.rows + s
 
     def reset(self):
         self.pos = self.rows = 0
@@ -303,6 +315,7 @@ class Decoder:
         g = self.gpu
         g.write(b["ids"], t)
         g.write(b["positions"], np.arange(self.pos, self.pos + s, dtype=np.int32))
+        g.write(b["row_positions"], np.arange(self.rows, self.rows + s, dtype=np.int32))
         g.write(b["write_index"], np.array([self.rows], np.int32))
         g.write(b["kv_len"], np.array([self.rows + s], np.int32))
         self._forward(s, b)
@@ -318,30 +331,37 @@ class Decoder:
         g = self.gpu
         b = self._buffers(1)
         self._set_decode_state(b, first_token)
-        if self.program is not None and not g.program_is_current(self.program):
+        if self.program is not None and not (g.program_is_current(self.program) and (self.cut_program is None or g.program_is_current(self.cut_program))):
             # a longer prompt since the recording made the context replace a work buffer the program's launches address
-            g.program_destroy(self.program)
-            self.program = None
+            self._drop_programs()
         if self.stack is not None:
             self._decode_buffers = b                 # one launch per step already: nothing to record
             return
         if self.program is None:
             if self.eviction:                        # (of no keys: nothing draws weight, and no row is evicted)
                 g.write(b["kv_len"], np.zeros(1, np.int32))
-            self._forward(1, b)                      # eager warm-up at the current position
+            self._forward(1, b, cut=bool(self.eviction))     # eager warm-up at the current position
             g.sync()
             self._set_decode_state(b, first_token)
 
-            def issue():
-                self._forward(1, b)
-                if self.eviction:                    # the next row goes behind those that stay
+            def issue(cut):
+                self._forward(1, b, cut)
+                if cut:                              # the next row goes behind those that stay
                     g.copy(b["write_index"], b["kept_len"], 4)
                     g.copy(b["kv_len"], b["kept_len"], 4)
                 # advance the device-resident loop state: next id = argmax, positions/write index/kv length += 1; the token
                 # is also logged at the position it was produced at, so that a run of steps needs no read-back per step
-                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["kv_len"]] + ([] if self.eviction else [b["write_index"]]),
+                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["kv_len"]] + ([] if cut else [b["write_index"]]),
                                      log=self.history, log_index=b["positions"], log_capacity=self.log_capacity)
-            self.program = g.record_program(issue)
+            self.program = g.record_program(lambda: issue(False))
+            if self.eviction:                        # the step that takes the caches past their limit is a program of its own
+                self.cut_program = g.record_program(lambda: issue(True))
+
+    def _drop_programs(self):
+        for p in (self.program, self.cut_program):
+            if p is not None:
+                self.gpu.program_destroy(p)
+        self.program = self.cut_program = None
 
     def _set_decode_state(self, b, token):
         g = self.gpu
@@ -354,7 +374,7 @@ class Decoder:
         """One decode step whose loop state stays on the device: the recorded program, or with the one-launch stack the five
         launches themselves."""
         if self.stack is None:
-            self.gpu.program_execute(self.program)
+            self.gpu.program_execute(self.cut_program if self._due(1) else self.program)
             return
         b, g = self._decode_buffers, self.gpu
         self._forward(1, b)
@@ -394,9 +414,7 @@ class Decoder:
         return int(self.gpu.download(self.token, np.int32, (1,))[0])
 
     def close(self):
-        if self.program is not None:
-            self.gpu.program_destroy(self.program)
-            self.program = None
+        self._drop_programs()
         if self.stack is not None:
             self.gpu.decoder_stack_destroy(self.stack)
             self.stack = None
@@ -408,7 +426,7 @@ class Decoder:
         for bufs in self.state.values():
             for t in bufs.values():
                 t.free()
-        for t in [self.embed, self.gamma, self.one, self.logits, self.token, self.history] + self.drawn + ([self.page_table] if self.page_table else []):
+        for t in [self.embed, self.gamma, self.one, self.logits, self.token, self.history] + self.drawn + ([self.page_table] if self.page_table else []) + (self.linear or []):
             t.free()
 
 

@@ -379,6 +379,25 @@ def test_evict_long(gpu):
     free(cache, wd, ld)
 
 
+def test_evict_in_place_a_part_of_the_heads_at_a_time(gpu):
+    """rows that take more than the memory between holds at once: 20 heads of 4096 rows of 4 KiB"""
+    rng = np.random.default_rng(2)
+    pages = Pages(rng, be.F16, 2, 1, 16, 10, 1024)
+    pages.p, pages.width, pages.pages = 64, 66, 133
+    pages.k = np.arange(133 * 10 * 64 * 1024, dtype=np.uint32).astype(np.uint16).reshape(133, 10, 64, 1024)
+    pages.k ^= np.arange(133 * 10 * 64, dtype=np.uint32).astype(np.uint16).reshape(133, 10, 64, 1)
+    pages.v = pages.k[::-1].copy()
+    pages.table = rng.permutation(133)[:132].reshape(2, 66).astype(np.int32)
+    weights = weigh(rng, (2, 10, 66 * 64), "plain")
+    cache, wd, ld = pages.upload(gpu), gpu.upload(weights), gpu.upload(np.array([4200, 4224], np.int32))
+    gpu.step_evict_paged(cache, wd, ld, wd, ld, 4096, first=1, recent=100)
+    _, want_len, want_w = evict(pages, weights, [4200, 4224], 4096, 4096, 1, 100)
+    assert np.array_equal(gpu.download(ld, np.int32, (2,)), want_len) and np.array_equal(gpu.download(wd, np.float32, weights.shape), want_w)
+    for buf, want in ((cache.k_pages, pages.k), (cache.v_pages, pages.v)):
+        assert np.array_equal(gpu.download(buf, np.uint16, want.shape), want)
+    free(cache, wd, ld)
+
+
 # ---------------------------------------------------------------------------------------------------------------- together
 def steps_together(gpu, record):
     """Tokens appended, attended to with weights kept, evicted in place every time a sequence passes its limit; against numpy at every step."""

@@ -82,6 +82,13 @@ def refusals(lib, ctx, at):
     say(("append", "rows"), append(good, s=W * P + 1), INV)
     say(("append", "in a pool"), append(good, k=at(1) + pool - 16), INV)
     say(("append", "in the table"), append(good, v=at(2)), INV)
+    say(("append", "index in a pool"), append(good, index=at(0) + 8), INV)
+    say(("rotary_append", "positions in a pool"), rappend(good, rotary(), pos=at(1) + 8), INV)
+    say(("rotary_append", "q over positions"), rappend(good, rotary(), qo=at(8)), INV)
+    say(("rotary_append", "q over the index"), rappend(good, rotary(), qo=at(5)), INV)
+    say(("read", "over the index"), read(good, v=at(5)), INV)
+    say(("attention", "over the lengths"), attend(good, out=at(5)), INV)
+    say(("attention", "over the positions"), attend(good, weights=at(9), query_positions=at(9) + 8), INV)
     for change in BAD_ROTARY:
         say(("rotary_append", str(change)), rappend(good, rotary(**change)), INV)
         say(("rotary", str(change)), lib.aionhip_step_rotary(ctx, at(6), at(7), at(8), be.F32, B, S, HQ, D, ref(rotary(**change))), INV)
