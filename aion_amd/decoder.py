@@ -330,7 +330,7 @@ class Decoder:
         eagerly first so that every scratch buffer has its final size; it is then rolled back)."""
         g = self.gpu
         b = self._buffers(1)
-        self._set_decode_state(b, first_token)
+        self._set_decode_state(b, first_token, self.pos)
         if self.program is not None and not (g.program_is_current(self.program) and (self.cut_program is None or g.program_is_current(self.cut_program))):
             # a longer prompt since the recording made the context replace a work buffer the program's launches address
             self._drop_programs()
@@ -342,7 +342,7 @@ class Decoder:
                 g.write(b["kv_len"], np.zeros(1, np.int32))
             self._forward(1, b, cut=bool(self.eviction))     # eager warm-up at the current position
             g.sync()
-            self._set_decode_state(b, first_token)
+            self._set_decode_state(b, first_token, self.pos)
 
             def issue(cut):
                 self._forward(1, b, cut)
@@ -363,12 +363,12 @@ class Decoder:
                 self.gpu.program_destroy(p)
         self.program = self.cut_program = None
 
-    def _set_decode_state(self, b, token):
-        g = self.gpu
+    def _set_decode_state(self, b, token, pos):
+        g, rows = self.gpu, pos - self.pos + self.rows
         g.write(b["ids"], np.array([token], np.int32))
-        g.write(b["positions"], np.array([self.pos], np.int32))
-        g.write(b["write_index"], np.array([self.rows], np.int32))
-        g.write(b["kv_len"], np.array([self.rows + 1], np.int32))
+        g.write(b["positions"], np.array([pos], np.int32))
+        g.write(b["write_index"], np.array([rows], np.int32))
+        g.write(b["kv_len"], np.array([rows + 1], np.int32))
 
     def _step_on_device(self):
         """One decode step whose loop state stays on the device: the recorded program, or with the one-launch stack the five
@@ -408,7 +408,7 @@ class Decoder:
     def decode_step_eager(self, token):
         """The same step without a program (used by tests to check the replayed graph)."""
         b = self._buffers(1)
-        self._set_decode_state(b, token)
+        self._set_decode_state(b, token, self.pos)
         self._forward(1, b)
         self._advanced(1)
         return int(self.gpu.download(self.token, np.int32, (1,))[0])
