@@ -137,7 +137,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
     int t_begin = wave * a.nseg + seg;
     // the pages of the half tiles of 32 steps, one to a lane; -1: none
     auto fetch_pages = [&](int step0) __attribute__((always_inline)) {
-        const int e = (int)((unsigned)((t_begin + (step0 + (lane >> 1)) * stride) * TILE_KEYS + (lane & 1) * 16) >> a.table.shift);
+        const int e = (int)(((unsigned)(t_begin + (step0 + (lane >> 1)) * stride) * TILE_KEYS + (lane & 1) * 16u) >> a.table.shift);
         return e >= 0 && e < a.table.width ? pages[e] : -1;
     };
     int ids = fetch_pages(0);
@@ -788,7 +788,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: queries are f32, f16 or bf16, not dtype %d", p->q_dtype);
     if (p->h_q == 0 || p->h_q % p->h_kv != 0) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention_paged: h_q %zu is not a multiple of h_kv %zu", p->h_q, p->h_kv);
     if (weights_before && !weights) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "attention_paged: weights to add to, and none to write");
-    if (!p->batch || !p->l_q) return AIONHIP_OK;
+    if (!p->batch || (!p->l_q && (!weights || weights == weights_before))) return AIONHIP_OK;
     const size_t groups = p->h_q / p->h_kv;
     if (p->h_q > 65535 || p->l_q > 0x7FFFFFFF / 16 / groups || p->batch * p->h_kv > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
     const size_t rows = p->l_q * groups, units = p->batch * p->h_kv, q_bytes = units * rows * c->d * (p->q_dtype == AIONHIP_F32 ? 4 : 2), out_bytes = units * rows * c->d * 4;
@@ -814,7 +814,8 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     a.d = (int)c->d, a.q_dtype = p->q_dtype, a.kv_dtype = c->dtype;
     a.scale = p->scale, a.soft_cap = p->attn_logits_soft_cap;
     a.win_left = p->window_left, a.win_right = p->window_right, a.win_chunk = p->window_chunk;
-    const bool fast = (c->d == 64 || c->d == 128 || c->d == 256) && (p->out & 15) == 0;
+    const bool none = p->l_q == 0;               // the weights stay what they were
+    const bool fast = (c->d == 64 || c->d == 128 || c->d == 256) && (p->out & 15) == 0 && !none;
     a.nseg = 1;
     bool once = false;
     if (fast) {
@@ -823,10 +824,11 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         if (!a.positions && a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + TILE_KEYS);
         const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
         a.nseg = segments(wgs, tiles, min(a.rows_total, 16), a.d, cus);
-        once = (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
+        once = a.row_tiles == 1 && (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
-    if ((size_t)a.row_tiles * a.nseg > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
-    if (weights && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
+    if ((fast ? (size_t)a.row_tiles * a.nseg * (c->d == 256 ? Cfg<256>::NW : Cfg<128>::NW) * 64 : rows * 256) > paged::MAX_THREADS)
+        return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
+    if (weights && rows && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take more than 4 GiB; ask for weights with fewer queries", units * rows, T);
     const size_t meetings = a.nseg > 1 ? units * a.row_tiles : 0, partial_bytes = meetings * a.nseg * (16 * c->d + 32) * 4;
     const size_t stats_bytes = weights ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
@@ -842,7 +844,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     }
     if (fast) {
         if (const int rc = c->dtype == AIONHIP_F16 ? launch_head<AIONHIP_F16>(ctx, a, (int)p->batch, once) : launch_head<AIONHIP_BF16>(ctx, a, (int)p->batch, once)) return rc;
-    } else {
+    } else if (!none) {
         ProfScope scope(ctx, "paged_generic");
         launch_k(ctx, paged_generic_kernel, dim3((unsigned)rows, (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
         LAUNCH_CHECK(ctx, "paged_generic");
@@ -850,7 +852,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     if (weights) {
         ProfScope scope(ctx, "paged_weights");
         launch_k(ctx, paged_weights_kernel, dim3((unsigned)((T + 1023) / 1024), (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
-        LAUNCH_CHECK(ctx, fast ? "paged_attn" : "paged_generic");
+        LAUNCH_CHECK(ctx, "paged_weights");
     }
     return AIONHIP_OK;
 }

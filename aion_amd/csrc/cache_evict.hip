@@ -246,7 +246,8 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "evict_paged: table_out is the cache's own, or %zu entries of %zu rows do not hold %zu", e->width_out, c->page_rows, e->limit);
     if (!c->batch) return AIONHIP_OK;
     const size_t cap_out = e->table_out ? e->width_out * c->page_rows : cap, units = c->batch * c->h_kv;
-    const size_t limit = min(e->limit, cap), kept_bytes = units * e->limit * 4;
+    // (a limit that no sequence passes may be any number: the list of what stays, and the memory between, are of the rows there can be)
+    const size_t limit = min(e->limit, cap), keep = min(e->keep, limit), kept_bytes = units * e->limit * 4, listed = e->kept ? e->limit : limit;
     if (units > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "evict_paged: dimension too large");
     const size_t w_bytes = units * cap * 4, wo_bytes = units * cap_out * 4, l_bytes = c->batch * 4, t_bytes = c->batch * e->width_out * 4;
     const bool same_w = e->weights_out == e->weights, same_l = e->lengths_out == e->kv_lengths;
@@ -258,12 +259,12 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
         overlap(e->table_out, t_bytes, e->lengths_out, l_bytes) || overlap(e->table_out, t_bytes, e->kept, kept_bytes) || overlap(e->table_out, t_bytes, c->k_pages, pool_bytes(c)) ||
         overlap(e->table_out, t_bytes, c->v_pages, pool_bytes(c)) || in_cache(c, e->weights, w_bytes) || in_cache(c, e->kv_lengths, l_bytes))
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "evict_paged: an operand that is written overlaps another");
-    const size_t row_bytes = c->d * 4, counts_bytes = (c->batch * 4 + 255) / 256 * 256, list_bytes = e->kept ? 0 : (kept_bytes + 255) / 256 * 256;
+    const size_t row_bytes = c->d * 4, counts_bytes = (c->batch * 4 + 255) / 256 * 256, list_bytes = e->kept ? 0 : (units * listed * 4 + 255) / 256 * 256;
     // in place: as many heads of sequences at once as the memory between takes
-    const size_t group = e->table_out || !e->keep ? units : min(units, max((size_t)1, HELD_BYTES / (e->keep * row_bytes)));
-    if (const int rc = ensure_scratch2(ctx, counts_bytes + list_bytes + (e->table_out ? 0 : group * e->keep * row_bytes))) return rc;
+    const size_t group = e->table_out || !keep ? units : min(units, max((size_t)1, HELD_BYTES / (keep * row_bytes)));
+    if (const int rc = ensure_scratch2(ctx, counts_bytes + list_bytes + (e->table_out ? 0 : group * keep * row_bytes))) return rc;
     int *counts = (int *)ctx->scratch2, *kept = e->kept ? dp<int>(e->kept) : (int *)((char *)ctx->scratch2 + counts_bytes);
-    const Select s{dp<const float>(e->weights), dp<const int>(e->kv_lengths), dp<float>(e->weights_out), kept, counts, (int)c->h_kv, (int)cap, (int)cap_out, (int)e->limit, (int)e->keep,
+    const Select s{dp<const float>(e->weights), dp<const int>(e->kv_lengths), dp<float>(e->weights_out), kept, counts, (int)c->h_kv, (int)cap, (int)cap_out, (int)listed, (int)keep,
                    (int)e->first, (int)e->recent, e->table_out ? 0 : 1, e->table_out || e->kept ? 1 : 0};
     {
         ProfScope scope(ctx, "evict_select");
@@ -273,13 +274,13 @@ extern "C" int aionhip_step_evict_paged(aionhip_ctx *ctx, const aionhip_paged_ca
         LAUNCH_CHECK(ctx, "evict_select");
     }
     Move m{{dp<unsigned char>(c->k_pages), dp<unsigned char>(c->v_pages)}, (unsigned char *)ctx->scratch2 + counts_bytes + list_bytes, kept, counts, dp<int>(e->lengths_out),
-           dp<const int>(e->kv_lengths), table_of(c), table_of(c), (int)c->h_kv, (int)c->d, (int)e->limit, (int)cap, (int)e->keep, 0, (int)(c->d / 8), 0};
+           dp<const int>(e->kv_lengths), table_of(c), table_of(c), (int)c->h_kv, (int)c->d, (int)listed, (int)cap, (int)keep, 0, (int)(c->d / 8), 0};
     ProfScope scope(ctx, "evict_move");
     if (e->table_out) {
         m.to.pages = dp<const int>(e->table_out);
         m.to.width = (int)e->width_out;
     }
-    const size_t rows = 256 / m.lanes, most = e->table_out ? limit : min(e->keep, limit);
+    const size_t rows = 256 / m.lanes, most = e->table_out ? limit : keep;
     for (size_t u = 0; u < units; u += 65535 < group ? 65535 : group) {
         const size_t n = min(units - u, min(group, (size_t)65535));
         m.first_unit = (int)u;

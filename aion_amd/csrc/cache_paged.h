@@ -8,7 +8,7 @@
 
 namespace paged {
 
-constexpr size_t MIN_PAGE = 16, MAX_PAGE = 1024, MAX_HEAD = 1024, MAX_ROWS = 0x7FFFFFC0;
+constexpr size_t MIN_PAGE = 16, MAX_PAGE = 1024, MAX_HEAD = 1024, MAX_ROWS = 0x7FFFFFC0, MAX_THREADS = 0xFFFFFFFF;      // (of a launch, along one axis of its grid)
 
 struct Table {
     const int *pages;

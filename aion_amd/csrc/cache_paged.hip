@@ -279,12 +279,10 @@ constexpr size_t ONCE_BYTES = (size_t)128 << 20;
 // the launch of `tokens` rows; `rotary` null or of no pairs: nothing turns
 int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rotary *rotary, size_t tokens, int dtype, int cache_dtype) {
     if (rotary && rotary->dims) {
-        if (const int rc = turn_table(ctx, rotary, &a.turns)) return rc;
         a.dims = (int)rotary->dims;
         a.interleaved = rotary->interleaved ? 1 : 0;
         a.magnitude = rotary->magnitude;
     }
-    if (tokens > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
     const int each = pairs_each(dtype);
     a.turning = (a.dims / 2 + each - 1) / each;
     a.pieces = a.turning + (a.d - a.dims + 2 * each - 1) / (2 * each);
@@ -295,6 +293,10 @@ int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rot
     const bool once = tokens * slots * a.d * (dtype == AIONHIP_F32 ? 8 : 4) >= ONCE_BYTES;
     const dim3 grid((unsigned)tokens, (unsigned)((slots + a.heads_wg * heads - 1) / (a.heads_wg * heads)));
     const unsigned threads = (unsigned)((a.heads_wg * a.pieces + 63) / 64 * 64);
+    if (tokens > MAX_THREADS / threads) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
+    if (a.dims) {
+        if (const int rc = turn_table(ctx, rotary, &a.turns)) return rc;
+    }
     ProfScope scope(ctx, who);
     auto go = [&](auto dt, auto ct) {
         constexpr int DT = decltype(dt)::value, CT = decltype(ct)::value;
@@ -384,7 +386,7 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *c, aion
     if (overlap(k_out, bytes, v_out, bytes) || overlap(k_out, bytes, first, c->batch * 4) || overlap(v_out, bytes, first, c->batch * 4))
         return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: the rows of keys and values overlap each other or the indices");
     if (in_cache(c, k_out, bytes) || in_cache(c, v_out, bytes)) return set_err(ctx, AIONHIP_INVALID_ARGUMENT, "read_paged: rows lie in the cache");
-    if ((total + 255) / 256 > 0x7FFFFFFF) return set_err(ctx, AIONHIP_UNSUPPORTED, "read_paged: too many rows for one launch");
+    if (total > MAX_THREADS - 255) return set_err(ctx, AIONHIP_UNSUPPORTED, "read_paged: too many rows for one launch");
     const ReadArgs a{{dp<const unsigned char>(c->k_pages), dp<const unsigned char>(c->v_pages)}, {dp<void>(k_out), dp<void>(v_out)}, dp<const int>(first), table_of(c), (int)s, (int)c->h_kv,
                      (int)c->d};
     const bool f16 = c->dtype == AIONHIP_F16;

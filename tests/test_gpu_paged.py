@@ -580,3 +580,39 @@ def test_the_kernels_by_name(gpu):
         bits, _ = source(rng, (1, 1, 2, d), be.F32)
         attend(gpu, pages, bits, be.F32, 0.1, lengths=[20])
         assert gpu.last_kernel() == name
+
+
+# ---------------------------------------------------------------------------------------------------------------- the ends of the ranges
+@pytest.mark.parametrize("d", [64, 72])
+def test_weights_of_no_queries_are_those_before(gpu, d):
+    rng = np.random.default_rng(12)
+    pages = Pages(rng, be.F16, 2, 5, 32, 2, d)
+    cache, q, out, ld = pages.upload(gpu), gpu.zeros(64), gpu.zeros(64), gpu.upload(np.array([150, 20], np.int32))
+    before = rng.standard_normal((2, 2, 160)).astype(np.float32)
+    bd, w = gpu.upload(before), gpu.upload(np.full(before.shape, np.nan, np.float32))
+    for given, want in ((bd, before), (None, np.zeros_like(before))):
+        gpu.step_attention_paged(out, q, cache, 0, 8, 0.125, kv_lengths=ld, weights=w, weights_before=given)
+        assert np.array_equal(gpu.download(w, np.float32, before.shape), want)
+    gpu.step_attention_paged(out, q, cache, 0, 8, 0.125, kv_lengths=ld, weights=bd, weights_before=bd)
+    assert np.array_equal(gpu.download(bd, np.float32, before.shape), before)
+    free(cache, q, out, ld, bd, w)
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(80, 1, 128), (33, 1, 64), (40, 2, 256)])
+def test_more_query_heads_to_a_kv_head_than_a_tile_has_rows(gpu, hq, hkv, d):
+    rng = np.random.default_rng(13)
+    pages = Pages(rng, be.F16, 2, 9, 32, hkv, d)
+    bits, q = source(rng, (2, 1, hq, d), be.F32)
+    check(gpu, pages, bits, q, be.F32, d ** -0.5, lengths=[288, 65])
+
+
+@pytest.mark.parametrize("keep", [7, 2 ** 31 - 65])
+def test_a_limit_far_past_the_capacity_cuts_nothing_and_takes_no_memory_for_it(gpu, keep):
+    rng = np.random.default_rng(14)
+    pages = Pages(rng, be.F16, 2, 5, 16, 2, 64)
+    weights = weigh(rng, (2, 2, 80), "plain")
+    cache, wd, ld, lo = pages.upload(gpu), gpu.upload(weights), gpu.upload(np.array([80, 99], np.int32)), gpu.alloc(8)
+    gpu.step_evict_paged(cache, wd, ld, wd, lo, keep, limit=2 ** 31 - 65, first=1, recent=2)
+    assert np.array_equal(gpu.download(lo, np.int32, (2,)), [80, 80]) and np.array_equal(gpu.download(wd, np.float32, weights.shape), weights)
+    assert pages.same(gpu, cache)
+    free(cache, wd, ld, lo)

@@ -125,6 +125,11 @@ def refusals(lib, ctx, at):
     say(("attention", "heads"), attend(good, h_q=1 << 17), UNS)
     say(("attention", "queries"), attend(good, l_q=1 << 30), UNS)
     wide = cache(at, table_width=1 << 20, page_table=1 << 47)
+    far = [1 << 46, 1 << 47, 1 << 48]
+    say(("rotary", "rows of one launch"), lib.aionhip_step_rotary(ctx, far[0], far[1], far[2], be.F32, 1, 1 << 27, 1, D, ref(rotary())), UNS)
+    say(("append", "rows of one launch"), append(cache(at, table_width=1 << 26, batch=4, page_table=far[0]), k=far[1], v=far[2], s=1 << 26), UNS)
+    say(("read", "rows of one launch"), read(cache(at, table_width=1 << 26, batch=4, page_table=far[0]), k=far[1], v=far[2], s=1 << 28), UNS)
+    say(("attention", "queries of one launch"), attend(cache(at, d=72), out=far[0], q=far[1], l_q=1 << 24, d_k=72, d_v=72), UNS)
     say(("attention", "scores"), attend(wide, weights=1 << 50, l_q=64, cap=P << 20), UNS)
     for change in (dict(weights=0), dict(kv_lengths=0), dict(weights_out=0), dict(lengths_out=0), dict(keep=41), dict(first=27), dict(recent=29), dict(limit=1 << 31), dict(width_out=2),
                    dict(table_out=0), dict(table_out=at(2)), dict(weights_out=at(9)), dict(weights_out=at(9) + 16), dict(lengths_out=at(10)), dict(kept=at(9)), dict(kept=at(10) + 4),
