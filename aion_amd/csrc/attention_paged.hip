@@ -1,7 +1,7 @@
 // Attention over caches in pages (the layout: cache_paged.h): one to a few tokens a sequence, f32 accuracy, and with it what each key's probabilities add up to.
 //
-// paged_attn_kernel - head sizes 64, 128, 256. A workgroup has sixteen query rows of one KV head (position-major, query head fastest) and one segment of their keys; its
-//   wavefronts take tiles of 32 keys in turn:
+// paged_attn_kernel - head sizes 64, 128, 256. A workgroup has sixteen query rows of one KV head (position-major, query head fastest), one segment of their keys and, in small
+//   calls, a share of the value columns; its wavefronts take tiles of 32 keys in turn:
 //       S^T[keys x rows] = K[keys x d] . Q^T[d x rows]          O^T[d x rows] += V^T[d x keys] . P^T[keys x rows]
 //   K goes from the pages to registers in the order the matrix instruction wants it, V through LDS, where it is read transposed. Sixteen keys lie in one page, so a
 //   page number is a scalar to each half tile: a lane fetches one of the next 64, and they become addresses without a load in between.
@@ -30,7 +30,7 @@ struct PagedArgs {
     float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
     unsigned *tickets;
     Table table;
-    int T, tpad, L, Hkv, groups, rows_total, row_tiles, nseg;
+    int T, tpad, L, Hkv, groups, rows_total, row_tiles, nseg, shares;
     int d, q_dtype, kv_dtype;
     float scale, soft_cap;
     unsigned win_left, win_right, win_chunk;
@@ -50,12 +50,13 @@ __device__ __forceinline__ void row_keys(const PagedArgs &a, int b, int li, int 
 }
 
 constexpr int MOST_SEGMENTS = 256;      // of a row tile
-template <int D>
+constexpr int wavefronts(int d) { return d == 256 ? 8 : 4; }     // of a workgroup
+template <int D, int SHARES>
 struct Cfg {
-    static constexpr int NW = D == 256 ? 8 : 4;                  // wavefronts of a workgroup
-    static constexpr int ROW = D * 2, TILE = TILE_KEYS * ROW;
-    static constexpr int SLOT = 16 * (D + 4) + 32;               // a wavefront's results where they meet: [16][D + 4], 16 references, 16 sums
-    static constexpr int PART = 16 * D + 32;                     // a segment's results in memory: [16][D], [16] (reference, sum)
+    static constexpr int NW = wavefronts(D), DV = D / SHARES;    // value columns of a workgroup
+    static constexpr int ROW = D * 2, V_ROW = DV * 2, TILE = TILE_KEYS * V_ROW;
+    static constexpr int SLOT = 16 * (DV + 4) + 32;              // a wavefront's results where they meet: [16][DV + 4], 16 references, 16 sums
+    static constexpr int PART = 16 * DV + 32;                    // a segment's results in memory: [16][DV], [16] (reference, sum)
     static constexpr int MOST = MOST_SEGMENTS;
     static constexpr int MEET = NW * SLOT * 4, JOIN = (16 * MOST + 64) * 4 + NW * 64 * 16;          // LDS where wavefronts, where segments meet
     static constexpr int MAIN = NW * TILE > MEET ? (NW * TILE > JOIN ? NW * TILE : JOIN) : MEET > JOIN ? MEET : JOIN;
@@ -68,9 +69,9 @@ __device__ __forceinline__ u32x4 lds_read(unsigned addr) {
     return x;
 }
 
-// One row's share of one wavefront, a key at a time: what its lanes have of the sums (columns lane, lane + 64, ..), its reference and its sum. See paged_attn_kernel.
-template <int D>
-__device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, int r, int rows_total, int L, int lo, int hi, int t_begin, int steps, int stride, float (&o)[D / 64],
+// One row's share of one wavefront, a key at a time: what its lanes have of the sums (columns dv0 + lane, dv0 + lane + 64, ..), its reference and its sum. See paged_attn_kernel.
+template <int D, int DV>
+__device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, int r, int rows_total, int L, int lo, int hi, int t_begin, int steps, int stride, int dv0, float (&o)[DV / 64],
                                                      float &top_out, float &sum_out) {
     const int lane = threadIdx.x & 63, li = r / a.groups, gi = r - li * a.groups;
     const size_t qbase = (((size_t)b * L + li) * (a.Hkv * a.groups) + hk * a.groups + gi) * D;
@@ -78,8 +79,9 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
         q[j] = load_scalar(a.q, a.q_dtype, qbase + lane + 64 * j);
-        o[j] = 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < DV / 64; ++j) o[j] = 0.f;
 #pragma unroll 1
     for (int i = 0; i < steps; ++i)
 #pragma unroll 1
@@ -94,11 +96,11 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
             for (int j = 0; j < D / 64; ++j) dot += q[j] * load_scalar(a.k, a.kv_dtype, at + lane + 64 * j);
             dot = lanes_sum(dot);
             const float s = a.soft_cap > 0.f ? a.soft_cap * LOG2E * tanhf(dot * (a.scale / a.soft_cap)) : dot * (a.scale * LOG2E);
-            if (a.scores && lane == 0) a.scores[((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key] = s;
+            if (a.scores && lane == 0 && dv0 == 0) a.scores[((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key] = s;
             const float top = fmaxf(ref, s), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + HEAD_ROOM);
             l = l * alpha + p;
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) o[j] = o[j] * alpha + p * load_scalar(a.v, a.kv_dtype, at + lane + 64 * j);
+            for (int j = 0; j < DV / 64; ++j) o[j] = o[j] * alpha + p * load_scalar(a.v, a.kv_dtype, at + dv0 + lane + 64 * j);
             ref = top;
         }
     top_out = ref;
@@ -106,13 +108,13 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
 }
 
 // QP: how many halves a query element is the sum of. MULTI: several queries a sequence, whose keys may differ (of one query all rows see the same). ONCE: keys and values
-// go past the caches. The leading arguments, 14 words, arrive in SGPRs with the wavefront. heads: KV heads, query heads of each << 16;
+// go past the caches. SHARES: workgroups that divide the value columns. The leading arguments, 14 words, arrive in SGPRs with the wavefront. heads: KV heads, query heads of each << 16;
 // form: segments, log2 of a page's rows << 12, query type << 16, rows of the queries in LDS << 24.
-template <int KV, int D, int QP, bool MULTI, bool ONCE>
-__global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
+template <int KV, int D, int QP, bool MULTI, bool ONCE, int SHARES>
+__global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
                                                                      unsigned heads, unsigned form, PagedArgs tail) {
-    using C = Cfg<D>;
-    constexpr int NW = C::NW, KK = D / 32, MT = D / 16;
+    using C = Cfg<D, SHARES>;
+    constexpr int NW = C::NW, DV = C::DV, KK = D / 32, MT = DV / 16;
     constexpr int PP = KV == AIONHIP_F16 ? 2 : 3;                // parts of a probability
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     PagedArgs a = tail;
@@ -126,7 +128,8 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int rows_total = L * a.groups;
-    const int rt = rows_total <= 16 ? 0 : blockIdx.x / a.nseg, seg = blockIdx.x - rt * a.nseg, hk = blockIdx.y, b = blockIdx.z;
+    const int share = SHARES == 1 ? 0 : blockIdx.x % SHARES, dv0 = share * DV, place = blockIdx.x / SHARES;
+    const int rt = rows_total <= 16 ? 0 : place / a.nseg, seg = place - rt * a.nseg, hk = blockIdx.y, b = blockIdx.z;
     const int unit = b * a.Hkv + hk;
     const int len_raw = kv_lengths ? kv_lengths[b] : 0;
 
@@ -216,8 +219,8 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
     };
     // V: 1 KiB an instruction, straight into LDS. 16-byte chunk c of key k lies at slot c ^ (2 * ((k >> 2) & 3)) ^ (8 * (k & 1)) of its row (the last term for rows
     // of 256 bytes and more), so that the sixteen keys of a transposing read fall on distinct banks.
-    constexpr int NVI = C::TILE / 1024, KEYS_PER_VI = 1024 / C::ROW;
-    const int v_key_in = (lane * 16) / C::ROW, v_slot = ((lane * 16) % C::ROW) / 16;
+    constexpr int NVI = C::TILE / 1024, KEYS_PER_VI = 1024 / C::V_ROW;
+    const int v_key_in = (lane * 16) / C::V_ROW, v_slot = ((lane * 16) % C::V_ROW) / 16;
     constexpr int NON_TEMPORAL = 2;                              // the nt bit of a buffer access
     (void)v_slot; (void)vp; (void)NON_TEMPORAL;
     auto load_v = [&](int t, int id0, int id1) __attribute__((always_inline)) {
@@ -229,8 +232,8 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
 #pragma unroll
             for (int i = 0; i < NVI / 2; ++i) {
                 const int key = i * KEYS_PER_VI + v_key_in;
-                const int chunk = v_slot ^ (2 * ((key >> 2) & 3)) ^ (D >= 128 ? 8 * (key & 1) : 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(vs + (h * (NVI / 2) + i) * 1024), 16, key * C::ROW + chunk * 16, 0, 0, ONCE ? NON_TEMPORAL : 0);
+                const int chunk = v_slot ^ (2 * ((key >> 2) & 3)) ^ (DV >= 128 ? 8 * (key & 1) : 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(vs + (h * (NVI / 2) + i) * 1024), 16, key * C::ROW + dv0 * 2 + chunk * 16, 0, 0, ONCE ? NON_TEMPORAL : 0);
             }
         }
 #endif
@@ -313,13 +316,13 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
     const float cap_log2 = a.soft_cap * LOG2E;
 
     const int tr_r = (lane >> 2) & 3, tr_q = lane & 3;
-    const unsigned v_rowaddr = (unsigned)(size_t)(lds_void *)vs + (unsigned)((4 * g + tr_r) * C::ROW + (tr_q & 1) * 8);
-    const unsigned v_slot_l = (unsigned)(((tr_q >> 1) ^ (2 * g) ^ (D >= 128 ? 8 * (tr_r & 1) : 0)) << 4);
+    const unsigned v_rowaddr = (unsigned)(size_t)(lds_void *)vs + (unsigned)((4 * g + tr_r) * C::V_ROW + (tr_q & 1) * 8);
+    const unsigned v_slot_l = (unsigned)(((tr_q >> 1) ^ (2 * g) ^ (DV >= 128 ? 8 * (tr_r & 1) : 0)) << 4);
     auto v_operand = [&](unsigned vr, unsigned vl, auto mt_c) __attribute__((always_inline)) {
         constexpr int mt = decltype(mt_c)::value;
         const unsigned addr = vr + (vl ^ (unsigned)(mt << 5));
         u32x2 a0, a1;
-        asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3" : "=&v"(a0), "=&v"(a1) : "v"(addr), "n"(16 * C::ROW) : "memory");
+        asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3" : "=&v"(a0), "=&v"(a1) : "v"(addr), "n"(16 * C::V_ROW) : "memory");
         return u32x4{a0.x, a0.y, a1.x, a1.y};
     };
 
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
                 p[j] = key >= lo && key < hi && (j < 4 ? ok0 : ok1) ? p[j] : MASKED;
             }
         }
-        if (a.scores) {
+        if (a.scores && share == 0) {
             if (row_ok) {
                 *(f32x4 *)(scores + key0 + g * 4) = f32x4{p[0], p[1], p[2], p[3]};
                 *(f32x4 *)(scores + key0 + 16 + g * 4) = f32x4{p[4], p[5], p[6], p[7]};
@@ -457,10 +460,10 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
 #pragma unroll 1
             for (int i = 0; i < 16; ++i) {
                 if (!(spoilt >> i & 0x0001000100010001ull)) continue;
-                float o[D / 64], top, sum;
-                walk_again<D>(a, b, hk, rt * 16 + i, rows_total, L, __builtin_amdgcn_readlane(lo, i), __builtin_amdgcn_readlane(hi, i), t_begin, steps, stride, o, top, sum);
+                float o[DV / 64], top, sum;
+                walk_again<D, DV>(a, b, hk, rt * 16 + i, rows_total, L, __builtin_amdgcn_readlane(lo, i), __builtin_amdgcn_readlane(hi, i), t_begin, steps, stride, dv0, o, top, sum);
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) ((float *)vs)[lane + 64 * j] = o[j];
+                for (int j = 0; j < DV / 64; ++j) ((float *)vs)[lane + 64 * j] = o[j];
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 if (n == i) {
 #pragma unroll
@@ -478,13 +481,13 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
     auto put = [&](int row, int col, f32x4 o, float top, float l) __attribute__((always_inline)) {
         const int rr = rt * 16 + row, l2 = L > 1 ? rr / a.groups : 0, g2 = rr - l2 * a.groups;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        *(f32x4 *)(a.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + col) = o * inv;
-        if (a.stats && col == 0) a.stats[(size_t)unit * rows_total + rr] = float2{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
+        *(f32x4 *)(a.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + dv0 + col) = o * inv;
+        if (a.stats && dv0 + col == 0) a.stats[(size_t)unit * rows_total + rr] = float2{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
     };
     // Device-scope accesses: written through, read at the point where the XCDs' caches agree.
     constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access
     (void)DEVICE_SCOPE;
-    const int meeting = unit * a.row_tiles + rt;
+    const int meeting = (unit * a.row_tiles + rt) * SHARES + share;
     [[maybe_unused]] float *const slots = a.partial + (size_t)meeting * a.nseg * C::PART;
 #if defined(__HIP_DEVICE_COMPILE__)
     const __amdgpu_buffer_rsrc_t slots_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)slots, 0, (unsigned)(a.nseg * C::PART * 4), 0x00027000);
@@ -495,8 +498,8 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
             return;
         }
 #if defined(__HIP_DEVICE_COMPILE__)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), slots_rsrc, (seg * C::PART + row * D + col) * 4, 0, DEVICE_SCOPE);
-        if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(l)}, slots_rsrc, (seg * C::PART + 16 * D + row * 2) * 4, 0, DEVICE_SCOPE);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), slots_rsrc, (seg * C::PART + row * DV + col) * 4, 0, DEVICE_SCOPE);
+        if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(l)}, slots_rsrc, (seg * C::PART + 16 * DV + row * 2) * 4, 0, DEVICE_SCOPE);
 #endif
     };
     if (te - tb <= a.nseg) {                                     // the first wavefront has all there is
@@ -511,19 +514,19 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
         if (row_ok) {
             float *w = mg + wave * C::SLOT;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) *(f32x4 *)(w + n * (D + 4) + mt * 16 + g * 4) = acc[mt];
-            if (g == 0) { w[16 * (D + 4) + n] = ref; w[16 * (D + 4) + 16 + n] = l_run; }
+            for (int mt = 0; mt < MT; ++mt) *(f32x4 *)(w + n * (DV + 4) + mt * 16 + g * 4) = acc[mt];
+            if (g == 0) { w[16 * (DV + 4) + n] = ref; w[16 * (DV + 4) + 16 + n] = l_run; }
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < rows * (D / 4); e += NW * 64) {
-            const int row = e / (D / 4), col = (e % (D / 4)) * 4;
+        for (int e = threadIdx.x; e < rows * (DV / 4); e += NW * 64) {
+            const int row = e / (DV / 4), col = (e % (DV / 4)) * 4;
             float rw[NW], lw[NW], top = MASKED, l = 0.f;
             f32x4 ow[NW], o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
-                rw[w] = mg[w * C::SLOT + 16 * (D + 4) + row];
-                lw[w] = mg[w * C::SLOT + 16 * (D + 4) + 16 + row];
-                ow[w] = *(const f32x4 *)(mg + w * C::SLOT + row * (D + 4) + col);
+                rw[w] = mg[w * C::SLOT + 16 * (DV + 4) + row];
+                lw[w] = mg[w * C::SLOT + 16 * (DV + 4) + 16 + row];
+                ow[w] = *(const f32x4 *)(mg + w * C::SLOT + row * (DV + 4) + col);
                 top = fmaxf(top, rw[w]);
             }
 #pragma unroll
@@ -561,11 +564,11 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
             st[i][j] = u32x2{__float_as_uint(MASKED), 0u};
 #if defined(__HIP_DEVICE_COMPILE__)
             if (wave + i * NW < rows && lane + 64 * j < live)
-                st[i][j] = __builtin_amdgcn_raw_buffer_load_b64(slots_rsrc, ((lane + 64 * j) * C::PART + 16 * D + (wave + i * NW) * 2) * 4, 0, DEVICE_SCOPE);
+                st[i][j] = __builtin_amdgcn_raw_buffer_load_b64(slots_rsrc, ((lane + 64 * j) * C::PART + 16 * DV + (wave + i * NW) * 2) * 4, 0, DEVICE_SCOPE);
 #endif
         }
     // A thread has four columns of a row; where there are more threads than that, several share the segments. Eight parts at a time, the next eight asked for ahead.
-    const int pieces = rows * (D / 4), sets = max(1, NW * 64 / pieces), set = (int)threadIdx.x / pieces;
+    const int pieces = rows * (DV / 4), sets = max(1, NW * 64 / pieces), set = (int)threadIdx.x / pieces;
     const bool mine = set < sets;
     int e = (int)threadIdx.x - set * pieces, s0 = set;
     u32x4 x[2][8];
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
             [[maybe_unused]] const int s = s0 + j * sets;        // (past the last segment: past the buffer's end, which reads as zeros)
             to[j] = u32x4{0u, 0u, 0u, 0u};
 #if defined(__HIP_DEVICE_COMPILE__)
-            to[j] = __builtin_amdgcn_raw_buffer_load_b128(slots_rsrc, s < live && e < pieces ? (s * C::PART + e / (D / 4) * D + e % (D / 4) * 4) * 4 : 0x7FFFFFF0, 0, DEVICE_SCOPE);
+            to[j] = __builtin_amdgcn_raw_buffer_load_b128(slots_rsrc, s < live && e < pieces ? (s * C::PART + e / (DV / 4) * DV + e % (DV / 4) * 4) * 4 : 0x7FFFFFF0, 0, DEVICE_SCOPE);
 #endif
         }
     };
@@ -605,7 +608,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
         const int e2 = last ? e + NW * 64 : e, s2 = last ? set : s0 + 8 * sets;
         const bool more = !last || (sets == 1 && e2 - (int)threadIdx.x < pieces);
         if (more) ask(next, e2, s2);
-        const int row = min(e / (D / 4), 15);
+        const int row = min(e / (DV / 4), 15);
 #pragma unroll
         for (int j = 0; j < 8; ++j) o += __builtin_bit_cast(f32x4, now[j]) * (s0 + j * sets < live ? s_f[row * C::MOST + s0 + j * sets] : 0.f);
         if (last) {
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(Cfg<D>::NW * 64, D == 256 ? 2 : 3) void paged_attn_
                 if (set == 0)
                     for (int i = 1; i < sets; ++i) o += s_o[i * pieces + threadIdx.x];
             }
-            if (mine && set == 0 && e < pieces) put(row, e % (D / 4) * 4, o, s_top[row], s_l[row]);
+            if (mine && set == 0 && e < pieces) put(row, e % (DV / 4) * 4, o, s_top[row], s_l[row]);
             o = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         e = e2, s0 = s2;
@@ -721,21 +724,24 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
     if (a.stats && threadIdx.x == 0) a.stats[(size_t)unit * a.rows_total + r] = float2{top > MASKED ? top : 0.f, inv};
 }
 
-template <int KV, int D, int QP, bool MULTI, bool ONCE>
+template <int KV, int D, int QP, bool MULTI, bool ONCE, int SHARES = 1>
 int launch(aionhip_ctx *ctx, const PagedArgs &a, int batch) {
-    const auto kernel = paged_attn_kernel<KV, D, QP, MULTI, ONCE>;
+    using C = Cfg<D, SHARES>;
+    const auto kernel = paged_attn_kernel<KV, D, QP, MULTI, ONCE, SHARES>;
     const int q_rows = D == 256 && a.rows_total <= 8 ? 8 : 16;
-    const size_t lds = Cfg<D>::MAIN + QP * q_rows * Cfg<D>::ROW + 64;
+    const size_t lds = C::MAIN + QP * q_rows * C::ROW + 64;
     static std::atomic<uint64_t> attr{0};
-    if (const int rc = allow_lds(ctx, attr, (const void *)kernel, Cfg<D>::MAIN + QP * 16 * Cfg<D>::ROW + 64)) return rc;
+    if (const int rc = allow_lds(ctx, attr, (const void *)kernel, C::MAIN + QP * 16 * C::ROW + 64)) return rc;
     ProfScope scope(ctx, "paged_attn");
-    launch_k(ctx, kernel, dim3((unsigned)(a.row_tiles * a.nseg), (unsigned)a.Hkv, (unsigned)batch), dim3(Cfg<D>::NW * 64), lds, a.kv_lengths, a.q, a.table.pages, a.k, a.v, a.T, a.L,
+    launch_k(ctx, kernel, dim3((unsigned)(a.row_tiles * a.nseg * SHARES), (unsigned)a.Hkv, (unsigned)batch), dim3(C::NW * 64), lds, a.kv_lengths, a.q, a.table.pages, a.k, a.v, a.T, a.L,
              (unsigned)a.Hkv | (unsigned)a.groups << 16, (unsigned)a.nseg | (unsigned)a.table.shift << 12 | (unsigned)a.q_dtype << 16 | (unsigned)q_rows << 24, a);
     LAUNCH_CHECK(ctx, "paged_attn");
     return AIONHIP_OK;
 }
 template <int KV, int D, int QP>
 int launch_form(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
+    if constexpr (D > 64)
+        if (a.shares > 1) return a.L > 1 ? launch<KV, D, QP, true, false, D / 64>(ctx, a, batch) : launch<KV, D, QP, false, false, D / 64>(ctx, a, batch);
     if (a.L > 1) return launch<KV, D, QP, true, false>(ctx, a, batch);
     return once ? launch<KV, D, QP, false, true>(ctx, a, batch) : launch<KV, D, QP, false, false>(ctx, a, batch);
 }
@@ -751,24 +757,34 @@ int launch_head(aionhip_ctx *ctx, const PagedArgs &a, int batch, bool once) {
     return launch_parts<KV, 256>(ctx, a, batch, once);
 }
 
-// Key segments of a row tile. As many as give each CU two workgroups at once (one of head size 256, whose LDS does not hold two), or four (two) in turn where the sequences alone
-// fill the CUs, since these are of uneven lengths: 32 sequences of up to 16384 keys, 8 heads of 128, 253 us in four segments, 263 in two, 277 in one. Fewer where joining them
-// costs more than they save, by what both take, us: a tile of a wavefront, its bytes through the CU's L1 (64 a clock), the wavefronts' meeting, and the workgroup that
-// joins, NW * 8 KiB of parts to a memory round trip. One token over 4015 keys, one head of 256 for 8, 126 segments 18.4 us, 16 15.3.
-int segments(long wgs, long tiles, int rows, int d, long cus) {
+// How a row tile is split: key segments, and shares of the value columns (each share computes all of the scores; the reads of V, the second product, the meetings and the
+// joining are divided). As many segments as give each CU two workgroups at once (one of head size 256, whose LDS does not hold two), or four (two) in turn where the sequences alone
+// fill the CUs, since these are of uneven lengths: 32 sequences of up to 16384 keys, 8 heads of 128, 253 us in four segments, 263 in two, 277 in one. Fewer, and in shares of 64
+// columns while those leave no CU with two workgroups, where that is less by what the parts of a call took one by one, us: a tile (a CU has only so many loads
+// in flight, so that two workgroups on one take 1.4 to 1.6 times as long), whole rows of V on their way through the first one, the wavefronts' meeting, the segments' joining,
+// of which the workgroup that joins reads NW * 8 KiB of parts to a memory round trip. Over 40 shapes the choice is within 8 % of the best of 30 on all but one (12).
+// One token, one head of 256 for 8, whole / in four shares, us: 100 keys 7.8 / 6.4, 531 10.4 / 7.3, 2048 11.0 / 8.4, 8192 14.6 / 9.8, 131072 38 / 54; 8 heads of 128 for 32, whole / in two: 100 keys
+// 6.2 / 5.5, 531 7.5 / 6.9, 2048 7.4 / 7.3, 8192 (whole in 32 segments, which two shares have no room for) 10.0 / 13.1.
+struct Split { int segments, shares; };
+Split split_of(long wgs, long tiles, int rows, int d, long cus) {
     const long at_once = d == 256 ? 1 : 2;
-    const int nw = d == 256 ? Cfg<256>::NW : Cfg<128>::NW;
-    const long room = wgs >= cus ? (2 * at_once * cus + wgs - 1) / wgs : max(1L, at_once * cus / wgs);
-    const float tile_us = 0.8f + 1.2f * d / 256, fill_us = 0.22f * d / 256, part_bytes = (float)rows * d * 4;
-    long best = max(1L, min(min(room, tiles), (long)MOST_SEGMENTS));
+    const int nw = wavefronts(d);
+    Split best{1, 1};
     float least = INFINITY;
-    for (long n = best;; n = (n + 1) / 2) {
-        const float joins = n > 1 ? 0.7f * ceilf(n * part_bytes / (nw * 8192)) : 0.f;
-        const float us = tile_us * ((tiles + n * nw - 1) / (n * nw)) + fill_us * ((tiles + n - 1) / n) + (tiles > n ? 1.f : 0.f) + joins;
-        if (us < least) least = us, best = n;
-        if (n == 1) break;
+    for (int shares = 1; shares == 1 || (shares == d / 64 && wgs * shares <= cus); shares = d / 64) {
+        const long room = shares > 1 ? cus / (wgs * shares) : wgs >= cus ? (2 * at_once * cus + wgs - 1) / wgs : max(1L, at_once * cus / wgs);
+        const float tile_us = d == 256 ? (shares > 1 ? 0.55f : 0.6f) : (shares > 1 ? 0.45f : 0.35f) * d / 128, whole_us = shares > 1 ? 0.f : d == 256 ? 1.5f : 0.5f, meet_us = (d == 256 ? 2.f : 0.6f) / shares, part_bytes = (float)rows * d * 4 / shares;
+        for (long n = max(1L, min(min(room, tiles), (long)MOST_SEGMENTS));; n = (n + 1) / 2) {
+            const long each = (tiles + n - 1) / n;
+            const bool two = wgs * n * shares > cus;             // workgroups of a CU: they share what it has of loads in flight
+            const float us = whole_us + tile_us * each * (!two ? 1.f : d == 64 ? 1.4f : 1.6f) + (two ? 0.5f : 0.f) + (each > 1 ? meet_us : 0.f) +
+                             (n > 1 ? 1.f + 0.25f * nw + 0.7f * n * part_bytes / (nw * 8192) : 0.f);
+            if (us < least) least = us, best = Split{(int)n, shares};
+            if (n == 1) break;
+        }
+        if (shares == d / 64) break;
     }
-    return (int)best;
+    return best;
 }
 
 // keys and values of this many bytes go past the caches: what is read once a step would push out what is read again. One token over 131072 keys, 8 heads of 128 (512 MiB),
@@ -816,21 +832,22 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     a.win_left = p->window_left, a.win_right = p->window_right, a.win_chunk = p->window_chunk;
     const bool none = p->l_q == 0;               // the weights stay what they were
     const bool fast = (c->d == 64 || c->d == 128 || c->d == 256) && (p->out & 15) == 0 && !none;
-    a.nseg = 1;
+    a.nseg = a.shares = 1;
     bool once = false;
     if (fast) {
         // Behind a window there are no more keys than it shows to the call's consecutive queries.
         long keys = a.T;
         if (!a.positions && a.win_chunk == 0 && a.win_right < (unsigned)a.T && a.win_left < (unsigned)a.T) keys = min(keys, (long)a.win_left + (long)a.win_right + a.L + TILE_KEYS);
         const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
-        a.nseg = segments(wgs, tiles, min(a.rows_total, 16), a.d, cus);
+        const Split split = split_of(wgs, tiles, min(a.rows_total, 16), a.d, cus);
+        a.nseg = split.segments, a.shares = split.shares;
         once = a.row_tiles == 1 && (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
-    if ((fast ? (size_t)a.row_tiles * a.nseg * (c->d == 256 ? Cfg<256>::NW : Cfg<128>::NW) * 64 : rows * 256) > paged::MAX_THREADS)
+    if ((fast ? (size_t)a.row_tiles * a.nseg * a.shares * (c->d == 256 ? wavefronts(256) : wavefronts(128)) * 64 : rows * 256) > paged::MAX_THREADS)
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
     if (weights && rows && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take more than 4 GiB; ask for weights with fewer queries", units * rows, T);
-    const size_t meetings = a.nseg > 1 ? units * a.row_tiles : 0, partial_bytes = meetings * a.nseg * (16 * c->d + 32) * 4;
+    const size_t meetings = a.nseg > 1 ? units * a.row_tiles * a.shares : 0, partial_bytes = meetings * a.nseg * (16 * c->d / a.shares + 32) * 4;
     const size_t stats_bytes = weights ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
     if (const int rc = ensure_scratch2(ctx, partial_bytes + stats_bytes + scores_bytes)) return rc;
     if (meetings) {
@@ -852,7 +869,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     if (weights) {
         ProfScope scope(ctx, "paged_weights");
         launch_k(ctx, paged_weights_kernel, dim3((unsigned)((T + 1023) / 1024), (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
-        LAUNCH_CHECK(ctx, "paged_weights");
+        LAUNCH_CHECK(ctx, none ? "paged_weights" : fast ? "paged_attn" : "paged_generic");
     }
     return AIONHIP_OK;
 }

@@ -616,3 +616,24 @@ def test_a_limit_far_past_the_capacity_cuts_nothing_and_takes_no_memory_for_it(g
     assert np.array_equal(gpu.download(lo, np.int32, (2,)), [80, 80]) and np.array_equal(gpu.download(wd, np.float32, weights.shape), weights)
     assert pages.same(gpu, cache)
     free(cache, wd, ld, lo)
+
+
+@pytest.mark.parametrize("hq, hkv, d, lengths", [(8, 1, 256, [3]), (8, 1, 256, [32]), (8, 1, 256, [33, 700]), (6, 2, 256, [1500, 0, 31]), (4, 4, 256, [2100]), (32, 8, 128, [31]), (32, 8, 128, [1001, 33]),
+                                               (2, 1, 128, [5000, 1, 64])])
+@pytest.mark.parametrize("l", [1, 3])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_value_columns_in_shares(gpu, dtype, hq, hkv, d, lengths, l):
+    """few workgroups: the columns are dealt out, the weights come from one share of them, and rows that end as no number are walked by each"""
+    rng = np.random.default_rng(15)
+    pages = Pages(rng, dtype, len(lengths), -(-max(lengths) // 32) + 1, 32, hkv, d)
+    bits, q = source(rng, (len(lengths), l, hq, d), be.F32)
+    check(gpu, pages, bits, q, be.F32, d ** -0.5, lengths=lengths)
+    # an infinite value in one column of the last step but one, which the first of three queries does not see
+    near, drawn = attention(q, pages, l, hq, d ** -0.5, lengths=lengths)
+    pages.v[pages.page(0, lengths[0] - 2), hkv - 1, (lengths[0] - 2) % 32, d - 70] = to_bits(np.array([np.inf], np.float32), dtype)[0]
+    got, weights = attend(gpu, pages, bits, be.F32, d ** -0.5, lengths=lengths)
+    hit = np.zeros(got.shape, bool)
+    hit[0, max(0, l - 2):, -(hq // hkv):, d - 70] = True
+    assert (got[hit] == np.inf).all()
+    near.out[hit] = got[hit] = 0.0
+    assert near.close(got).all() and near.weights_close(weights, drawn, l * hq // hkv).all()
