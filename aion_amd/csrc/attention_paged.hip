@@ -6,8 +6,8 @@
 //   K goes from the pages to registers in the order the matrix instruction wants it, V through LDS, where it is read transposed. Sixteen keys lie in one page, so a
 //   page number is a scalar to each half tile: a lane fetches one of the next 64, and they become addresses without a load in between.
 //   Accuracy: q and P enter the products as sums of halves (two f16, three bf16; q that comes in the cache's type as it is), K and V are exact, sums are f32.
-//   The workgroup that ends last adds the segments of its rows.
-// paged_weights_kernel - what the keys draw, from the scores that the first kernel left.
+//   The workgroup that ends last adds the segments of its rows and, where the capacity is small, what the keys draw.
+// paged_weights_kernel - what the keys draw elsewhere, from the scores that the first kernel left.
 // paged_generic_kernel - other head sizes: a wavefront a key at a time, f32. It is there so that every shape has a path.
 #include "attention_common.h"
 #include "cache_paged.h"
@@ -28,6 +28,7 @@ struct PagedArgs {
     const float *weights_before;
     float *weights;
     float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
+    int draws;                // the workgroup that ends last adds up the weights itself
     unsigned *tickets;
     Table table;
     int T, tpad, L, Hkv, groups, rows_total, row_tiles, nseg, shares;
@@ -96,7 +97,8 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
             for (int j = 0; j < D / 64; ++j) dot += q[j] * load_scalar(a.k, a.kv_dtype, at + lane + 64 * j);
             dot = lanes_sum(dot);
             const float s = a.soft_cap > 0.f ? a.soft_cap * LOG2E * tanhf(dot * (a.scale / a.soft_cap)) : dot * (a.scale * LOG2E);
-            if (a.scores && lane == 0 && dv0 == 0) a.scores[((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key] = s;
+            if (a.scores && lane == 0 && dv0 == 0)
+                __hip_atomic_store(a.scores + ((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             const float top = fmaxf(ref, s), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + HEAD_ROOM);
             l = l * alpha + p;
 #pragma unroll
@@ -329,6 +331,11 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     f32x4 acc[MT];
     float ref = MASKED, l_run = 0.f;                             // l_run: of this lane's keys
     float *scores = a.scores + ((size_t)unit * rows_total + r) * a.tpad;
+    constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access: written through, read at the point where the XCDs' caches agree
+    (void)DEVICE_SCOPE;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const __amdgpu_buffer_rsrc_t scores_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(a.scores + (size_t)unit * rows_total * a.tpad), 0, a.draws ? (unsigned)(rows_total * a.tpad * 4) : 0u, 0x00027000);
+#endif
     // MORE: another tile of this wavefront follows (two copies of the body, so that every path requests K and V in the same order and the count of loads in flight holds)
     auto tile = [&](int t, bool ok0, bool ok1, int next0, int next1, auto more_c) __attribute__((always_inline)) {
         constexpr bool more = decltype(more_c)::value;
@@ -368,10 +375,17 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
             }
         }
         if (a.scores && share == 0) {
-            if (row_ok) {
+            if (row_ok && !a.draws) {
                 *(f32x4 *)(scores + key0 + g * 4) = f32x4{p[0], p[1], p[2], p[3]};
                 *(f32x4 *)(scores + key0 + 16 + g * 4) = f32x4{p[4], p[5], p[6], p[7]};
             }
+#if defined(__HIP_DEVICE_COMPILE__)
+            if (row_ok && a.draws) {
+                const int at = (r * a.tpad + key0 + g * 4) * 4;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]}), scores_rsrc, at, 0, DEVICE_SCOPE);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{p[4], p[5], p[6], p[7]}), scores_rsrc, at + 64, 0, DEVICE_SCOPE);
+            }
+#endif
         }
         if (more) {
             load_k(t + stride, next0, next1);
@@ -478,15 +492,49 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     l_run = groups4_sum(l_run);
 
     const int rows = min(16, rows_total - rt * 16);
+    float2 *const s_stat = (float2 *)qs;                         // (the queries are dead)
     auto put = [&](int row, int col, f32x4 o, float top, float l) __attribute__((always_inline)) {
         const int rr = rt * 16 + row, l2 = L > 1 ? rr / a.groups : 0, g2 = rr - l2 * a.groups;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *(f32x4 *)(a.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + dv0 + col) = o * inv;
-        if (a.stats && dv0 + col == 0) a.stats[(size_t)unit * rows_total + rr] = float2{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
+        if (a.scores && dv0 + col == 0) {
+            const float2 st{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
+            if (a.draws) s_stat[row] = st;
+            else a.stats[(size_t)unit * rows_total + rr] = st;
+        }
     };
-    // Device-scope accesses: written through, read at the point where the XCDs' caches agree.
-    constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access
-    (void)DEVICE_SCOPE;
+    // What the keys draw, in calls of few scores: a thread has four keys and adds the rows' probabilities in order, as paged_weights_kernel does.
+    auto draw = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const bool in_place = a.weights == a.weights_before;
+        for (int key = (int)threadIdx.x * 4; key < a.T; key += NW * 256) {
+            const bool seen = key < uni_hi && key + 4 > uni_lo;
+            if (in_place && !seen) continue;
+            const size_t at = (size_t)unit * a.T + key;
+            f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f}, before = w;
+            if (a.weights_before) __builtin_memcpy(&before, a.weights_before + at, 16);
+            u32x4 x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = u32x4{0u, 0u, 0u, 0u};
+#if defined(__HIP_DEVICE_COMPILE__)
+                if (seen && i < rows) x[i] = __builtin_amdgcn_raw_buffer_load_b128(scores_rsrc, (i * a.tpad + key) * 4, 0, DEVICE_SCOPE);
+#endif
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (i >= rows) break;
+                const int from = MULTI ? __builtin_amdgcn_readlane(lo, i) : lo, end = MULTI ? __builtin_amdgcn_readlane(hi, i) : hi;
+                const float2 st = s_stat[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (key + j >= from && key + j < end) w[j] += __builtin_amdgcn_exp2f(__uint_as_float(x[i][j]) - st.x) * st.y;
+            }
+            w += before;
+            __builtin_memcpy(a.weights + at, &w, 16);
+        }
+    };
     const int meeting = (unit * a.row_tiles + rt) * SHARES + share;
     [[maybe_unused]] float *const slots = a.partial + (size_t)meeting * a.nseg * C::PART;
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -539,7 +587,10 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
             publish(row, col, o, top, l);
         }
     }
-    if (live <= 1) return;
+    if (live <= 1) {
+        if (a.draws && share == 0) draw();
+        return;
+    }
 
     // ---- the workgroup that ends last adds the segments: each publishes its part, waits until the stores have been acknowledged and takes a ticket; whoever draws the
     // last one finds all of them. Nobody waits for anybody.
@@ -625,9 +676,11 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         return more;
     };
     while (round(x[0], x[1]) && round(x[1], x[0])) {}
+    if (a.draws && share == 0) draw();
 }
 
 // What the keys draw: a thread has four of them, of 1024 to a workgroup, and adds the rows' probabilities in order. stats: a row's reference and the reciprocal of its sum.
+// 8 sequences over 9001 keys, 4 heads for 16: 4.3 us, 6.9 MB read and written; a launch and two dependent loads bound it.
 constexpr int WEIGH_ROWS = 64;
 __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
     __shared__ float2 s_stat[WEIGH_ROWS];
@@ -791,6 +844,11 @@ Split split_of(long wgs, long tiles, int rows, int d, long cus) {
 // 101 -> 91 us; 55 MB, which the memory-side cache holds from step to step, 14.2 us, and 16.9 past it.
 constexpr size_t ONCE_BYTES = (size_t)192 << 20;
 
+// Up to this capacity the workgroup that ends last adds up what the keys draw, in two rounds of its threads; past it a launch of its own does, which takes about five us more
+// than no weights at whatever length. us a weighed token, within the launch / in one of their own / without weights: one head of 256 for 8, 500 keys 9.4 / 12.9 / 7.8, 2000 11.4 / 14.3 / 8.9,
+// 4000 13.6 / 15.7 / 9.9, 8000 17.3 / 16.8 / 10.8; 8 heads of 128 for 32, 1000 keys 9.5 / 12.4 / 8.1, 2000 11.1 / 13.1 / 8.6, 4000 13.7 / 13.8 / 9.3, 8000 18.9 / 15.7 / 10.8.
+constexpr int draws_keys(int d) { return wavefronts(d) * 64 * 4 * 2; }
+
 }  // namespace
 
 extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_attention *p, const aionhip_paged_cache *c, aionhip_handle weights_before, aionhip_handle weights) {
@@ -847,8 +905,9 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
     if (weights && rows && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take more than 4 GiB; ask for weights with fewer queries", units * rows, T);
+    a.draws = fast && weights && a.row_tiles == 1 && T <= (size_t)draws_keys(a.d) ? 1 : 0;
     const size_t meetings = a.nseg > 1 ? units * a.row_tiles * a.shares : 0, partial_bytes = meetings * a.nseg * (16 * c->d / a.shares + 32) * 4;
-    const size_t stats_bytes = weights ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
+    const size_t stats_bytes = weights && !a.draws ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
     if (const int rc = ensure_scratch2(ctx, partial_bytes + stats_bytes + scores_bytes)) return rc;
     if (meetings) {
         if (const int rc = ensure_tickets(ctx, meetings * MEET_TICKET_WORDS * sizeof(unsigned))) return rc;
@@ -866,7 +925,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         launch_k(ctx, paged_generic_kernel, dim3((unsigned)rows, (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
         LAUNCH_CHECK(ctx, "paged_generic");
     }
-    if (weights) {
+    if (weights && !a.draws) {
         ProfScope scope(ctx, "paged_weights");
         launch_k(ctx, paged_weights_kernel, dim3((unsigned)((T + 1023) / 1024), (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
         LAUNCH_CHECK(ctx, none ? "paged_weights" : fast ? "paged_attn" : "paged_generic");

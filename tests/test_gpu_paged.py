@@ -637,3 +637,30 @@ def test_value_columns_in_shares(gpu, dtype, hq, hkv, d, lengths, l):
     assert (got[hit] == np.inf).all()
     near.out[hit] = got[hit] = 0.0
     assert near.close(got).all() and near.weights_close(weights, drawn, l * hq // hkv).all()
+
+
+@pytest.mark.parametrize("d, hq, hkv, width", [(64, 4, 2, 64), (64, 4, 2, 65), (128, 8, 2, 64), (128, 8, 2, 65), (256, 8, 1, 128), (256, 8, 1, 129)])
+@pytest.mark.parametrize("apart", [True, False])
+def test_weights_within_the_launch_and_in_one_of_their_own(gpu, d, hq, hkv, width, apart):
+    """capacities on either side of where a launch of its own adds them up; sequences without keys, entries that are no page, steps nobody sees keep what they had"""
+    rng = np.random.default_rng(16)
+    pages = Pages(rng, be.F16, 3, width, 32, hkv, d)
+    pages.table[0, 3] = -1
+    lengths = [width * 32, 0, 70]
+    bits, q = source(rng, (3, 2, hq, d), be.F32)
+    before = rng.standard_normal((3, hkv, width * 32)).astype(np.float32)
+    near, drawn = attention(q, pages, 2, hq, d ** -0.5, lengths=lengths)
+    cache, qd, out, ld = pages.upload(gpu), gpu.upload(bits), gpu.alloc(bits.nbytes), gpu.upload(np.array(lengths, np.int32))
+    bd = gpu.upload(before)
+    w = gpu.upload(np.full(before.shape, np.nan, np.float32)) if apart else bd
+    want, size = before.astype(np.float64), np.abs(before).astype(np.float64)
+    for _ in range(2):
+        gpu.step_attention_paged(out, qd, cache, 2, hq, d ** -0.5, kv_lengths=ld, weights=w, weights_before=bd)
+        got = gpu.download(w, np.float32, before.shape)
+        want, size = (before + drawn, np.abs(before) + drawn) if apart else (want + drawn, size + drawn)
+        assert near.close(gpu.download(out, np.float32, bits.shape)).all()
+        # (a rounding for each addition to what was there, and what the weights themselves may be off by)
+        bound = 2 * near.reach.max() * (d + 16) * 2.0 ** -24 + 2 * (near.keys.max() / 32 + 64) * 2.0 ** -24 + 2.0 ** -21
+        assert (np.abs(got - want) <= 2 * drawn * (np.expm1(bound) + (2 * hq // hkv + 1) * 2.0 ** -24) + 2 * 2.0 ** -24 * size + 1e-37).all()
+        assert np.array_equal(got[1], before[1]) and np.array_equal(got[2, :, 70:], before[2, :, 70:]) and np.array_equal(got[0, :, 96:128], before[0, :, 96:128])
+    free(cache, qd, out, ld, *([bd, w] if apart else [bd]))
