@@ -692,6 +692,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
     const size_t at = (size_t)unit * a.T + key;
     f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
     const int len = a.kv_lengths ? a.kv_lengths[b] : 0;
+    bool seen = a.weights != a.weights_before;   // (in place what nobody sees stays as it is: a capacity may be far past the lengths)
     for (int r0 = 0; r0 < a.rows_total; r0 += WEIGH_ROWS) {
         const int rows = min(WEIGH_ROWS, a.rows_total - r0);
         if (r0) __syncthreads();
@@ -707,6 +708,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
             for (int i = 0; i < rows; ++i) {
                 const int2 see = s_keys[i];
                 if (key >= see.y || key + 4 <= see.x) continue;
+                seen = true;
                 const f32x4 s = *(const f32x4 *)(a.scores + ((size_t)unit * a.rows_total + r0 + i) * a.tpad + key);
                 const float2 st = s_stat[i];
 #pragma unroll
@@ -714,7 +716,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
                     if (key + j >= see.x && key + j < see.y) w[j] += __builtin_amdgcn_exp2f(s[j] - st.x) * st.y;
             }
     }
-    if (key < a.T) {                             // (a capacity is a multiple of sixteen)
+    if (key < a.T && seen) {                     // (a capacity is a multiple of sixteen)
         if (a.weights_before) {
             f32x4 before;
             __builtin_memcpy(&before, a.weights_before + at, 16);
