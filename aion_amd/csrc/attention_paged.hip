@@ -31,6 +31,7 @@ struct PagedArgs {
     const float *weights_before;
     float *weights;
     float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
+    int beside;               // workgroups that read the same keys lie side by side behind one L2
     int draws;                // the workgroup that ends last adds up the weights itself
     unsigned *tickets;
     Table table;
@@ -114,7 +115,7 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
 
 // QP: how many halves a query element is the sum of. MULTI: several queries a sequence, whose keys may differ (of one query all rows see the same). ONCE: keys and values
 // go past the caches. SHARES: workgroups that divide the value columns. The leading arguments, 14 words, arrive in SGPRs with the wavefront. heads: KV heads, query heads of each << 16;
-// form: segments, log2 of a page's rows << 12, query type << 16, rows of the queries in LDS << 24.
+// form: segments, log2 of a page's rows << 12, query type << 16, rows of the queries in LDS << 24, whether the grid is of one dimension << 31.
 template <int KV, int D, int QP, bool MULTI, bool ONCE, int SHARES>
 __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_attn_kernel(const int *kv_lengths, const void *q, const int *table, const unsigned char *k, const unsigned char *v, int T, int queries,
                                                                      unsigned heads, unsigned form, PagedArgs tail) {
@@ -129,12 +130,26 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     a.nseg = (int)(form & 0xFFFu), a.table.shift = (int)(form >> 12 & 0xFu), a.q_dtype = (int)(form >> 16 & 0xFFu);
     a.table.width = T >> a.table.shift;
     a.k = k, a.v = v, a.kv_dtype = KV;
-    const int q_rows = D == 256 ? (int)(form >> 24) : 16;        // 8 or 16
+    const int q_rows = D == 256 ? (int)(form >> 24 & 0x1Fu) : 16;        // 8 or 16
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int rows_total = L * a.groups;
-    const int share = SHARES == 1 ? 0 : blockIdx.x % SHARES, dv0 = share * DV, place = blockIdx.x / SHARES;
-    const int rt = rows_total <= 16 ? 0 : place / a.nseg, seg = place - rt * a.nseg, hk = blockIdx.y, b = blockIdx.z;
+    int rt = 0, share = 0, seg, hk = blockIdx.y, b = blockIdx.z;
+    if (form >> 31) {
+        // Workgroups are dealt to the eight XCDs in turn, so of eight streams of keys (segments of heads of sequences) the first workgroups, a row tile's share, lie next to each other, then
+        // their second ones, and so on: those of a stream run side by side behind one L2.
+        const unsigned kinds = (unsigned)(a.row_tiles * SHARES), streams = gridDim.x / kinds, first = blockIdx.x / (8 * kinds) * 8, beside = min(8u, streams - first);
+        const unsigned within = blockIdx.x - first * kinds, kind = within / beside;
+        unsigned stream = first + within - kind * beside;
+        rt = (int)(kind / SHARES), share = (int)(kind % SHARES);
+        seg = (int)(stream % (unsigned)a.nseg), stream /= (unsigned)a.nseg;
+        hk = (int)(stream % (unsigned)a.Hkv), b = (int)(stream / (unsigned)a.Hkv);
+    } else {
+        const int place = blockIdx.x / SHARES;
+        share = blockIdx.x % SHARES;
+        rt = rows_total <= 16 ? 0 : place / a.nseg, seg = place - rt * a.nseg;
+    }
+    const int dv0 = share * DV;
     const int unit = b * a.Hkv + hk;
     const int len_raw = kv_lengths ? kv_lengths[b] : 0;
 
@@ -333,11 +348,11 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
 
     f32x4 acc[MT];
     float ref = MASKED, l_run = 0.f;                             // l_run: of this lane's keys
-    float *scores = a.scores + ((size_t)unit * rows_total + r) * a.tpad;
     constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access: written through, read at the point where the XCDs' caches agree
     (void)DEVICE_SCOPE;
 #if defined(__HIP_DEVICE_COMPILE__)
-    const __amdgpu_buffer_rsrc_t scores_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(a.scores + (size_t)unit * rows_total * a.tpad), 0, a.draws ? (unsigned)(rows_total * a.tpad * 4) : 0u, 0x00027000);
+    const __amdgpu_buffer_rsrc_t scores_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(a.scores + ((size_t)unit * rows_total + rt * 16) * a.tpad), 0,
+                                                                                 a.scores ? (unsigned)min(16, rows_total - rt * 16) * (unsigned)a.tpad * 4u : 0u, 0x00027000);
 #endif
     // MORE: another tile of this wavefront follows (two copies of the body, so that every path requests K and V in the same order and the count of loads in flight holds)
     auto tile = [&](int t, bool ok0, bool ok1, int next0, int next1, auto more_c) __attribute__((always_inline)) {
@@ -377,19 +392,19 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
                 p[j] = key >= lo && key < hi && (j < 4 ? ok0 : ok1) ? p[j] : MASKED;
             }
         }
-        if (a.scores && share == 0) {
-            if (row_ok && !a.draws) {
-                *(f32x4 *)(scores + key0 + g * 4) = f32x4{p[0], p[1], p[2], p[3]};
-                *(f32x4 *)(scores + key0 + 16 + g * 4) = f32x4{p[4], p[5], p[6], p[7]};
-            }
 #if defined(__HIP_DEVICE_COMPILE__)
-            if (row_ok && a.draws) {
-                const int at = (r * a.tpad + key0 + g * 4) * 4;
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]}), scores_rsrc, at, 0, DEVICE_SCOPE);
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{p[4], p[5], p[6], p[7]}), scores_rsrc, at + 64, 0, DEVICE_SCOPE);
+        if (a.scores && share == 0 && row_ok) {
+            const int at = (int)((unsigned)(n * a.tpad + g * 4) * 4u);
+            const u32x4 lower = __builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]}), upper = __builtin_bit_cast(u32x4, f32x4{p[4], p[5], p[6], p[7]});
+            if (a.draws) {
+                __builtin_amdgcn_raw_buffer_store_b128(lower, scores_rsrc, at, key0 * 4, DEVICE_SCOPE);
+                __builtin_amdgcn_raw_buffer_store_b128(upper, scores_rsrc, at + 64, key0 * 4, DEVICE_SCOPE);
+            } else {                               // (written through they would cost a long call a tenth)
+                __builtin_amdgcn_raw_buffer_store_b128(lower, scores_rsrc, at, key0 * 4, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(upper, scores_rsrc, at + 64, key0 * 4, 0);
             }
-#endif
         }
+#endif
         if (more) {
             load_k(t + stride, next0, next1);
             asm volatile("" ::: "memory");         // requested here, ahead of the counted wait for V below
@@ -590,95 +605,92 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
             publish(row, col, o, top, l);
         }
     }
-    if (live <= 1) {
-        if (a.draws && share == 0) draw();
-        return;
-    }
-
-    // ---- the workgroup that ends last adds the segments: each publishes its part, waits until the stores have been acknowledged and takes a ticket; whoever draws the
-    // last one finds all of them. Nobody waits for anybody.
-    __syncthreads();
-    int *s_ticket = (int *)lds;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) *s_ticket = (int)__hip_atomic_fetch_add(a.tickets + meeting * MEET_TICKET_WORDS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (*s_ticket != live - 1) return;
-    if (threadIdx.x == 0) __hip_atomic_store(a.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    float *s_f = (float *)lds, *s_top = s_f + 16 * C::MOST, *s_l = s_top + 16;      // factors of the segments of each row
-    f32x4 *s_o = (f32x4 *)(lds + (16 * C::MOST + 64) * 4);
-    // A wavefront derives the segments' factors for every NW-th row, a lane to a segment; all are asked for at once.
-    constexpr int EACH = 16 / NW;
-    u32x2 st[EACH][C::MOST / 64];
+    if (live > 1) {
+        // ---- the workgroup that ends last adds the segments: each publishes its part, waits until the stores have been acknowledged and takes a ticket; whoever draws the
+        // last one finds all of them. Nobody waits for anybody.
+        __syncthreads();
+        int *s_ticket = (int *)lds;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) *s_ticket = (int)__hip_atomic_fetch_add(a.tickets + meeting * MEET_TICKET_WORDS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (*s_ticket != live - 1) return;
+        if (threadIdx.x == 0) __hip_atomic_store(a.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        float *s_f = (float *)lds, *s_top = s_f + 16 * C::MOST, *s_l = s_top + 16;      // factors of the segments of each row
+        f32x4 *s_o = (f32x4 *)(lds + (16 * C::MOST + 64) * 4);
+        // A wavefront derives the segments' factors for every NW-th row, a lane to a segment; all are asked for at once.
+        constexpr int EACH = 16 / NW;
+        u32x2 st[EACH][C::MOST / 64];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
+        for (int i = 0; i < EACH; ++i)
 #pragma unroll
-        for (int j = 0; j < C::MOST / 64; ++j) {
-            st[i][j] = u32x2{__float_as_uint(MASKED), 0u};
+            for (int j = 0; j < C::MOST / 64; ++j) {
+                st[i][j] = u32x2{__float_as_uint(MASKED), 0u};
 #if defined(__HIP_DEVICE_COMPILE__)
-            if (wave + i * NW < rows && lane + 64 * j < live)
-                st[i][j] = __builtin_amdgcn_raw_buffer_load_b64(slots_rsrc, ((lane + 64 * j) * C::PART + 16 * DV + (wave + i * NW) * 2) * 4, 0, DEVICE_SCOPE);
+                if (wave + i * NW < rows && lane + 64 * j < live)
+                    st[i][j] = __builtin_amdgcn_raw_buffer_load_b64(slots_rsrc, ((lane + 64 * j) * C::PART + 16 * DV + (wave + i * NW) * 2) * 4, 0, DEVICE_SCOPE);
 #endif
-        }
-    // A thread has four columns of a row; where there are more threads than that, several share the segments. Eight parts at a time, the next eight asked for ahead.
-    const int pieces = rows * (DV / 4), sets = max(1, NW * 64 / pieces), set = (int)threadIdx.x / pieces;
-    const bool mine = set < sets;
-    int e = (int)threadIdx.x - set * pieces, s0 = set;
-    u32x4 x[2][8];
-    auto ask = [&](u32x4 (&to)[8], int e, int s0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            [[maybe_unused]] const int s = s0 + j * sets;        // (past the last segment: past the buffer's end, which reads as zeros)
-            to[j] = u32x4{0u, 0u, 0u, 0u};
-#if defined(__HIP_DEVICE_COMPILE__)
-            to[j] = __builtin_amdgcn_raw_buffer_load_b128(slots_rsrc, s < live && e < pieces ? (s * C::PART + e / (DV / 4) * DV + e % (DV / 4) * 4) * 4 : 0x7FFFFFF0, 0, DEVICE_SCOPE);
-#endif
-        }
-    };
-    ask(x[0], e, s0);
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int row = wave + i * NW;
-        if (row >= rows) break;
-        float top = MASKED, sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < C::MOST / 64; ++j) top = fmaxf(top, __uint_as_float(st[i][j].x));
-        top = lanes_max(top);
-#pragma unroll
-        for (int j = 0; j < C::MOST / 64; ++j) {
-            const float sr = __uint_as_float(st[i][j].x), f = sr > MASKED ? __builtin_amdgcn_exp2f(sr - top) : 1.f;
-            s_f[row * C::MOST + lane + 64 * j] = lane + 64 * j < live ? f : 0.f;
-            sum += __uint_as_float(st[i][j].y) * f;
-        }
-        sum = lanes_sum(sum);
-        if (lane == 0) s_top[row] = top, s_l[row] = sum;
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    // one round: eight parts added, and the piece written with its last ones; false: none are left
-    auto round = [&](u32x4 (&now)[8], u32x4 (&next)[8]) __attribute__((always_inline)) {
-        const bool last = s0 + 8 * sets - set >= live;           // (the same for all threads)
-        const int e2 = last ? e + NW * 64 : e, s2 = last ? set : s0 + 8 * sets;
-        const bool more = !last || (sets == 1 && e2 - (int)threadIdx.x < pieces);
-        if (more) ask(next, e2, s2);
-        const int row = min(e / (DV / 4), 15);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o += __builtin_bit_cast(f32x4, now[j]) * (s0 + j * sets < live ? s_f[row * C::MOST + s0 + j * sets] : 0.f);
-        if (last) {
-            if (sets > 1) {
-                s_o[threadIdx.x] = o;
-                __syncthreads();
-                if (set == 0)
-                    for (int i = 1; i < sets; ++i) o += s_o[i * pieces + threadIdx.x];
             }
-            if (mine && set == 0 && e < pieces) put(row, e % (DV / 4) * 4, o, s_top[row], s_l[row]);
-            o = f32x4{0.f, 0.f, 0.f, 0.f};
+        // A thread has four columns of a row; where there are more threads than that, several share the segments. Eight parts at a time, the next eight asked for ahead.
+        const int pieces = rows * (DV / 4), sets = max(1, NW * 64 / pieces), set = (int)threadIdx.x / pieces;
+        const bool mine = set < sets;
+        int e = (int)threadIdx.x - set * pieces, s0 = set;
+        u32x4 x[2][8];
+        auto ask = [&](u32x4 (&to)[8], int e, int s0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                [[maybe_unused]] const int s = s0 + j * sets;        // (past the last segment: past the buffer's end, which reads as zeros)
+                to[j] = u32x4{0u, 0u, 0u, 0u};
+#if defined(__HIP_DEVICE_COMPILE__)
+                to[j] = __builtin_amdgcn_raw_buffer_load_b128(slots_rsrc, s < live && e < pieces ? (s * C::PART + e / (DV / 4) * DV + e % (DV / 4) * 4) * 4 : 0x7FFFFFF0, 0, DEVICE_SCOPE);
+#endif
+            }
+        };
+        ask(x[0], e, s0);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int row = wave + i * NW;
+            if (row >= rows) break;
+            float top = MASKED, sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < C::MOST / 64; ++j) top = fmaxf(top, __uint_as_float(st[i][j].x));
+            top = lanes_max(top);
+#pragma unroll
+            for (int j = 0; j < C::MOST / 64; ++j) {
+                const float sr = __uint_as_float(st[i][j].x), f = sr > MASKED ? __builtin_amdgcn_exp2f(sr - top) : 1.f;
+                s_f[row * C::MOST + lane + 64 * j] = lane + 64 * j < live ? f : 0.f;
+                sum += __uint_as_float(st[i][j].y) * f;
+            }
+            sum = lanes_sum(sum);
+            if (lane == 0) s_top[row] = top, s_l[row] = sum;
         }
-        e = e2, s0 = s2;
-        return more;
-    };
-    while (round(x[0], x[1]) && round(x[1], x[0])) {}
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        // one round: eight parts added, and the piece written with its last ones; false: none are left
+        auto round = [&](u32x4 (&now)[8], u32x4 (&next)[8]) __attribute__((always_inline)) {
+            const bool last = s0 + 8 * sets - set >= live;           // (the same for all threads)
+            const int e2 = last ? e + NW * 64 : e, s2 = last ? set : s0 + 8 * sets;
+            const bool more = !last || (sets == 1 && e2 - (int)threadIdx.x < pieces);
+            if (more) ask(next, e2, s2);
+            const int row = min(e / (DV / 4), 15);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o += __builtin_bit_cast(f32x4, now[j]) * (s0 + j * sets < live ? s_f[row * C::MOST + s0 + j * sets] : 0.f);
+            if (last) {
+                if (sets > 1) {
+                    s_o[threadIdx.x] = o;
+                    __syncthreads();
+                    if (set == 0)
+                        for (int i = 1; i < sets; ++i) o += s_o[i * pieces + threadIdx.x];
+                }
+                if (mine && set == 0 && e < pieces) put(row, e % (DV / 4) * 4, o, s_top[row], s_l[row]);
+                o = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            e = e2, s0 = s2;
+            return more;
+        };
+        while (round(x[0], x[1]) && round(x[1], x[0])) {}
+    }
     if (a.draws && share == 0) draw();
 }
 
@@ -693,6 +705,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
     f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
     const int len = a.kv_lengths ? a.kv_lengths[b] : 0;
     bool seen = a.weights != a.weights_before;   // (in place what nobody sees stays as it is: a capacity may be far past the lengths)
+    if (!seen && a.kv_lengths && (int)blockIdx.x * 1024 >= len) return;
     for (int r0 = 0; r0 < a.rows_total; r0 += WEIGH_ROWS) {
         const int rows = min(WEIGH_ROWS, a.rows_total - r0);
         if (r0) __syncthreads();
@@ -791,8 +804,12 @@ int launch(aionhip_ctx *ctx, const PagedArgs &a, int batch) {
     static std::atomic<uint64_t> attr{0};
     if (const int rc = allow_lds(ctx, attr, (const void *)kernel, C::MAIN + QP * 16 * C::ROW + 64)) return rc;
     ProfScope scope(ctx, "paged_attn");
-    launch_k(ctx, kernel, dim3((unsigned)(a.row_tiles * a.nseg * SHARES), (unsigned)a.Hkv, (unsigned)batch), dim3(C::NW * 64), lds, a.kv_lengths, a.q, a.table.pages, a.k, a.v, a.T, a.L,
-             (unsigned)a.Hkv | (unsigned)a.groups << 16, (unsigned)a.nseg | (unsigned)a.table.shift << 12 | (unsigned)a.q_dtype << 16 | (unsigned)q_rows << 24, a);
+    // (one dimension where keys are read by several workgroups, if it takes them all)
+    const size_t wgs = (size_t)a.row_tiles * a.nseg * SHARES * a.Hkv * batch;
+    const bool flat = a.beside && wgs <= paged::MAX_THREADS / (C::NW * 64);
+    const dim3 grid = flat ? dim3((unsigned)wgs) : dim3((unsigned)(a.row_tiles * a.nseg * SHARES), (unsigned)a.Hkv, (unsigned)batch);
+    launch_k(ctx, kernel, grid, dim3(C::NW * 64), lds, a.kv_lengths, a.q, a.table.pages, a.k, a.v, a.T, a.L,
+             (unsigned)a.Hkv | (unsigned)a.groups << 16, (unsigned)a.nseg | (unsigned)a.table.shift << 12 | (unsigned)a.q_dtype << 16 | (unsigned)q_rows << 24 | (flat ? 1u << 31 : 0u), a);
     LAUNCH_CHECK(ctx, "paged_attn");
     return AIONHIP_OK;
 }
@@ -904,12 +921,15 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
         const Split split = split_of(wgs, tiles, min(a.rows_total, 16), a.d, cus);
         a.nseg = split.segments, a.shares = split.shares;
+        // Five queries of 32 sequences over 8192 keys, 32 heads on 8 of 128 (two row tiles), 305 -> 203 us; 7 over 62761, 5 sequences, 363 -> 244. Shares of few tiles do not wait for what places
+        // them: one token, one head of 256 for 8, 4096 keys 10.0 in plain order and 10.5 so, 32768 20.0 and 17.3.
+        a.beside = a.row_tiles > 1 || (a.shares > 1 && tiles >= 8L * a.nseg);
         once = a.row_tiles == 1 && (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
     if ((fast ? (size_t)a.row_tiles * a.nseg * a.shares * (c->d == 256 ? wavefronts(256) : wavefronts(128)) * 64 : rows * 256) > paged::MAX_THREADS)
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
-    if (weights && rows && units > ((size_t)4 << 30) / (rows * a.tpad * 4))
-        return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take more than 4 GiB; ask for weights with fewer queries", units * rows, T);
+    if (weights && rows && units > (((size_t)4 << 30) - 1) / (rows * a.tpad * 4))
+        return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take 4 GiB or more; ask for weights with fewer queries", units * rows, T);
     a.draws = fast && weights && a.row_tiles == 1 && T <= (size_t)draws_keys(a.d) ? 1 : 0;
     const size_t meetings = a.nseg > 1 ? units * a.row_tiles * a.shares : 0, partial_bytes = meetings * a.nseg * (16 * c->d / a.shares + 32) * 4;
     const size_t stats_bytes = weights && !a.draws ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;

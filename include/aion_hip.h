@@ -406,7 +406,7 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, 
  * aionhip_step_attention, which shares the keys among 128 rows: 4096 tokens of 32 heads on 8 of 128 656 us over the pages, 143 with the rows read back first.
  * weights (0: none), f32 [batch, h_kv, capacity]: weights = weights_before (the same shape, the same buffer or 0, which counts as zeros) + the probability of
  * each key, summed over the queries and the query heads of its KV head. What aionhip_step_evict_paged goes by. AIONHIP_UNSUPPORTED where the scores (4 bytes a
- * query row and key of the capacity) would take more than 4 GiB of scratch memory: ask with the last queries of a long prompt alone. */
+ * query row and key of the capacity) would take 4 GiB of scratch memory or more: ask with the last queries of a long prompt alone. */
 int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_attention *p, const aionhip_paged_cache *cache, aionhip_handle weights_before, aionhip_handle weights);
 /* Eviction: of each sequence longer than `limit` every KV head keeps `keep` rows (first + recent <= keep <= limit): the `first` oldest, the `recent` newest, and of
  * those between them the ones of greatest weight, of equal weights the oldest (a NaN is the greatest, -0 equals 0). A head's rows keep their order and become steps 0 .. keep - 1;

@@ -664,3 +664,13 @@ def test_weights_within_the_launch_and_in_one_of_their_own(gpu, d, hq, hkv, widt
         assert (np.abs(got - want) <= 2 * drawn * (np.expm1(bound) + (2 * hq // hkv + 1) * 2.0 ** -24) + 2 * 2.0 ** -24 * size + 1e-37).all()
         assert np.array_equal(got[1], before[1]) and np.array_equal(got[2, :, 70:], before[2, :, 70:]) and np.array_equal(got[0, :, 96:128], before[0, :, 96:128])
     free(cache, qd, out, ld, *([bd, w] if apart else [bd]))
+
+
+@pytest.mark.parametrize("b, l, hq, hkv, d, lengths", [(1, 5, 16, 2, 64, [700]), (3, 9, 8, 2, 128, [300, 0, 40]), (5, 3, 8, 1, 256, [9, 500, 64, 2, 333]), (1, 1, 8, 1, 256, [17000]), (2, 1, 4, 1, 128, [5000, 4097]),
+                                                     (1, 40, 8, 1, 128, [2100])])
+def test_workgroups_that_read_the_same_keys_side_by_side(gpu, b, l, hq, hkv, d, lengths):
+    """row tiles and shares whose streams of keys are no multiple of eight, with and without weights"""
+    rng = np.random.default_rng(17)
+    pages = Pages(rng, be.F16, b, -(-max(lengths) // 64) + 1, 64, hkv, d)
+    bits, q = source(rng, (b, l, hq, d), be.F32)
+    check(gpu, pages, bits, q, be.F32, d ** -0.5, lengths=lengths)
