@@ -392,8 +392,9 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
                 p[j] = key >= lo && key < hi && (j < 4 ? ok0 : ok1) ? p[j] : MASKED;
             }
         }
+        const bool scored = a.scores && share == 0;              // (some lane of every wavefront has a row)
 #if defined(__HIP_DEVICE_COMPILE__)
-        if (a.scores && share == 0 && row_ok) {
+        if (scored && row_ok) {
             const int at = (int)((unsigned)(n * a.tpad + g * 4) * 4u);
             const u32x4 lower = __builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]}), upper = __builtin_bit_cast(u32x4, f32x4{p[4], p[5], p[6], p[7]});
             if (a.draws) {
@@ -440,8 +441,9 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
                 w -= from_half_bits<KV>((unsigned short)(both >> 16));
             }
         }
-        // V has landed once only the younger K loads are outstanding (loads complete in order); the tile is this wavefront's alone
-        if (more) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * KK));
+        // V has landed once only what is younger is outstanding, K and the two stores of scores (they complete in order); the tile is this wavefront's alone
+        if (more && scored) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * KK + 2));
+        else if (more) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * KK));
         else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         asm volatile("" ::: "memory");
         if (!full) {
@@ -694,18 +696,21 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     if (a.draws && share == 0) draw();
 }
 
-// What the keys draw: a thread has four of them, of 1024 to a workgroup, and adds the rows' probabilities in order. stats: a row's reference and the reciprocal of its sum.
-// 8 sequences over 9001 keys, 4 heads for 16: 4.3 us, 6.9 MB read and written; a launch and two dependent loads bound it.
+// What the keys draw: a thread has KEYS of them and adds the rows' probabilities in order, AHEAD rows asked for before the first is used. stats: a row's reference and the reciprocal of
+// its sum. What it costs is the rows' loads one after another where there are few keys, so a thread has one and eight rows ahead (64 rows of 8 heads over 4000 keys 9 us; four keys, a
+// row at a time, 33), and the bytes of the scores where there are many, so it has four and four ahead (32 sequences, 8 heads, over 8192 keys 10 us).
 constexpr int WEIGH_ROWS = 64;
+constexpr size_t WEIGH_MANY = (size_t)512 << 10;
+template <int KEYS, int AHEAD>
 __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
     __shared__ float2 s_stat[WEIGH_ROWS];
     __shared__ int2 s_keys[WEIGH_ROWS];
-    const int hk = blockIdx.y, b = blockIdx.z, unit = b * a.Hkv + hk, tid = threadIdx.x, key = (int)blockIdx.x * 1024 + tid * 4;
+    const int hk = blockIdx.y, b = blockIdx.z, unit = b * a.Hkv + hk, tid = threadIdx.x, key = ((int)blockIdx.x * 256 + tid) * KEYS;
     const size_t at = (size_t)unit * a.T + key;
-    f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
+    float w[KEYS] = {};
     const int len = a.kv_lengths ? a.kv_lengths[b] : 0;
     bool seen = a.weights != a.weights_before;   // (in place what nobody sees stays as it is: a capacity may be far past the lengths)
-    if (!seen && a.kv_lengths && (int)blockIdx.x * 1024 >= len) return;
+    if (!seen && a.kv_lengths && (int)blockIdx.x * 256 * KEYS >= len) return;
     for (int r0 = 0; r0 < a.rows_total; r0 += WEIGH_ROWS) {
         const int rows = min(WEIGH_ROWS, a.rows_total - r0);
         if (r0) __syncthreads();
@@ -717,25 +722,32 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(PagedArgs a) {
             s_stat[tid] = a.stats[(size_t)unit * a.rows_total + r];
         }
         __syncthreads();
-        if (key < a.T)
-            for (int i = 0; i < rows; ++i) {
-                const int2 see = s_keys[i];
-                if (key >= see.y || key + 4 <= see.x) continue;
-                seen = true;
-                const f32x4 s = *(const f32x4 *)(a.scores + ((size_t)unit * a.rows_total + r0 + i) * a.tpad + key);
-                const float2 st = s_stat[i];
+        if (key < a.T) {
+            const float *from = a.scores + ((size_t)unit * a.rows_total + r0) * a.tpad + key;
+            for (int i0 = 0; i0 < rows; i0 += AHEAD) {
+                float s[AHEAD][KEYS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (key + j >= see.x && key + j < see.y) w[j] += __builtin_amdgcn_exp2f(s[j] - st.x) * st.y;
+                for (int i = 0; i < AHEAD; ++i) __builtin_memcpy(s[i], from + (size_t)min(i0 + i, rows - 1) * a.tpad, sizeof s[i]);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int2 see = s_keys[min(i0 + i, rows - 1)];
+                    const float2 st = s_stat[min(i0 + i, rows - 1)];
+                    const int end = i0 + i < rows ? see.y : 0;
+                    seen |= key < end && key + KEYS > see.x;
+#pragma unroll
+                    for (int j = 0; j < KEYS; ++j) w[j] += key + j >= see.x && key + j < end ? __builtin_amdgcn_exp2f(s[i][j] - st.x) * st.y : 0.f;
+                }
             }
+        }
     }
     if (key < a.T && seen) {                     // (a capacity is a multiple of sixteen)
         if (a.weights_before) {
-            f32x4 before;
-            __builtin_memcpy(&before, a.weights_before + at, 16);
-            w += before;
+            float before[KEYS];
+            __builtin_memcpy(before, a.weights_before + at, sizeof w);
+#pragma unroll
+            for (int j = 0; j < KEYS; ++j) w[j] += before[j];
         }
-        __builtin_memcpy(a.weights + at, &w, 16);
+        __builtin_memcpy(a.weights + at, w, sizeof w);
     }
 }
 
@@ -952,7 +964,10 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
     }
     if (weights && !a.draws) {
         ProfScope scope(ctx, "paged_weights");
-        launch_k(ctx, paged_weights_kernel, dim3((unsigned)((T + 1023) / 1024), (unsigned)p->h_kv, (unsigned)p->batch), dim3(256), 0, a);
+        // (measured at the kernel)
+        const size_t keys = units * T >= WEIGH_MANY ? 4 : 1;
+        launch_k(ctx, keys == 4 ? paged_weights_kernel<4, 4> : paged_weights_kernel<1, 8>, dim3((unsigned)((T + 256 * keys - 1) / (256 * keys)), (unsigned)p->h_kv, (unsigned)p->batch),
+                 dim3(256), 0, a);
         LAUNCH_CHECK(ctx, none ? "paged_weights" : fast ? "paged_attn" : "paged_generic");
     }
     return AIONHIP_OK;
