@@ -15,6 +15,7 @@
 #include "attention_common.h"
 #include "cache_paged.h"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace {
@@ -31,6 +32,7 @@ struct PagedArgs {
     const float *weights_before;
     float *weights;
     float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
+    int streams;              // of keys: segments of heads of sequences
     int beside;               // workgroups that read the same keys lie side by side behind one L2
     int draws;                // the workgroup that ends last adds up the weights itself
     unsigned *tickets;
@@ -52,6 +54,25 @@ __device__ __forceinline__ void row_keys(const PagedArgs &a, int b, int li, int 
     if (pos < 0) return;
     window_keys(a.win_left, a.win_right, a.win_chunk, pos, len, lo, hi);
     if (hi < lo) hi = lo;
+}
+
+// The arguments behind the leading ones, read where they are used: left to itself the compiler asks for all of them at the kernel's start and waits there for the lines that only its end
+// needs. One token over 531 keys, one head of 256 for 8: 8.0 -> 7.5 us.
+struct KernelArgs {
+    const void *pointers[5];
+    int numbers[4];
+    PagedArgs tail;
+};
+static_assert(offsetof(KernelArgs, tail) == 56, "paged_attn_kernel's arguments");
+__device__ __forceinline__ PagedArgs late_args() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef const __attribute__((address_space(4))) char *Bytes;
+    Bytes at = (Bytes)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(KernelArgs, tail);
+    asm volatile("" : "+s"(at));
+    return *(const __attribute__((address_space(4))) PagedArgs *)at;
+#else
+    return PagedArgs{};
+#endif
 }
 
 constexpr int MOST_SEGMENTS = 256;      // of a row tile
@@ -138,7 +159,8 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     if (form >> 31) {
         // Workgroups are dealt to the eight XCDs in turn, so of eight streams of keys (segments of heads of sequences) the first workgroups, a row tile's share, lie next to each other, then
         // their second ones, and so on: those of a stream run side by side behind one L2.
-        const unsigned kinds = (unsigned)(a.row_tiles * SHARES), streams = gridDim.x / kinds, first = blockIdx.x / (8 * kinds) * 8, beside = min(8u, streams - first);
+        const PagedArgs z = late_args();
+        const unsigned kinds = (unsigned)(z.row_tiles * SHARES), streams = (unsigned)z.streams, first = blockIdx.x / (8 * kinds) * 8, beside = min(8u, streams - first);
         const unsigned within = blockIdx.x - first * kinds, kind = within / beside;
         unsigned stream = first + within - kind * beside;
         rt = (int)(kind / SHARES), share = (int)(kind % SHARES);
@@ -511,29 +533,30 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     }
     l_run = groups4_sum(l_run);
 
+    const PagedArgs z = late_args();
     const int rows = min(16, rows_total - rt * 16);
     float2 *const s_stat = (float2 *)qs;                         // (the queries are dead)
     auto put = [&](int row, int col, f32x4 o, float top, float l) __attribute__((always_inline)) {
         const int rr = rt * 16 + row, l2 = L > 1 ? rr / a.groups : 0, g2 = rr - l2 * a.groups;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        *(f32x4 *)(a.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + dv0 + col) = o * inv;
+        *(f32x4 *)(z.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + dv0 + col) = o * inv;
         if (a.scores && dv0 + col == 0) {
             const float2 st{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
-            if (a.draws) s_stat[row] = st;
-            else a.stats[(size_t)unit * rows_total + rr] = st;
+            if (z.draws) s_stat[row] = st;
+            else z.stats[(size_t)unit * rows_total + rr] = st;
         }
     };
     // What the keys draw, in calls of few scores: a thread has four keys and adds the rows' probabilities in order, as paged_weights_kernel does.
     auto draw = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const bool in_place = a.weights == a.weights_before;
+        const bool in_place = z.weights == z.weights_before;
         for (int key = (int)threadIdx.x * 4; key < a.T; key += NW * 256) {
             const bool seen = key < uni_hi && key + 4 > uni_lo;
             if (in_place && !seen) continue;
             const size_t at = (size_t)unit * a.T + key;
             f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f}, before = w;
-            if (a.weights_before) __builtin_memcpy(&before, a.weights_before + at, 16);
+            if (z.weights_before) __builtin_memcpy(&before, z.weights_before + at, 16);
             u32x4 x[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -552,11 +575,11 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
                     if (key + j >= from && key + j < end) w[j] += __builtin_amdgcn_exp2f(__uint_as_float(x[i][j]) - st.x) * st.y;
             }
             w += before;
-            __builtin_memcpy(a.weights + at, &w, 16);
+            __builtin_memcpy(z.weights + at, &w, 16);
         }
     };
-    const int meeting = (unit * a.row_tiles + rt) * SHARES + share;
-    [[maybe_unused]] float *const slots = a.partial + (size_t)meeting * a.nseg * C::PART;
+    const int meeting = (unit * z.row_tiles + rt) * SHARES + share;
+    [[maybe_unused]] float *const slots = z.partial + (size_t)meeting * a.nseg * C::PART;
 #if defined(__HIP_DEVICE_COMPILE__)
     const __amdgpu_buffer_rsrc_t slots_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)slots, 0, (unsigned)(a.nseg * C::PART * 4), 0x00027000);
 #endif
@@ -614,10 +637,10 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         int *s_ticket = (int *)lds;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0) *s_ticket = (int)__hip_atomic_fetch_add(a.tickets + meeting * MEET_TICKET_WORDS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) *s_ticket = (int)__hip_atomic_fetch_add(z.tickets + meeting * MEET_TICKET_WORDS, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (*s_ticket != live - 1) return;
-        if (threadIdx.x == 0) __hip_atomic_store(a.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) __hip_atomic_store(z.tickets + meeting * MEET_TICKET_WORDS, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         float *s_f = (float *)lds, *s_top = s_f + 16 * C::MOST, *s_l = s_top + 16;      // factors of the segments of each row
         f32x4 *s_o = (f32x4 *)(lds + (16 * C::MOST + 64) * 4);
@@ -693,7 +716,7 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         };
         while (round(x[0], x[1]) && round(x[1], x[0])) {}
     }
-    if (a.draws && share == 0) draw();
+    if (z.draws && share == 0) draw();
 }
 
 // What the keys draw: a thread has KEYS of them and adds the rows' probabilities in order, AHEAD rows asked for before the first is used. stats: a row's reference and the reciprocal of
@@ -942,6 +965,7 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: dimension too large");
     if (weights && rows && units > (((size_t)4 << 30) - 1) / (rows * a.tpad * 4))
         return set_err(ctx, AIONHIP_UNSUPPORTED, "attention_paged: the scores of %zu rows over %zu keys take 4 GiB or more; ask for weights with fewer queries", units * rows, T);
+    a.streams = (int)(units * (size_t)a.nseg);
     a.draws = fast && weights && a.row_tiles == 1 && T <= (size_t)draws_keys(a.d) ? 1 : 0;
     const size_t meetings = a.nseg > 1 ? units * a.row_tiles * a.shares : 0, partial_bytes = meetings * a.nseg * (16 * c->d / a.shares + 32) * 4;
     const size_t stats_bytes = weights && !a.draws ? (units * rows * 8 + 255) / 256 * 256 : 0, scores_bytes = weights ? units * rows * a.tpad * 4 : 0;
