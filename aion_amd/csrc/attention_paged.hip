@@ -8,7 +8,7 @@
 //   Accuracy: q and P enter the products as sums of halves (two f16, three bf16; q that comes in the cache's type as it is), K and V are exact, sums are f32.
 //   The workgroup that ends last adds the segments of its rows and, where the capacity is small, what the keys draw.
 //   What bounds it, us: large calls HBM (one token over 131072 keys, 8 heads of 128 for 32, 90, 6.0 TB/s; 32 sequences of up to 16384 252, 6.3 TB/s, the last tenth of it
-//   the unevenness of the sequences); small ones a chain of latencies (531 keys, one head of 256 for 8, 7.3: launch 4, length and page, keys and values, products, one
+//   the unevenness of the sequences); small ones a chain of latencies (531 keys, one head of 256 for 8, 7.5: launch 4, length and page, keys and values, products, one
 //   exchange between the segments). Five queries, 4 sequences over 3001 keys, 32 heads of 128: 35, 4.6 TB/s.
 // paged_weights_kernel - what the keys draw elsewhere, from the scores that the first kernel left.
 // paged_generic_kernel - other head sizes: a wavefront a key at a time, f32. It is there so that every shape has a path.

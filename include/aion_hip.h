@@ -403,7 +403,7 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, 
  * the row was turned by. f32 accuracy (about 1e-6) whatever aionhip_set_attention_precise says. A query that sees no key, or only scores of minus infinity, gets zeros; what is not
  * finite reaches the queries that see it and no others. Head sizes 64, 128 and 256 run on the matrix pipe (out at a multiple of 16 bytes), others on a slow kernel. Made for one to a few tokens: of more
  * query rows to a KV head than sixteen, every sixteen walk the keys on their own. A long prompt is better read back (aionhip_step_read_paged) and run by
- * aionhip_step_attention, which shares the keys among 128 rows: 4096 tokens of 32 heads on 8 of 128 656 us over the pages, 143 with the rows read back first.
+ * aionhip_step_attention, which shares the keys among 128 rows: 4096 tokens of 32 heads on 8 of 128 620 us over the pages, 143 with the rows read back first.
  * weights (0: none), f32 [batch, h_kv, capacity]: weights = weights_before (the same shape, the same buffer or 0, which counts as zeros) + the probability of
  * each key, summed over the queries and the query heads of its KV head. What aionhip_step_evict_paged goes by. AIONHIP_UNSUPPORTED where the scores (4 bytes a
  * query row and key of the capacity) would take 4 GiB of scratch memory or more: ask with the last queries of a long prompt alone. */
