@@ -37,9 +37,12 @@ __device__ __forceinline__ void load_n(const void *src, size_t i, int n, float (
     typename Elem<DT>::T h[N];
     const auto *p = (const typename Elem<DT>::T *)src + i;
     if (n == N) {
-        if constexpr (ONCE && sizeof h == 16) {
-            const u32x4 w = __builtin_nontemporal_load((const u32x4u<sizeof h[0]> *)p);
-            __builtin_memcpy(h, &w, sizeof h);
+        if constexpr (ONCE && sizeof h >= 16) {
+#pragma unroll
+            for (size_t k = 0; k < sizeof h / 16; ++k) {
+                const u32x4 w = __builtin_nontemporal_load((const u32x4u<sizeof h[0]> *)p + k);
+                __builtin_memcpy((char *)h + 16 * k, &w, 16);
+            }
         } else {
             __builtin_memcpy(h, p, sizeof h);
         }
@@ -57,10 +60,13 @@ __device__ __forceinline__ void store_n(void *dst, size_t i, int n, const float 
     for (int j = 0; j < N; ++j) h[j] = from_f32<DT>(x[j]);
     auto *p = (typename Elem<DT>::T *)dst + i;
     if (n == N) {
-        if constexpr (ONCE && sizeof h == 16) {
-            u32x4u<sizeof h[0]> w;
-            __builtin_memcpy(&w, h, sizeof h);
-            __builtin_nontemporal_store(w, (u32x4u<sizeof h[0]> *)p);
+        if constexpr (ONCE && sizeof h >= 16) {
+#pragma unroll
+            for (size_t k = 0; k < sizeof h / 16; ++k) {
+                u32x4u<sizeof h[0]> w;
+                __builtin_memcpy(&w, (const char *)h + 16 * k, 16);
+                __builtin_nontemporal_store(w, (u32x4u<sizeof h[0]> *)p + k);
+            }
         } else {
             __builtin_memcpy(p, h, sizeof h);
         }
@@ -189,6 +195,55 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotate a) {
     }
 }
 
+// The same where a head does not come apart into whole pieces (62 of 64 elements turning in halves: runs at odd places, and short ones): a thread has eight neighbouring elements of a
+// row whatever they are; the angles, and what they turn with in the other half, come through LDS, where element and pair e lie at [e % 8][e / 8], so that neighbouring threads meet
+// neighbouring banks. Every element is the sum that rope_rotate writes for its side, with the same bits. us in pieces / so:
+// 14 x 132 bf16 rows of 32 + 32 + 32 heads of 128, 106 elements turning in halves, 54 / 32; 37 x 30 f16 of 96 heads, 116 turning, 34 / 22; 2 x 1863 f16 of 24 heads of 64, 50 as neighbours,
+// 17 / 11. Four heads to a thread, as above, are no faster here. Whole pieces are faster by themselves: 8000 tokens, 60, would take 72 this way.
+template <int DT, int CT, bool ONCE>
+__global__ __launch_bounds__(256) void rotary_rows_kernel(Rotate a) {
+#pragma clang fp contract(off)
+    __shared__ float rows[8][256], sines[8][MAX_HEAD / 16], cosines[8][MAX_HEAD / 16];
+    const int chunks = a.d >> 3, slot0 = (int)threadIdx.x / chunks, at = ((int)threadIdx.x - slot0 * chunks) * 8;
+    const size_t tok = blockIdx.x;
+    const int slot = (int)blockIdx.y * a.heads_wg + slot0, half = a.dims >> 1;
+    const bool mine = slot0 < a.heads_wg && slot < a.h_q + 2 * a.h_kv, is_q = slot < a.h_q, is_v = slot >= a.h_q + a.h_kv;
+    const int head = is_q ? slot : slot - a.h_q - (is_v ? a.h_kv : 0);
+    const size_t from = (tok * (is_q ? a.h_q : a.h_kv) + head) * a.d + at;
+    float x[8] = {};
+    if (mine) load_n<DT, 8, ONCE>(is_q ? a.q : is_v ? a.v : a.k, from, 8, x);
+    const int pos = half > 0 ? a.positions[tok] : 0;               // (an append alone has none)
+    for (int pair = (int)threadIdx.x; pair < half; pair += (int)blockDim.x) {
+        float sn, cs;
+        sincos_turn(a.turns[pair] * (unsigned long)(long)pos, sn, cs);
+        sines[pair & 7][pair >> 3] = sn * a.magnitude;
+        cosines[pair & 7][pair >> 3] = cs * a.magnitude;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rows[j][threadIdx.x] = x[j];
+    __syncthreads();
+    if (!mine) return;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int e = at + j;
+        const bool upper = a.interleaved ? j & 1 : e >= half;
+        const int pair = max(0, min(a.interleaved ? e >> 1 : upper ? e - half : e, half - 1)), with = upper ? max(0, e - half) : min(e + half, a.d - 1);
+        const float own = x[j], beside = x[j ^ 1], across = rows[with & 7][slot0 * chunks + (with >> 3)], sn = sines[pair & 7][pair >> 3], cs = cosines[pair & 7][pair >> 3];
+        const float turned = own * cs + (a.interleaved ? beside : across) * (upper ? sn : -sn);
+        y[j] = e < a.dims && !is_v ? turned : own;
+    }
+    if (is_q) {
+        store_n<DT, 8, ONCE>(a.q_out, from, 8, y);
+    } else if (a.write_index) {
+        const size_t seq = (unsigned)tok / (unsigned)a.s_len;
+        const long step = (long)a.write_index[seq] + (long)(tok - seq * (unsigned)a.s_len);
+        const int page = step >= 0 && step < (long)MAX_ROWS ? page_of(a.table, seq, (int)step) : -1;
+        if (page >= 0)
+            store_n<CT, 8>(is_v ? a.v_pages : a.k_pages, ((((size_t)page * a.h_kv + head) << a.table.shift) + ((int)step & ((1 << a.table.shift) - 1))) * a.d + at, 8, y);
+    }
+}
+
 struct ReadArgs {
     const unsigned char *pages[2];
     void *out[2];
@@ -288,10 +343,14 @@ int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rot
     a.turning = (a.dims / 2 + each - 1) / each;
     a.pieces = a.turning + (a.d - a.dims + 2 * each - 1) / (2 * each);
     const int slots = a.h_q + 2 * a.h_kv;
+    const bool once = tokens * slots * a.d * (dtype == AIONHIP_F32 ? 8 : 4) >= ONCE_BYTES;
+    // (f32 rows past the caches, 56 x 214 of 12 heads of 256, 196 elements turning: 61 us in pieces, 64 so)
+    const bool whole = (a.interleaved ? a.dims % (2 * each) : a.dims / 2 % each) == 0 && (a.d - a.dims) % (2 * each) == 0;
+    const bool by_rows = !whole && a.d % 8 == 0 && !(once && dtype == AIONHIP_F32);
+    if (by_rows) a.pieces = a.d / 8;
     a.heads_wg = min(256 / a.pieces, slots);                             // (heads of up to 1024 have 129 pieces at most)
     // (measured at the kernel)
-    const int heads = tokens >= 1024 && a.h_kv ? 4 : 1;
-    const bool once = tokens * slots * a.d * (dtype == AIONHIP_F32 ? 8 : 4) >= ONCE_BYTES;
+    const int heads = !by_rows && tokens >= 1024 && a.h_kv ? 4 : 1;
     const dim3 grid((unsigned)tokens, (unsigned)((slots + a.heads_wg * heads - 1) / (a.heads_wg * heads)));
     const unsigned threads = (unsigned)((a.heads_wg * a.pieces + 63) / 64 * 64);
     if (tokens > MAX_THREADS / threads) return set_err(ctx, AIONHIP_UNSUPPORTED, "%s: too many rows for one launch", who);
@@ -301,7 +360,9 @@ int launch_rotary(aionhip_ctx *ctx, const char *who, Rotate a, const aionhip_rot
     ProfScope scope(ctx, who);
     auto go = [&](auto dt, auto ct) {
         constexpr int DT = decltype(dt)::value, CT = decltype(ct)::value;
-        if (heads == 1) launch_k(ctx, once ? rotary_kernel<DT, CT, 1, true> : rotary_kernel<DT, CT, 1, false>, grid, dim3(threads), 0, a);
+        constexpr bool PAST = DT != AIONHIP_F32;
+        if (by_rows) launch_k(ctx, once ? rotary_rows_kernel<DT, CT, PAST> : rotary_rows_kernel<DT, CT, false>, grid, dim3(threads), 0, a);
+        else if (heads == 1) launch_k(ctx, once ? rotary_kernel<DT, CT, 1, true> : rotary_kernel<DT, CT, 1, false>, grid, dim3(threads), 0, a);
         else launch_k(ctx, once ? rotary_kernel<DT, CT, 4, true> : rotary_kernel<DT, CT, 4, false>, grid, dim3(threads), 0, a);
     };
     auto types = [&](auto dt) {

@@ -674,3 +674,49 @@ def test_workgroups_that_read_the_same_keys_side_by_side(gpu, b, l, hq, hkv, d, 
     pages = Pages(rng, be.F16, b, -(-max(lengths) // 64) + 1, 64, hkv, d)
     bits, q = source(rng, (b, l, hq, d), be.F32)
     check(gpu, pages, bits, q, be.F32, d ** -0.5, lengths=lengths)
+
+
+@pytest.mark.parametrize("dtype", [be.F32] + TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d, dims, h", [(64, 62, 5), (64, 2, 3), (8, 6, 40), (72, 30, 7), (256, 150, 2), (1024, 1022, 1), (1024, 6, 3), (136, 134, 300)])
+@pytest.mark.parametrize("rows", [7, 1030])
+def test_rotary_of_heads_that_do_not_come_apart_evenly(gpu, dtype, interleaved, d, dims, h, rows):
+    if rows > 7 and h * d > 8192:
+        h = 9
+    rng = np.random.default_rng(dims)
+    r = be.Rotary(dims, base=10000.0, interleaved=interleaved, magnitude=1.25)
+    bits, x = source(rng, (1, rows, h, d), dtype)
+    positions = rng.integers(-5, 300000, (1, rows)).astype(np.int32)
+    xd, pd = gpu.upload(bits), gpu.upload(positions)
+    out = gpu.alloc(bits.nbytes)
+    gpu.step_rotary(out, xd, pd, 1, rows, h, d, r, dtype=dtype)
+    got = gpu.download(out, storage(dtype), bits.shape)
+    assert turned_close(to_f64(got, dtype), x, positions, r, dtype).all()
+    gpu.step_rotary(xd, xd, pd, 1, rows, h, d, r, dtype=dtype)
+    assert np.array_equal(gpu.download(xd, storage(dtype), bits.shape).view(np.uint8), got.view(np.uint8))
+    for buf in (xd, pd, out):
+        buf.free()
+
+
+@pytest.mark.parametrize("src", [be.F32] + TYPES)
+@pytest.mark.parametrize("hq, h, d, dims, s", [(4, 2, 64, 62, 3), (7, 3, 72, 30, 1), (5, 5, 72, 0, 9), (8, 1, 256, 150, 1100), (32, 8, 128, 106, 2)])
+def test_append_of_heads_that_do_not_come_apart_evenly(gpu, src, hq, h, d, dims, s):
+    """q as the step alone has it, keys from the turned f32 values, values as they came; and the append without turning"""
+    rng = np.random.default_rng(d + s)
+    pages = Pages(rng, be.F16, 2, -(-s // 32) + 1, 32, h, d)
+    r = be.Rotary(dims, base=500000.0)
+    (qb, q), (kb, k), (vb, v) = source(rng, (2, s, hq, d), src), source(rng, (2, s, h, d), src), source(rng, (2, s, h, d), src)
+    positions, start = rng.integers(0, 5000, (2, s)).astype(np.int32), np.array([5, 17], np.int32)
+    cache, qd, kd, vd, pd, sd = pages.upload(gpu), gpu.upload(qb), gpu.upload(kb), gpu.upload(vb), gpu.upload(positions), gpu.upload(start)
+    out, ko, vo = gpu.alloc(qb.nbytes), gpu.alloc(k.size * 4), gpu.alloc(k.size * 4)
+    gpu.step_rotary_append_paged(cache, r, out, qd, kd, vd, pd, sd, s, hq, dtype=src)
+    assert turned_close(to_f64(gpu.download(out, storage(src), qb.shape), src), q, positions, r, src).all()
+    gpu.step_read_paged(cache, ko, vo, sd, s)
+    assert turned_close(gpu.download(ko, np.float32, k.shape).astype(np.float64), k, positions, r, be.F16).all()
+    plain = to_f64(to_bits(v.astype(np.float32), be.F16), be.F16)
+    assert np.array_equal(gpu.download(vo, np.float32, v.shape), plain)
+    gpu.step_append_paged(cache, vd, kd, sd, s, src_dtype=src)
+    gpu.step_read_paged(cache, ko, vo, sd, s)
+    assert np.array_equal(gpu.download(ko, np.float32, v.shape), plain)
+    assert np.array_equal(gpu.download(vo, np.float32, k.shape), to_f64(to_bits(k.astype(np.float32), be.F16), be.F16))
+    free(cache, qd, kd, vd, pd, sd, out, ko, vo)
