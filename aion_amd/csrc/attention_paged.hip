@@ -956,8 +956,8 @@ extern "C" int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_atte
         const long cus = ctx->cu_count > 0 ? ctx->cu_count : 256, wgs = (long)units * a.row_tiles, tiles = (keys + TILE_KEYS - 1) / TILE_KEYS;
         const Split split = split_of(wgs, tiles, min(a.rows_total, 16), a.d, cus);
         a.nseg = split.segments, a.shares = split.shares;
-        // Five queries of 32 sequences over 8192 keys, 32 heads on 8 of 128 (two row tiles), 305 -> 203 us; 7 over 62761, 5 sequences, 363 -> 244. Shares of few tiles do not wait for what places
-        // them: one token, one head of 256 for 8, 4096 keys 10.0 in plain order and 10.5 so, 32768 20.0 and 17.3.
+        // Five queries of 32 sequences of up to 8192 keys, 32 heads on 8 of 128 (two row tiles), 237 -> 180 us (four queries, one tile, 156); 7 of 5 sequences of up to 62761, 310 -> 232. Shares
+        // of few tiles do not wait for what places them: one token, one head of 256 for 8, 4096 keys 10.0 in plain order and 10.5 so, 32768 20.0 and 17.3.
         a.beside = a.row_tiles > 1 || (a.shares > 1 && tiles >= 8L * a.nseg);
         once = a.row_tiles == 1 && (size_t)units * keys * c->d * 4 >= ONCE_BYTES;
     }
