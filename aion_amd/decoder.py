@@ -180,7 +180,7 @@ class Decoder:
         self.history = gpu.alloc(self.log_capacity * 4)  # token produced at each position (decode program's log)
         self.state = {}        # S -> activation buffers
         self.program = self.cut_program = None
-        self.pos = self.rows = 0                         # tokens of the text, rows of the caches (fewer, once rows have been evicted)
+        self._pos = self.gone = 0                        # tokens of the text; of their rows, how many eviction has taken
         if one_launch and not cfg.quant_cache and not cfg.page_rows:               # (the one-launch form reads linear f16 caches)
             layers = [{"wq": self.w["l%d.wq" % l], "wk": self.w["l%d.wk" % l], "wv": self.w["l%d.wv" % l], "wo": self.w["l%d.wo" % l],
                        "w_gate": self.w["l%d.wgate" % l], "w_up": self.w["l%d.wup" % l], "w_down": self.w["l%d.wdown" % l],
@@ -294,14 +294,34 @@ class Decoder:
         """Whether s tokens more take the caches past their limit: how many rows there are is known here, which ones stay is not."""
         return bool(self.eviction) and self.rows + s > self.eviction[1]
 
+    @property
+    def pos(self):
+        """Tokens of the text so far. May be set: the text goes on from there, over what was behind. Under eviction only to 0, which is reset(): which rows a shorter text would still have,
+        and what its keys had drawn, is not kept."""
+        return self._pos
+
+    @pos.setter
+    def pos(self, pos):
+        if self.eviction and pos != self._pos:
+            if pos:
+                raise ValueError("pos %d: under eviction a text goes on from its end (%d) or begins anew (0)" % (pos, self._pos))
+            self.reset()
+        self._pos = pos
+
+    @property
+    def rows(self):
+        """Rows of the caches: fewer than the text has tokens, once rows have been evicted."""
+        return self._pos - self.gone
+
     def _advanced(self, s):
         """The text and the caches are s tokens further."""
         due = self._due(s)
-        self.pos += s
-        self.rows = self.eviction[0] if due else self.rows + s
+        self._pos += s
+        if due:
+            self.gone = self._pos - self.eviction[0]
 
     def reset(self):
-        self.pos = self.rows = 0
+        self._pos = self.gone = 0
         for w in self.drawn:
             self.gpu.write(w, np.zeros(w.nbytes // 4, np.float32))
 
@@ -364,7 +384,7 @@ class Decoder:
         self.program = self.cut_program = None
 
     def _set_decode_state(self, b, token, pos):
-        g, rows = self.gpu, pos - self.pos + self.rows
+        g, rows = self.gpu, pos - self.gone
         g.write(b["ids"], np.array([token], np.int32))
         g.write(b["positions"], np.array([pos], np.int32))
         g.write(b["write_index"], np.array([rows], np.int32))

@@ -1,0 +1,161 @@
+"""Where a decoder writes its rows after `pos` has been set: with a stand-in for the backend that keeps what is written, and on the GPU against a decoder that has seen nothing else."""
+import numpy as np
+import pytest
+
+from aion_amd import backend as be
+from aion_amd.decoder import Decoder, DecoderConfig, SyntheticWeights
+
+SHAPE = dict(layers=2, hidden=256, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1024)
+KINDS = {"linear": {}, "q8": dict(cache_dtype=be.Q8_0), "pages": dict(page_rows=16), "evicting": dict(page_rows=16, evict_keep=16, evict_limit=36)}
+
+
+class Buffer:
+    def __init__(self, nbytes):
+        self.nbytes, self.value, self.handle = nbytes, None, 0
+
+    def view(self, offset):
+        return self
+
+
+class Backend:
+    """Takes every step, runs none: buffers keep what the host wrote, step_advance_state counts."""
+
+    def alloc(self, nbytes):
+        return Buffer(nbytes)
+
+    zeros = alloc
+
+    def upload(self, x):
+        return Buffer(np.asarray(x).nbytes)
+
+    def upload_weight(self, *a):
+        return Buffer(0)
+
+    def cache_quant_bytes(self, *a):
+        return 64
+
+    def paged_cache(self, *a):
+        return be.PagedCache(*a)
+
+    def write(self, buf, x):
+        buf.value = np.array(x)
+
+    def copy(self, dst, src, nbytes):
+        dst.value = np.array(src.value)
+
+    def download(self, buf, dtype, shape=None, offset=0):
+        return np.zeros(shape, dtype)
+
+    def step_advance_state(self, dst, src, n, counters, **kw):
+        for c in counters:
+            c.value = c.value + 1
+
+    def step_evict_paged(self, cache, w, lengths, wo, lengths_out, keep, limit, first, recent):
+        lengths_out.value = np.minimum(lengths.value, keep) if lengths.value[0] > limit else np.array(lengths.value)
+
+    def record_program(self, issue):
+        return issue
+
+    def program_execute(self, program):
+        program()
+
+    def program_is_current(self, program):
+        return True
+
+    def step_attention_matmul(self, *a, **kw):
+        return True
+
+    def __getattr__(self, name):
+        return lambda *a, **kw: None
+
+
+def state(d, s):
+    b = d._buffers(s)
+    return int(b["positions"].value[0]), int(b["write_index"].value[0]), int(b["kv_len"].value[0])
+
+
+class Blank(SyntheticWeights):
+    def blocks(self, name):
+        return np.zeros(0, np.uint8)
+
+
+def blank(kind):
+    cfg = DecoderConfig(max_seq=40, **KINDS[kind], **SHAPE)
+    return Decoder(Backend(), cfg, Blank(cfg, 1))
+
+
+@pytest.mark.parametrize("kind", ["linear", "q8", "pages"])
+def test_rows_go_where_pos_says(kind):
+    d = blank(kind)
+    for _ in range(4):                                       # as many prompts as there are, each from the beginning
+        d.pos = 0
+        d.prefill(np.zeros(16, np.int32))
+        assert state(d, 16) == (0, 0, 16) and (d.pos, d.rows) == (16, 16)
+    for _ in range(4):
+        d.pos = 16
+        d.begin_decode(3)
+        assert state(d, 1) == (16, 16, 17)
+        d.decode_run(12)
+        assert state(d, 1) == (28, 28, 29) and d.rows == 28
+    d.pos = 20
+    d.prefill(np.zeros(7, np.int32))
+    assert state(d, 7) == (20, 20, 27)
+    with pytest.raises(ValueError):
+        d.prefill(np.zeros(14, np.int32))
+
+
+def test_under_eviction_a_text_goes_on_or_begins_anew():
+    d = blank("evicting")
+    for again in range(2):
+        d.prefill(np.zeros(20, np.int32))
+        for pos in (19, 21, 1):
+            with pytest.raises(ValueError):
+                d.pos = pos
+        d.pos = 20
+        d.prefill(np.zeros(17, np.int32))
+        assert state(d, 17) == (20, 20, 37) and (d.pos, d.rows, d.gone) == (37, 16, 21)
+        d.begin_decode(3)
+        assert state(d, 1) == (37, 16, 17)
+        d.decode_run(20)
+        assert state(d, 1) == (57, 36, 37) and d.rows == 36
+        d.decode_step()                                      # the 37th row passes the limit
+        assert state(d, 1) == (58, 16, 17) and (d.pos, d.rows) == (58, 16)
+        with pytest.raises(ValueError):
+            d.pos = 57
+        for w in d.drawn:
+            w.value = None
+        d.pos = 0                                            # as reset()
+        assert d.rows == 0 and all((w.value == 0).all() for w in d.drawn)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind, one_launch", [("linear", False), ("linear", True), ("q8", False), ("pages", False)])
+def test_a_text_taken_back_is_the_text_of_a_fresh_decoder(gpu, kind, one_launch):
+    cfg = DecoderConfig(max_seq=150, **KINDS[kind], **SHAPE)
+    weights = SyntheticWeights(cfg, 3)
+    rng = np.random.default_rng(1)
+    first, second = (rng.integers(0, cfg.vocab, 70).astype(np.int32) for _ in range(2))
+    d = Decoder(gpu, cfg, weights, one_launch=one_launch)
+    fresh, other = (Decoder(gpu, cfg, weights, one_launch=one_launch) for _ in range(2))
+    try:
+        d.begin_decode(d.prefill(first))
+        d.decode_run(30)
+        d.pos = 0
+        a, b = d.prefill(second), fresh.prefill(second)
+        assert a == b and np.array_equal(d.logits_host(), fresh.logits_host())
+        d.begin_decode(a)
+        fresh.begin_decode(b)
+        want = fresh.decode_run(30)
+        assert np.array_equal(d.decode_run(30), want) and np.array_equal(d.logits_host(), fresh.logits_host())
+        for _ in range(3):                                   # the same run again and again
+            d.pos = second.size
+            d.begin_decode(a)
+            assert np.array_equal(d.decode_run(30), want) and np.array_equal(d.logits_host(), fresh.logits_host())
+        d.pos = 40                                           # the rest of the prompt once more, in front of another end of the text
+        other.prefill(second)                                # (of 40 tokens alone the prompt's own sums would be split otherwise)
+        other.pos = 40
+        assert d.prefill(first[:25]) == other.prefill(first[:25]) and np.array_equal(d.logits_host(), other.logits_host())
+    finally:
+        d.close()
+        fresh.close()
+        other.close()
