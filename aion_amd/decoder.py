@@ -176,8 +176,8 @@ class Decoder:
         self.one = gpu.upload(np.ones(1, np.int32))
         self.logits = gpu.alloc(cfg.vocab * 4)
         self.token = gpu.alloc(4)
-        self.log_capacity = cfg.max_seq if not self.eviction else max(cfg.max_seq, 1 << 16)
-        self.history = gpu.alloc(self.log_capacity * 4)  # token produced at each position (decode program's log)
+        self.history = gpu.alloc(cfg.max_seq * 4)        # the tokens that a run of decode steps has produced, the first at 0
+        self.logged = gpu.upload(np.zeros(1, np.int32))  # how many
         self.state = {}        # S -> activation buffers
         self.program = self.cut_program = None
         self._pos = self.gone = 0                        # tokens of the text; of their rows, how many eviction has taken
@@ -370,9 +370,9 @@ class Decoder:
                     g.copy(b["write_index"], b["kept_len"], 4)
                     g.copy(b["kv_len"], b["kept_len"], 4)
                 # advance the device-resident loop state: next id = argmax, positions/write index/kv length += 1; the token
-                # is also logged at the position it was produced at, so that a run of steps needs no read-back per step
-                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["kv_len"]] + ([] if cut else [b["write_index"]]),
-                                     log=self.history, log_index=b["positions"], log_capacity=self.log_capacity)
+                # is also logged behind those before it, so that a run of steps needs no read-back per step
+                g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["kv_len"], self.logged] + ([] if cut else [b["write_index"]]),
+                                     log=self.history, log_index=self.logged, log_capacity=self.cfg.max_seq)
             self.program = g.record_program(lambda: issue(False))
             if self.eviction:                        # the step that takes the caches past their limit is a program of its own
                 self.cut_program = g.record_program(lambda: issue(True))
@@ -398,8 +398,8 @@ class Decoder:
             return
         b, g = self._decode_buffers, self.gpu
         self._forward(1, b)
-        g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["write_index"], b["kv_len"]],
-                             log=self.history, log_index=b["positions"], log_capacity=self.cfg.max_seq)
+        g.step_advance_state(b["ids"], self.token, 1, [b["positions"], b["write_index"], b["kv_len"], self.logged],
+                             log=self.history, log_index=self.logged, log_capacity=self.cfg.max_seq)
 
     def decode_step(self, read_token=True):
         """One decode step on the device-resident state; returns the token it produced (a 4-byte read-back)."""
@@ -413,14 +413,17 @@ class Decoder:
 
     def decode_run(self, n):
         """Replays the decode program n times back to back (nothing is read back in between: the loop state and the token
-        log live on the device) and returns the n tokens."""
-        if self.pos + n > self.log_capacity:
-            raise ValueError("token log exhausted" if self.eviction else "cache capacity exhausted")
-        start = self.pos
-        for _ in range(n):
-            self._step_on_device()
-            self._advanced(1)
-        tokens = self.gpu.download(self.history, np.int32, (n,), offset=start * 4)
+        log live on the device; under eviction, where the text may outgrow the log, the log is read whenever it is full) and returns the n tokens."""
+        if not self.eviction and self.pos + n > self.cfg.max_seq:
+            raise ValueError("cache capacity exhausted")
+        tokens = np.zeros(n, np.int32)
+        for start in range(0, n, self.cfg.max_seq):
+            run = min(n - start, self.cfg.max_seq)
+            self.gpu.write(self.logged, np.zeros(1, np.int32))
+            for _ in range(run):
+                self._step_on_device()
+                self._advanced(1)
+            tokens[start:start + run] = self.gpu.download(self.history, np.int32, (run,))
         if self.stack is not None:
             self.gpu.decoder_stack_status(self.stack)      # raises if a launch gave up waiting (its tokens would be invalid)
         return tokens
@@ -446,7 +449,7 @@ class Decoder:
         for bufs in self.state.values():
             for t in bufs.values():
                 t.free()
-        for t in [self.embed, self.gamma, self.one, self.logits, self.token, self.history] + self.drawn + ([self.page_table] if self.page_table else []) + (self.linear or []):
+        for t in [self.embed, self.gamma, self.one, self.logits, self.token, self.history, self.logged] + self.drawn + ([self.page_table] if self.page_table else []) + (self.linear or []):
             t.free()
 
 

@@ -26,7 +26,9 @@ class Backend:
     zeros = alloc
 
     def upload(self, x):
-        return Buffer(np.asarray(x).nbytes)
+        b = Buffer(np.asarray(x).nbytes)
+        b.value = np.array(x)
+        return b
 
     def upload_weight(self, *a):
         return Buffer(0)
@@ -44,9 +46,17 @@ class Backend:
         dst.value = np.array(src.value)
 
     def download(self, buf, dtype, shape=None, offset=0):
-        return np.zeros(shape, dtype)
+        return np.zeros(shape, dtype) if buf.value is None else buf.value[offset // 4:offset // 4 + shape[0]].copy()
 
-    def step_advance_state(self, dst, src, n, counters, **kw):
+    def step_argmax(self, token, logits, rows, columns):
+        token.value = np.array([0 if token.value is None else int(token.value[0]) + 1], np.int32)
+
+    def step_advance_state(self, dst, src, n, counters, log, log_index, log_capacity):
+        at = int(log_index.value[0])
+        if at < log_capacity:
+            if log.value is None:
+                log.value = np.full(log.nbytes // 4, -1, np.int32)
+            log.value[at] = src.value[0]
         for c in counters:
             c.value = c.value + 1
 
@@ -128,6 +138,23 @@ def test_under_eviction_a_text_goes_on_or_begins_anew():
         assert d.rows == 0 and all((w.value == 0).all() for w in d.drawn)
 
 
+@pytest.mark.parametrize("kind, runs", [("linear", [5, 0, 18]), ("evicting", [3, 0, 40, 41, 200, 66000, 7])])
+def test_a_run_returns_its_tokens_however_long_the_text_is(kind, runs):
+    """the stand-in's tokens are numbered; under eviction the text passes the caches and any log of it"""
+    d = blank(kind)
+    d.prefill(np.zeros(16, np.int32))
+    d.begin_decode(3)
+    d.decode_step(read_token=False)                          # (not a run's)
+    at = int(d.token.value[0])
+    for n in runs:
+        assert np.array_equal(d.decode_run(n), at + 1 + np.arange(n))
+        at += n
+    assert d.pos == 17 + sum(runs)
+    if kind == "linear":
+        with pytest.raises(ValueError):
+            d.decode_run(1)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind, one_launch", [("linear", False), ("linear", True), ("q8", False), ("pages", False)])
 def test_a_text_taken_back_is_the_text_of_a_fresh_decoder(gpu, kind, one_launch):
@@ -159,3 +186,19 @@ def test_a_text_taken_back_is_the_text_of_a_fresh_decoder(gpu, kind, one_launch)
         d.close()
         fresh.close()
         other.close()
+
+
+@pytest.mark.gpu
+def test_a_run_longer_than_the_log(gpu):
+    cfg = DecoderConfig(max_seq=40, **KINDS["evicting"], **SHAPE)
+    weights = SyntheticWeights(cfg, 3)
+    prompt = np.random.default_rng(2).integers(0, cfg.vocab, 33).astype(np.int32)
+    a, b = (Decoder(gpu, cfg, weights) for _ in range(2))
+    try:
+        a.begin_decode(a.prefill(prompt))
+        b.begin_decode(b.prefill(prompt))
+        want = [b.decode_step() for _ in range(170)]
+        assert list(a.decode_run(130)) + list(a.decode_run(40)) == want
+    finally:
+        a.close()
+        b.close()
