@@ -138,6 +138,9 @@ def hash_name(name):
     return h
 
 
+PROMPT_ROWS = 64        # caches in pages: longer prompts attend to keys and values read back in order; of them that many last queries say what the keys draw
+
+
 class Decoder:
     def __init__(self, gpu, cfg, weights, on_weight=None, one_launch=False):
         """on_weight(name, host_array) is called for every tensor (the tests feed the oracle with it)."""
@@ -199,13 +202,19 @@ class Decoder:
         c, g = self.cfg, self.gpu
         f = 4 * s
         b = {
-            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4), "kept_len": g.alloc(4), "row_positions": g.alloc(4 * s),
+            "ids": g.alloc(4 * s), "positions": g.alloc(4 * s), "write_index": g.alloc(4), "kv_len": g.alloc(4),
             "x": g.alloc(f * c.hidden), "h": g.alloc(f * c.hidden), "o": g.alloc(f * c.hidden),
             "q": g.alloc(f * c.q_dim), "qr": g.alloc(f * c.q_dim), "att": g.alloc(f * c.q_dim),
             "k": g.alloc(f * c.kv_dim), "kr": g.alloc(f * c.kv_dim), "v": g.alloc(f * c.kv_dim),
             "gate": g.alloc(f * c.ffn), "up": g.alloc(f * c.ffn), "act": g.alloc(f * c.ffn),
-            "hl": g.alloc(4 * c.hidden), "tail": g.alloc(4 * min(s, 64) * c.q_dim),
+            "hl": g.alloc(4 * c.hidden),
         }
+        if c.page_rows and s > PROMPT_ROWS:
+            b["row_positions"] = g.alloc(4 * s)
+        if self.eviction:
+            b["kept_len"] = g.alloc(4)
+            if s > PROMPT_ROWS:
+                b["tail"] = g.alloc(4 * PROMPT_ROWS * c.q_dim)
         self.state[s] = b
         return b
 
@@ -269,7 +278,7 @@ class Decoder:
         c, g, p, cache = self.cfg, self.gpu, "l%d." % l, self.caches[l]
         g.step_rmsnorm_matmul([self.w[p + "wq"], self.w[p + "wk"], self.w[p + "wv"]], b["x"], self.gamma, s, [b["q"], b["k"], b["v"]], c.eps)
         g.step_rotary_append_paged(cache, self.rotary, b["qr"], b["q"], b["k"], b["v"], b["positions"], b["write_index"], s, c.heads)
-        asked = min(s, 64)
+        asked = min(s, PROMPT_ROWS)
         if asked < s:
             # a prompt: its keys and values in order, for the kernel that shares them among many rows
             n = self.rows + s
@@ -335,7 +344,8 @@ class Decoder:
         g = self.gpu
         g.write(b["ids"], t)
         g.write(b["positions"], np.arange(self.pos, self.pos + s, dtype=np.int32))
-        g.write(b["row_positions"], np.arange(self.rows, self.rows + s, dtype=np.int32))
+        if "row_positions" in b:
+            g.write(b["row_positions"], np.arange(self.rows, self.rows + s, dtype=np.int32))
         g.write(b["write_index"], np.array([self.rows], np.int32))
         g.write(b["kv_len"], np.array([self.rows + s], np.int32))
         self._forward(s, b)

@@ -155,6 +155,12 @@ def test_a_run_returns_its_tokens_however_long_the_text_is(kind, runs):
             d.decode_run(1)
 
 
+@pytest.mark.parametrize("kind, s, more", [("linear", 100, set()), ("linear", 1, set()), ("q8", 100, set()), ("pages", 64, set()), ("pages", 65, {"row_positions"}), ("evicting", 1, {"kept_len"}),
+                                           ("evicting", 65, {"kept_len", "row_positions", "tail"})])
+def test_only_caches_in_pages_cost_what_they_need(kind, s, more):
+    assert set(blank(kind)._buffers(s)) & {"kept_len", "row_positions", "tail"} == more
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind, one_launch", [("linear", False), ("linear", True), ("q8", False), ("pages", False)])
 def test_a_text_taken_back_is_the_text_of_a_fresh_decoder(gpu, kind, one_launch):
