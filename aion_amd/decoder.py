@@ -6,8 +6,10 @@ src/bench/models.zig:433-536, trimmed to a plain pre-norm block): Gather -> per 
 MatMul o -> add -> RMSNorm -> MatMul gate,up -> gate(gelu) -> MatMul down -> add] ->
 RMSNorm -> MatMul lm_head -> ArgMax. With `cache_dtype` Q8_0 or Q4_0 the keys and values are quantised as they are appended
 (SequenceAppend takes the f32 rows, no Cast) and attention reads the codes. With `page_rows` the caches are pools of pages under one
-page table; q and k turn as `rotary` says, and with `evict_keep` a sequence that passes `evict_limit` rows keeps that many of them, the ones
-whose keys have drawn the most attention, decided on the device at every step: the text may then be longer than the caches. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
+page table; q and k turn as `rotary` says, and with `evict_keep` a sequence that passes `evict_limit` rows keeps that many of them: the first, the newest, and the ones
+whose keys have drawn the most attention, decided on the device at every step. The text may then be longer than the caches, though no prompt may (it is refused whole, before
+anything is evicted for it). What keys draw is counted from the queries of every decode step and of a prompt's last 64 tokens, so that a text handed over in
+several prompts counts more queries, and may keep other rows, than in one. q4_0 weights are [K,N] quant_axis 0 MatMul operands (the
 only q4 layout aion has), q8_0 weights are [N,K] quant_axis 1 MatMulNT operands.
 
 Prefill runs the steps eagerly; the single-token decode step is recorded once into a program
@@ -45,7 +47,7 @@ class DecoderConfig:
     evict_keep: int = 0              # caches in pages: rows that a sequence keeps when it passes evict_limit; 0: no eviction
     evict_limit: int = 0             # 0: max_seq - 1
     evict_first: int = 4             # of those, the oldest and the newest that stay in any case
-    evict_recent: int = 0            # 0: a quarter of evict_keep
+    evict_recent: int = None         # None: a quarter of evict_keep
 
     @property
     def q_dim(self):
@@ -71,7 +73,7 @@ class DecoderConfig:
             raise ValueError("evict_keep: eviction is from caches in pages (page_rows)")
         limit = self.evict_limit or self.max_seq - 1
         first = min(self.evict_first, self.evict_keep)
-        recent = min(self.evict_recent or self.evict_keep // 4, self.evict_keep - first)
+        recent = min(self.evict_keep // 4 if self.evict_recent is None else self.evict_recent, self.evict_keep - first)
         if not self.evict_keep <= limit < self.max_seq:
             raise ValueError("evict_keep %d <= evict_limit %d < max_seq %d must hold" % (self.evict_keep, limit, self.max_seq))
         return self.evict_keep, limit, first, recent

@@ -161,6 +161,12 @@ def test_only_caches_in_pages_cost_what_they_need(kind, s, more):
     assert set(blank(kind)._buffers(s)) & {"kept_len", "row_positions", "tail"} == more
 
 
+def test_no_newest_rows_need_stay():
+    cfg = lambda **kw: DecoderConfig(max_seq=64, page_rows=16, evict_keep=16, **SHAPE, **kw).eviction()  # noqa: E731
+    assert cfg(evict_recent=0) == (16, 63, 4, 0) and cfg(evict_recent=0, evict_first=0) == (16, 63, 0, 0)
+    assert cfg() == cfg(evict_recent=None) == (16, 63, 4, 4) and cfg(evict_recent=40) == (16, 63, 4, 12)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind, one_launch", [("linear", False), ("linear", True), ("q8", False), ("pages", False)])
 def test_a_text_taken_back_is_the_text_of_a_fresh_decoder(gpu, kind, one_launch):
