@@ -64,27 +64,29 @@ __device__ __forceinline__ int scan_all(int v, int *red, int &total) {
 // (25.5), ranks instead of weights in registers (the same), 64 neighbouring rows to a wavefront, with masks and counts of bits in place of sums (30).
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
-    constexpr int CHUNK = THREADS * SELECT_EACH, COPIES = THREADS / 256, OWN = DIGITS / THREADS;
+    constexpr unsigned CHUNK = THREADS * SELECT_EACH;
+    constexpr int COPIES = THREADS / 256, OWN = DIGITS / THREADS;
     __shared__ int hist[DIGITS * COPIES], red[THREADS / 64], s_digit, s_above;
     const int b = blockIdx.y, head = blockIdx.x, tid = threadIdx.x;
     const size_t unit = (size_t)b * a.h + head;
-    const int n = max(0, min(a.lengths[b], a.cap));
-    const bool cut = n > a.limit;
-    const int count = cut ? a.keep : n;
+    // (steps are unsigned: a capacity goes up to 2^31 - 64, and the places after a chunk, or a thread's last row, past 2^31)
+    const unsigned n = (unsigned)max(0, min(a.lengths[b], a.cap)), limit = (unsigned)a.limit, cap_out = (unsigned)a.cap_out;
+    const bool cut = n > limit;
+    const int count = cut ? a.keep : (int)n;
     if (head == 0 && tid == 0) a.counts[b] = cut || !a.in_place ? count : -1;
     const float *w = a.weights + unit * a.cap;
     float *out = a.weights_out + unit * a.cap_out;
     int *kept = a.kept + unit * a.limit;
     if (!cut) {
         if (a.tell)
-            for (int i = tid; i < a.limit; i += THREADS) kept[i] = i < n ? i : -1;
+            for (unsigned i = tid; i < limit; i += THREADS) kept[i] = i < n ? (int)i : -1;
         if (out != w)                             // (in place an uncut sequence costs nothing but the look at its length)
-            for (int i = tid; i < a.cap_out; i += THREADS) out[i] = i < n ? w[i] : 0.f;
+            for (unsigned i = tid; i < cap_out; i += THREADS) out[i] = i < n ? w[i] : 0.f;
         return;
     }
-    const int lo = a.first, hi = n - a.recent;
-    auto load = [&](int chunk, float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
-        const int i = chunk * CHUNK + tid * SELECT_EACH;
+    const unsigned lo = (unsigned)a.first, hi = n - (unsigned)a.recent;
+    auto load = [&](unsigned chunk, float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+        const unsigned i = chunk * CHUNK + (unsigned)tid * SELECT_EACH;
         if (i + SELECT_EACH <= n) {
             __builtin_memcpy(x, w + i, sizeof x);
         } else {
@@ -94,7 +96,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
     };
     float held[HELD][SELECT_EACH];
 #pragma unroll
-    for (int c = 0; c < HELD; ++c)
+    for (unsigned c = 0; c < HELD; ++c)
         if (c * CHUNK < n) load(c, held[c]);
     int want = a.keep - a.first - a.recent;
     unsigned prefix = 0;
@@ -105,8 +107,8 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
             const int bits = shift == 0 ? 10 : 11;
             for (int i = tid; i < DIGITS * COPIES; i += THREADS) hist[i] = 0;
             __syncthreads();
-            auto add = [&](int chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
-                const int i = chunk * CHUNK + tid * SELECT_EACH;
+            auto add = [&](unsigned chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+                const unsigned i = chunk * CHUNK + (unsigned)tid * SELECT_EACH;
 #pragma unroll
                 for (int j = 0; j < SELECT_EACH; ++j) {
                     const unsigned r = rank_of(x[j]);
@@ -115,9 +117,9 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
                 }
             };
 #pragma unroll
-            for (int c = 0; c < HELD; ++c)
+            for (unsigned c = 0; c < HELD; ++c)
                 if (c * CHUNK < n) add(c, held[c]);
-            for (int c = HELD; c * CHUNK < n; ++c) {
+            for (unsigned c = HELD; c * CHUNK < n; ++c) {
                 float x[SELECT_EACH];
                 load(c, x);
                 add(c, x);
@@ -145,8 +147,8 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
     // `want` of the rows whose rank is `prefix` stay, the oldest of them. Chunks in order: what is read of a chunk lies behind everything written so far, and its ranks have been
     // taken when the workgroup meets, so that weights may move in place.
     int sure = 0, equal = 0;                      // rows before the chunk that stay whatever `want` is, and of that rank
-    auto place = [&](int chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
-        const int i = chunk * CHUNK + tid * SELECT_EACH;
+    auto place = [&](unsigned chunk, const float (&x)[SELECT_EACH]) __attribute__((always_inline)) {
+        const unsigned i = chunk * CHUNK + (unsigned)tid * SELECT_EACH;
         unsigned stays = 0, same = 0;
 #pragma unroll
         for (int j = 0; j < SELECT_EACH; ++j) {
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
             const bool mine = stays >> j & 1u, alike = same >> j & 1u;
             if (mine || (alike && e < want)) {
                 const int to = s + min(e, want);
-                kept[to] = i + j;
+                kept[to] = (int)(i + j);
                 out[to] = x[j];
             }
             s += mine ? 1 : 0;
@@ -173,16 +175,16 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Select a) {
         equal += (int)((unsigned)total >> 16);
     };
 #pragma unroll
-    for (int c = 0; c < HELD; ++c)
+    for (unsigned c = 0; c < HELD; ++c)
         if (c * CHUNK < n) place(c, held[c]);
-    for (int c = HELD; c * CHUNK < n; ++c) {
+    for (unsigned c = HELD; c * CHUNK < n; ++c) {
         float x[SELECT_EACH];
         load(c, x);
         place(c, x);
     }
     __syncthreads();
-    for (int i = a.keep + tid; i < a.limit; i += THREADS) kept[i] = -1;
-    for (int i = a.keep + tid; i < a.cap_out; i += THREADS) out[i] = 0.f;
+    for (unsigned i = (unsigned)(a.keep + tid); i < limit; i += THREADS) kept[i] = -1;
+    for (unsigned i = (unsigned)(a.keep + tid); i < cap_out; i += THREADS) out[i] = 0.f;
 }
 
 struct Move {
@@ -209,8 +211,9 @@ __global__ __launch_bounds__(256) void move_kernel(Move a) {
     if (row >= rows) return;
     const int *kept = a.kept + (size_t)unit * a.limit;
     const int mask = (1 << a.from.shift) - 1;
-    for (int to = (int)blockIdx.x * rows + row; to < count; to += a.parts * rows) {
-        const int from = kept[to];
+    const unsigned places = (unsigned)max(count, 0), stride = (unsigned)(a.parts * rows);         // (unsigned: a stride behind the last place may pass 2^31)
+    for (unsigned place = blockIdx.x * (unsigned)rows + row; place < places; place += stride) {
+        const int to = (int)place, from = kept[to];
         if (MODE != TO_PAGES && from == to) continue;
         const int source = page_of(a.from, b, from), target = MODE == HOLD ? 0 : page_of(a.to, b, to);
         if (source < 0 || target < 0) continue;

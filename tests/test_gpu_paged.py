@@ -720,3 +720,43 @@ def test_append_of_heads_that_do_not_come_apart_evenly(gpu, src, hq, h, d, dims,
     assert np.array_equal(gpu.download(ko, np.float32, v.shape), plain)
     assert np.array_equal(gpu.download(vo, np.float32, k.shape), to_f64(to_bits(k.astype(np.float32), be.F16), be.F16))
     free(cache, qd, kd, vd, pd, sd, out, ko, vo)
+
+
+@pytest.mark.parametrize("cut", [False, True])
+def test_evict_where_steps_end_at_two_to_the_31(cut):
+    """the largest capacity there is, all but two of its entries no page: rows move where both ends are on one"""
+    gpu = be.HipBackend(0)                                               # (26 GB, and scratch memory that goes with the context)
+    rng = np.random.default_rng(31)
+    p, d = 1024, 8
+    width = 0x7FFFFFC0 // p
+    cap = width * p
+    limit, first, recent = cap - 5000 if cut else cap, 3, 700
+    keep = cap - 6000 if cut else cap
+    pages = Pages(rng, be.F16, 1, 1, p, 1, d, pages=3)
+    table, table_out = np.full(width, -1, np.int32), np.full(width, -1, np.int32)
+    table[-1], table_out[-1 if not cut else -6] = 2, 1
+    kd, vd, td, to = (gpu.upload(x) for x in (pages.k, pages.v, table, table_out))
+    cache = gpu.paged_cache(kd, vd, td, 3, 1, width, p, 1, d)
+    wd, wo, kept, ld, lo = gpu.zeros(cap * 4), gpu.alloc(cap * 4), gpu.alloc(limit * 4), gpu.upload(np.array([2 ** 31 - 1], np.int32)), gpu.alloc(4)
+    tail = rng.random(20000).astype(np.float32)                          # the last rows have weights, all others none
+    gpu.write(wd, tail, offset=(cap - 20000) * 4)
+    gpu.step_evict_paged(cache, wd, ld, wo, lo, keep, limit=limit, first=first, recent=recent, table_out=to, width_out=width, kept=kept)
+    assert gpu.download(lo, np.int32, (1,))[0] == keep
+    # every weighed row stays, and of the others the oldest
+    old = keep - 20000
+    want = np.concatenate((np.arange(old - 9000, old), np.arange(cap - 20000, cap)))
+    assert np.array_equal(gpu.download(kept, np.int32, (29000,), offset=(keep - 29000) * 4), want)
+    assert np.array_equal(gpu.download(kept, np.int32, (9000,)), np.arange(9000)) and (gpu.download(kept, np.int32, (limit - keep,), offset=keep * 4) == -1).all()
+    weights = gpu.download(wo, np.float32, (cap - keep + 29000,), offset=(keep - 29000) * 4)
+    assert np.array_equal(weights, np.concatenate((np.zeros(9000, np.float32), tail, np.zeros(cap - keep, np.float32))))
+    # the source's page holds the last 1024 steps; the target's one page of places
+    page = width - (6 if cut else 1)
+    for which, (pool, buf) in enumerate(((pages.k, kd), (pages.v, vd))):
+        for to_step in range(page * p, min((page + 1) * p, keep)):
+            t = cap - (keep - to_step)                                   # (a place among the weighed rows)
+            if t // p == width - 1:
+                pool[1, :, to_step % p] = pool[2, :, t % p]
+        assert np.array_equal(gpu.download(buf, np.float16, pool.shape), pool), which
+    for buf in (kd, vd, td, to, wd, wo, kept, ld, lo):
+        buf.free()
+    gpu.close()
