@@ -501,7 +501,8 @@ class HipBackend:
 
     def step_evict_paged(self, cache, weights, kv_lengths, weights_out, lengths_out, keep, limit=None, first=0, recent=0, table_out=None, width_out=0, kept=None):
         """Sequences of more than `limit` (None: keep) rows keep `keep` of them: the `first` oldest, the `recent` newest, the ones of greatest weight between. table_out
-        None: in place; else the kept rows are copied to its pages. kept i32 [b, h_kv, limit]: the steps they were."""
+        None: in place; else the kept rows are copied to its pages. kept i32 [b, h_kv, limit]: the steps they were. Every step below kv_lengths lies on a page (a page that was
+        given back in the middle of a sequence would come back as whatever its steps' new places held)."""
         e = hip.Eviction(weights.handle, kv_lengths.handle, weights_out.handle, lengths_out.handle, table_out.handle if table_out is not None else 0,
                          kept.handle if kept is not None else 0, width_out, keep if limit is None else limit, keep, first, recent)
         self._check(self._lib.aionhip_step_evict_paged(self._ctx, cache.ref, C.byref(e)))

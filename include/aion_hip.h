@@ -411,7 +411,8 @@ int aionhip_step_attention_paged(aionhip_ctx *ctx, const aionhip_attention *p, c
 /* Eviction: of each sequence longer than `limit` every KV head keeps `keep` rows (first + recent <= keep <= limit): the `first` oldest, the `recent` newest, and of
  * those between them the ones of greatest weight, of equal weights the oldest (a NaN is the greatest, -0 equals 0). A head's rows keep their order and become steps 0 .. keep - 1;
  * which steps remain differs from head to head, how many does not. A sequence of up to `limit` rows keeps all. Decided on the device: a recorded
- * program may hold the step and run it every token.
+ * program may hold the step and run it every token. Every step below the length of a sequence that is cut or copied lies on a page: the choice looks at weights alone, and of a step on
+ * an entry that is no page nothing moves, so that the step it becomes, where that one has a page, shows what the page held there before.
  *   weights  f32 [batch, h_kv, capacity], kv_lengths i32 [batch]
  *   table_out 0: in place. The rows move within the cache's own pages (none of them shared with another sequence), a sequence of up to `limit` rows is left alone;
  *     rows go through up to 256 MiB of the context's scratch memory (a head's rows at least) on the way.
