@@ -23,9 +23,12 @@ using namespace attn;
 using paged::Table;
 
 constexpr float MASKED = -INFINITY;
-// Probabilities are held as 2^(s - ref + HEAD_ROOM), the reference being raised only when a score passes it by more than SLACK: 2^14 at most fits f16, and what f16
-// pairs round away lies 2^-31 below the largest.
-constexpr float HEAD_ROOM = 6.f, SLACK = 8.f;
+// Probabilities are held as 2^(s - ref + HEAD_ROOM), 2^15 at most, which fits f16; a pair of f16 rounds to 2^-22 of itself or 2^-25, whichever is more. So the reference goes by the tile: it is
+// raised when the tile's largest score passes it by more than SLACK, and over f16 values lowered when that lies more than DROP below it, by up to DEPTH below the largest score of all.
+// What a key loses is then 2^-31 of the largest probability of its own tile of 32, and an answer 2^-26 of the largest value, however many keys there are. (A reference that only rises loses
+// as much of the row's largest with every key: of a hundred thousand keys 22 nats below one whose value is zero nothing was left.) DEPTH keeps the sums, 2^31 keys of 65504 times
+// 2^(15 + 64) at most, and the factors between segments in f32. Three bf16 need no lowering.
+constexpr float HEAD_ROOM = 10.f, SLACK = 5.f, DROP = 4.f, DEPTH = 64.f;
 
 struct PagedArgs {
     float *out, *partial, *scores;
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
     };
 
     f32x4 acc[MT];
-    float ref = MASKED, l_run = 0.f;                             // l_run: of this lane's keys
+    float ref = MASKED, peak = MASKED, l_run = 0.f;              // peak: the largest score; l_run: of this lane's keys
     constexpr int DEVICE_SCOPE = 16;                             // the sc1 bit of a buffer access: written through, read at the point where the XCDs' caches agree
     (void)DEVICE_SCOPE;
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -434,9 +437,12 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
         mx = groups4_max(mx);
-        if (__any(mx > ref + SLACK)) {
-            const float ref_new = fmaxf(ref, mx), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - ref_new) : 0.f;
-            if (ref_new > ref) {
+        peak = fmaxf(peak, mx);
+        const float ref_new = KV == AIONHIP_F16 ? fmaxf(mx, peak - DEPTH) : mx;
+        const bool moves = ref_new > ref + SLACK || (KV == AIONHIP_F16 && mx > MASKED && ref_new < ref - DROP);
+        if (__any(moves)) {
+            if (moves) {
+                const float alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - ref_new) : 0.f;
                 l_run *= alpha;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[mt] *= alpha;

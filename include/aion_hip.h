@@ -400,7 +400,8 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, 
 /* aionhip_step_attention over pages: out, q, batch, l_q, h_q, q_dtype, scale, soft cap and window as there; k and v are 0, t_kv is the capacity, h_kv, d_k = d_v and kv_dtype
  * are the cache's, rolling is 0. kv_lengths 0: every sequence fills its capacity; a length past it counts as the capacity. query_positions 0: the queries are the last
  * l_q steps, kv_lengths[b] - l_q + i (one before the first step sees nothing) - and so a position is the row in the cache, which after an eviction is no longer the position that
- * the row was turned by. f32 accuracy (about 1e-6) whatever aionhip_set_attention_precise says. A query that sees no key, or only scores of minus infinity, gets zeros; what is not
+ * the row was turned by. f32 accuracy whatever aionhip_set_attention_precise says: about 1e-6 of
+ * the sum of the probabilities times their values' magnitudes, and over f16 pages 2^-26 of the largest value that the query sees, however many keys there are. A query that sees no key, or only scores of minus infinity, gets zeros; what is not
  * finite reaches the queries that see it and no others. Head sizes 64, 128 and 256 run on the matrix pipe (out at a multiple of 16 bytes), others on a slow kernel. Made for one to a few tokens: of more
  * query rows to a KV head than sixteen, every sixteen walk the keys on their own. A long prompt is better read back (aionhip_step_read_paged) and run by
  * aionhip_step_attention, which shares the keys among 128 rows: 4096 tokens of 32 heads on 8 of 128 620 us over the pages, 143 with the rows read back first.
