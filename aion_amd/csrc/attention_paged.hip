@@ -23,18 +23,21 @@ using namespace attn;
 using paged::Table;
 
 constexpr float MASKED = -INFINITY;
-// Probabilities are held as 2^(s - ref + HEAD_ROOM), 2^15 at most, which fits f16; a pair of f16 rounds to 2^-22 of itself or 2^-25, whichever is more. So the reference goes by the tile: it is
+// Probabilities are held as 2^(s - ref + head_room), over f16 2^15 at most, which fits f16; a pair of f16 rounds to 2^-22 of itself or 2^-25, whichever is more. So the reference goes by the tile: it is
 // raised when the tile's largest score passes it by more than SLACK, and over f16 values lowered when that lies more than DROP below it, by up to DEPTH below the largest score of all.
 // What a key loses is then 2^-31 of the largest probability of its own tile of 32, and an answer 2^-26 of the largest value, however many keys there are. (A reference that only rises loses
 // as much of the row's largest with every key: of a hundred thousand keys 22 nats below one whose value is zero nothing was left.) DEPTH keeps the sums, 2^31 keys of 65504 times
-// 2^(15 + 64) at most, and the factors between segments in f32. Three bf16 need no lowering.
-constexpr float HEAD_ROOM = 10.f, SLACK = 5.f, DROP = 4.f, DEPTH = 64.f;
+// 2^(15 + 64) at most, and the factors between segments in f32. Three bf16 need no lowering, and no room above: below one
+// the sums have room for values that bf16 has and f16 has not, up to 2^100 whatever their number (with the room that f16 takes, values were infinite from 2^112 on).
+constexpr float SLACK = 5.f, DROP = 4.f, DEPTH = 64.f, LOW = -16.f;
+__host__ __device__ constexpr float head_room(int kv) { return kv == AIONHIP_F16 ? 10.f : LOW; }
+__host__ __device__ constexpr float two_to(float e) { return e < 0.f ? 1.f / two_to(-e) : (float)(1 << (int)e); }
 
 struct PagedArgs {
     float *out, *partial, *scores;
     const float *weights_before;
     float *weights;
-    float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum
+    float2 *stats;            // of each row: its reference (log2) and the reciprocal of its sum of 2^(s - reference)
     int streams;              // of keys: segments of heads of sequences
     int beside;               // workgroups that read the same keys lie side by side behind one L2
     int draws;                // the workgroup that ends last adds up the weights itself
@@ -127,7 +130,7 @@ __device__ __forceinline__ void walk_again(const PagedArgs &a, int b, int hk, in
             const float s = a.soft_cap > 0.f ? a.soft_cap * LOG2E * tanhf(dot * (a.scale / a.soft_cap)) : dot * (a.scale * LOG2E);
             if (a.scores && lane == 0 && dv0 == 0)
                 __hip_atomic_store(a.scores + ((size_t)(b * a.Hkv + hk) * rows_total + r) * a.tpad + key, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float top = fmaxf(ref, s), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + HEAD_ROOM);
+            const float top = fmaxf(ref, s), alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + head_room(a.kv_dtype));
             l = l * alpha + p;
 #pragma unroll
             for (int j = 0; j < DV / 64; ++j) o[j] = o[j] * alpha + p * load_scalar(a.v, a.kv_dtype, at + dv0 + lane + 64 * j);
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
                 ref = ref_new;
             }
         }
-        const float base = (ref > MASKED ? ref : 0.f) - HEAD_ROOM;
+        const float base = (ref > MASKED ? ref : 0.f) - head_room(KV);
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -547,7 +550,7 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *(f32x4 *)(z.out + (((size_t)b * L + l2) * (a.Hkv * a.groups) + hk * a.groups + g2) * D + dv0 + col) = o * inv;
         if (a.scores && dv0 + col == 0) {
-            const float2 st{(top > MASKED ? top : 0.f) - HEAD_ROOM, inv};
+            const float2 st{top > MASKED ? top : 0.f, inv * two_to(head_room(KV))};
             if (z.draws) s_stat[row] = st;
             else z.stats[(size_t)unit * rows_total + rr] = st;
         }
@@ -812,7 +815,7 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
         if (a.scores && lane == 0) a.scores[((size_t)unit * a.rows_total + r) * a.tpad + key] = s;
         if (page < 0) continue;
         const float top = fmaxf(ref, s);
-        const float alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f));
+        const float alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - top) : 1.f, p = __builtin_amdgcn_exp2f(s - (top > MASKED ? top : 0.f) + LOW);
         l = l * alpha + p;
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
@@ -833,7 +836,7 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedArgs a) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int c = threadIdx.x; c < a.d; c += 256) a.out[qbase + c] = (s_o[0][c] * f[0] + s_o[1][c] * f[1] + s_o[2][c] * f[2] + s_o[3][c] * f[3]) * inv;
-    if (a.stats && threadIdx.x == 0) a.stats[(size_t)unit * a.rows_total + r] = float2{top > MASKED ? top : 0.f, inv};
+    if (a.stats && threadIdx.x == 0) a.stats[(size_t)unit * a.rows_total + r] = float2{top > MASKED ? top : 0.f, inv * two_to(LOW)};
 }
 
 template <int KV, int D, int QP, bool MULTI, bool ONCE, int SHARES = 1>

@@ -401,8 +401,9 @@ int aionhip_step_read_paged(aionhip_ctx *ctx, const aionhip_paged_cache *cache, 
  * are the cache's, rolling is 0. kv_lengths 0: every sequence fills its capacity; a length past it counts as the capacity. query_positions 0: the queries are the last
  * l_q steps, kv_lengths[b] - l_q + i (one before the first step sees nothing) - and so a position is the row in the cache, which after an eviction is no longer the position that
  * the row was turned by. f32 accuracy whatever aionhip_set_attention_precise says: about 1e-6 of
- * the sum of the probabilities times their values' magnitudes, and over f16 pages 2^-26 of the largest value that the query sees, however many keys there are. A query that sees no key, or only scores of minus infinity, gets zeros; what is not
- * finite reaches the queries that see it and no others. Head sizes 64, 128 and 256 run on the matrix pipe (out at a multiple of 16 bytes), others on a slow kernel. Made for one to a few tokens: of more
+ * the sum of the probabilities times their values' magnitudes, and over f16 pages 2^-26 of the largest value that the query sees, however many keys there are; of bf16 values
+ * up to 2^100 (larger ones may sum to infinity). A query that sees no key, or only scores of minus infinity, gets zeros; what is not finite reaches the queries that see it
+ * and no others. Head sizes 64, 128 and 256 run on the matrix pipe (out at a multiple of 16 bytes), others on a slow kernel. Made for one to a few tokens: of more
  * query rows to a KV head than sixteen, every sixteen walk the keys on their own. A long prompt is better read back (aionhip_step_read_paged) and run by
  * aionhip_step_attention, which shares the keys among 128 rows: 4096 tokens of 32 heads on 8 of 128 620 us over the pages, 143 with the rows read back first.
  * weights (0: none), f32 [batch, h_kv, capacity]: weights = weights_before (the same shape, the same buffer or 0, which counts as zeros) + the probability of

@@ -69,3 +69,17 @@ def test_tiles_far_apart(gpu, d, score):
     off = np.repeat(np.stack([largest @ np.abs(to_f64(pages.v, be.F16).transpose(1, 0, 2, 3).reshape(2, -1, d)[g, :n]) for g in range(2)]), 4, axis=0)[None, None] * 2.0 ** -31
     assert near.close(near.out + np.maximum(np.abs(got - near.out) - off, 0.0)).all(), np.abs(got / near.out - 1).max()
     assert near.weights_close(weights, drawn, 4).all()
+
+
+@pytest.mark.parametrize("hq, h, d", [(4, 2, 64), (8, 2, 128), (8, 1, 256), (2, 1, 72)])
+@pytest.mark.parametrize("n", [1, 20, 3001])
+@pytest.mark.parametrize("size", [100, 112, 120])
+def test_values_past_the_range_of_f16(gpu, hq, h, d, n, size):
+    """values of 2^size: their sum over the keys is far past f32's range before it is divided by that of the probabilities where a key counts for 2^15 or one"""
+    if n > 1000 and size > 112:
+        n = 200
+    pages, near, drawn = peaked(np.random.default_rng(d), be.BF16, n, hq, h, d, lambda t: t % 5 * 0.5, lambda t: np.full(t.size, 2.0 ** size))
+    q = np.zeros((1, 1, hq, d), np.float32)
+    q[..., 0] = 1.0
+    got, weights = attend(gpu, pages, q, be.F32, 1.0, lengths=[n])
+    assert near.close(got).all() and near.weights_close(weights, drawn, hq // h).all()
