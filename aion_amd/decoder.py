@@ -78,6 +78,12 @@ class DecoderConfig:
             raise ValueError("evict_keep %d <= evict_limit %d < max_seq %d must hold" % (self.evict_keep, limit, self.max_seq))
         return self.evict_keep, limit, first, recent
 
+    def turning(self):
+        """How q and k turn on caches in pages."""
+        if self.rotary is not None and not self.page_rows:
+            raise ValueError("rotary: linear caches turn the whole head by rope_base (page_rows)")
+        return self.rotary or be.Rotary(self.head_dim, base=self.rope_base)
+
     def cache_bytes(self, gpu):
         """Bytes of one layer's cache of keys (or values)."""
         if self.page_rows:
@@ -147,6 +153,7 @@ class Decoder:
     def __init__(self, gpu, cfg, weights, on_weight=None, one_launch=False):
         """on_weight(name, host_array) is called for every tensor (the tests feed the oracle with it)."""
         self.gpu, self.cfg = gpu, cfg
+        self.eviction, self.rotary = cfg.eviction(), cfg.turning()
         self.stack = None
         layout = be.ROWS_NK if cfg.wdtype == be.Q8_0 else be.KMAJOR_KN
         self.w = {}
@@ -169,8 +176,6 @@ class Decoder:
         kv_bytes = cfg.cache_bytes(gpu)
         self.kc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
         self.vc = [gpu.zeros(kv_bytes) for _ in range(cfg.layers)]
-        self.eviction = cfg.eviction()
-        self.rotary = cfg.rotary or be.Rotary(cfg.head_dim, base=cfg.rope_base)
         self.page_table, self.caches, self.drawn, self.linear = None, [], [], None
         if cfg.page_rows:
             self.page_table = gpu.upload(np.arange(cfg.pages, dtype=np.int32))
@@ -474,8 +479,8 @@ class SessionDecoder:
 
     def __init__(self, gpu, cfg, weights, fusion=None):
         from . import session as ss
-        if cfg.page_rows:
-            raise ValueError("page_rows: aion's step list has no caches in pages")
+        if cfg.page_rows or cfg.rotary is not None or cfg.evict_keep:
+            raise ValueError("page_rows, rotary, evict_keep: aion's step list has no caches in pages")
         self.ss, self.gpu, self.cfg = ss, gpu, cfg
         self.sess = ss.Session(gpu)
         if fusion is not None:

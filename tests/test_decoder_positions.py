@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from aion_amd import backend as be
-from aion_amd.decoder import Decoder, DecoderConfig, SyntheticWeights
+from aion_amd.decoder import Decoder, DecoderConfig, SessionDecoder, SyntheticWeights
 
 SHAPE = dict(layers=2, hidden=256, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1024)
 KINDS = {"linear": {}, "q8": dict(cache_dtype=be.Q8_0), "pages": dict(page_rows=16), "evicting": dict(page_rows=16, evict_keep=16, evict_limit=36)}
@@ -165,6 +165,17 @@ def test_no_newest_rows_need_stay():
     cfg = lambda **kw: DecoderConfig(max_seq=64, page_rows=16, evict_keep=16, **SHAPE, **kw).eviction()  # noqa: E731
     assert cfg(evict_recent=0) == (16, 63, 4, 0) and cfg(evict_recent=0, evict_first=0) == (16, 63, 0, 0)
     assert cfg() == cfg(evict_recent=None) == (16, 63, 4, 4) and cfg(evict_recent=40) == (16, 63, 4, 12)
+
+
+def test_what_only_caches_in_pages_have_is_refused_elsewhere():
+    for options in (dict(rotary=be.Rotary(32)), dict(evict_keep=16), dict(cache_dtype=be.Q8_0, rotary=be.Rotary(64))):
+        cfg = DecoderConfig(max_seq=64, **options, **SHAPE)
+        with pytest.raises(ValueError):
+            Decoder(Backend(), cfg, Blank(cfg, 1))
+        with pytest.raises(ValueError):
+            SessionDecoder(Backend(), cfg, Blank(cfg, 1))
+    cfg = DecoderConfig(max_seq=64, page_rows=16, rotary=be.Rotary(32), **SHAPE)
+    assert Decoder(Backend(), cfg, Blank(cfg, 1)).rotary is cfg.rotary
 
 
 @pytest.mark.gpu
