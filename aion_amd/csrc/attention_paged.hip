@@ -27,9 +27,10 @@ constexpr float MASKED = -INFINITY;
 // raised when the tile's largest score passes it by more than SLACK, and over f16 values lowered when that lies more than DROP below it, by up to DEPTH below the largest score of all.
 // What a key loses is then 2^-31 of the largest probability of its own tile of 32, and an answer 2^-26 of the largest value, however many keys there are. (A reference that only rises loses
 // as much of the row's largest with every key: of a hundred thousand keys 22 nats below one whose value is zero nothing was left.) DEPTH keeps the sums, 2^31 keys of 65504 times
-// 2^(15 + 64) at most, and the factors between segments in f32. Three bf16 need no lowering, and no room above: below one
+// 2^(15 + 64) at most, and the factors between segments in f32. A reference is a whole number, so that sums come from one to another without a rounding (a thousand of which, where tiles
+// lie far apart in turn, were 2e-6). Three bf16 need no lowering, and no room above: below one
 // the sums have room for values that bf16 has and f16 has not, up to 2^100 whatever their number (with the room that f16 takes, values were infinite from 2^112 on).
-constexpr float SLACK = 5.f, DROP = 4.f, DEPTH = 64.f, LOW = -16.f;
+constexpr float SLACK = 5.f, DROP = 3.f, DEPTH = 64.f, LOW = -16.f;
 __host__ __device__ constexpr float head_room(int kv) { return kv == AIONHIP_F16 ? 10.f : LOW; }
 __host__ __device__ constexpr float two_to(float e) { return e < 0.f ? 1.f / two_to(-e) : (float)(1 << (int)e); }
 
@@ -441,11 +442,11 @@ __global__ __launch_bounds__(wavefronts(D) * 64, D == 256 ? 2 : 3) void paged_at
         float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
         mx = groups4_max(mx);
         peak = fmaxf(peak, mx);
-        const float ref_new = KV == AIONHIP_F16 ? fmaxf(mx, peak - DEPTH) : mx;
+        const float ref_new = __builtin_ceilf(KV == AIONHIP_F16 ? fmaxf(mx, peak - DEPTH) : mx);
         const bool moves = ref_new > ref + SLACK || (KV == AIONHIP_F16 && mx > MASKED && ref_new < ref - DROP);
         if (__any(moves)) {
             if (moves) {
-                const float alpha = ref > MASKED ? __builtin_amdgcn_exp2f(ref - ref_new) : 0.f;
+                const float alpha = ref > MASKED ? __builtin_amdgcn_ldexpf(1.f, (int)fmaxf(fminf(ref - ref_new, 200.f), -200.f)) : 0.f;
                 l_run *= alpha;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[mt] *= alpha;

@@ -83,3 +83,23 @@ def test_values_past_the_range_of_f16(gpu, hq, h, d, n, size):
     q[..., 0] = 1.0
     got, weights = attend(gpu, pages, q, be.F32, 1.0, lengths=[n])
     assert near.close(got).all() and near.weights_close(weights, drawn, hq // h).all()
+
+
+@pytest.mark.parametrize("dtype", [be.F16, be.BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_sums_keep_their_size_while_the_reference_moves(gpu, dtype, d):
+    """Two keys of equal score and opposite values, at either end of a text whose tiles lie ten powers of two and more apart in turn: each wavefront's sums are brought to another reference up to a
+    thousand times in between, and the answer is zero as long as that loses nothing. Each probability is off by 2^-23 (exp2) and 2^-22 (its halves) at most, and by 2^-23 in each of two meetings: 2^-20."""
+    b, n = 1024, 131072 if d < 256 else 65536
+    rng = np.random.default_rng(0)
+    high, low = -16.5 + 3 * rng.random(n // 128), -23.5 - 8 * rng.random(n // 128)
+    level = np.where(np.arange(n // 128) % 2 == 1, high, low)
+    pages, _, _ = peaked(rng, dtype, n, 1, 1, d, lambda t: np.where((t == 0) | (t == n - 1), 0.0, level[t // 128]), lambda t: np.zeros(t.size))
+    pages.v[0, 0, 0], pages.v[-1, 0, -1] = to_bits(np.array([1.0, -1.0], np.float32), dtype)
+    pages.b, pages.table = b, np.repeat(pages.table, b, axis=0)
+    q = np.zeros((b, 1, 1, d), np.float32)
+    q[..., 0] = 1.0
+    got, _ = attend(gpu, pages, q, be.F32, 1.0, lengths=[n] * b, weigh=False)
+    launch = gpu.last_launch()
+    assert launch["grid"][0] == 1 and n // 32 // (launch["block"][0] // 64) >= 256                     # (one segment)
+    assert np.abs(got).max() <= 2.0 ** -20, np.abs(got).max()
