@@ -199,8 +199,8 @@ struct Move {
 };
 // The rows that stay, keys and values together, a 16-byte piece of each to a thread. TO_PAGES: to pages of their own. In place the rows go through memory outside the cache (HOLD,
 // then BACK), as one that moves may lie where another goes to; those in front of the first that leaves do not move. 4 sequences of 32768 rows of 8 heads of 128 cut to 8192:
-// 55.4 us to pages of their own, 4.9 TB/s of rows of 256 bytes picked from four times as many. In place 95 with the choice of the rows, and one of 4352 cut to 4096 27
-// (193 and 86 by workgroups that moved all rows of a few columns in order).
+// 53.2 us to pages of their own, 5.0 TB/s of rows of 256 bytes picked from four times as many. In place 106 with the choice of the rows (24, then 42 and 40), and one of 4352 cut to
+// 4096 27 (193 and 86 by workgroups that moved all rows of a few columns in order).
 enum { TO_PAGES, HOLD, BACK };
 template <int MODE>
 __global__ __launch_bounds__(256) void move_kernel(Move a) {
